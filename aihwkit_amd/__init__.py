@@ -6,6 +6,6 @@ and GPU tile classes with ``forward`` / ``backward`` / ``update`` taking torch t
 arithmetic runs in ``lib/librpu_amd.so`` (HIP kernels for gfx950) through the C ABI of
 ``include/rpu_amd.h``.
 """
-from . import rpu_base  # noqa: F401
+from . import digital, rpu_base  # noqa: F401
 
-__all__ = ["rpu_base"]
+__all__ = ["digital", "rpu_base"]

@@ -42,6 +42,19 @@ class UpdateParams(C.Structure):
     ]
 
 
+class DropoutParams(C.Structure):
+    """``rpu_dropout_params``."""
+
+    _fields_ = [("p", C.c_double), ("seed", C.c_uint64), ("call", u32), ("reserved", u32), ("call_dev", C.c_void_p)]
+
+
+class Adapters(C.Structure):
+    """``rpu_adapters``."""
+
+    _fields_ = [("a_dev", C.c_void_p), ("b_dev", C.c_void_p), ("scale_dev", C.c_void_p), ("n", i32), ("in_size", i32),
+                ("out_size", i32), ("rank", i32), ("w_dtype", i32), ("reserved", i32)]
+
+
 class DeviceParams(C.Structure):
     """``rpu_device_params``."""
 
@@ -212,6 +225,21 @@ SYMBOLS = {
     "rpu_tile_profile_name": (C.c_char_p, [_P, C.c_int]),
     "rpu_philox4x32_10": (C.c_int, [C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32)]),
     "rpu_philox4x32_10_device": (C.c_int, [C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.POINTER(C.c_uint32), C.c_int]),
+    "rpu_dropout": (C.c_int, [_P, C.c_long, _P, C.c_long, _P, C.c_long, C.c_int, C.c_int, C.c_int, C.POINTER(DropoutParams),
+                              C.c_int, _P]),
+    "rpu_layer_norm": (C.c_int, [_P, C.c_long, _P, _P, C.c_int, _P, C.c_long, _P, _P, C.c_int, C.c_int, C.c_int, C.c_float,
+                                 C.c_int, _P]),
+    "rpu_layer_norm_backward_scratch": (C.c_size_t, [C.c_int, C.c_int]),
+    "rpu_layer_norm_backward": (C.c_int, [_P, C.c_long, _P, C.c_long, _P, _P, _P, C.c_int, _P, C.c_long, _P, C.c_long, _P, _P,
+                                          C.c_int, C.c_int, C.c_int, _P, C.c_size_t, C.c_int, _P]),
+    "rpu_adapter_plan_bytes": (C.c_size_t, [C.c_int, C.c_int]),
+    "rpu_adapter_plan": (C.c_int, [_P, C.c_int, C.c_int, _P, C.c_size_t, C.c_int, _P]),
+    "rpu_adapter_forward": (C.c_int, [C.POINTER(Adapters), _P, C.c_long, _P, _P, C.c_size_t, C.POINTER(DropoutParams), _P,
+                                      C.c_long, _P, C.c_long, _P, C.c_int, C.c_int, C.c_int, _P]),
+    "rpu_adapter_backward_scratch": (C.c_size_t, [C.POINTER(Adapters), C.c_int]),
+    "rpu_adapter_backward": (C.c_int, [C.POINTER(Adapters), _P, C.c_long, _P, C.c_long, _P, _P, C.c_size_t,
+                                       C.POINTER(DropoutParams), _P, C.c_long, _P, C.c_long, _P, _P, C.c_int, C.c_int, _P,
+                                       C.c_size_t, C.c_int, _P]),
     "rpu_device_allocation_count": (C.c_long, []),
     "rpu_last_error": (C.c_char_p, []),
     "rpu_abi_version": (C.c_int, []),

@@ -1,0 +1,235 @@
+// The digital operators beside the tiles (dropout, layer norm, low-rank adapters): argument blocks, launches, and what their
+// kernels share.  Tensors are rows of a unit column stride in one of three types; everything is computed in 32 bits.
+#pragma once
+#include "../../include/rpu_amd.h"
+#include "bf16_parts.h"
+#include "philox.h"
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace rpu_amd {
+
+struct MatrixDev { // rows at p + row * ld; p null: not given
+  void *p;
+  long ld;
+};
+
+// Dropout of element (row, column): half column % 8 of the Philox block of counter (column / 8, row, call, RNG_DROPOUT), u,
+// is dropped below the limit round(p 2^32): u < limit / 2^16, or u equal to it and the same half of the block of
+// RNG_DROPOUT_LOW below limit % 2^16.  32 bits decide, at the price of 16: one element in 65536 needs the second block.
+struct DropDev {
+  uint32_t high, low; // the limit's halves (high = 65536: all)
+  float scale;        // of what is kept, 1 / (1 - p)
+  PhiloxKey key;
+  uint32_t call;
+  const int64_t *call_dev; // added to `call` when the kernel runs; null: nothing is
+  int on;
+};
+
+struct DropoutArgs {
+  MatrixDev x, base, out;
+  int rows, cols;
+  DropDev drop;
+};
+void launch_dropout(const DropoutArgs &a, int dtype, int cus, hipStream_t s);
+
+struct NormArgs {
+  MatrixDev x, out;
+  const void *w, *b; // null: ones, zeros
+  float *mean, *rstd;
+  int rows, cols;
+  float eps;
+};
+void launch_layer_norm(const NormArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+
+struct NormBackwardArgs {
+  MatrixDev d, x, base, dx;
+  const float *mean, *rstd;
+  const void *w;       // null: ones
+  void *dw, *db;       // null: not wanted (both)
+  float *part;         // [parts][2][cols]
+  int rows, cols, parts;
+};
+int layer_norm_parts(int rows, int cols, int cus); // workgroups of the backward pass, each of which leaves sums of its rows
+void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtype, hipStream_t s);
+
+// Rows grouped by adapter: what launch_adapter_plan writes, one array of ints.
+//   order [rows]       rows by adapter, in their order within each; those without one last
+//   seg [n + 2]        seg[a]: where adapter a begins in `order`; seg[n]: the rows without one; seg[n + 1] = rows
+//   tiles [4 * tiles]  {adapter or -1, first place in `order`, rows (0: none), 0}: at most tile_rows rows each
+//   chunks [4 * chunks]  the same in longer pieces for the gradients, of adapters only; the last number is the slot for the
+//                      chunk's sums, -1 if it holds all rows of its adapter
+//   first [n + 1]      first[a]: the first chunk of adapter a
+//   tile_first [n + 2], slot_first [n + 1]  the same of the tiles and of the slots
+//   other [rows]       scratch
+struct AdapterPlan {
+  int rows, n;
+  int tile_rows, chunk_rows;
+  int max_tiles, max_chunks, max_slots;
+  size_t order, seg, tiles, chunks, first, tile_first, slot_first, other, words; // offsets in ints, total
+};
+AdapterPlan adapter_plan(int rows, int n);
+void launch_adapter_plan(const int *index, int *plan, const AdapterPlan &p, hipStream_t s);
+constexpr int ADAPTER_FEW_ROWS = 64; // up to so many rows a forward call groups them by itself
+constexpr int ADAPTER_MAX_RANK = 128;
+constexpr int ADAPTER_MAX = 65535;
+
+struct AdapterRowsArgs {
+  MatrixDev in, base, out;     // forward: x, base, y; backward: d, base, dx
+  const void *w_in, *w_out;    // forward: a, b; backward: b, a
+  const float *scale;
+  float *hidden;               // [rows][rank]: a drop(x), or scale b^T d; null: not wanted
+  const int *index;            // without a plan
+  const int *plan;             // null: the rows are grouped from `index`
+  AdapterPlan p;
+  int rows, n, rank, in_size, out_size;
+  DropDev drop;                // of the input (forward) or of the output (backward)
+};
+void launch_adapter_forward(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+void launch_adapter_backward_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+
+struct AdapterGradArgs {
+  MatrixDev x, d;
+  const float *hidden, *up;    // [rows][rank]: a drop(x) and scale b^T d
+  const float *scale;
+  void *da, *db;               // [n][rank][in], [n][out][rank]
+  float *part;                 // [max_slots][rank * (in + out)]
+  const int *plan;
+  AdapterPlan p;
+  int rows, n, rank, in_size, out_size;
+  DropDev drop;
+};
+void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+
+#if defined(__HIPCC__)
+// ---- eight neighbouring values of a row -------------------------------------------------------------------------------
+// Rows begin at any element: loads and stores of 16 bytes from any address that a value may have.
+typedef uint32_t u32x4_from2 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t u32x4_from4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x2_from2 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t u32x2_from4 __attribute__((ext_vector_type(2), aligned(4)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+struct Values8 {
+  float v[8];
+};
+
+__device__ __forceinline__ float to_float(float v) { return v; }
+__device__ __forceinline__ float to_float(__bf16 v) { return __uint_as_float((uint32_t)__builtin_bit_cast(uint16_t, v) << 16); }
+__device__ __forceinline__ float to_float(_Float16 v) { return (float)v; }
+
+template <typename T> struct Packed8; // the eight values as they are stored
+template <> struct Packed8<float> {
+  u32x4_from4 q[2];
+};
+template <> struct Packed8<__bf16> {
+  u32x4_from2 q;
+};
+template <> struct Packed8<_Float16> {
+  u32x4_from2 q;
+};
+__device__ __forceinline__ Packed8<float> load8(const float *p) {
+  const u32x4_from4 *s = reinterpret_cast<const u32x4_from4 *>(p);
+  return {{s[0], s[1]}};
+}
+__device__ __forceinline__ Packed8<__bf16> load8(const __bf16 *p) { return {*reinterpret_cast<const u32x4_from2 *>(p)}; }
+__device__ __forceinline__ Packed8<_Float16> load8(const _Float16 *p) { return {*reinterpret_cast<const u32x4_from2 *>(p)}; }
+
+__device__ __forceinline__ Values8 widen(const Packed8<float> &p) {
+  Values8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = __uint_as_float(p.q[i >> 2][i & 3]);
+  return r;
+}
+__device__ __forceinline__ Values8 widen(const Packed8<__bf16> &p) {
+  Values8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    r.v[2 * i] = __uint_as_float(p.q[i] << 16);
+    r.v[2 * i + 1] = __uint_as_float(p.q[i] & 0xffff0000u);
+  }
+  return r;
+}
+__device__ __forceinline__ Values8 widen(const Packed8<_Float16> &p) {
+  Values8 r;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const f16x2 h = __builtin_bit_cast(f16x2, (uint32_t)p.q[i]);
+    r.v[2 * i] = (float)h.x;
+    r.v[2 * i + 1] = (float)h.y;
+  }
+  return r;
+}
+// the first `count` of eight values (all where count >= 8), zeros behind them
+template <typename T> __device__ __forceinline__ Values8 read8(const T *p, int count) {
+  if (count >= 8) return widen(load8(p));
+  Values8 r;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) r.v[i] = i < count ? to_float(p[i]) : 0.0f;
+  return r;
+}
+
+// One rounding, to nearest even, from the 32 bits that everything was computed in.
+__device__ __forceinline__ uint32_t pack2(float a, float b, __bf16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, _Float16) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, f16x2));
+}
+__device__ __forceinline__ void store8(float *p, const Values8 &r) {
+  u32x4_from4 *d = reinterpret_cast<u32x4_from4 *>(p);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    u32x4_from4 q;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(r.v[4 * h + i]);
+    d[h] = q;
+  }
+}
+template <typename T> __device__ __forceinline__ void store8(T *p, const Values8 &r) {
+  u32x4_from2 q;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) q[i] = pack2(r.v[2 * i], r.v[2 * i + 1], T{});
+  *reinterpret_cast<u32x4_from2 *>(p) = q;
+}
+template <typename T> __device__ __forceinline__ void write8(T *p, const Values8 &r, int count) {
+  if (count >= 8) {
+    store8(p, r);
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) p[i] = (T)r.v[i];
+}
+
+// ---- dropout ----------------------------------------------------------------------------------------------------------
+__device__ __forceinline__ uint32_t drop_call(const DropDev &d) { return d.call + (d.call_dev ? (uint32_t)*d.call_dev : 0u); }
+
+// bit h: element 8 * block + h of the row is kept
+__device__ __forceinline__ uint32_t drop_kept(const DropDev &d, uint32_t call, uint32_t row, uint32_t block) {
+  const Philox4 r = philox4x32_10(block, row, call, RNG_DROPOUT, d.key.k0, d.key.k1);
+  uint32_t kept = 0, even = 0;
+#pragma unroll
+  for (int h = 0; h < 8; ++h) {
+    const uint32_t u = h & 1 ? r.v[h >> 1] >> 16 : r.v[h >> 1] & 0xffffu;
+    kept |= u > d.high ? 1u << h : 0u;
+    even |= u == d.high ? 1u << h : 0u;
+  }
+  if (even) {
+    const Philox4 q = philox4x32_10(block, row, call, RNG_DROPOUT_LOW, d.key.k0, d.key.k1);
+#pragma unroll
+    for (int h = 0; h < 8; ++h) {
+      const uint32_t v = h & 1 ? q.v[h >> 1] >> 16 : q.v[h >> 1] & 0xffffu;
+      kept |= v >= d.low ? even & (1u << h) : 0u;
+    }
+  }
+  return kept;
+}
+// What is dropped is zero whatever it was (an infinity, a NaN), never zero times it.
+__device__ __forceinline__ void drop_apply(const DropDev &d, uint32_t kept, Values8 &r) {
+#pragma unroll
+  for (int h = 0; h < 8; ++h) r.v[h] = kept & (1u << h) ? r.v[h] * d.scale : 0.0f;
+}
+#endif
+
+} // namespace rpu_amd

@@ -1,0 +1,41 @@
+// Dropout whose mask is drawn again wherever it is needed and never stored: out = base + drop(x).  The backward pass is the
+// same map of the gradient.
+#include "digital.h"
+
+#include <algorithm>
+
+namespace rpu_amd {
+namespace {
+
+// A thread takes eight neighbouring elements, one Philox block, at a time.
+template <typename T> __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
+  const T *x = static_cast<const T *>(a.x.p), *base = static_cast<const T *>(a.base.p);
+  T *out = static_cast<T *>(a.out.p);
+  const uint32_t blocks = ((uint32_t)a.cols + 7u) / 8u, call = drop_call(a.drop);
+  const uint64_t total = (uint64_t)a.rows * blocks;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
+    const uint32_t row = (uint32_t)(i / blocks), block = (uint32_t)(i % blocks);
+    const int left = a.cols - (int)(block * 8u);
+    const long col = (long)block * 8;
+    Values8 v = read8(x + row * a.x.ld + col, left);
+    drop_apply(a.drop, drop_kept(a.drop, call, row, block), v);
+    if (base) {
+      const Values8 r = read8(base + row * a.base.ld + col, left);
+#pragma unroll
+      for (int h = 0; h < 8; ++h) v.v[h] += r.v[h];
+    }
+    write8(out + row * a.out.ld + col, v, left);
+  }
+}
+
+} // namespace
+
+void launch_dropout(const DropoutArgs &a, int dtype, int cus, hipStream_t s) {
+  const uint64_t total = (uint64_t)a.rows * (((uint64_t)a.cols + 7) / 8);
+  const dim3 grid((unsigned)std::min<uint64_t>((total + 255) / 256, (uint64_t)cus * 16));
+  if (dtype == RPU_F32) hipLaunchKernelGGL(k_dropout<float>, grid, dim3(256), 0, s, a);
+  else if (dtype == RPU_F16) hipLaunchKernelGGL(k_dropout<_Float16>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_dropout<__bf16>, grid, dim3(256), 0, s, a);
+}
+
+} // namespace rpu_amd

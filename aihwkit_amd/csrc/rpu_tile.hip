@@ -3,6 +3,7 @@
 // buffers of the kernels.  It plays the role of the reference's RPUPulsed (src/rpucuda/rpu_pulsed.{h,cpp})
 // and RPUCudaPulsed (src/rpucuda/cuda/rpucuda_pulsed.{h,cu}) pair.
 #include "../../include/rpu_amd.h"
+#include "entry.h"
 #include "kernels.h"
 #include "rpu_host.h"
 
@@ -26,14 +27,6 @@
 static __device__ __align__(256) unsigned char scratch[RPU_NOALLOC_MAX_SCRATCH_BYTES];
 
 namespace rpu_amd {
-
-#define RPU_HIP_CHECK(expr)                                                                         \
-  do {                                                                                              \
-    hipError_t _e = (expr);                                                                         \
-    if (_e != hipSuccess) {                                                                         \
-      throw RpuError(std::string("HIP error: ") + hipGetErrorString(_e) + " in " #expr);            \
-    }                                                                                               \
-  } while (0)
 
 namespace {
 
@@ -194,24 +187,6 @@ private:
     const auto after = std::lower_bound(s.begin(), s.end(), std::make_pair(to, (uintptr_t)0)); // the first that begins at or behind `to`
     return after != s.begin() && (after - 1)->second > from;
   }
-};
-
-class DeviceGuard {
-public:
-  explicit DeviceGuard(int device) {
-    RPU_HIP_CHECK(hipGetDevice(&prev_));
-    if (device != prev_) {
-      RPU_HIP_CHECK(hipSetDevice(device));
-      changed_ = true;
-    }
-  }
-  ~DeviceGuard() {
-    if (changed_) (void)hipSetDevice(prev_);
-  }
-
-private:
-  int prev_ = 0;
-  bool changed_ = false;
 };
 
 __global__ void k_philox_probe(uint32_t c0, uint32_t c1, uint32_t c2, uint32_t c3, uint32_t k0, uint32_t k1,
@@ -2393,26 +2368,14 @@ struct rpu_tile {
   Tile t;
 };
 
-namespace {
-thread_local std::string g_last_error;
-
-template <typename F> int guarded(F &&f) {
-  try {
-    f();
-    return 0;
-  } catch (const std::exception &e) {
-    g_last_error = e.what();
-    return 1;
-  } catch (...) {
-    g_last_error = "unknown error";
-    return 2;
-  }
+std::string &rpu_amd::last_error() {
+  static thread_local std::string message;
+  return message;
 }
-} // namespace
 
 extern "C" {
 
-const char *rpu_last_error(void) { return g_last_error.c_str(); }
+const char *rpu_last_error(void) { return last_error().c_str(); }
 int rpu_abi_version(void) { return RPU_AMD_ABI_VERSION; }
 
 int rpu_tile_config_default(rpu_tile_config *cfg, int device_kind) {

@@ -719,6 +719,94 @@ int rpu_group_set_round_wait_test_hook(rpu_group_t *group, int spin_limit, int e
  * for `beyond` bytes more than it needs. */
 int rpu_tile_set_exact_scratch_test_hook(rpu_tile_t *tile, size_t beyond);
 
+/* ---- digital operators beside the tiles ------------------------------------------------------
+ *
+ * No counterparts in the reference's rpucuda, which leaves them to torch: what stands digitally between and beside analog
+ * tiles of a network and is trained there, where the tiles' programmed weights are not any more.  They hold no state: every
+ * call gets its operands, outputs and scratch memory from the caller, all on GPU `device_id` (-1 = current), and is enqueued
+ * on `stream`; nothing waits on the host and nothing is allocated, so that calls can be captured into HIP graphs.
+ *
+ * Matrices are rows of unit column stride, `*_ld` values apart (column slices of larger matrices are read and written in
+ * place; ld >= columns wherever there is more than one row).  `dtype`: the type of all matrices of a call that are not named
+ * otherwise; they are computed in 32 bits and rounded once, to nearest even, when they are stored.
+ * `base_dev` (null: none): a matrix that is added to the result before that rounding; it may be the output itself, and
+ * operands that are only read may overlap each other.  Any other overlap of an output with an operand or another output is
+ * refused where an entry point does not allow it by name. */
+enum rpu_dtype {
+  RPU_F32 = 0,
+  RPU_F16 = 1,
+  RPU_BF16 = 2
+};
+
+/* Dropout: element (row, column) is dropped with probability p and otherwise scaled by 1 / (1 - p).  Whether it is dropped is
+ * a function of (seed, call, row, column) alone and is not stored: with limit = round(p 2^32), u and v half-words
+ * column % 8 (low half of word 0, high half of word 0, ...) of the Philox4x32-10 blocks of key (seed low, seed high) and
+ * counters (column / 8, row, call, 18) and (column / 8, row, call, 19), it is dropped if u < limit / 2^16, or
+ * u = limit / 2^16 and v < limit % 2^16.  What is dropped counts as zero, also where it is infinite or NaN. */
+typedef struct rpu_dropout_params {
+  double p;                /* [0, 1]; at 0 nothing is drawn, at 1 everything is dropped */
+  uint64_t seed;
+  uint32_t call;           /* a number of its own for every mask that is drawn with one seed */
+  uint32_t reserved;       /* 0 */
+  const int64_t *call_dev; /* null, or a number on the GPU that is added to `call` (mod 2^32) when the kernel runs: a captured
+                              step draws new masks in every replay if the caller counts it up in between */
+} rpu_dropout_params;
+
+/* out = base + dropout(x), [rows][cols]; out may be x.  The backward pass is the same call on the gradient. */
+int rpu_dropout(const void *x_dev, long x_ld, const void *base_dev, long base_ld, void *out_dev, long out_ld, int dtype,
+                int rows, int cols, const rpu_dropout_params *params, int device_id, void *stream);
+
+/* Layer norm of rows: out = (x - mean) rstd w + b with the mean of the row and rstd = (mean((x - mean)^2) + eps)^-1/2, both
+ * stored for the backward pass ([rows]).  w, b: [cols], of `w_dtype` (RPU_F32 or `dtype`); null: ones, zeros.  out may be x. */
+int rpu_layer_norm(const void *x_dev, long x_ld, const void *w_dev, const void *b_dev, int w_dtype, void *out_dev, long out_ld,
+                   float *mean_dev, float *rstd_dev, int dtype, int rows, int cols, float eps, int device_id, void *stream);
+
+/* Its gradients: with h = (x - mean) rstd and g = d w, dx = base + rstd (g - mean(g) - h mean(g h)), dw = sum over rows d h,
+ * db = sum over rows d (of `w_dtype`, both or neither; zeros for no rows).  dx may be d or x.  Sums over rows are added in a
+ * fixed order.  scratch: rpu_layer_norm_backward_scratch bytes (no less for other GPUs), used until the call's work is done. */
+size_t rpu_layer_norm_backward_scratch(int rows, int cols);
+int rpu_layer_norm_backward(const void *d_dev, long d_ld, const void *x_dev, long x_ld, const float *mean_dev,
+                            const float *rstd_dev, const void *w_dev, int w_dtype, const void *base_dev, long base_ld,
+                            void *dx_dev, long dx_ld, void *dw_dev, void *db_dev, int dtype, int rows, int cols,
+                            void *scratch_dev, size_t scratch_bytes, int device_id, void *stream);
+
+/* Low-rank adapters of one projection in_size -> out_size, of which every row of a call takes one:
+ *   forward   hidden = a x,  y = base + scale b hidden      (a [rank][in_size], b [out_size][rank] of the row's adapter)
+ *   backward  up = scale b^T d,  dx = base + a^T up,  da = sum over the adapter's rows up x^T,  db = scale sum d hidden^T
+ * where x is dropout(x) if `drop` is given (null: no dropout) and dx then the dropout of a^T up with the same mask.
+ * a_dev [n][rank][in_size] and b_dev [n][out_size][rank] are dense and of w_dtype: any type with dtype RPU_F32, `dtype`
+ * otherwise.  rank 1 .. RPU_ADAPTER_MAX_RANK (an adapter of a smaller rank: zeros in the rest), n 1 .. RPU_ADAPTER_MAX. */
+#define RPU_ADAPTER_MAX_RANK 128
+#define RPU_ADAPTER_MAX 65535
+typedef struct rpu_adapters {
+  const void *a_dev, *b_dev;
+  const float *scale_dev; /* [n] */
+  int32_t n, in_size, out_size, rank, w_dtype, reserved;
+} rpu_adapters;
+
+/* index_dev [rows]: the adapter of every row; a row whose number is not in 0 .. n - 1 has none (y = base, hidden = 0, dx =
+ * base, no part in da and db).  Groups the rows by adapter into plan_dev, rpu_adapter_plan_bytes(rows, n) bytes, for any
+ * number of forward and backward calls on as many rows and adapters, of whatever sizes; the order of the rows of an adapter is kept, so that the
+ * sums over them do not depend on the run. */
+size_t rpu_adapter_plan_bytes(int rows, int n);
+int rpu_adapter_plan(const int32_t *index_dev, int rows, int n, void *plan_dev, size_t plan_bytes, int device_id, void *stream);
+
+/* Rows up to which rpu_adapter_forward takes the index alone (plan_dev null): few rows are grouped within the call. */
+#define RPU_ADAPTER_FEW_ROWS 64
+/* hidden_dev [rows][rank], float, dense (null: not wanted).  y may be base, but no other operand. */
+int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_ld, const int32_t *index_dev,
+                        const void *plan_dev, size_t plan_bytes, const rpu_dropout_params *drop, const void *base_dev,
+                        long base_ld, void *y_dev, long y_ld, float *hidden_dev, int dtype, int rows, int device_id,
+                        void *stream);
+
+/* da_dev, db_dev: laid out and typed like a and b, zeros for adapters without rows.  dx may be base, but no other operand.
+ * scratch: rpu_adapter_backward_scratch bytes, used until the call's work is done. */
+size_t rpu_adapter_backward_scratch(const rpu_adapters *adapters, int rows);
+int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d_ld, const void *x_dev, long x_ld,
+                         const float *hidden_dev, const void *plan_dev, size_t plan_bytes, const rpu_dropout_params *drop,
+                         const void *base_dev, long base_ld, void *dx_dev, long dx_ld, void *da_dev, void *db_dev, int dtype,
+                         int rows, void *scratch_dev, size_t scratch_bytes, int device_id, void *stream);
+
 /* ---- inspection hooks (mirror the reference's debug hooks) ------------------------------ */
 
 /* After rpu_tile_update with a stochastic pulse type: copies the packed pulse words of that call
