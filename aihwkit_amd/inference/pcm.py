@@ -7,11 +7,12 @@ single-pair conductance converter of converter/conductance.py:24-82), ``GlobalDr
 to the host, perturbs them in torch and writes them back; here the perturbation runs on the tile's matrix in HBM.
 """
 import ctypes as C
-from typing import List, Optional
+from typing import List, Optional, Union
 
 import torch
 
 from .._cabi import PcmNoiseParams, check, lib
+from ..digital import AdapterRows, LowRankAdapters
 from ..rpu_base import devices, tiles
 
 
@@ -164,11 +165,16 @@ class InferenceTile:
             out.mul_(self.alpha)
         return out
 
-    def forward(self, x_input: torch.Tensor, is_test: bool = False, bias: bool = False) -> torch.Tensor:
+    def forward(self, x_input: torch.Tensor, is_test: bool = False, bias: bool = False,
+                adapters: Optional[LowRankAdapters] = None, rows: Optional[Union[torch.Tensor, AdapterRows]] = None) -> torch.Tensor:
         """Analog forward; in evaluation mode the output is scaled by the drift compensation (inference.py:264-282).
         ``bias``: the tile's last input column is the bias column and ``x_input`` comes without it (the tile adds the
-        column of ones, as the reference's ``forward(x_input, bias=True)`` does)."""
-        out = self._gpu().forward(x_input, bias, False, False, is_test, False)
+        column of ones, as the reference's ``forward(x_input, bias=True)`` does).
+        ``adapters``, ``rows``: digital low-rank adapters of ``x_input`` (without the bias column) that are added to the
+        compensated output, each row's by ``rows`` (see ``LowRankAdapters.forward``); the reference has no counterpart."""
+        if (adapters is None) != (rows is None):
+            raise RuntimeError("adapters and the rows' choice of them (rows) come together")
+        out = self._gpu().forward(x_input, bias, False, False, is_test, adapters is not None)
         if is_test and self.drift_compensation is not None and self.alpha != 1.0 and not self._alpha_in_tile:
             out = out * self.alpha
-        return out
+        return out if adapters is None else adapters.forward(x_input, rows, base=out, out=out)
