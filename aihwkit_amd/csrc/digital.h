@@ -77,17 +77,26 @@ constexpr int ADAPTER_MAX = 65535;
 
 struct AdapterRowsArgs {
   MatrixDev in, base, out;     // forward: x, base, y; backward: d, base, dx
-  const void *w_in, *w_out;    // forward: a, b; backward: b, a
+  const void *w_in, *w_out;    // [n][rank][in_size], [n][out_size][rank]: forward a, b; backward b, a with both exchanged
   const float *scale;
   float *hidden;               // [rows][rank]: a drop(x), or scale b^T d; null: not wanted
   const int *index;            // without a plan
   const int *plan;             // null: the rows are grouped from `index`
   AdapterPlan p;
   int rows, n, rank, in_size, out_size;
+  int back;
   DropDev drop;                // of the input (forward) or of the output (backward)
 };
-void launch_adapter_forward(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
-void launch_adapter_backward_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+void launch_adapter_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
+
+struct AdapterTurnArgs {
+  const void *a, *b;
+  void *a_turned, *b_turned;   // [n][in][rank], [n][rank][out], of adapters with rows
+  const int *plan;
+  AdapterPlan p;
+  int n, rank, in_size, out_size;
+};
+void launch_adapter_turn(const AdapterTurnArgs &a, int w_dtype, int cus, hipStream_t s);
 
 struct AdapterGradArgs {
   MatrixDev x, d;

@@ -5,6 +5,7 @@
 //
 //   k_adapter_plan   groups the rows by adapter (a stable counting sort) and cuts the groups into tiles and chunks
 //   k_adapter_rows   a tile of rows through both thin products, hidden and up never leave the workgroup in between
+//   k_adapter_turn   for the backward pass: the matrices with ranks and columns exchanged, so that it is the forward pass
 //   k_adapter_grads  sums over the rows of a chunk, for 128 columns of dA or dB
 //   k_adapter_join   adds the chunks of an adapter in their order, zeros for adapters without rows
 #include "digital.h"
@@ -13,6 +14,10 @@
 
 namespace rpu_amd {
 namespace {
+
+template <int V> struct Int {
+  static constexpr int value = V;
+};
 
 constexpr int PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
 
@@ -157,18 +162,160 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
   cut(plan + p.chunks, p.max_chunks, first, p.n, p.chunk_rows, slot_first);
 }
 
-constexpr int WAVES = 4;
+// ---- eight terms, or four ranks, of both operands of a product, as the matrix instructions take them ------------------
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
-__device__ __forceinline__ f32x4 mfma(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// rows of float: products on the fp32 instructions, whatever the weights are stored as
+template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) == 2> struct Pipe {
+  using X = Packed8<T>;
+  using W = Packed8<TW>;
+  using V = f32x4; // four ranks of hidden
+  static __device__ __forceinline__ f32x4 multiply(f32x4 a, f32x4 b, f32x4 c) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
+    return c;
+  }
+  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) {
+    const Values8 a = widen(w), b = widen(x);
+    c = multiply(f32x4{a.v[0], a.v[1], a.v[2], a.v[3]}, f32x4{b.v[0], b.v[1], b.v[2], b.v[3]}, c);
+    return multiply(f32x4{a.v[4], a.v[5], a.v[6], a.v[7]}, f32x4{b.v[4], b.v[5], b.v[6], b.v[7]}, c);
+  }
+  static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x.q[i >> 2][i & 3] = kept & (1u << i) ? x.q[i >> 2][i & 3] : 0u;
+  }
+  template <int RT> static __device__ __forceinline__ float split(const f32x4 (&v)[RT], V (&to)[RT]) {
+#pragma unroll
+    for (int q = 0; q < RT; ++q) to[q] = v[q];
+    return 1.0f;
+  }
+  using R = f32x4; // four ranks of a weight row
+  static __device__ __forceinline__ R four(const float *p) { return *reinterpret_cast<const f32x4_unaligned *>(p); }
+  template <typename H> static __device__ __forceinline__ R four(const H *p) {
+    const u32x2_from2 w = *reinterpret_cast<const u32x2_from2 *>(p);
+    const Values8 v = widen(Packed8<H>{u32x4_from2{w[0], w[1], 0u, 0u}});
+    return R{v.v[0], v.v[1], v.v[2], v.v[3]};
+  }
+  static __device__ __forceinline__ void put(R &r, int i, TW w) { r[i] = to_float(w); }
+  template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT][2], int j, const V (&v)[RT], f32x4 c) {
+#pragma unroll
+    for (int q = 0; q < RT; ++q) c = multiply(w[q][j], v[q], c);
+    return c;
+  }
+};
 
-// A product of 16 x 16 results takes, per lane, column lane % 16 of one operand and row lane % 16 of the other, four terms at
-// a time, of which the lane has term lane / 16.  Terms may come in any order that both operands share: a lane reads eight
-// neighbouring terms at once and hands them out one by one.  The result has, per lane, column lane % 16 and rows
-// 4 (lane / 16) + 0 .. 3.  With the weights as rows that is: lane % 16 = the row of x, and four neighbouring ranks -- the
-// very operand that the second product wants, so hidden goes from one to the other through registers (and LDS where waves
-// share the terms).
-template <typename T, typename TW, int RT, int MT, bool BACK> __global__ __launch_bounds__(64 * WAVES) void k_adapter_rows(AdapterRowsArgs a) {
-  constexpr int RP = 16 * RT, PITCH = RP + 4;
+// 16-bit rows with weights of their type: exact products, sums in 32 bits.  hidden, which is not one of their numbers, goes into the
+// second product as the sum of some that are, against the same weights again: three bf16 parts, which are all of its 24 bits; two
+// halves, 22 bits (an error of 2^-23, twice that of a float, far below the 2^-11 of what is stored in the end).
+template <typename T> struct Pipe<T, T, true> {
+  using X = Packed8<T>;
+  using W = Packed8<T>;
+  struct V {
+    u32x4 upper; // the first two parts
+    u32x2 third;
+  };
+  static __device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
+    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  }
+  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) { return multiply(w.q, x.q, c); }
+  static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) x.q[i] &= (kept & (1u << 2 * i) ? 0xffffu : 0u) | (kept & (2u << 2 * i) ? 0xffff0000u : 0u);
+  }
+  static __device__ __forceinline__ uint32_t cut(float a, float b) { return (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u); }
+  static __device__ __forceinline__ float rest(float v, float part) { return __builtin_isfinite(v) ? v - part : 0.0f; }
+  // returns what the second product has to be multiplied by
+  template <int RT> static __device__ __forceinline__ float split(const f32x4 (&v)[RT], V (&to)[RT]) {
+    float lift = 1.0f, drop = 1.0f;
+    if constexpr (__is_same(T, _Float16)) { // hidden may leave the range of halves: the largest of the row becomes 2^14 .. 2^15
+      float most = 0.0f;
+#pragma unroll
+      for (int q = 0; q < RT; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = __builtin_isfinite(v[q][i]) ? fmaxf(most, fabsf(v[q][i])) : most;
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased; smaller rows than 2^-97 round to steps of 2^-135
+      lift = __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);
+      drop = __uint_as_float((uint32_t)(exponent - 14) << 23);
+    }
+#pragma unroll
+    for (int q = 0; q < RT; ++q)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const float a = v[q][2 * h] * lift, b = v[q][2 * h + 1] * lift;
+        if constexpr (__is_same(T, __bf16)) { // cut off, not rounded: the largest float stays finite
+          const uint32_t high = cut(a, b);
+          const float a1 = rest(a, __uint_as_float(high << 16)), b1 = rest(b, __uint_as_float(high & 0xffff0000u));
+          const uint32_t mid = cut(a1, b1);
+          to[q].upper[h] = high;
+          to[q].upper[2 + h] = mid;
+          to[q].third[h] = cut(a1 - __uint_as_float(mid << 16), b1 - __uint_as_float(mid & 0xffff0000u)); // eight bits are left
+        } else {
+          const uint32_t high = pack2(a, b, T{});
+          const f16x2 r = __builtin_bit_cast(f16x2, high);
+          to[q].upper[h] = high;
+          to[q].upper[2 + h] = pack2(rest(a, (float)r.x), rest(b, (float)r.y), T{});
+        }
+      }
+    return drop;
+  }
+  using R = u32x2;
+  static __device__ __forceinline__ R four(const T *p) { return *reinterpret_cast<const u32x2_from2 *>(p); }
+  static __device__ __forceinline__ void put(R &r, int i, T w) {
+    const uint32_t bits = (uint32_t)__builtin_bit_cast(uint16_t, w);
+    r[i >> 1] = i & 1 ? r[i >> 1] | bits << 16 : bits;
+  }
+  template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT][2], int j, const V (&v)[RT], f32x4 c) {
+#pragma unroll
+    for (int q = 0; q < RT; ++q) c = multiply(u32x4{w[q][j][0], w[q][j][1], w[q][j][0], w[q][j][1]}, v[q].upper, c);
+    if constexpr (__is_same(T, __bf16)) { // the third parts of two tiles of ranks at a time
+#pragma unroll
+      for (int q = 0; q < RT; q += 2) {
+        const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q][j] : R{};
+        const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
+        c = multiply(u32x4{w[q][j][0], w[q][j][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
+      }
+    }
+    return c;
+  }
+};
+
+// the first `count` of eight stored values, zeros behind them
+template <typename T> __device__ __forceinline__ Packed8<T> load8_first(const T *p, int count) {
+  if (count >= 8) return load8(p);
+  Packed8<T> r = {};
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+    if (i < count) {
+      if constexpr (__is_same(T, float)) r.q[i >> 2][i & 3] = __float_as_uint(p[i]);
+      else r.q[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << 16 * (i & 1);
+    }
+  return r;
+}
+template <typename T> __device__ __forceinline__ void clear_unless(Packed8<T> &r, bool kept) {
+  if constexpr (__is_same(T, float)) {
+    r.q[0] = kept ? r.q[0] : u32x4_from4{};
+    r.q[1] = kept ? r.q[1] : u32x4_from4{};
+  } else {
+    r.q = kept ? r.q : u32x4_from2{};
+  }
+}
+
+constexpr int WAVES = 8;
+
+// A product of 16 x 16 results takes, per lane, row lane % 16 of one operand and column lane % 16 of the other, and of the terms
+// those of lane / 16.  Terms may come in any order that both operands share: a lane reads eight neighbouring ones at once.  The
+// result has, per lane, column lane % 16 and rows 4 (lane / 16) + 0 .. 3.  With the weights as rows that is: lane % 16 = the
+// row of x, and four neighbouring ranks -- the very operand that the second product wants, and there four neighbouring columns
+// of y, eight with the weights' rows dealt accordingly.
+// The workgroup's waves share the terms of the first product, add their parts up in LDS, and share the columns of the second;
+// nothing but x, base, y and the weights (which come from L2) is moved.  FULL: the rank fills its tiles of 16.
+template <typename T, typename TW, int RT, int MT, bool FULL> __global__ __launch_bounds__(64 * WAVES) void k_adapter_rows(AdapterRowsArgs a) {
+  using P = Pipe<T, TW>;
+  constexpr int RP = 16 * RT, PITCH = RP + 4, TILES = MT * RT;
+  constexpr int DEEP = RT <= 2 ? 4 / MT : RT == 4 ? 2 / MT : 1; // steps of 32 terms whose loads are under way together
   __shared__ float red[WAVES][16 * MT][PITCH];
   __shared__ int rows_of[64];
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, lm = lane & 15, kg = lane >> 4;
@@ -210,102 +357,196 @@ template <typename T, typename TW, int RT, int MT, bool BACK> __global__ __launc
   const TW *w_in = static_cast<const TW *>(a.w_in) + (long)adapter * a.rank * a.in_size;
   const TW *w_out = static_cast<const TW *>(a.w_out) + (long)adapter * a.rank * a.out_size;
   const float scale = a.scale[adapter];
+  const bool drop_in = a.drop.on && !a.back, drop_out = a.drop.on && a.back;
   const uint32_t call = a.drop.on ? drop_call(a.drop) : 0;
+  const int full_steps = a.in_size / 32;
 
   for (int m0 = 0; m0 < count; m0 += 16 * MT) {
     long row[MT];
+    const T *x_at[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) row[mt] = rows_of[min(m0 + 16 * mt + lm, count - 1)]; // rows beyond the last repeat it and are not stored
+    for (int mt = 0; mt < MT; ++mt) { // rows beyond the last repeat it and are not stored
+      row[mt] = rows_of[min(m0 + 16 * mt + lm, count - 1)];
+      x_at[mt] = in + row[mt] * a.in.ld;
+    }
     f32x4 sum[MT][RT] = {};
-    for (int k0 = 32 * wave; k0 < a.in_size; k0 += 32 * WAVES) {
-      const int col = k0 + 8 * kg, left = a.in_size - col;
-      Values8 w[RT];
+    // `n` steps, WAVES apart; not whole: the one that the terms end in; masked: of an input that goes through dropout
+    const auto steps = [&](int step, auto n, auto whole, auto masked) {
+      constexpr int N = decltype(n)::value;
+      typename P::X x[N][MT];
+      typename P::W w[N][RT];
 #pragma unroll
-      for (int q = 0; q < RT; ++q) {
-        const int rank = 16 * q + lm;
-        if (BACK) {
+      for (int s = 0; s < N; ++s) {
+        const int col = (step + s * WAVES) * 32 + 8 * kg, left = decltype(whole)::value ? 8 : a.in_size - col;
 #pragma unroll
-          for (int j = 0; j < 8; ++j) w[q].v[j] = rank < a.rank && j < left ? to_float(w_in[(long)(col + j) * a.rank + rank]) : 0.0f;
-        } else {
-          w[q] = read8(w_in + (long)min(rank, a.rank - 1) * a.in_size + col, rank < a.rank ? left : 0);
+        for (int mt = 0; mt < MT; ++mt) x[s][mt] = decltype(whole)::value ? load8(x_at[mt] + col) : load8_first(x_at[mt] + col, left);
+#pragma unroll
+        for (int q = 0; q < RT; ++q) {
+          const int rank = 16 * q + lm;
+          const TW *at = w_in + (long)(FULL ? rank : min(rank, a.rank - 1)) * a.in_size + col;
+          w[s][q] = decltype(whole)::value ? load8(at) : load8_first(at, left);
+          if (!FULL) clear_unless(w[s][q], rank < a.rank);
         }
       }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        Values8 x = read8(in + row[mt] * a.in.ld + col, left);
-        if (!BACK && a.drop.on) drop_apply(a.drop, drop_kept(a.drop, call, (uint32_t)row[mt], (uint32_t)col / 8u), x);
+      for (int s = 0; s < N; ++s) {
+        const uint32_t block = (uint32_t)(step + s * WAVES) * 4u + (uint32_t)kg;
 #pragma unroll
-        for (int q = 0; q < RT; ++q)
+        for (int mt = 0; mt < MT; ++mt) {
+          if (decltype(masked)::value) P::keep(x[s][mt], drop_kept(a.drop, call, (uint32_t)row[mt], block)); // scaled below
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[mt][q] = mfma(w[q].v[j], x.v[j], sum[mt][q]);
+          for (int q = 0; q < RT; ++q) sum[mt][q] = P::terms(w[s][q], x[s][mt], sum[mt][q]);
+        }
       }
+    };
+    int step = wave;
+    if (drop_in) { // drawing the masks takes longer than the loads
+      for (; step < full_steps; step += WAVES) steps(step, Int<1>{}, Int<1>{}, Int<1>{});
+      if (step == full_steps && step * 32 < a.in_size) steps(step, Int<1>{}, Int<0>{}, Int<1>{});
+    } else {
+      for (; step + (DEEP - 1) * WAVES < full_steps; step += DEEP * WAVES) steps(step, Int<DEEP>{}, Int<1>{}, Int<0>{});
+      if (DEEP > 1)
+        for (; step < full_steps; step += WAVES) steps(step, Int<1>{}, Int<1>{}, Int<0>{});
+      if (step == full_steps && step * 32 < a.in_size) steps(step, Int<1>{}, Int<0>{}, Int<0>{});
     }
-    // the waves' shares of the terms, added in their order by every wave
+
+    // the waves' parts, added in their order: tile t by wave t % WAVES
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
       for (int q = 0; q < RT; ++q) *reinterpret_cast<f32x4 *>(&red[wave][16 * mt + lm][16 * q + 4 * kg]) = sum[mt][q];
     __syncthreads();
+    for (int t = wave; t < TILES; t += WAVES) {
+      const int mt = t / RT, q = t % RT, m = m0 + 16 * mt + lm;
+      float *at = &red[0][16 * mt + lm][16 * q + 4 * kg];
+      f32x4 v = *reinterpret_cast<const f32x4 *>(at);
+#pragma unroll
+      for (int w = 1; w < WAVES; ++w) v += *reinterpret_cast<const f32x4 *>(at + w * 16 * MT * PITCH);
+      if (drop_in) v *= a.drop.scale;
+      const f32x4 scaled = v * scale;
+      if (a.hidden && !blockIdx.y && m < count) {
+        float *to = a.hidden + (long)rows_of[m] * a.rank + 16 * q + 4 * kg;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (FULL || 16 * q + 4 * kg + i < a.rank) to[i] = a.back ? scaled[i] : v[i];
+      }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) // padding is zero also where a row holds an infinity, whose product with it is none
+        at[i] = FULL || 16 * q + 4 * kg + i < a.rank ? scaled[i] : 0.0f;
+    }
+    __syncthreads();
+    typename P::V hidden[MT][RT];
+    float lift[MT];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-      const int m = m0 + 16 * mt + lm;
 #pragma unroll
-      for (int q = 0; q < RT; ++q) {
-        f32x4 v = *reinterpret_cast<const f32x4 *>(&red[0][16 * mt + lm][16 * q + 4 * kg]);
-#pragma unroll
-        for (int w = 1; w < WAVES; ++w) v += *reinterpret_cast<const f32x4 *>(&red[w][16 * mt + lm][16 * q + 4 * kg]);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int rank = 16 * q + 4 * kg + i;
-          const float scaled = v[i] * scale;
-          if (a.hidden && !blockIdx.y && mt % WAVES == wave && m < count && rank < a.rank) a.hidden[row[mt] * a.rank + rank] = BACK ? scaled : v[i];
-          sum[mt][q][i] = rank < a.rank ? scaled : 0.0f; // also where a row holds an infinity, whose product with the padding is none
-        }
-      }
+      for (int q = 0; q < RT; ++q) sum[mt][q] = *reinterpret_cast<const f32x4 *>(&red[0][16 * mt + lm][16 * q + 4 * kg]);
+      lift[mt] = P::split(sum[mt], hidden[mt]) * (drop_out ? a.drop.scale : 1.0f);
     }
-    for (int unit = unit0 + wave; unit < unit1; unit += WAVES) {
-      f32x4 acc[MT][2] = {};
-      const int col = unit * 32 + 8 * kg, left = a.out_size - col; // of the lane's results
+
+    const auto columns = [&](int unit0, auto n, auto whole, auto masked) { // `n` units, WAVES apart
+      constexpr int N = decltype(n)::value;
+      Packed8<T> add[N][MT];
+      typename P::R w[N][RT][2];
 #pragma unroll
-      for (int q = 0; q < RT; ++q)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          // row lm of the operand is the column whose result ends up beside its neighbours
-          const int c = min(unit * 32 + (lm >> 2) * 8 + j * 4 + (lm & 3), a.out_size - 1);
-          f32x4 w;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int rank = 16 * q + 4 * kg + i;
-            const long at = BACK ? (long)min(rank, a.rank - 1) * a.out_size + c : (long)c * a.rank + min(rank, a.rank - 1);
-            w[i] = rank < a.rank ? to_float(w_out[at]) : 0.0f;
-          }
+      for (int u = 0; u < N; ++u) {
+        const int unit = unit0 + u * WAVES, col = unit * 32 + 8 * kg;
+        if (base) {
 #pragma unroll
           for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[mt][j] = mfma(w[i], sum[mt][q][i], acc[mt][j]);
+            add[u][mt] = decltype(whole)::value ? load8(base + row[mt] * a.base.ld + col) : load8_first(base + row[mt] * a.base.ld + col, a.out_size - col);
         }
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        if (m0 + 16 * mt + lm >= count) continue;
-        Values8 v;
+        for (int q = 0; q < RT; ++q)
 #pragma unroll
-        for (int h = 0; h < 8; ++h) v.v[h] = acc[mt][h >> 2][h & 3];
-        if (BACK && a.drop.on) drop_apply(a.drop, drop_kept(a.drop, call, (uint32_t)row[mt], (uint32_t)col / 8u), v);
-        if (base) {
-          const Values8 add = read8(base + row[mt] * a.base.ld + col, left);
+          for (int j = 0; j < 2; ++j) {
+            int c = unit * 32 + (lm >> 2) * 8 + j * 4 + (lm & 3); // the column whose result ends up beside its neighbours
+            if (!decltype(whole)::value) c = min(c, a.out_size - 1);
+            const int rank = 16 * q + 4 * kg;
+            if (FULL) {
+              w[u][q][j] = P::four(w_out + (long)c * a.rank + rank);
+            } else {
 #pragma unroll
-          for (int h = 0; h < 8; ++h) v.v[h] += add.v[h];
-        }
-        write8(out + row[mt] * a.out.ld + col, v, left);
+              for (int i = 0; i < 4; ++i) P::put(w[u][q][j], i, rank + i < a.rank ? w_out[(long)c * a.rank + min(rank + i, a.rank - 1)] : (TW)0.0f);
+            }
+          }
       }
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        const int unit = unit0 + u * WAVES, col = unit * 32 + 8 * kg, left = decltype(whole)::value ? 8 : a.out_size - col;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+          f32x4 acc[2] = {};
+#pragma unroll
+          for (int j = 0; j < 2; ++j) acc[j] = P::ranks(w[u], j, hidden[mt], acc[j]);
+          if (m0 + 16 * mt + lm >= count) continue;
+          Values8 v;
+#pragma unroll
+          for (int h = 0; h < 8; ++h) v.v[h] = acc[h >> 2][h & 3] * lift[mt];
+          if (decltype(masked)::value) {
+            const uint32_t kept = drop_kept(a.drop, call, (uint32_t)row[mt], (uint32_t)unit * 4u + (uint32_t)kg);
+#pragma unroll
+            for (int h = 0; h < 8; ++h) v.v[h] = kept & (1u << h) ? v.v[h] : 0.0f;
+          }
+          if (base) {
+            const Values8 b = widen(add[u][mt]);
+#pragma unroll
+            for (int h = 0; h < 8; ++h) v.v[h] += b.v[h];
+          }
+          if (decltype(whole)::value) store8(out + row[mt] * a.out.ld + col, v);
+          else write8(out + row[mt] * a.out.ld + col, v, left);
+        }
+      }
+    };
+    constexpr int WIDE = RT * MT == 1 ? 4 : RT * MT == 2 ? 2 : 1; // units whose loads are under way together
+    const int whole_units = min(unit1, a.out_size / 32);
+    int unit = unit0 + wave;
+    if (drop_out) {
+      for (; unit < whole_units; unit += WAVES) columns(unit, Int<1>{}, Int<1>{}, Int<1>{});
+      if (unit < unit1) columns(unit, Int<1>{}, Int<0>{}, Int<1>{});
+    } else {
+      for (; unit + (WIDE - 1) * WAVES < whole_units; unit += WIDE * WAVES) columns(unit, Int<WIDE>{}, Int<1>{}, Int<0>{});
+      if (WIDE > 1)
+        for (; unit < whole_units; unit += WAVES) columns(unit, Int<1>{}, Int<1>{}, Int<0>{});
+      if (unit < unit1) columns(unit, Int<1>{}, Int<0>{}, Int<0>{});
     }
     __syncthreads();
   }
 }
 
+// The matrices of the adapters that have rows with ranks and columns exchanged: with them the backward pass of rows is the
+// forward pass.
+template <typename TW> __global__ __launch_bounds__(256) void k_adapter_turn(AdapterTurnArgs a) {
+  __shared__ TW tile[64][65];
+  const int *seg = a.plan + a.p.seg;
+  const int t = (int)threadIdx.x, fast = t & 63, slow = t >> 6;
+  const int a_tiles = (a.in_size + 63) / 64, b_tiles = (a.out_size + 63) / 64, rank_tiles = (a.rank + 63) / 64;
+  for (int adapter = (int)blockIdx.y; adapter < a.n; adapter += (int)gridDim.y) {
+    if (seg[adapter + 1] == seg[adapter]) continue;
+    for (int k = (int)blockIdx.x; k < (a_tiles + b_tiles) * rank_tiles; k += (int)gridDim.x) {
+      const int c = k / rank_tiles, r0 = k % rank_tiles * 64;
+      const bool of_a = c < a_tiles;
+      // a: [rank][in] -> [in][rank], b: [out][rank] -> [rank][out]
+      const int rows = of_a ? a.rank : a.out_size, cols = of_a ? a.in_size : a.rank;
+      const int row0 = of_a ? r0 : (c - a_tiles) * 64, col0 = of_a ? c * 64 : r0;
+      const long at = (long)adapter * rows * cols;
+      const TW *from = static_cast<const TW *>(of_a ? a.a : a.b) + at;
+      TW *to = static_cast<TW *>(of_a ? a.a_turned : a.b_turned) + at;
+      __syncthreads();
+      for (int i = slow; i < 64 && row0 + i < rows; i += 4)
+        if (col0 + fast < cols) tile[i][fast] = from[(long)(row0 + i) * cols + col0 + fast];
+      __syncthreads();
+      for (int i = slow; i < 64 && col0 + i < cols; i += 4)
+        if (row0 + fast < rows) to[(long)(col0 + i) * rows + row0 + fast] = tile[fast][i];
+    }
+  }
+}
+
+constexpr int GRAD_WAVES = 4;
+
 // 128 columns of dA (of x, against up) or of dB (of d, against scale hidden).  A wave takes 16 rows of its chunk at a time; lane
 // % 16 reads eight neighbouring columns of four rows, and product j of a row takes column 8 (lane % 16) + j.
-template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * WAVES) void k_adapter_grads(AdapterGradArgs a) {
+template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * GRAD_WAVES) void k_adapter_grads(AdapterGradArgs a) {
   __shared__ float sums[32 * RT][64];
   const int4 chunk = reinterpret_cast<const int4 *>(a.plan + a.p.chunks)[blockIdx.x];
   const int adapter = chunk.x, count = chunk.z;
@@ -322,7 +563,7 @@ template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * WAV
   const uint32_t call = drop ? drop_call(a.drop) : 0;
   const int col = c0 + 8 * lm, left = width - col, rank0 = 16 * RT * (int)blockIdx.z;
   f32x4 acc[8][RT] = {};
-  for (int g = wave; g * 16 < count; g += WAVES) {
+  for (int g = wave; g * 16 < count; g += GRAD_WAVES) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int at = 16 * g + 4 * kg + i;
@@ -335,11 +576,11 @@ template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * WAV
         const int rank = rank0 + 16 * q + lm;
         const float u = valid && rank < a.rank ? factor[row * a.rank + rank] * scale : 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) acc[j][q] = mfma(x.v[j], u, acc[j][q]);
+        for (int j = 0; j < 8; ++j) acc[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[j], u, acc[j][q], 0, 0, 0);
       }
     }
   }
-  for (int from = 0; from < WAVES; ++from) { // the waves' sums, added in their order
+  for (int from = 0; from < GRAD_WAVES; ++from) { // the waves' sums, added in their order
     if (wave == from) {
 #pragma unroll
       for (int e = 0; e < 32 * RT; ++e) {
@@ -350,7 +591,7 @@ template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * WAV
     }
     __syncthreads();
   }
-  if (wave != WAVES - 1) return;
+  if (wave != GRAD_WAVES - 1) return;
   const bool whole = chunk.w < 0; // nothing to join
   float *part = a.part + (long)chunk.w * a.rank * ((long)a.in_size + a.out_size) + (of_a ? 0 : (long)a.rank * a.in_size);
 #pragma unroll
@@ -402,9 +643,6 @@ template <typename F> void with_types(int dtype, int w_dtype, F &&f) {
   else if (w_dtype == RPU_F16) f(float{}, _Float16{});
   else f(float{}, __bf16{});
 }
-template <int V> struct Int {
-  static constexpr int value = V;
-};
 template <typename F> void with_rank_tiles(int rank, F &&f) {
   if (rank <= 16) f(Int<1>{});
   else if (rank <= 32) f(Int<2>{});
@@ -412,8 +650,10 @@ template <typename F> void with_rank_tiles(int rank, F &&f) {
   else f(Int<8>{});
 }
 
-template <bool BACK> void launch_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) {
-  const int tile_rows = a.plan ? a.p.tile_rows : (a.rows + 15) / 16 * 16, tiles = a.plan ? a.p.max_tiles : a.rows;
+} // namespace
+
+void launch_adapter_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) {
+  const int tile_rows = a.plan ? a.p.tile_rows : a.rows, tiles = a.plan ? a.p.max_tiles : a.rows;
   // tiles that leave CUs idle share their output columns among several workgroups, each of which makes hidden for itself
   const int units = (a.out_size + 31) / 32;
   const int slices = std::max(1, std::min(units / WAVES, cus / std::max(tiles, 1)));
@@ -422,22 +662,31 @@ template <bool BACK> void launch_rows(const AdapterRowsArgs &a, int dtype, int w
     using T = decltype(x);
     using TW = decltype(w);
     with_rank_tiles(a.rank, [&](auto rt) {
-      constexpr int RT = decltype(rt)::value;
-      constexpr int MOST = RT <= 2 ? 4 : 2; // groups of 16 rows at a time: what the registers and LDS hold
-      if (tile_rows <= 16) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 1, BACK>), grid, dim3(64 * WAVES), 0, s, a);
-      else if (tile_rows <= 32) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 2, BACK>), grid, dim3(64 * WAVES), 0, s, a);
-      else hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, MOST, BACK>), grid, dim3(64 * WAVES), 0, s, a);
+      constexpr int RT = decltype(rt)::value, MOST = RT <= 4 ? 2 : 1; // groups of 16 rows at a time: what registers and LDS hold
+      const bool full = a.rank == 16 * RT;
+      if (tile_rows <= 16 || MOST == 1) {
+        if (full) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 1, true>), grid, dim3(64 * WAVES), 0, s, a);
+        else hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 1, false>), grid, dim3(64 * WAVES), 0, s, a);
+      } else {
+        if (full) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, MOST, true>), grid, dim3(64 * WAVES), 0, s, a);
+        else hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, MOST, false>), grid, dim3(64 * WAVES), 0, s, a);
+      }
     });
   });
 }
 
-} // namespace
+void launch_adapter_turn(const AdapterTurnArgs &a, int w_dtype, int cus, hipStream_t s) {
+  const int tiles = ((a.in_size + 63) / 64 + (a.out_size + 63) / 64) * ((a.rank + 63) / 64);
+  const dim3 grid((unsigned)std::min(tiles, std::max(1, cus * 8 / std::min(a.n, cus * 8))), (unsigned)std::min(a.n, cus * 8));
+  if (w_dtype == RPU_F32) hipLaunchKernelGGL(k_adapter_turn<float>, grid, dim3(256), 0, s, a);
+  else hipLaunchKernelGGL(k_adapter_turn<uint16_t>, grid, dim3(256), 0, s, a);
+}
 
 AdapterPlan adapter_plan(int rows, int n) {
   AdapterPlan p{};
   p.rows = rows;
   p.n = n;
-  p.tile_rows = rows <= 2048 ? 16 : rows <= 16384 ? 32 : 64;
+  p.tile_rows = rows <= 16384 ? 16 : 32;
   p.chunk_rows = 64;
   while (p.chunk_rows < 1024 && rows / p.chunk_rows > 32) p.chunk_rows *= 2;
   // every group of rows but for one may end with a piece that is not full
@@ -466,9 +715,6 @@ void launch_adapter_plan(const int *index, int *plan, const AdapterPlan &p, hipS
   hipLaunchKernelGGL(k_adapter_plan, dim3(1), dim3(PLAN_THREADS), 0, s, index, plan, p);
 }
 
-void launch_adapter_forward(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) { launch_rows<false>(a, dtype, w_dtype, cus, s); }
-void launch_adapter_backward_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) { launch_rows<true>(a, dtype, w_dtype, cus, s); }
-
 void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) {
   const unsigned slices = (unsigned)(((long)a.in_size + 127) / 128 + ((long)a.out_size + 127) / 128);
   const long values = (long)a.rank * ((long)a.in_size + a.out_size);
@@ -479,7 +725,7 @@ void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int 
     if (a.rows)
       with_rank_tiles(a.rank, [&](auto rt) {
         constexpr int RT = decltype(rt)::value, AT_ONCE = RT < 4 ? RT : 4; // more sums than that of 64 ranks leave the registers
-        hipLaunchKernelGGL((k_adapter_grads<T, TW, AT_ONCE>), dim3((unsigned)a.p.max_chunks, slices, RT / AT_ONCE), dim3(64 * WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_adapter_grads<T, TW, AT_ONCE>), dim3((unsigned)a.p.max_chunks, slices, RT / AT_ONCE), dim3(64 * GRAD_WAVES), 0, s, a);
       });
     hipLaunchKernelGGL(k_adapter_join<TW>, join, dim3(256), 0, s, a);
   });

@@ -116,11 +116,23 @@ void check_plan(const void *plan, size_t bytes, const AdapterPlan &p) {
   if (bytes < p.words * sizeof(int)) throw RpuError("The row plan is too small for this many rows and adapters.");
   if ((uintptr_t)plan % 16) throw RpuError("The row plan is not aligned to 16 bytes.");
 }
-size_t backward_scratch(const rpu_adapters *a, int rows) { // up [rows][rank], then the chunks' sums
-  const AdapterPlan p = adapter_plan(rows, a->n);
-  const size_t up = ((size_t)rows * a->rank + 3) / 4 * 4;
-  return sizeof(float) * (up + (size_t)p.max_slots * a->rank * ((size_t)a->in_size + a->out_size));
-}
+struct BackwardScratch { // offsets in bytes
+  size_t up, part, a_turned, b_turned, bytes;
+  BackwardScratch(const rpu_adapters *a, int rows) {
+    const AdapterPlan p = adapter_plan(rows, a->n);
+    const size_t e = value_size(a->w_dtype);
+    bytes = 0;
+    up = take(4 * (size_t)rows * a->rank);
+    part = take(4 * (size_t)p.max_slots * a->rank * ((size_t)a->in_size + a->out_size));
+    a_turned = take(rows ? e * a->n * a->rank * a->in_size : 0);
+    b_turned = take(rows ? e * a->n * a->rank * a->out_size : 0);
+  }
+  size_t take(size_t n) {
+    const size_t from = bytes;
+    bytes += (n + 15) / 16 * 16;
+    return from;
+  }
+};
 
 } // namespace
 } // namespace rpu_amd
@@ -291,7 +303,7 @@ int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_
     a.in_size = w.in_size;
     a.out_size = w.out_size;
     a.drop = d;
-    launch_adapter_forward(a, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
+    launch_adapter_rows(a, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
     check_launch();
   });
 }
@@ -299,9 +311,9 @@ int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_
 size_t rpu_adapter_backward_scratch(const rpu_adapters *adapters, int rows) {
   if (!adapters || rows < 0 || rows > MOST_ROWS || adapters->n < 1 || adapters->n > RPU_ADAPTER_MAX || adapters->rank < 1 ||
       adapters->rank > RPU_ADAPTER_MAX_RANK || adapters->in_size < 1 || adapters->out_size < 1 || adapters->in_size > MOST_ADAPTER_COLS ||
-      adapters->out_size > MOST_ADAPTER_COLS)
+      adapters->out_size > MOST_ADAPTER_COLS || (adapters->w_dtype != RPU_F32 && adapters->w_dtype != RPU_F16 && adapters->w_dtype != RPU_BF16))
     return 0;
-  return backward_scratch(adapters, rows);
+  return BackwardScratch(adapters, rows).bytes;
 }
 
 int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d_ld, const void *x_dev, long x_ld,
@@ -314,7 +326,8 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
     const rpu_adapters &w = *adapters;
     const AdapterPlan p = adapter_plan(rows, w.n);
     check_plan(plan_dev, plan_bytes, p);
-    const size_t e = value_size(dtype), we = value_size(w.w_dtype), need = backward_scratch(adapters, rows);
+    const BackwardScratch s(adapters, rows);
+    const size_t e = value_size(dtype), we = value_size(w.w_dtype), need = s.bytes;
     if (scratch_bytes < need) throw RpuError("The scratch memory is too small.");
     if ((uintptr_t)scratch_dev % 4) throw RpuError("The scratch memory is not aligned to 4 bytes.");
     const size_t of_a = we * w.n * w.rank * (size_t)w.in_size, of_b = we * w.n * w.rank * (size_t)w.out_size;
@@ -324,13 +337,13 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
     const std::vector<Span> written{matrix("dx", dx_dev, dx_ld, rows, w.in_size, e), dense("da", da_dev, of_a), dense("db", db_dev, of_b),
                                     dense("the scratch memory", scratch_dev, need)};
     for (size_t k = 0; k < written.size(); ++k) {
-      for (const Span &s : read) apart(written[k], s);
+      for (const Span &r : read) apart(written[k], r);
       for (size_t i = 0; i < k; ++i) apart(written[k], written[i]);
       if (base_dev) apart(written[k], matrix("the base", base_dev, base_ld, rows, w.in_size, e), k == 0);
     }
     const DropDev drop_of_x = drop_dev(drop);
     const Gpu gpu(device_id);
-    float *up = (float *)scratch_dev, *part = up + ((size_t)rows * w.rank + 3) / 4 * 4;
+    float *up = (float *)((char *)scratch_dev + s.up), *part = (float *)((char *)scratch_dev + s.part);
     AdapterGradArgs g{};
     g.x = {const_cast<void *>(x_dev), x_ld};
     g.d = {const_cast<void *>(d_dev), d_ld};
@@ -349,12 +362,14 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
     g.out_size = w.out_size;
     g.drop = drop_of_x;
     if (rows) {
+      AdapterTurnArgs turn{w.a_dev, w.b_dev, (char *)scratch_dev + s.a_turned, (char *)scratch_dev + s.b_turned, g.plan, p, w.n, w.rank, w.in_size, w.out_size};
+      launch_adapter_turn(turn, w.w_dtype, gpu.cus(), (hipStream_t)stream);
       AdapterRowsArgs a{};
       a.in = g.d;
       a.base = {const_cast<void *>(base_dev), base_ld};
       a.out = {dx_dev, dx_ld};
-      a.w_in = w.b_dev;
-      a.w_out = w.a_dev;
+      a.w_in = turn.b_turned;
+      a.w_out = turn.a_turned;
       a.scale = w.scale_dev;
       a.hidden = up;
       a.plan = g.plan;
@@ -365,7 +380,8 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
       a.in_size = w.out_size;
       a.out_size = w.in_size;
       a.drop = drop_of_x;
-      launch_adapter_backward_rows(a, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
+      a.back = 1;
+      launch_adapter_rows(a, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
     }
     launch_adapter_grads(g, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
     check_launch();
