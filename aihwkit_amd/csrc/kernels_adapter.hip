@@ -27,17 +27,108 @@ __device__ __forceinline__ void wave_sync() {
   __builtin_amdgcn_wave_barrier();
 }
 // lanes whose digit is this lane's (lanes with `valid` only)
-__device__ __forceinline__ uint64_t same_digit(int digit, bool valid) {
+__device__ __forceinline__ uint64_t same_digit(int digit, bool valid, int bits) {
   uint64_t mask = __ballot(valid);
-#pragma unroll
-  for (int b = 0; b < 8; ++b) {
+  for (int b = 0; b < bits; ++b) {
     const bool bit = (digit >> b) & 1;
     const uint64_t with = __ballot(valid && bit);
     mask &= bit ? with : ~with;
   }
   return mask;
 }
+// piece i of a list: key, first place, rows, slot
+__device__ __forceinline__ int4 plan_piece(int i, const int *firsts, const int *seg, const int *slots, int keys, int n, int piece) {
+  int lo = 0, hi = keys; // the last key that begins at or before piece i
+  while (lo < hi) {
+    const int mid = (lo + hi) / 2;
+    if (firsts[mid + 1] <= i) lo = mid + 1;
+    else hi = mid;
+  }
+  if (lo >= keys) return {-1, 0, 0, 0};
+  const int at = seg[lo] + (i - firsts[lo]) * piece;
+  return {lo < n ? lo : -1, at, min(piece, seg[lo + 1] - at), slots && slots[lo + 1] > slots[lo] ? slots[lo] + i - firsts[lo] : -1};
+}
 
+// Few adapters (a byte holds a key) and rows that LDS holds the keys of: one trip to memory for the index, everything else in
+// LDS.
+constexpr int PLAN_LDS_ROWS = 65536, PLAN_LDS_KEYS = 256;
+__global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan_lds(const int *index, int *plan, AdapterPlan p) {
+  __shared__ uint8_t key_of[PLAN_LDS_ROWS];
+  __shared__ int hist[PLAN_WAVES][PLAN_LDS_KEYS], sums[4][4], firsts[4][PLAN_LDS_KEYS + 1]; // of rows, tiles, chunks, slots
+  const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = p.n + 1, bits = 32 - __clz(p.n);
+  const uint64_t below = (1ull << lane) - 1;
+  const int share = (p.rows + PLAN_THREADS - 1) / PLAN_THREADS * 64, begin = min(wave * share, p.rows), end = min(begin + share, p.rows);
+  for (int from = 0; from < p.rows; from += 8 * PLAN_THREADS) {
+    int v[8];
+#pragma unroll
+    for (int u = 0; u < 8; ++u) v[u] = from + u * PLAN_THREADS + tid < p.rows ? index[from + u * PLAN_THREADS + tid] : 0;
+#pragma unroll
+    for (int u = 0; u < 8; ++u)
+      if (from + u * PLAN_THREADS + tid < p.rows) key_of[from + u * PLAN_THREADS + tid] = (uint8_t)adapter_key(v[u], p.n);
+  }
+  for (int i = tid; i < PLAN_WAVES * PLAN_LDS_KEYS; i += PLAN_THREADS) (&hist[0][0])[i] = 0;
+  __syncthreads();
+  for (int from = begin; from < end; from += 64) {
+    const bool valid = from + lane < end;
+    const int key = valid ? key_of[from + lane] : 0;
+    const uint64_t same = same_digit(key, valid, bits);
+    if (valid && !(same & below)) hist[wave][key] += __popcll(same);
+    wave_sync();
+  }
+  __syncthreads();
+  int count[4] = {};
+  if (tid < PLAN_LDS_KEYS) { // a key's rows: those of wave 0 first
+    for (int w = 0; w < PLAN_WAVES; ++w) {
+      const int c = hist[w][tid];
+      hist[w][tid] = count[0];
+      count[0] += c;
+    }
+    count[1] = (count[0] + p.tile_rows - 1) / p.tile_rows;
+    count[2] = tid < p.n ? (count[0] + p.chunk_rows - 1) / p.chunk_rows : 0;
+    count[3] = count[2] > 1 ? count[2] : 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      int upto = count[c];
+      for (int m = 1; m < 64; m <<= 1) {
+        const int v = __shfl_up(upto, m);
+        if (lane >= m) upto += v;
+      }
+      if (lane == 63) sums[wave][c] = upto;
+      count[c] = upto - count[c];
+    }
+  }
+  __syncthreads();
+  if (tid < PLAN_LDS_KEYS) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      for (int w = 0; w < wave; ++w) count[c] += sums[w][c];
+      firsts[c][tid] = count[c];
+      if (tid == PLAN_LDS_KEYS - 1) firsts[c][PLAN_LDS_KEYS] = sums[0][c] + sums[1][c] + sums[2][c] + sums[3][c];
+    }
+  }
+  __syncthreads();
+  int *order = plan + p.order;
+  for (int from = begin; from < end; from += 64) {
+    const bool valid = from + lane < end;
+    const int key = valid ? key_of[from + lane] : 0;
+    const uint64_t same = same_digit(key, valid, bits);
+    if (valid) order[firsts[0][key] + hist[wave][key] + __popcll(same & below)] = from + lane;
+    wave_sync();
+    if (valid && !(same & below)) hist[wave][key] += __popcll(same);
+    wave_sync();
+  }
+  for (int i = tid; i < p.max_tiles; i += PLAN_THREADS)
+    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, firsts[1], firsts[0], nullptr, keys, p.n, p.tile_rows);
+  for (int i = tid; i < p.max_chunks; i += PLAN_THREADS)
+    reinterpret_cast<int4 *>(plan + p.chunks)[i] = plan_piece(i, firsts[2], firsts[0], firsts[3], p.n, p.n, p.chunk_rows);
+  for (int i = tid; i <= keys; i += PLAN_THREADS) plan[p.seg + i] = i < PLAN_LDS_KEYS + 1 ? firsts[0][i] : p.rows;
+  for (int i = tid; i <= p.n; i += PLAN_THREADS) {
+    plan[p.first + i] = firsts[2][i];
+    plan[p.slot_first + i] = firsts[3][i];
+  }
+}
+
+// Any number of rows and adapters: the lists go through memory, keys of more than a byte in two rounds of the sort.
 __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index, int *plan, AdapterPlan p) {
   __shared__ int hist[PLAN_WAVES][256], start[256], sums[PLAN_WAVES][3];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, keys = p.n + 1;
@@ -49,16 +140,28 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
   const int passes = keys <= 256 ? 1 : 2; // eight bits each
   for (int pass = 0; pass < passes; ++pass) {
     int *to = pass == passes - 1 ? order : other;
+    const auto walk = [&](auto &&f) { // over the wave's rows, 64 at a time; the loads of eight times that are under way together
+      for (int from = begin; from < end; from += 8 * 64) {
+        int row[8], key[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) row[u] = pass && from + 64 * u + lane < end ? other[from + 64 * u + lane] : from + 64 * u + lane;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) key[u] = from + 64 * u + lane < end ? adapter_key(index[row[u]], p.n) : 0;
+#pragma unroll
+        for (int u = 0; u < 8; ++u) {
+          const bool valid = from + 64 * u + lane < end;
+          if (from + 64 * u >= end) break; // all lanes
+          const int digit = (key[u] >> (8 * pass)) & 255;
+          f(row[u], digit, same_digit(digit, valid, 8), valid);
+        }
+      }
+    };
     for (int i = tid; i < PLAN_WAVES * 256; i += PLAN_THREADS) hist[i >> 8][i & 255] = 0;
     __syncthreads();
-    for (int from = begin; from < end; from += 64) {
-      const bool valid = from + lane < end;
-      const int row = valid ? (pass ? other[from + lane] : from + lane) : 0;
-      const int digit = (adapter_key(index[row], p.n) >> (8 * pass)) & 255;
-      const uint64_t same = same_digit(digit, valid);
+    walk([&](int, int digit, uint64_t same, bool valid) {
       if (valid && !(same & below)) hist[wave][digit] += __popcll(same);
       wave_sync();
-    }
+    });
     __syncthreads();
     if (tid < 256) { // a digit's rows: those of wave 0 first
       int sum = 0;
@@ -84,16 +187,12 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
       for (int i = 0; i < 4; ++i) start[4 * lane + i] = upto - sum + own[i];
     }
     __syncthreads();
-    for (int from = begin; from < end; from += 64) {
-      const bool valid = from + lane < end;
-      const int row = valid ? (pass ? other[from + lane] : from + lane) : 0;
-      const int digit = (adapter_key(index[row], p.n) >> (8 * pass)) & 255;
-      const uint64_t same = same_digit(digit, valid);
+    walk([&](int row, int digit, uint64_t same, bool valid) {
       if (valid) to[start[digit] + hist[wave][digit] + __popcll(same & below)] = row;
       wave_sync();
       if (valid && !(same & below)) hist[wave][digit] += __popcll(same);
       wave_sync();
-    }
+    });
     __syncthreads();
   }
   // where every key begins: a key without rows where the next one does
@@ -141,25 +240,10 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
     slot_first[p.n] = count[2];
   }
   __syncthreads();
-  const auto cut = [&](int *list, int most, const int *firsts, int n_keys, int piece, const int *slots) {
-    for (int i = tid; i < most; i += PLAN_THREADS) {
-      int lo = 0, hi = n_keys; // the last key that begins at or before piece i
-      while (lo < hi) {
-        const int mid = (lo + hi) / 2;
-        if (firsts[mid + 1] <= i) lo = mid + 1;
-        else hi = mid;
-      }
-      int4 entry = {-1, 0, 0, 0};
-      if (lo < n_keys) {
-        const int at = seg[lo] + (i - firsts[lo]) * piece;
-        const int slot = slots && slots[lo + 1] > slots[lo] ? slots[lo] + i - firsts[lo] : -1;
-        entry = {lo < p.n ? lo : -1, at, min(piece, seg[lo + 1] - at), slot};
-      }
-      reinterpret_cast<int4 *>(list)[i] = entry;
-    }
-  };
-  cut(plan + p.tiles, p.max_tiles, tile_first, keys, p.tile_rows, nullptr);
-  cut(plan + p.chunks, p.max_chunks, first, p.n, p.chunk_rows, slot_first);
+  for (int i = tid; i < p.max_tiles; i += PLAN_THREADS)
+    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, tile_first, seg, nullptr, keys, p.n, p.tile_rows);
+  for (int i = tid; i < p.max_chunks; i += PLAN_THREADS)
+    reinterpret_cast<int4 *>(plan + p.chunks)[i] = plan_piece(i, first, seg, slot_first, p.n, p.n, p.chunk_rows);
 }
 
 // ---- eight terms, or four ranks, of both operands of a product, as the matrix instructions take them ------------------
@@ -533,11 +617,20 @@ template <typename TW> __global__ __launch_bounds__(256) void k_adapter_turn(Ada
       const TW *from = static_cast<const TW *>(of_a ? a.a : a.b) + at;
       TW *to = static_cast<TW *>(of_a ? a.a_turned : a.b_turned) + at;
       __syncthreads();
-      for (int i = slow; i < 64 && row0 + i < rows; i += 4)
-        if (col0 + fast < cols) tile[i][fast] = from[(long)(row0 + i) * cols + col0 + fast];
+      TW v[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int r = row0 + slow + 4 * i;
+        v[i] = from[(long)min(r, rows - 1) * cols + min(col0 + fast, cols - 1)];
+      }
+#pragma unroll
+      for (int i = 0; i < 16; ++i) tile[slow + 4 * i][fast] = v[i];
       __syncthreads();
-      for (int i = slow; i < 64 && col0 + i < cols; i += 4)
-        if (row0 + fast < rows) to[(long)(col0 + i) * rows + row0 + fast] = tile[fast][i];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        const int c = col0 + slow + 4 * i;
+        if (c < cols && row0 + fast < rows) to[(long)c * rows + row0 + fast] = tile[fast][slow + 4 * i];
+      }
     }
   }
 }
@@ -629,7 +722,15 @@ template <typename TW> __global__ __launch_bounds__(256) void k_adapter_join(Ada
     const int begin = slots[adapter], end = slots[adapter + 1];
     for (long e = (long)blockIdx.x * 256 + threadIdx.x; e < all; e += (long)gridDim.x * 256) {
       float sum = 0.0f;
-      for (int c = begin; c < end; ++c) sum += a.part[c * all + e];
+      int c = begin;
+      for (; c + 8 <= end; c += 8) {
+        float v[8];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) v[u] = a.part[(c + u) * all + e];
+#pragma unroll
+        for (int u = 0; u < 8; ++u) sum += v[u];
+      }
+      for (; c < end; ++c) sum += a.part[c * all + e];
       if (e < of_a) static_cast<TW *>(a.da)[adapter * of_a + e] = (TW)sum;
       else static_cast<TW *>(a.db)[adapter * (all - of_a) + e - of_a] = (TW)sum;
     }
@@ -712,7 +813,8 @@ AdapterPlan adapter_plan(int rows, int n) {
 }
 
 void launch_adapter_plan(const int *index, int *plan, const AdapterPlan &p, hipStream_t s) {
-  hipLaunchKernelGGL(k_adapter_plan, dim3(1), dim3(PLAN_THREADS), 0, s, index, plan, p);
+  if (p.rows <= PLAN_LDS_ROWS && p.n < PLAN_LDS_KEYS) hipLaunchKernelGGL(k_adapter_plan_lds, dim3(1), dim3(PLAN_THREADS), 0, s, index, plan, p);
+  else hipLaunchKernelGGL(k_adapter_plan, dim3(1), dim3(PLAN_THREADS), 0, s, index, plan, p);
 }
 
 void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) {

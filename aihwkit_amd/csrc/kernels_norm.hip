@@ -125,11 +125,12 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
   }
 }
 
+constexpr int backward_threads(int threads_of_a_row) { return threads_of_a_row == 64 ? 512 : threads_of_a_row; }
 // Backward pass of rows of up to 8 * TPR * V columns.  A workgroup adds d and d h of its rows up in registers and leaves the
 // sums in part[workgroup]; k_layer_norm_join adds those.
 template <typename T, typename TW, int TPR, int V>
-__global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_layer_norm_backward(NormBackwardArgs a) {
-  constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
+__global__ __launch_bounds__(backward_threads(TPR)) void k_layer_norm_backward(NormBackwardArgs a) {
+  constexpr int THREADS = backward_threads(TPR), ROWS = THREADS / TPR;
   __shared__ float room[THREADS / 64];
   __shared__ Values8 sums[ROWS > 1 ? 2 * TPR * V : 1];
   const int t = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
@@ -261,8 +262,17 @@ template <typename TW> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_laye
   const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6;
   const long col = (long)blockIdx.x * 64 + lane, width = 2l * a.cols;
   float sum = 0.0f;
-  if (col < width)
-    for (int p = wave; p < a.parts; p += JOIN_WAVES) sum += a.part[p * width + col];
+  if (col < width) {
+    int p = wave;
+    for (; p + 7 * JOIN_WAVES < a.parts; p += 8 * JOIN_WAVES) { // eight loads under way together
+      float v[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) v[u] = a.part[(p + u * JOIN_WAVES) * width + col];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) sum += v[u];
+    }
+    for (; p < a.parts; p += JOIN_WAVES) sum += a.part[p * width + col];
+  }
   sums[wave][lane] = sum;
   __syncthreads();
   if (wave || col >= width) return;
@@ -281,7 +291,7 @@ template <typename F> void with_types(int dtype, int w_dtype, F &&f) {
 
 // threads to a row of the backward pass, and their groups of eight columns each
 constexpr int BACKWARD_LONGEST = 1024 * 16;
-int backward_rows(int cols) { return cols <= 1024 ? 4 : 1; } // rows that a workgroup works on at a time
+int backward_rows(int cols) { return cols <= 1024 ? 8 : 1; } // rows that a workgroup works on at a time
 
 } // namespace
 
@@ -302,7 +312,7 @@ void launch_layer_norm(const NormArgs &a, int dtype, int w_dtype, int cus, hipSt
 
 int layer_norm_parts(int rows, int cols, int cus) {
   const long groups = ((long)rows + backward_rows(cols) - 1) / backward_rows(cols);
-  return (int)std::min((groups + 3) / 4, (long)cus * 2);
+  return (int)std::min((groups + 1) / 2, (long)cus);
 }
 
 void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtype, hipStream_t s) {
@@ -311,8 +321,8 @@ void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtyp
     using TW = decltype(w);
     const dim3 grid((unsigned)a.parts);
     if (a.parts) {
-      if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 1>), grid, dim3(256), 0, s, a);
-      else if (a.cols <= 1024) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 2>), grid, dim3(256), 0, s, a);
+      if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 1>), grid, dim3(512), 0, s, a);
+      else if (a.cols <= 1024) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 2>), grid, dim3(512), 0, s, a);
       else if (a.cols <= 2048) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 256, 1>), grid, dim3(256), 0, s, a);
       else if (a.cols <= 4096) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 256, 2>), grid, dim3(256), 0, s, a);
       else if (a.cols <= 8192) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 1024, 1>), grid, dim3(1024), 0, s, a);
