@@ -5,7 +5,8 @@
 //
 // Every function handles the plain case -- contiguous float32 tensors of the right sizes on the GPU -- and returns None
 // for everything else without having done anything: the caller (rpu_base/tiles.py) then takes its general path, which
-// converts what can be converted and words the errors.  A failing C entry point raises RuntimeError with its message, and
+// converts what can be converted and words the errors (for the digital operators, digital/: any of their types, and matrices
+// whose rows are apart).  A failing C entry point raises RuntimeError with its message, and
 // so does a C++ exception on the way to it.  Pointers and streams are taken before the GIL is released: nothing between
 // the two can throw.
 #include <torch/csrc/autograd/python_variable.h>
@@ -15,6 +16,7 @@
 #include <ATen/TensorSubclassLikeUtils.h>
 #include <c10/hip/HIPStream.h>
 
+#include <algorithm>
 #include <vector>
 
 #include "../../include/rpu_amd.h"
@@ -266,6 +268,344 @@ PyObject *group_update(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&] { return group_update_checked(a, n); });
 }
 
+// ---- digital operators beside the tiles ------------------------------------------------------------------------------
+
+int rpu_type(const at::Tensor &t) {
+  switch (t.scalar_type()) {
+  case at::kFloat: return RPU_F32;
+  case at::kHalf: return RPU_F16;
+  case at::kBFloat16: return RPU_BF16;
+  default: return -1;
+  }
+}
+
+// a tensor whose last dimension holds the columns and the others together the rows
+struct Rows {
+  const at::Tensor *t = nullptr;
+  int type = -1;
+  int64_t rows = 0, cols = 0;
+  long ld = 0;
+  bool take(PyObject *o) {
+    t = stored(o);
+    if (!t || !t->is_cuda() || t->dim() < 1 || (type = rpu_type(*t)) < 0) return false;
+    cols = t->size(-1);
+    if (cols < 1 || cols > 0x7fffffff) return false;
+    rows = t->numel() / cols;
+    if (rows > 0x7fffffff) return false;
+    ld = (long)cols;
+    if (t->dim() == 2 && t->size(0) > 1) {
+      ld = (long)t->stride(0);
+      return (cols == 1 || t->stride(1) == 1) && ld >= cols;
+    }
+    return t->is_contiguous();
+  }
+  bool like(const Rows &o) const { return type == o.type && t->device() == o.t->device(); }
+  const void *in() const { return t ? t->const_data_ptr() : nullptr; }
+  void *out() const { return t->data_ptr(); }
+};
+
+// an operand that may be None, beside `x` and of the given shape
+bool take_beside(PyObject *o, const Rows &x, at::IntArrayRef shape, Rows &r) {
+  if (o == Py_None) return true;
+  return r.take(o) && r.like(x) && r.t->sizes() == shape;
+}
+
+// the given output, or a new tensor; false: not the plain case
+bool take_out(PyObject *o, const Rows &x, at::IntArrayRef shape, at::Tensor &keep, Rows &r) {
+  if (o != Py_None) {
+    if (!take_beside(o, x, shape, r)) return false;
+    keep = *r.t;
+    return true;
+  }
+  keep = at::empty(shape, x.t->options().requires_grad(false));
+  r.t = &keep;
+  r.type = x.type;
+  r.cols = keep.size(-1);
+  r.rows = keep.numel() / std::max<int64_t>(r.cols, 1);
+  r.ld = (long)r.cols;
+  return true;
+}
+
+// a dense vector of `count` values (None: null); types: bit t allows rpu_dtype t
+bool take_vector(PyObject *o, const Rows &x, int64_t count, int types, const at::Tensor *&t) {
+  t = nullptr;
+  if (o == Py_None) return true;
+  t = stored(o);
+  if (!t || !t->is_cuda() || t->device() != x.t->device() || t->numel() != count || !t->is_contiguous()) return false;
+  const int type = rpu_type(*t);
+  return type >= 0 && ((types >> type) & 1);
+}
+
+// (p, seed, call) given as plain numbers
+bool take_drop(PyObject *p, PyObject *seed, PyObject *call, rpu_dropout_params &d) {
+  if (!PyFloat_CheckExact(p) || !PyLong_CheckExact(seed) || !PyLong_CheckExact(call)) return false;
+  d = {};
+  d.p = PyFloat_AS_DOUBLE(p);
+  const unsigned long long s = PyLong_AsUnsignedLongLong(seed), c = PyLong_AsUnsignedLongLong(call);
+  if (PyErr_Occurred()) {
+    PyErr_Clear();
+    return false;
+  }
+  if (c > 0xffffffffull || !(d.p >= 0.0 && d.p <= 1.0)) return false;
+  d.seed = s;
+  d.call = (uint32_t)c;
+  return true;
+}
+
+PyObject *tuple_of(at::Tensor a, at::Tensor b, at::Tensor c, int n) { // an undefined tensor becomes None
+  THPObjectPtr result(PyTuple_New(n));
+  if (!result) return nullptr;
+  at::Tensor *all[3] = {&a, &b, &c};
+  for (int i = 0; i < n; ++i) {
+    PyObject *item = THPVariable_Wrap(std::move(*all[i]));
+    if (!item) return nullptr;
+    PyTuple_SET_ITEM(result.get(), i, item);
+  }
+  return result.release();
+}
+
+// (x, p, seed, call, base, out, non_blocking) -> out, or None
+PyObject *dropout_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 7) return PyErr_Format(PyExc_TypeError, "7 arguments expected"), nullptr;
+  Rows x, base, out;
+  rpu_dropout_params d;
+  at::Tensor y;
+  if (!x.take(a[0]) || !take_drop(a[1], a[2], a[3], d) || !take_beside(a[4], x, x.t->sizes(), base) ||
+      !take_out(a[5], x, x.t->sizes(), y, out))
+    Py_RETURN_NONE;
+  const hipStream_t s = stream_of(*x.t);
+  void *yp = out.out(); // before the pointers of operands, which it may be one of
+  const void *xp = x.in(), *bp = base.in();
+  const int device = x.t->device().index();
+  const bool ok = call([&] { return rpu_dropout(xp, x.ld, bp, base.ld, yp, out.ld, x.type, (int)x.rows, (int)x.cols, &d, device, s); }, s, truth(a[6]));
+  return ok ? THPVariable_Wrap(std::move(y)) : nullptr;
+}
+PyObject *dropout(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return dropout_checked(a, n); });
+}
+
+at::Tensor per_row(const Rows &x, int64_t values) { // float, of the leading dimensions of x (values < 0: those alone)
+  c10::SmallVector<int64_t, 6> dims(x.t->sizes().begin(), x.t->sizes().end() - 1);
+  if (values >= 0) dims.push_back(values);
+  return at::empty(dims, x.t->options().dtype(at::kFloat).requires_grad(false));
+}
+
+// (x, weight, bias, eps, out, non_blocking) -> (y, mean, rstd), or None
+PyObject *layer_norm_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 6) return PyErr_Format(PyExc_TypeError, "6 arguments expected"), nullptr;
+  Rows x, out;
+  at::Tensor y;
+  const at::Tensor *w, *b;
+  if (!x.take(a[0]) || !PyFloat_CheckExact(a[3])) Py_RETURN_NONE;
+  const int types = 1 << RPU_F32 | 1 << x.type;
+  if (!take_vector(a[1], x, x.cols, types, w) || !take_vector(a[2], x, x.cols, types, b) || (w && b && w->scalar_type() != b->scalar_type()) ||
+      !take_out(a[4], x, x.t->sizes(), y, out))
+    Py_RETURN_NONE;
+  at::Tensor mean = per_row(x, -1), rstd = per_row(x, -1);
+  const hipStream_t s = stream_of(*x.t);
+  const float eps = (float)PyFloat_AS_DOUBLE(a[3]);
+  const int w_type = w ? rpu_type(*w) : b ? rpu_type(*b) : RPU_F32, device = x.t->device().index();
+  void *yp = out.out();
+  const void *xp = x.in(), *wp = w ? w->const_data_ptr() : nullptr, *bp = b ? b->const_data_ptr() : nullptr;
+  float *mp = out_data(mean), *rp = out_data(rstd);
+  const bool ok = call(
+      [&] { return rpu_layer_norm(xp, x.ld, wp, bp, w_type, yp, out.ld, mp, rp, x.type, (int)x.rows, (int)x.cols, eps, device, s); }, s, truth(a[5]));
+  return ok ? tuple_of(std::move(y), std::move(mean), std::move(rstd), 3) : nullptr;
+}
+PyObject *layer_norm(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return layer_norm_checked(a, n); });
+}
+
+at::Tensor scratch_of(const Rows &x, size_t bytes) { return at::empty({(int64_t)bytes}, x.t->options().dtype(at::kByte).requires_grad(false)); }
+
+// (d, x, mean, rstd, weight, base, out, non_blocking) -> (dx, dweight, dbias), or None
+PyObject *layer_norm_backward_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 8) return PyErr_Format(PyExc_TypeError, "8 arguments expected"), nullptr;
+  Rows d, x, base, out;
+  at::Tensor dx, dw, db, scratch;
+  const at::Tensor *mean, *rstd, *w;
+  if (!x.take(a[1]) || !d.take(a[0]) || !d.like(x) || d.t->sizes() != x.t->sizes()) Py_RETURN_NONE;
+  if (!take_vector(a[2], x, x.rows, 1 << RPU_F32, mean) || !take_vector(a[3], x, x.rows, 1 << RPU_F32, rstd) || !mean || !rstd ||
+      !take_vector(a[4], x, x.cols, 1 << RPU_F32 | 1 << x.type, w) || !take_beside(a[5], x, x.t->sizes(), base) ||
+      !take_out(a[6], x, x.t->sizes(), dx, out))
+    Py_RETURN_NONE;
+  size_t bytes = 0;
+  if (w) {
+    dw = at::empty(w->sizes(), w->options().requires_grad(false));
+    db = at::empty(w->sizes(), w->options().requires_grad(false));
+    bytes = rpu_layer_norm_backward_scratch((int)x.rows, (int)x.cols);
+    scratch = scratch_of(x, bytes);
+  }
+  const hipStream_t s = stream_of(*x.t);
+  const int device = x.t->device().index(), w_type = w ? rpu_type(*w) : RPU_F32;
+  void *dxp = out.out(), *dwp = w ? dw.data_ptr() : nullptr, *dbp = w ? db.data_ptr() : nullptr, *sp = w ? scratch.data_ptr() : nullptr;
+  const void *dp = d.in(), *xp = x.in(), *bp = base.in(), *wp = w ? w->const_data_ptr() : nullptr;
+  const float *mp = data(*mean), *rp = data(*rstd);
+  const bool ok = call(
+      [&] {
+        return rpu_layer_norm_backward(dp, d.ld, xp, x.ld, mp, rp, wp, w_type, bp, base.ld, dxp, out.ld, dwp, dbp, x.type, (int)x.rows, (int)x.cols, sp,
+                                       bytes, device, s);
+      },
+      s, truth(a[7]));
+  return ok ? tuple_of(std::move(dx), std::move(dw), std::move(db), 3) : nullptr;
+}
+PyObject *layer_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return layer_norm_backward_checked(a, n); });
+}
+
+const at::Tensor *index_of(PyObject *o) {
+  const at::Tensor *t = stored(o);
+  return t && t->is_cuda() && t->scalar_type() == at::kInt && t->is_contiguous() && t->numel() <= 0x7fffffff ? t : nullptr;
+}
+
+// The matrices of adapters and the rows that they are beside.
+struct AdapterCall {
+  rpu_adapters w{};
+  Rows x;
+  // a, b, scale, x: [n][rank][in], [n][out][rank], [n], rows of in values
+  bool take(PyObject *a, PyObject *b, PyObject *scale, PyObject *rows) {
+    const at::Tensor *at = stored(a), *bt = stored(b), *st = stored(scale);
+    if (!at || !bt || !st || !x.take(rows)) return false;
+    if (at->dim() != 3 || bt->dim() != 3 || st->dim() != 1 || !at->is_contiguous() || !bt->is_contiguous() || !st->is_contiguous()) return false;
+    const auto device = x.t->device();
+    if (at->device() != device || bt->device() != device || st->device() != device) return false;
+    const int type = rpu_type(*at);
+    if (type < 0 || rpu_type(*bt) != type || st->scalar_type() != at::kFloat) return false;
+    if (bt->size(0) != at->size(0) || st->size(0) != at->size(0) || bt->size(2) != at->size(1) || at->size(2) != x.cols) return false;
+    if (at->size(0) > 0x7fffffff || at->size(1) > 0x7fffffff || bt->size(1) > 0x7fffffff) return false;
+    w.a_dev = at->const_data_ptr();
+    w.b_dev = bt->const_data_ptr();
+    w.scale_dev = data(*st);
+    w.n = (int)at->size(0);
+    w.rank = (int)at->size(1);
+    w.in_size = (int)at->size(2);
+    w.out_size = (int)bt->size(1);
+    w.w_dtype = type;
+    return true;
+  }
+};
+
+// the plan of an index; undefined: not the plain case
+at::Tensor plan_for(const at::Tensor &index, int64_t n) {
+  const size_t bytes = n >= 1 && n <= RPU_ADAPTER_MAX ? rpu_adapter_plan_bytes((int)index.numel(), (int)n) : 0;
+  return bytes ? at::empty({(int64_t)bytes}, index.options().dtype(at::kByte).requires_grad(false)) : at::Tensor();
+}
+
+// (index, n adapters) -> the plan (bytes on the GPU), or None
+PyObject *adapter_plan_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 2) return PyErr_Format(PyExc_TypeError, "2 arguments expected"), nullptr;
+  const at::Tensor *index = index_of(a[0]);
+  if (!index) Py_RETURN_NONE;
+  const long adapters = integer(a[1]);
+  at::Tensor plan = plan_for(*index, adapters);
+  if (!plan.defined()) Py_RETURN_NONE;
+  const hipStream_t s = stream_of(*index);
+  const int32_t *ip = static_cast<const int32_t *>(index->const_data_ptr());
+  void *pp = plan.data_ptr();
+  const int rows = (int)index->numel(), device = index->device().index();
+  const size_t bytes = (size_t)plan.numel();
+  const bool ok = call([&] { return rpu_adapter_plan(ip, rows, (int)adapters, pp, bytes, device, s); }, s, true);
+  return ok ? THPVariable_Wrap(std::move(plan)) : nullptr;
+}
+PyObject *adapter_plan(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return adapter_plan_checked(a, n); });
+}
+
+// The rows of a call: a plan of as many rows and adapters (checked by the caller), or an index, which is grouped first unless its rows are
+// few.
+struct GroupedRows {
+  const at::Tensor *index = nullptr;
+  at::Tensor plan;
+  bool make = false;
+  bool take(PyObject *index_or_none, PyObject *plan_or_none, const AdapterCall &c, int64_t few) {
+    if (plan_or_none != Py_None) {
+      const at::Tensor *p = stored(plan_or_none);
+      if (!p || !p->is_cuda() || p->device() != c.x.t->device() || !p->is_contiguous()) return false;
+      plan = *p;
+      return true;
+    }
+    index = index_of(index_or_none);
+    if (!index || index->device() != c.x.t->device() || index->numel() != c.x.rows) return false;
+    if (index->numel() <= few) return true;
+    plan = plan_for(*index, c.w.n);
+    make = true;
+    return plan.defined();
+  }
+};
+
+// (a, b, scale, x, index, plan, base, out, return_hidden, p, seed, call, non_blocking) -> (y, hidden or None), or None
+PyObject *adapter_forward_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments expected"), nullptr;
+  AdapterCall c;
+  Rows base, out;
+  rpu_dropout_params d;
+  GroupedRows g;
+  at::Tensor y, hidden;
+  if (!c.take(a[0], a[1], a[2], a[3]) || !take_drop(a[9], a[10], a[11], d) || !g.take(a[4], a[5], c, RPU_ADAPTER_FEW_ROWS)) Py_RETURN_NONE;
+  c10::SmallVector<int64_t, 6> dims(c.x.t->sizes().begin(), c.x.t->sizes().end());
+  dims.back() = c.w.out_size;
+  if (!take_beside(a[6], c.x, dims, base) || !take_out(a[7], c.x, dims, y, out)) Py_RETURN_NONE;
+  if (truth(a[8])) hidden = per_row(c.x, c.w.rank);
+  const hipStream_t s = stream_of(*c.x.t);
+  const int rows = (int)c.x.rows, device = c.x.t->device().index();
+  const int32_t *ip = g.index ? static_cast<const int32_t *>(g.index->const_data_ptr()) : nullptr;
+  void *pp = g.plan.defined() ? g.plan.data_ptr() : nullptr, *yp = out.out();
+  const size_t bytes = g.plan.defined() ? (size_t)g.plan.nbytes() : 0;
+  const void *xp = c.x.in(), *bp = base.in();
+  float *hp = hidden.defined() ? out_data(hidden) : nullptr;
+  const bool ok = call(
+      [&] {
+        if (g.make)
+          if (const int rc = rpu_adapter_plan(ip, rows, c.w.n, pp, bytes, device, s)) return rc;
+        return rpu_adapter_forward(&c.w, xp, c.x.ld, ip, pp, bytes, &d, bp, base.ld, yp, out.ld, hp, c.x.type, rows, device, s);
+      },
+      s, truth(a[12]));
+  return ok ? tuple_of(std::move(y), std::move(hidden), {}, 2) : nullptr;
+}
+PyObject *adapter_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return adapter_forward_checked(a, n); });
+}
+
+// (a, b, scale, d, x, index, plan, hidden, base, out, p, seed, call, non_blocking) -> (dx, da, db), or None
+PyObject *adapter_backward_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 14) return PyErr_Format(PyExc_TypeError, "14 arguments expected"), nullptr;
+  AdapterCall c;
+  Rows dy, base, out;
+  rpu_dropout_params d;
+  GroupedRows g;
+  at::Tensor dx;
+  if (!c.take(a[0], a[1], a[2], a[4]) || !take_drop(a[10], a[11], a[12], d) || !g.take(a[5], a[6], c, -1)) Py_RETURN_NONE;
+  c10::SmallVector<int64_t, 6> dims(c.x.t->sizes().begin(), c.x.t->sizes().end());
+  dims.back() = c.w.out_size;
+  const at::Tensor *hidden;
+  if (!dy.take(a[3]) || !dy.like(c.x) || dy.t->sizes() != at::IntArrayRef(dims) || !take_vector(a[7], c.x, c.x.rows * c.w.rank, 1 << RPU_F32, hidden) || !hidden ||
+      !take_beside(a[8], c.x, c.x.t->sizes(), base) || !take_out(a[9], c.x, c.x.t->sizes(), dx, out))
+    Py_RETURN_NONE;
+  const at::Tensor &wa = *stored(a[0]), &wb = *stored(a[1]);
+  at::Tensor da = at::empty(wa.sizes(), wa.options().requires_grad(false)), db = at::empty(wb.sizes(), wb.options().requires_grad(false));
+  const size_t scratch_bytes = rpu_adapter_backward_scratch(&c.w, (int)c.x.rows);
+  at::Tensor scratch = scratch_of(c.x, scratch_bytes);
+  const hipStream_t s = stream_of(*c.x.t);
+  const int rows = (int)c.x.rows, device = c.x.t->device().index();
+  const int32_t *ip = g.index ? static_cast<const int32_t *>(g.index->const_data_ptr()) : nullptr;
+  void *pp = g.plan.data_ptr(), *dxp = out.out(), *dap = da.data_ptr(), *dbp = db.data_ptr(), *sp = scratch.data_ptr();
+  const size_t bytes = (size_t)g.plan.nbytes();
+  const void *dp = dy.in(), *xp = c.x.in(), *bp = base.in();
+  const float *hp = data(*hidden);
+  const bool ok = call(
+      [&] {
+        if (g.make)
+          if (const int rc = rpu_adapter_plan(ip, rows, c.w.n, pp, bytes, device, s)) return rc;
+        return rpu_adapter_backward(&c.w, dp, dy.ld, xp, c.x.ld, hp, pp, bytes, &d, bp, base.ld, dxp, out.ld, dap, dbp, c.x.type, rows, sp, scratch_bytes,
+                                    device, s);
+      },
+      s, truth(a[13]));
+  return ok ? tuple_of(std::move(dx), std::move(da), std::move(db), 3) : nullptr;
+}
+PyObject *adapter_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return adapter_backward_checked(a, n); });
+}
+
 PyMethodDef methods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(backward)), METH_FASTCALL, nullptr},
@@ -273,6 +613,12 @@ PyMethodDef methods[] = {
     {"group_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_forward)), METH_FASTCALL, nullptr},
     {"group_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_backward)), METH_FASTCALL, nullptr},
     {"group_update", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(group_update)), METH_FASTCALL, nullptr},
+    {"dropout", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(dropout)), METH_FASTCALL, nullptr},
+    {"layer_norm", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm)), METH_FASTCALL, nullptr},
+    {"layer_norm_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(layer_norm_backward)), METH_FASTCALL, nullptr},
+    {"adapter_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_plan)), METH_FASTCALL, nullptr},
+    {"adapter_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_forward)), METH_FASTCALL, nullptr},
+    {"adapter_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_backward)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "rpu_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -4,7 +4,7 @@ from typing import Optional, Tuple, Union
 
 import torch
 
-from .._cabi import Adapters, check, lib
+from .._cabi import Adapters, check, lib, torch_calls
 from ._operands import DTYPES, Matrix, check_rows, drop_params, launch, like
 
 FEW_ROWS = 64   # RPU_ADAPTER_FEW_ROWS: a forward call groups so many rows by itself
@@ -27,12 +27,16 @@ class AdapterRows:
     def __init__(self, index: torch.Tensor, n_adapters: int):
         index = _check_index(index)
         self.n_adapters, self.rows, self.device = int(n_adapters), index.numel(), index.device
+        self._plan = torch_calls().adapter_plan(index, self.n_adapters)
+        if self._plan is not None:
+            self._bytes = self._plan.numel()
+            return
         self._bytes = 0
         if 1 <= self.n_adapters <= 65535:
             self._bytes = lib().rpu_adapter_plan_bytes(self.rows, self.n_adapters)
         if not self._bytes:
             raise RuntimeError("The number of adapters must be in 1 .. 65535, that of rows at most 2^28.")
-        self._plan = torch.empty(self._bytes // 4, dtype=torch.int32, device=index.device)
+        self._plan = torch.empty(self._bytes, dtype=torch.uint8, device=index.device)
         stream = torch.cuda.current_stream(index.device)
         check(lib().rpu_adapter_plan(index.data_ptr(), self.rows, self.n_adapters, self._plan.data_ptr(), self._bytes,
                                      index.device.index, C.c_void_p(stream.cuda_stream)))
@@ -60,6 +64,7 @@ class LowRankAdapters:
         if self.out_size < 1:
             raise RuntimeError("The sizes of the adapters must be positive.")
         self.a, self.b = a, b
+        self._a_shape, self._b_shape = a.shape, torch.Size((self.n_adapters, self.out_size, self.rank))
         self.scale = torch.ones(self.n_adapters, dtype=torch.float32, device=a.device) if scale is None else scale
         self._operand(a)
 
@@ -104,6 +109,18 @@ class LowRankAdapters:
             plan = AdapterRows(index, self.n_adapters)
         return index, plan
 
+    def _native(self, rows, x_input):
+        """(index, plan) for the native calls, (None, None) for what the general path has to look at."""
+        a, b = self.a, self.b
+        if not isinstance(a, torch.Tensor) or not isinstance(b, torch.Tensor) or not isinstance(x_input, torch.Tensor) or \
+                a.shape != self._a_shape or b.shape != self._b_shape:
+            return None, None
+        if not isinstance(rows, AdapterRows):
+            return rows, None
+        if rows.n_adapters != self.n_adapters or rows.rows * self.in_size != x_input.numel():
+            return None, None
+        return None, rows._plan
+
     def forward(self, x_input: torch.Tensor, rows: Union[torch.Tensor, AdapterRows], base: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None, return_hidden: bool = False, p: float = 0.0, seed: int = 0,
                 call: Union[int, torch.Tensor] = 0, non_blocking: bool = False
@@ -113,6 +130,12 @@ class LowRankAdapters:
         ``rows``: the adapter of every row, an int32 CUDA tensor, or ``AdapterRows`` that several calls share.  ``base``: the
         projection's output, which ``out`` may be.  Rows without adapter get ``base`` (zeros without it).  ``p``, ``seed`` and
         ``call`` are those of ``dropout``, applied to ``x_input``."""
+        index, plan = self._native(rows, x_input)
+        if index is not None or plan is not None:
+            done = torch_calls().adapter_forward(self.a, self.b, self.scale, x_input, index, plan, base, out, return_hidden, p, seed,
+                                                 call, non_blocking)
+            if done is not None:
+                return done if return_hidden else done[0]
         x = self._rows(x_input, self.in_size, "x_input")
         adapters = self._operand(x_input)
         shape = (*x_input.shape[:-1], self.out_size)
@@ -137,6 +160,12 @@ class LowRankAdapters:
         """``(dx, da, db)`` from the gradient ``d_input`` of ``y`` and what the forward pass took and left (``rows``, ``p``,
         ``seed`` and ``call`` as there).  ``base``: added to ``dx``, the input gradient of the projection; ``out`` (dx) may be
         it.  ``da`` and ``db`` are like ``a`` and ``b``, zeros for adapters without rows."""
+        index, plan = self._native(rows, x_input)
+        if index is not None or plan is not None:
+            done = torch_calls().adapter_backward(self.a, self.b, self.scale, d_input, x_input, index, plan, hidden, base, out, p, seed,
+                                                  call, non_blocking)
+            if done is not None:
+                return done
         x = self._rows(x_input, self.in_size, "x_input")
         adapters = self._operand(x_input)
         d = like(d_input, x_input, (*x_input.shape[:-1], self.out_size), "d_input")

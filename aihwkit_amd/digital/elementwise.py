@@ -4,7 +4,7 @@ from typing import Optional, Union
 
 import torch
 
-from .._cabi import lib
+from .._cabi import lib, torch_calls
 from ._operands import DTYPES, Matrix, check_rows, drop_params, launch, like
 
 
@@ -17,6 +17,9 @@ def dropout(x_input: torch.Tensor, p: float, seed: int, call: Union[int, torch.T
     with one seed, or an int64 tensor of one value on the GPU, read when the kernel runs, so that a captured step draws new
     masks in every replay.  Dropped elements count as zero also where they are infinite or NaN.  ``out`` may be ``x_input``
     or ``base``."""
+    done = torch_calls().dropout(x_input, p, seed, call, base, out, non_blocking)
+    if done is not None:
+        return done
     x = Matrix(check_rows(x_input, "x_input"), "x_input")
     add = None if base is None else like(base, x_input, x_input.shape, "base")
     params = drop_params(p, seed, call, x_input.device)

@@ -3,7 +3,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from .._cabi import lib
+from .._cabi import lib, torch_calls
 from ._operands import DTYPES, Matrix, check_rows, launch, like, vector
 
 
@@ -13,6 +13,9 @@ def layer_norm(x_input: torch.Tensor, weight: Optional[torch.Tensor] = None, bia
     """``(y, mean, rstd)`` with ``y = (x - mean) rstd weight + bias`` and ``rstd = (mean((x - mean)^2) + eps)^-1/2`` of every
     row; ``mean`` and ``rstd`` are float32, one value a row, for the backward pass.  ``weight`` and ``bias`` are float32 or of
     the type of ``x_input``, both alike; ``out`` may be ``x_input``."""
+    done = torch_calls().layer_norm(x_input, weight, bias, eps, out, non_blocking)
+    if done is not None:
+        return done
     x = Matrix(check_rows(x_input, "x_input"), "x_input")
     types = (torch.float32, x_input.dtype)
     w = vector(weight, x_input, x.cols, types, "weight")
@@ -39,6 +42,9 @@ def layer_norm_backward(d_input: torch.Tensor, x_input: torch.Tensor, mean: torc
     ``base`` is added to ``dx``: the gradient that reaches ``x`` past the norm.  ``dweight`` and ``dbias`` have the type of
     ``weight`` and are None without it.  ``out`` (dx) may be ``d_input``, ``x_input`` or ``base``.  Sums over rows are added in
     an order that depends on the sizes alone."""
+    done = torch_calls().layer_norm_backward(d_input, x_input, mean, rstd, weight, base, out, non_blocking)
+    if done is not None:
+        return done
     x = Matrix(check_rows(x_input, "x_input"), "x_input")
     d = like(d_input, x_input, x_input.shape, "d_input")
     mean = vector(mean, x_input, x.rows, (torch.float32,), "mean")

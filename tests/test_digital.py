@@ -165,8 +165,8 @@ def test_scratch_sizes_do_not_grow_with_rows_without_end():
     assert lib.rpu_layer_norm_backward_scratch(0, 768) == 0
     assert lib.rpu_layer_norm_backward_scratch(1, 768) == 2 * 768 * 4
     assert lib.rpu_layer_norm_backward_scratch(1 << 24, 768) == lib.rpu_layer_norm_backward_scratch(1 << 20, 768) <= 16 << 20
-    # as many adapters as rows: nothing has to be joined
-    assert lib.rpu_adapter_backward_scratch(C.byref(adapters(n=8)), 8) == 8 * 8 * 4
+    # as many adapters as rows: nothing has to be joined; up [8][8] and the matrices turned, [8][8][64 + 48] floats
+    assert lib.rpu_adapter_backward_scratch(C.byref(adapters(n=8)), 8) == 4 * 8 * 8 * (1 + 64 + 48)
 
 
 def test_python_calls_refuse_host_tensors_and_wrong_types():
