@@ -32,6 +32,18 @@ struct DropoutArgs {
   int rows, cols;
   DropDev drop;
 };
+// types of rows and adapter weights, and a number, as arguments of a generic function
+template <typename F> void with_adapter_types(int dtype, int w_dtype, F &&f) {
+  if (dtype == RPU_BF16) f(__bf16{}, __bf16{});
+  else if (dtype == RPU_F16) f(_Float16{}, _Float16{});
+  else if (w_dtype == RPU_F32) f(float{}, float{});
+  else if (w_dtype == RPU_F16) f(float{}, _Float16{});
+  else f(float{}, __bf16{});
+}
+template <int V> struct Int {
+  static constexpr int value = V;
+};
+
 void launch_dropout(const DropoutArgs &a, int dtype, int cus, hipStream_t s);
 
 struct NormArgs {
@@ -57,15 +69,16 @@ void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtyp
 // Rows grouped by adapter: what launch_adapter_plan writes, one array of ints.
 //   order [rows]       rows by adapter, in their order within each; those without one last
 //   seg [n + 2]        seg[a]: where adapter a begins in `order`; seg[n]: the rows without one; seg[n + 1] = rows
-//   tiles [4 * tiles]  {adapter or -1, first place in `order`, rows (0: none), 0}: at most tile_rows rows each
+//   tiles [4 * tiles]  {adapter or -1, first place in `order`, rows (0: none), 0}: at most ADAPTER_TILE_ROWS rows each
 //   chunks [4 * chunks]  the same in longer pieces for the gradients, of adapters only; the last number is the slot for the
 //                      chunk's sums, -1 if it holds all rows of its adapter
 //   first [n + 1]      first[a]: the first chunk of adapter a
 //   tile_first [n + 2], slot_first [n + 1]  the same of the tiles and of the slots
 //   other [rows]       scratch
+constexpr int ADAPTER_TILE_ROWS = 64;
 struct AdapterPlan {
   int rows, n;
-  int tile_rows, chunk_rows;
+  int chunk_rows;
   int max_tiles, max_chunks, max_slots;
   size_t order, seg, tiles, chunks, first, tile_first, slot_first, other, words; // offsets in ints, total
 };
@@ -79,12 +92,13 @@ struct AdapterRowsArgs {
   MatrixDev in, base, out;     // forward: x, base, y; backward: d, base, dx
   const void *w_in, *w_out;    // [n][rank][in_size], [n][out_size][rank]: forward a, b; backward b, a with both exchanged
   const float *scale;
-  float *hidden;               // [rows][rank]: a drop(x), or scale b^T d; null: not wanted
+  float *hidden;               // [rows][rank]: a drop(x), or scale b^T d; without a plan it may be null
   const int *index;            // without a plan
   const int *plan;             // null: the rows are grouped from `index`
   AdapterPlan p;
   int rows, n, rank, in_size, out_size;
   int back;
+  int units_each;              // few rows: 32 columns of the output each, of a workgroup (set by the launch)
   DropDev drop;                // of the input (forward) or of the output (backward)
 };
 void launch_adapter_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
@@ -112,6 +126,8 @@ struct AdapterGradArgs {
 void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int cus, hipStream_t s);
 
 #if defined(__HIPCC__)
+__device__ __forceinline__ int adapter_key(int index, int n) { return index >= 0 && index < n ? index : n; }
+
 // ---- eight neighbouring values of a row -------------------------------------------------------------------------------
 // Rows begin at any element: loads and stores of 16 bytes from any address that a value may have.
 typedef uint32_t u32x4_from2 __attribute__((ext_vector_type(4), aligned(2)));
@@ -169,13 +185,113 @@ __device__ __forceinline__ Values8 widen(const Packed8<_Float16> &p) {
   }
   return r;
 }
-// the first `count` of eight values (all where count >= 8), zeros behind them
-template <typename T> __device__ __forceinline__ Values8 read8(const T *p, int count) {
-  if (count >= 8) return widen(load8(p));
-  Values8 r;
+// a 16-bit value below seven others
+__device__ __forceinline__ u32x4 shift_in(u32x4 q, uint16_t v) {
+  return u32x4{q[0] << 16 | v, q[1] << 16 | q[0] >> 16, q[2] << 16 | q[1] >> 16, q[3] << 16 | q[2] >> 16};
+}
+// Eight values of a row from column `col` on, in two steps.  ahead8 only loads: where the row ends it begins earlier.  trim8, at the first
+// use, moves the values down, with zeros behind the last column.  In one step, or with a branch around the load, every load would be
+// waited for before the next begins: rows of fewer than eight columns, which cannot begin earlier, have kernels of their own (SHORT).
+template <bool SHORT, typename T> __device__ __forceinline__ Packed8<T> ahead8(const T *row, long col, long cols) {
+  if (!SHORT) return load8(row + min(col, cols - 8));
+  if (cols >= 8) return load8(row + min(col, cols - 8)); // a matrix beside a short one
+  Packed8<T> p = {};
+#pragma unroll 1
+  for (long i = cols - 1; i >= col; --i) {
+    if constexpr (sizeof(T) == 4) {
+      p.q[1] = u32x4{p.q[0][3], p.q[1][0], p.q[1][1], p.q[1][2]};
+      p.q[0] = u32x4{__float_as_uint(row[i]), p.q[0][0], p.q[0][1], p.q[0][2]};
+    } else {
+      p.q = shift_in(p.q, __builtin_bit_cast(uint16_t, row[i]));
+    }
+  }
+  return p;
+}
+template <typename T> __device__ __forceinline__ void trim8(Packed8<T> &p, long col, long cols) {
+  if (cols < 8 || col + 8 <= cols) return;
+  constexpr int WORDS = sizeof(T) == 4 ? 8 : 4;
+  int by = (int)min(col + 8 - cols, 8l); // values
+  uint32_t d[WORDS];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) r.v[i] = i < count ? to_float(p[i]) : 0.0f;
-  return r;
+  for (int i = 0; i < WORDS; ++i) {
+    if constexpr (sizeof(T) == 4) d[i] = p.q[i >> 2][i & 3];
+    else d[i] = p.q[i];
+  }
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) d[i] = by & 1 ? (d[i] >> 16 | (i + 1 < WORDS ? d[i + 1] << 16 : 0u)) : d[i];
+    by >>= 1;
+  }
+#pragma unroll
+  for (int step = 1; step <= WORDS; step *= 2)
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) d[i] = by & step ? (i + step < WORDS ? d[i + step] : 0u) : d[i];
+#pragma unroll
+  for (int i = 0; i < WORDS; ++i) {
+    if constexpr (sizeof(T) == 4) p.q[i >> 2][i & 3] = d[i];
+    else p.q[i] = d[i];
+  }
+}
+template <bool SHORT, typename T> __device__ __forceinline__ Values8 read8(const T *row, long col, long cols) {
+  Packed8<T> p = ahead8<SHORT>(row, col, cols);
+  trim8(p, col, cols);
+  return widen(p);
+}
+
+// ---- 16 bytes of neighbouring values of a row ---------------------------------------------------------------------------
+template <typename T> constexpr int CHUNK = 16 / (int)sizeof(T); // values
+template <typename T> struct Packed16 {
+  u32x4 q;
+};
+template <typename T> __device__ __forceinline__ Packed16<T> load16(const T *p) {
+  if constexpr (sizeof(T) == 4) return {*reinterpret_cast<const u32x4_from4 *>(p)};
+  else return {*reinterpret_cast<const u32x4_from2 *>(p)};
+}
+// the same two steps as for eight values
+template <bool SHORT, typename T> __device__ __forceinline__ Packed16<T> ahead16(const T *row, long col, long cols) {
+  if (!SHORT) return load16(row + min(col, cols - CHUNK<T>));
+  if (cols >= CHUNK<T>) return load16(row + min(col, cols - CHUNK<T>));
+  Packed16<T> p = {};
+#pragma unroll 1
+  for (long i = cols - 1; i >= col; --i) {
+    if constexpr (sizeof(T) == 4) p.q = u32x4{__float_as_uint(row[i]), p.q[0], p.q[1], p.q[2]};
+    else p.q = shift_in(p.q, __builtin_bit_cast(uint16_t, row[i]));
+  }
+  return p;
+}
+template <typename T> __device__ __forceinline__ void trim16(Packed16<T> &p, long col, long cols) {
+  if (cols < CHUNK<T> || col + CHUNK<T> <= cols) return;
+  u32x4 q = p.q;
+  int by = (int)min(col + CHUNK<T> - cols, (long)CHUNK<T>);
+  if constexpr (sizeof(T) == 2) {
+    if (by & 1) q = u32x4{q[0] >> 16 | q[1] << 16, q[1] >> 16 | q[2] << 16, q[2] >> 16 | q[3] << 16, q[3] >> 16};
+    by >>= 1;
+  }
+  if (by & 1) q = u32x4{q[1], q[2], q[3], 0u};
+  if (by & 2) q = u32x4{q[2], q[3], 0u, 0u};
+  p.q = by & 4 ? u32x4{} : q;
+}
+template <typename T> __device__ __forceinline__ void widen16(float (&v)[CHUNK<T>], const Packed16<T> &p) {
+  if constexpr (sizeof(T) == 4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = __uint_as_float(p.q[i]);
+  } else {
+    const Values8 r = widen(Packed8<T>{p.q});
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = r.v[i];
+  }
+}
+template <typename T> __device__ __forceinline__ void add16(float (&v)[CHUNK<T>], const Packed16<T> &p) {
+  float more[CHUNK<T>];
+  widen16(more, p);
+#pragma unroll
+  for (int i = 0; i < CHUNK<T>; ++i) v[i] += more[i];
+}
+
+// what one wave wrote to LDS is there for its other lanes (whose instructions keep their order)
+__device__ __forceinline__ void wave_sync() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
 }
 
 // One rounding, to nearest even, from the 32 bits that everything was computed in.
@@ -201,6 +317,7 @@ template <typename T> __device__ __forceinline__ void store8(T *p, const Values8
   for (int i = 0; i < 4; ++i) q[i] = pack2(r.v[2 * i], r.v[2 * i + 1], T{});
   *reinterpret_cast<u32x4_from2 *>(p) = q;
 }
+// the first `count` of eight values
 template <typename T> __device__ __forceinline__ void write8(T *p, const Values8 &r, int count) {
   if (count >= 8) {
     store8(p, r);
@@ -209,6 +326,24 @@ template <typename T> __device__ __forceinline__ void write8(T *p, const Values8
 #pragma unroll
   for (int i = 0; i < 8; ++i)
     if (i < count) p[i] = (T)r.v[i];
+}
+
+// the first `count` of 4 or 8 values
+template <typename T, int N> __device__ __forceinline__ void store_first(T *p, const float (&v)[N], int count) {
+  static_assert(N == 4 || N == 8);
+  if (count >= N) {
+    if constexpr (N == 8) {
+      store8(p, Values8{{v[0], v[1], v[2], v[3], v[4], v[5], v[6], v[7]}});
+    } else if constexpr (sizeof(T) == 4) {
+      *reinterpret_cast<f32x4_unaligned *>(p) = f32x4{v[0], v[1], v[2], v[3]};
+    } else {
+      *reinterpret_cast<u32x2_from2 *>(p) = u32x2{pack2(v[0], v[1], T{}), pack2(v[2], v[3], T{})};
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (i < count) p[i] = (T)v[i];
 }
 
 // ---- dropout ----------------------------------------------------------------------------------------------------------

@@ -4,7 +4,6 @@
 // x goes through dropout first where that is on; its mask is drawn again in all three places.
 //
 //   k_adapter_plan   groups the rows by adapter (a stable counting sort) and cuts the groups into tiles and chunks
-//   k_adapter_rows   a tile of rows through both thin products, hidden and up never leave the workgroup in between
 //   k_adapter_turn   for the backward pass: the matrices with ranks and columns exchanged, so that it is the forward pass
 //   k_adapter_grads  sums over the rows of a chunk, for 128 columns of dA or dB
 //   k_adapter_join   adds the chunks of an adapter in their order, zeros for adapters without rows
@@ -15,17 +14,8 @@
 namespace rpu_amd {
 namespace {
 
-template <int V> struct Int {
-  static constexpr int value = V;
-};
-
 constexpr int PLAN_THREADS = 1024, PLAN_WAVES = PLAN_THREADS / 64;
 
-__device__ __forceinline__ int adapter_key(int index, int n) { return index >= 0 && index < n ? index : n; }
-__device__ __forceinline__ void wave_sync() {
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-}
 // lanes whose digit is this lane's (lanes with `valid` only)
 __device__ __forceinline__ uint64_t same_digit(int digit, bool valid, int bits) {
   uint64_t mask = __ballot(valid);
@@ -83,7 +73,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan_lds(const int *in
       hist[w][tid] = count[0];
       count[0] += c;
     }
-    count[1] = (count[0] + p.tile_rows - 1) / p.tile_rows;
+    count[1] = (count[0] + ADAPTER_TILE_ROWS - 1) / ADAPTER_TILE_ROWS;
     count[2] = tid < p.n ? (count[0] + p.chunk_rows - 1) / p.chunk_rows : 0;
     count[3] = count[2] > 1 ? count[2] : 0;
 #pragma unroll
@@ -118,7 +108,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan_lds(const int *in
     wave_sync();
   }
   for (int i = tid; i < p.max_tiles; i += PLAN_THREADS)
-    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, firsts[1], firsts[0], nullptr, keys, p.n, p.tile_rows);
+    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, firsts[1], firsts[0], nullptr, keys, p.n, ADAPTER_TILE_ROWS);
   for (int i = tid; i < p.max_chunks; i += PLAN_THREADS)
     reinterpret_cast<int4 *>(plan + p.chunks)[i] = plan_piece(i, firsts[2], firsts[0], firsts[3], p.n, p.n, p.chunk_rows);
   for (int i = tid; i <= keys; i += PLAN_THREADS) plan[p.seg + i] = i < PLAN_LDS_KEYS + 1 ? firsts[0][i] : p.rows;
@@ -207,7 +197,7 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
   const auto pieces = [&](int k, int piece) { return (seg[k + 1] - seg[k] + piece - 1) / piece; };
   int count[3] = {}; // tiles, chunks, and those chunks that are not all of their adapter
   const auto add = [&](int k) {
-    count[0] += pieces(k, p.tile_rows);
+    count[0] += pieces(k, ADAPTER_TILE_ROWS);
     const int chunks = k < p.n ? pieces(k, p.chunk_rows) : 0;
     count[1] += chunks;
     count[2] += chunks > 1 ? chunks : 0;
@@ -241,361 +231,9 @@ __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan(const int *index,
   }
   __syncthreads();
   for (int i = tid; i < p.max_tiles; i += PLAN_THREADS)
-    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, tile_first, seg, nullptr, keys, p.n, p.tile_rows);
+    reinterpret_cast<int4 *>(plan + p.tiles)[i] = plan_piece(i, tile_first, seg, nullptr, keys, p.n, ADAPTER_TILE_ROWS);
   for (int i = tid; i < p.max_chunks; i += PLAN_THREADS)
     reinterpret_cast<int4 *>(plan + p.chunks)[i] = plan_piece(i, first, seg, slot_first, p.n, p.n, p.chunk_rows);
-}
-
-// ---- eight terms, or four ranks, of both operands of a product, as the matrix instructions take them ------------------
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
-// rows of float: products on the fp32 instructions, whatever the weights are stored as
-template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) == 2> struct Pipe {
-  using X = Packed8<T>;
-  using W = Packed8<TW>;
-  using V = f32x4; // four ranks of hidden
-  static __device__ __forceinline__ f32x4 multiply(f32x4 a, f32x4 b, f32x4 c) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[i], b[i], c, 0, 0, 0);
-    return c;
-  }
-  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) {
-    const Values8 a = widen(w), b = widen(x);
-    c = multiply(f32x4{a.v[0], a.v[1], a.v[2], a.v[3]}, f32x4{b.v[0], b.v[1], b.v[2], b.v[3]}, c);
-    return multiply(f32x4{a.v[4], a.v[5], a.v[6], a.v[7]}, f32x4{b.v[4], b.v[5], b.v[6], b.v[7]}, c);
-  }
-  static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) x.q[i >> 2][i & 3] = kept & (1u << i) ? x.q[i >> 2][i & 3] : 0u;
-  }
-  template <int RT> static __device__ __forceinline__ float split(const f32x4 (&v)[RT], V (&to)[RT]) {
-#pragma unroll
-    for (int q = 0; q < RT; ++q) to[q] = v[q];
-    return 1.0f;
-  }
-  using R = f32x4; // four ranks of a weight row
-  static __device__ __forceinline__ R four(const float *p) { return *reinterpret_cast<const f32x4_unaligned *>(p); }
-  template <typename H> static __device__ __forceinline__ R four(const H *p) {
-    const u32x2_from2 w = *reinterpret_cast<const u32x2_from2 *>(p);
-    const Values8 v = widen(Packed8<H>{u32x4_from2{w[0], w[1], 0u, 0u}});
-    return R{v.v[0], v.v[1], v.v[2], v.v[3]};
-  }
-  static __device__ __forceinline__ void put(R &r, int i, TW w) { r[i] = to_float(w); }
-  template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT][2], int j, const V (&v)[RT], f32x4 c) {
-#pragma unroll
-    for (int q = 0; q < RT; ++q) c = multiply(w[q][j], v[q], c);
-    return c;
-  }
-};
-
-// 16-bit rows with weights of their type: exact products, sums in 32 bits.  hidden, which is not one of their numbers, goes into the
-// second product as the sum of some that are, against the same weights again: three bf16 parts, which are all of its 24 bits; two
-// halves, 22 bits (an error of 2^-23, twice that of a float, far below the 2^-11 of what is stored in the end).
-template <typename T> struct Pipe<T, T, true> {
-  using X = Packed8<T>;
-  using W = Packed8<T>;
-  struct V {
-    u32x4 upper; // the first two parts
-    u32x2 third;
-  };
-  static __device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) { return multiply(w.q, x.q, c); }
-  static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) x.q[i] &= (kept & (1u << 2 * i) ? 0xffffu : 0u) | (kept & (2u << 2 * i) ? 0xffff0000u : 0u);
-  }
-  static __device__ __forceinline__ uint32_t cut(float a, float b) { return (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u); }
-  static __device__ __forceinline__ float rest(float v, float part) { return __builtin_isfinite(v) ? v - part : 0.0f; }
-  // returns what the second product has to be multiplied by
-  template <int RT> static __device__ __forceinline__ float split(const f32x4 (&v)[RT], V (&to)[RT]) {
-    float lift = 1.0f, drop = 1.0f;
-    if constexpr (__is_same(T, _Float16)) { // hidden may leave the range of halves: the largest of the row becomes 2^14 .. 2^15
-      float most = 0.0f;
-#pragma unroll
-      for (int q = 0; q < RT; ++q)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) most = __builtin_isfinite(v[q][i]) ? fmaxf(most, fabsf(v[q][i])) : most;
-      most = fmaxf(most, __shfl_xor(most, 16));
-      most = fmaxf(most, __shfl_xor(most, 32));
-      const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased; smaller rows than 2^-97 round to steps of 2^-135
-      lift = __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);
-      drop = __uint_as_float((uint32_t)(exponent - 14) << 23);
-    }
-#pragma unroll
-    for (int q = 0; q < RT; ++q)
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const float a = v[q][2 * h] * lift, b = v[q][2 * h + 1] * lift;
-        if constexpr (__is_same(T, __bf16)) { // cut off, not rounded: the largest float stays finite
-          const uint32_t high = cut(a, b);
-          const float a1 = rest(a, __uint_as_float(high << 16)), b1 = rest(b, __uint_as_float(high & 0xffff0000u));
-          const uint32_t mid = cut(a1, b1);
-          to[q].upper[h] = high;
-          to[q].upper[2 + h] = mid;
-          to[q].third[h] = cut(a1 - __uint_as_float(mid << 16), b1 - __uint_as_float(mid & 0xffff0000u)); // eight bits are left
-        } else {
-          const uint32_t high = pack2(a, b, T{});
-          const f16x2 r = __builtin_bit_cast(f16x2, high);
-          to[q].upper[h] = high;
-          to[q].upper[2 + h] = pack2(rest(a, (float)r.x), rest(b, (float)r.y), T{});
-        }
-      }
-    return drop;
-  }
-  using R = u32x2;
-  static __device__ __forceinline__ R four(const T *p) { return *reinterpret_cast<const u32x2_from2 *>(p); }
-  static __device__ __forceinline__ void put(R &r, int i, T w) {
-    const uint32_t bits = (uint32_t)__builtin_bit_cast(uint16_t, w);
-    r[i >> 1] = i & 1 ? r[i >> 1] | bits << 16 : bits;
-  }
-  template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT][2], int j, const V (&v)[RT], f32x4 c) {
-#pragma unroll
-    for (int q = 0; q < RT; ++q) c = multiply(u32x4{w[q][j][0], w[q][j][1], w[q][j][0], w[q][j][1]}, v[q].upper, c);
-    if constexpr (__is_same(T, __bf16)) { // the third parts of two tiles of ranks at a time
-#pragma unroll
-      for (int q = 0; q < RT; q += 2) {
-        const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q][j] : R{};
-        const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
-        c = multiply(u32x4{w[q][j][0], w[q][j][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
-      }
-    }
-    return c;
-  }
-};
-
-// the first `count` of eight stored values, zeros behind them
-template <typename T> __device__ __forceinline__ Packed8<T> load8_first(const T *p, int count) {
-  if (count >= 8) return load8(p);
-  Packed8<T> r = {};
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (i < count) {
-      if constexpr (__is_same(T, float)) r.q[i >> 2][i & 3] = __float_as_uint(p[i]);
-      else r.q[i >> 1] |= (uint32_t)__builtin_bit_cast(uint16_t, p[i]) << 16 * (i & 1);
-    }
-  return r;
-}
-template <typename T> __device__ __forceinline__ void clear_unless(Packed8<T> &r, bool kept) {
-  if constexpr (__is_same(T, float)) {
-    r.q[0] = kept ? r.q[0] : u32x4_from4{};
-    r.q[1] = kept ? r.q[1] : u32x4_from4{};
-  } else {
-    r.q = kept ? r.q : u32x4_from2{};
-  }
-}
-
-constexpr int WAVES = 8;
-
-// A product of 16 x 16 results takes, per lane, row lane % 16 of one operand and column lane % 16 of the other, and of the terms
-// those of lane / 16.  Terms may come in any order that both operands share: a lane reads eight neighbouring ones at once.  The
-// result has, per lane, column lane % 16 and rows 4 (lane / 16) + 0 .. 3.  With the weights as rows that is: lane % 16 = the
-// row of x, and four neighbouring ranks -- the very operand that the second product wants, and there four neighbouring columns
-// of y, eight with the weights' rows dealt accordingly.
-// The workgroup's waves share the terms of the first product, add their parts up in LDS, and share the columns of the second;
-// nothing but x, base, y and the weights (which come from L2) is moved.  FULL: the rank fills its tiles of 16.
-template <typename T, typename TW, int RT, int MT, bool FULL> __global__ __launch_bounds__(64 * WAVES) void k_adapter_rows(AdapterRowsArgs a) {
-  using P = Pipe<T, TW>;
-  constexpr int RP = 16 * RT, PITCH = RP + 4, TILES = MT * RT;
-  constexpr int DEEP = RT <= 2 ? 4 / MT : RT == 4 ? 2 / MT : 1; // steps of 32 terms whose loads are under way together
-  __shared__ float red[WAVES][16 * MT][PITCH];
-  __shared__ int rows_of[64];
-  const int lane = (int)threadIdx.x & 63, wave = (int)threadIdx.x >> 6, lm = lane & 15, kg = lane >> 4;
-  int adapter, count;
-  if (a.plan) {
-    const int4 tile = reinterpret_cast<const int4 *>(a.plan + a.p.tiles)[blockIdx.x];
-    adapter = tile.x;
-    count = tile.z;
-    if (!count) return;
-    if ((int)threadIdx.x < count) rows_of[threadIdx.x] = a.plan[a.p.order + tile.y + threadIdx.x];
-  } else { // the rows of the adapter of row blockIdx.x, unless an earlier row has it
-    const int key = lane < a.rows ? adapter_key(a.index[lane], a.n) : -1;
-    const int mine = __shfl(key, (int)blockIdx.x);
-    const uint64_t same = __ballot(key == mine);
-    if (same & ((1ull << blockIdx.x) - 1)) return;
-    adapter = mine < a.n ? mine : -1;
-    count = __popcll(same);
-    if (wave == 0 && ((same >> lane) & 1)) rows_of[__popcll(same & ((1ull << lane) - 1))] = lane;
-  }
-  __syncthreads();
-  const T *in = static_cast<const T *>(a.in.p), *base = static_cast<const T *>(a.base.p);
-  T *out = static_cast<T *>(a.out.p);
-  const int units = (a.out_size + 31) / 32; // of 32 columns, shared by the workgroups of the tile
-  const int unit0 = (int)((long)units * blockIdx.y / gridDim.y), unit1 = (int)((long)units * (blockIdx.y + 1) / gridDim.y);
-  if (adapter < 0) {
-    if (base != out || !base)
-      for (int m = wave; m < count; m += WAVES) {
-        const long row = rows_of[m];
-        for (int col = unit0 * 32 + lane * 8; col < min(unit1 * 32, a.out_size); col += 512) {
-          Values8 v = {};
-          if (base) v = read8(base + row * a.base.ld + col, a.out_size - col);
-          write8(out + row * a.out.ld + col, v, a.out_size - col);
-        }
-      }
-    if (a.hidden && !blockIdx.y)
-      for (int i = (int)threadIdx.x; i < count * a.rank; i += 64 * WAVES) a.hidden[(long)rows_of[i / a.rank] * a.rank + i % a.rank] = 0.0f;
-    return;
-  }
-  const TW *w_in = static_cast<const TW *>(a.w_in) + (long)adapter * a.rank * a.in_size;
-  const TW *w_out = static_cast<const TW *>(a.w_out) + (long)adapter * a.rank * a.out_size;
-  const float scale = a.scale[adapter];
-  const bool drop_in = a.drop.on && !a.back, drop_out = a.drop.on && a.back;
-  const uint32_t call = a.drop.on ? drop_call(a.drop) : 0;
-  const int full_steps = a.in_size / 32;
-
-  for (int m0 = 0; m0 < count; m0 += 16 * MT) {
-    long row[MT];
-    const T *x_at[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) { // rows beyond the last repeat it and are not stored
-      row[mt] = rows_of[min(m0 + 16 * mt + lm, count - 1)];
-      x_at[mt] = in + row[mt] * a.in.ld;
-    }
-    f32x4 sum[MT][RT] = {};
-    // `n` steps, WAVES apart; not whole: the one that the terms end in; masked: of an input that goes through dropout
-    const auto steps = [&](int step, auto n, auto whole, auto masked) {
-      constexpr int N = decltype(n)::value;
-      typename P::X x[N][MT];
-      typename P::W w[N][RT];
-#pragma unroll
-      for (int s = 0; s < N; ++s) {
-        const int col = (step + s * WAVES) * 32 + 8 * kg, left = decltype(whole)::value ? 8 : a.in_size - col;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) x[s][mt] = decltype(whole)::value ? load8(x_at[mt] + col) : load8_first(x_at[mt] + col, left);
-#pragma unroll
-        for (int q = 0; q < RT; ++q) {
-          const int rank = 16 * q + lm;
-          const TW *at = w_in + (long)(FULL ? rank : min(rank, a.rank - 1)) * a.in_size + col;
-          w[s][q] = decltype(whole)::value ? load8(at) : load8_first(at, left);
-          if (!FULL) clear_unless(w[s][q], rank < a.rank);
-        }
-      }
-#pragma unroll
-      for (int s = 0; s < N; ++s) {
-        const uint32_t block = (uint32_t)(step + s * WAVES) * 4u + (uint32_t)kg;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          if (decltype(masked)::value) P::keep(x[s][mt], drop_kept(a.drop, call, (uint32_t)row[mt], block)); // scaled below
-#pragma unroll
-          for (int q = 0; q < RT; ++q) sum[mt][q] = P::terms(w[s][q], x[s][mt], sum[mt][q]);
-        }
-      }
-    };
-    int step = wave;
-    if (drop_in) { // drawing the masks takes longer than the loads
-      for (; step < full_steps; step += WAVES) steps(step, Int<1>{}, Int<1>{}, Int<1>{});
-      if (step == full_steps && step * 32 < a.in_size) steps(step, Int<1>{}, Int<0>{}, Int<1>{});
-    } else {
-      for (; step + (DEEP - 1) * WAVES < full_steps; step += DEEP * WAVES) steps(step, Int<DEEP>{}, Int<1>{}, Int<0>{});
-      if (DEEP > 1)
-        for (; step < full_steps; step += WAVES) steps(step, Int<1>{}, Int<1>{}, Int<0>{});
-      if (step == full_steps && step * 32 < a.in_size) steps(step, Int<1>{}, Int<0>{}, Int<0>{});
-    }
-
-    // the waves' parts, added in their order: tile t by wave t % WAVES
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int q = 0; q < RT; ++q) *reinterpret_cast<f32x4 *>(&red[wave][16 * mt + lm][16 * q + 4 * kg]) = sum[mt][q];
-    __syncthreads();
-    for (int t = wave; t < TILES; t += WAVES) {
-      const int mt = t / RT, q = t % RT, m = m0 + 16 * mt + lm;
-      float *at = &red[0][16 * mt + lm][16 * q + 4 * kg];
-      f32x4 v = *reinterpret_cast<const f32x4 *>(at);
-#pragma unroll
-      for (int w = 1; w < WAVES; ++w) v += *reinterpret_cast<const f32x4 *>(at + w * 16 * MT * PITCH);
-      if (drop_in) v *= a.drop.scale;
-      const f32x4 scaled = v * scale;
-      if (a.hidden && !blockIdx.y && m < count) {
-        float *to = a.hidden + (long)rows_of[m] * a.rank + 16 * q + 4 * kg;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (FULL || 16 * q + 4 * kg + i < a.rank) to[i] = a.back ? scaled[i] : v[i];
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) // padding is zero also where a row holds an infinity, whose product with it is none
-        at[i] = FULL || 16 * q + 4 * kg + i < a.rank ? scaled[i] : 0.0f;
-    }
-    __syncthreads();
-    typename P::V hidden[MT][RT];
-    float lift[MT];
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-      for (int q = 0; q < RT; ++q) sum[mt][q] = *reinterpret_cast<const f32x4 *>(&red[0][16 * mt + lm][16 * q + 4 * kg]);
-      lift[mt] = P::split(sum[mt], hidden[mt]) * (drop_out ? a.drop.scale : 1.0f);
-    }
-
-    const auto columns = [&](int unit0, auto n, auto whole, auto masked) { // `n` units, WAVES apart
-      constexpr int N = decltype(n)::value;
-      Packed8<T> add[N][MT];
-      typename P::R w[N][RT][2];
-#pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const int unit = unit0 + u * WAVES, col = unit * 32 + 8 * kg;
-        if (base) {
-#pragma unroll
-          for (int mt = 0; mt < MT; ++mt)
-            add[u][mt] = decltype(whole)::value ? load8(base + row[mt] * a.base.ld + col) : load8_first(base + row[mt] * a.base.ld + col, a.out_size - col);
-        }
-#pragma unroll
-        for (int q = 0; q < RT; ++q)
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            int c = unit * 32 + (lm >> 2) * 8 + j * 4 + (lm & 3); // the column whose result ends up beside its neighbours
-            if (!decltype(whole)::value) c = min(c, a.out_size - 1);
-            const int rank = 16 * q + 4 * kg;
-            if (FULL) {
-              w[u][q][j] = P::four(w_out + (long)c * a.rank + rank);
-            } else {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) P::put(w[u][q][j], i, rank + i < a.rank ? w_out[(long)c * a.rank + min(rank + i, a.rank - 1)] : (TW)0.0f);
-            }
-          }
-      }
-#pragma unroll
-      for (int u = 0; u < N; ++u) {
-        const int unit = unit0 + u * WAVES, col = unit * 32 + 8 * kg, left = decltype(whole)::value ? 8 : a.out_size - col;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-          f32x4 acc[2] = {};
-#pragma unroll
-          for (int j = 0; j < 2; ++j) acc[j] = P::ranks(w[u], j, hidden[mt], acc[j]);
-          if (m0 + 16 * mt + lm >= count) continue;
-          Values8 v;
-#pragma unroll
-          for (int h = 0; h < 8; ++h) v.v[h] = acc[h >> 2][h & 3] * lift[mt];
-          if (decltype(masked)::value) {
-            const uint32_t kept = drop_kept(a.drop, call, (uint32_t)row[mt], (uint32_t)unit * 4u + (uint32_t)kg);
-#pragma unroll
-            for (int h = 0; h < 8; ++h) v.v[h] = kept & (1u << h) ? v.v[h] : 0.0f;
-          }
-          if (base) {
-            const Values8 b = widen(add[u][mt]);
-#pragma unroll
-            for (int h = 0; h < 8; ++h) v.v[h] += b.v[h];
-          }
-          if (decltype(whole)::value) store8(out + row[mt] * a.out.ld + col, v);
-          else write8(out + row[mt] * a.out.ld + col, v, left);
-        }
-      }
-    };
-    constexpr int WIDE = RT * MT == 1 ? 4 : RT * MT == 2 ? 2 : 1; // units whose loads are under way together
-    const int whole_units = min(unit1, a.out_size / 32);
-    int unit = unit0 + wave;
-    if (drop_out) {
-      for (; unit < whole_units; unit += WAVES) columns(unit, Int<1>{}, Int<1>{}, Int<1>{});
-      if (unit < unit1) columns(unit, Int<1>{}, Int<0>{}, Int<1>{});
-    } else {
-      for (; unit + (WIDE - 1) * WAVES < whole_units; unit += WIDE * WAVES) columns(unit, Int<WIDE>{}, Int<1>{}, Int<0>{});
-      if (WIDE > 1)
-        for (; unit < whole_units; unit += WAVES) columns(unit, Int<1>{}, Int<1>{}, Int<0>{});
-      if (unit < unit1) columns(unit, Int<1>{}, Int<0>{}, Int<0>{});
-    }
-    __syncthreads();
-  }
 }
 
 // The matrices of the adapters that have rows with ranks and columns exchanged: with them the backward pass of rows is the
@@ -638,8 +276,11 @@ template <typename TW> __global__ __launch_bounds__(256) void k_adapter_turn(Ada
 constexpr int GRAD_WAVES = 4;
 
 // 128 columns of dA (of x, against up) or of dB (of d, against scale hidden).  A wave takes 16 rows of its chunk at a time; lane
-// % 16 reads eight neighbouring columns of four rows, and product j of a row takes column 8 (lane % 16) + j.
-template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * GRAD_WAVES) void k_adapter_grads(AdapterGradArgs a) {
+// % 16 reads eight columns of four rows, 16 bytes beside those of its neighbours at a time, and product j of a row takes its column j.
+// Bound by the reads of x and d, which no other workgroup reads, and the products on the fp32 instructions: 8192 rows of 768 and 2304 floats,
+// rank 16, in 25.7 us (101 MB, 3.9 TB/s).  One group at a time, each waited for, 35 us; the next one under way with a branch around
+// every load 33 us.
+template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bounds__(64 * GRAD_WAVES, RT == 1 ? 3 : 1) void k_adapter_grads(AdapterGradArgs a) {
   __shared__ float sums[32 * RT][64];
   const int4 chunk = reinterpret_cast<const int4 *>(a.plan + a.p.chunks)[blockIdx.x];
   const int adapter = chunk.x, count = chunk.z;
@@ -654,24 +295,79 @@ template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * GRA
   const float scale = of_a ? 1.0f : a.scale[adapter];
   const bool drop = of_a && a.drop.on;
   const uint32_t call = drop ? drop_call(a.drop) : 0;
-  const int col = c0 + 8 * lm, left = width - col, rank0 = 16 * RT * (int)blockIdx.z;
+  constexpr int EACH = CHUNK<T>, PIECES = 8 / EACH, STEP = 16 * EACH; // columns of a load, loads of a row, columns of a load of 16 lanes
+  const int col = c0 + EACH * lm, rank0 = 16 * RT * (int)blockIdx.z;
   f32x4 acc[8][RT] = {};
-  for (int g = wave; g * 16 < count; g += GRAD_WAVES) {
+  // the next group is under way, and the rows of the one after it
+  struct Group {
+    Packed16<T> x[4][PIECES];
+    float u[4][RT];
+  };
+  const auto find = [&](int (&row)[4], int g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) row[i] = order[min(16 * g + 4 * kg + i, count - 1)]; // rows beyond the last repeat it
+  };
+  const auto fetch = [&](Group &next, const int (&row)[4]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int at = 16 * g + 4 * kg + i;
-      const bool valid = at < count;
-      const long row = order[min(at, count - 1)];
-      Values8 x = read8(static_cast<const T *>(m.p) + row * m.ld + col, valid ? left : 0);
-      if (drop) drop_apply(a.drop, drop_kept(a.drop, call, (uint32_t)row, (uint32_t)col / 8u), x);
+#pragma unroll
+      for (int h = 0; h < PIECES; ++h) next.x[i][h] = ahead16<SHORT>(static_cast<const T *>(m.p) + (long)row[i] * m.ld, col + STEP * h, width);
+#pragma unroll
+      for (int q = 0; q < RT; ++q) next.u[i][q] = factor[(long)row[i] * a.rank + min(rank0 + 16 * q + lm, a.rank - 1)];
+    }
+  };
+  const auto multiply = [&](Group &here, const int (&row)[4], int g) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const bool valid = 16 * g + 4 * kg + i < count;
+      Values8 x;
+#pragma unroll
+      for (int h = 0; h < PIECES; ++h) {
+        trim16(here.x[i][h], col + STEP * h, width);
+        float v[EACH];
+        widen16(v, here.x[i][h]);
+#pragma unroll
+        for (int j = 0; j < EACH; ++j) x.v[EACH * h + j] = v[j];
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) x.v[j] = valid ? x.v[j] : 0.0f; // whatever the row that stands in for it holds
+      if (drop) {
+        uint32_t kept;
+        if constexpr (PIECES == 1) {
+          kept = drop_kept(a.drop, call, (uint32_t)row[i], (uint32_t)col / 8u);
+        } else { // two neighbours hold half of two blocks each: each draws one
+          const uint32_t mine = drop_kept(a.drop, call, (uint32_t)row[i], (uint32_t)(col + STEP * (lm & 1)) / 8u), other = (uint32_t)__shfl_xor((int)mine, 1);
+          const uint32_t low = lm & 1 ? other : mine, high = lm & 1 ? mine : other, shift = col & 4;
+          kept = (low >> shift & 15u) | (high >> shift & 15u) << 4;
+        }
+        drop_apply(a.drop, kept, x);
+      }
 #pragma unroll
       for (int q = 0; q < RT; ++q) {
-        const int rank = rank0 + 16 * q + lm;
-        const float u = valid && rank < a.rank ? factor[row * a.rank + rank] * scale : 0.0f;
+        const float u = valid && rank0 + 16 * q + lm < a.rank ? here.u[i][q] * scale : 0.0f;
 #pragma unroll
         for (int j = 0; j < 8; ++j) acc[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(x.v[j], u, acc[j][q], 0, 0, 0);
       }
     }
+  };
+  const int groups = (count + 15) / 16;
+  int rows[2][4], last[4];
+  Group group[2];
+  if (wave < groups) {
+    find(rows[0], wave);
+    fetch(group[0], rows[0]);
+    find(rows[1], wave + GRAD_WAVES);
+  }
+  const auto step = [&](Group &here, Group &next, int (&row)[4], int (&ahead)[4], int g) {
+    if (g + GRAD_WAVES < groups) fetch(next, ahead);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) last[i] = row[i];
+    if (g + 2 * GRAD_WAVES < groups) find(row, g + 2 * GRAD_WAVES);
+    multiply(here, last, g);
+  };
+  for (int g = wave; g < groups; g += 2 * GRAD_WAVES) {
+    step(group[0], group[1], rows[0], rows[1], g);
+    if (g + GRAD_WAVES < groups) step(group[1], group[0], rows[1], rows[0], g + GRAD_WAVES);
   }
   for (int from = 0; from < GRAD_WAVES; ++from) { // the waves' sums, added in their order
     if (wave == from) {
@@ -693,21 +389,25 @@ template <typename T, typename TW, int RT> __global__ __launch_bounds__(64 * GRA
     if (rank >= a.rank) continue;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const int c = c0 + 32 * kg + 8 * i;
-      Values8 v;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) v.v[j] = acc[j][q][i];
-      if (of_a) {
-        const long at = (long)rank * a.in_size + c;
-        if (whole) write8(static_cast<TW *>(a.da) + (long)adapter * a.rank * a.in_size + at, v, width - c);
-        else write8(part + at, v, width - c);
-      } else {
+      for (int h = 0; h < PIECES; ++h) {
+        const int c = c0 + STEP * h + EACH * (4 * kg + i);
+        if (of_a) {
+          const long at = (long)rank * a.in_size + c;
+          float v[EACH];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          if (c + j >= width) continue;
-          const long at = (long)(c + j) * a.rank + rank;
-          if (whole) static_cast<TW *>(a.db)[(long)adapter * a.rank * a.out_size + at] = (TW)v.v[j];
-          else part[at] = v.v[j];
+          for (int j = 0; j < EACH; ++j) v[j] = acc[EACH * h + j][q][i];
+          if (whole) store_first(static_cast<TW *>(a.da) + (long)adapter * a.rank * a.in_size + at, v, width - c);
+          else store_first(part + at, v, width - c);
+        } else {
+#pragma unroll
+          for (int j = 0; j < EACH; ++j) {
+            if (c + j >= width) continue;
+            const long at = (long)(c + j) * a.rank + rank;
+            const float v = acc[EACH * h + j][q][i];
+            if (whole) static_cast<TW *>(a.db)[(long)adapter * a.rank * a.out_size + at] = (TW)v;
+            else part[at] = v;
+          }
         }
       }
     }
@@ -737,13 +437,6 @@ template <typename TW> __global__ __launch_bounds__(256) void k_adapter_join(Ada
   }
 }
 
-template <typename F> void with_types(int dtype, int w_dtype, F &&f) {
-  if (dtype == RPU_BF16) f(__bf16{}, __bf16{});
-  else if (dtype == RPU_F16) f(_Float16{}, _Float16{});
-  else if (w_dtype == RPU_F32) f(float{}, float{});
-  else if (w_dtype == RPU_F16) f(float{}, _Float16{});
-  else f(float{}, __bf16{});
-}
 template <typename F> void with_rank_tiles(int rank, F &&f) {
   if (rank <= 16) f(Int<1>{});
   else if (rank <= 32) f(Int<2>{});
@@ -752,29 +445,6 @@ template <typename F> void with_rank_tiles(int rank, F &&f) {
 }
 
 } // namespace
-
-void launch_adapter_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int cus, hipStream_t s) {
-  const int tile_rows = a.plan ? a.p.tile_rows : a.rows, tiles = a.plan ? a.p.max_tiles : a.rows;
-  // tiles that leave CUs idle share their output columns among several workgroups, each of which makes hidden for itself
-  const int units = (a.out_size + 31) / 32;
-  const int slices = std::max(1, std::min(units / WAVES, cus / std::max(tiles, 1)));
-  const dim3 grid((unsigned)tiles, (unsigned)slices);
-  with_types(dtype, w_dtype, [&](auto x, auto w) {
-    using T = decltype(x);
-    using TW = decltype(w);
-    with_rank_tiles(a.rank, [&](auto rt) {
-      constexpr int RT = decltype(rt)::value, MOST = RT <= 4 ? 2 : 1; // groups of 16 rows at a time: what registers and LDS hold
-      const bool full = a.rank == 16 * RT;
-      if (tile_rows <= 16 || MOST == 1) {
-        if (full) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 1, true>), grid, dim3(64 * WAVES), 0, s, a);
-        else hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, 1, false>), grid, dim3(64 * WAVES), 0, s, a);
-      } else {
-        if (full) hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, MOST, true>), grid, dim3(64 * WAVES), 0, s, a);
-        else hipLaunchKernelGGL((k_adapter_rows<T, TW, RT, MOST, false>), grid, dim3(64 * WAVES), 0, s, a);
-      }
-    });
-  });
-}
 
 void launch_adapter_turn(const AdapterTurnArgs &a, int w_dtype, int cus, hipStream_t s) {
   const int tiles = ((a.in_size + 63) / 64 + (a.out_size + 63) / 64) * ((a.rank + 63) / 64);
@@ -787,11 +457,10 @@ AdapterPlan adapter_plan(int rows, int n) {
   AdapterPlan p{};
   p.rows = rows;
   p.n = n;
-  p.tile_rows = rows <= 16384 ? 16 : 32;
   p.chunk_rows = 64;
   while (p.chunk_rows < 1024 && rows / p.chunk_rows > 32) p.chunk_rows *= 2;
   // every group of rows but for one may end with a piece that is not full
-  p.max_tiles = (int)std::min<long>(rows, ((long)rows + p.tile_rows - 1) / p.tile_rows + std::min(n, rows));
+  p.max_tiles = (int)std::min<long>(rows, ((long)rows + ADAPTER_TILE_ROWS - 1) / ADAPTER_TILE_ROWS + std::min(n, rows));
   p.max_chunks = (int)std::min<long>(rows, ((long)rows + p.chunk_rows - 1) / p.chunk_rows + std::min(n, rows));
   p.max_slots = (int)std::min<long>(p.max_chunks, 2l * rows / p.chunk_rows); // of adapters with more rows than a chunk
   size_t at = 0;
@@ -821,13 +490,15 @@ void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int 
   const unsigned slices = (unsigned)(((long)a.in_size + 127) / 128 + ((long)a.out_size + 127) / 128);
   const long values = (long)a.rank * ((long)a.in_size + a.out_size);
   const dim3 join((unsigned)std::max<long>(1, std::min<long>((values + 255) / 256, std::max(1, cus * 8 / a.n))), (unsigned)std::min(a.n, 65535));
-  with_types(dtype, w_dtype, [&](auto x, auto w) {
+  with_adapter_types(dtype, w_dtype, [&](auto x, auto w) {
     using T = decltype(x);
     using TW = decltype(w);
-    if (a.rows)
+    if (a.rows && std::min(a.in_size, a.out_size) < 8)
+      hipLaunchKernelGGL((k_adapter_grads<T, TW, 1, true>), dim3((unsigned)a.p.max_chunks, slices, (unsigned)(a.rank + 15) / 16), dim3(64 * GRAD_WAVES), 0, s, a);
+    else if (a.rows)
       with_rank_tiles(a.rank, [&](auto rt) {
         constexpr int RT = decltype(rt)::value, AT_ONCE = RT < 4 ? RT : 4; // more sums than that of 64 ranks leave the registers
-        hipLaunchKernelGGL((k_adapter_grads<T, TW, AT_ONCE>), dim3((unsigned)a.p.max_chunks, slices, RT / AT_ONCE), dim3(64 * GRAD_WAVES), 0, s, a);
+        hipLaunchKernelGGL((k_adapter_grads<T, TW, AT_ONCE, false>), dim3((unsigned)a.p.max_chunks, slices, RT / AT_ONCE), dim3(64 * GRAD_WAVES), 0, s, a);
       });
     hipLaunchKernelGGL(k_adapter_join<TW>, join, dim3(256), 0, s, a);
   });

@@ -8,7 +8,7 @@ namespace rpu_amd {
 namespace {
 
 // A thread takes eight neighbouring elements, one Philox block, at a time.
-template <typename T> __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
+template <typename T, bool SHORT> __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
   const T *x = static_cast<const T *>(a.x.p), *base = static_cast<const T *>(a.base.p);
   T *out = static_cast<T *>(a.out.p);
   const uint32_t blocks = ((uint32_t)a.cols + 7u) / 8u, call = drop_call(a.drop);
@@ -17,10 +17,15 @@ template <typename T> __global__ __launch_bounds__(256) void k_dropout(DropoutAr
     const uint32_t row = (uint32_t)(i / blocks), block = (uint32_t)(i % blocks);
     const int left = a.cols - (int)(block * 8u);
     const long col = (long)block * 8;
-    Values8 v = read8(x + row * a.x.ld + col, left);
-    drop_apply(a.drop, drop_kept(a.drop, call, row, block), v);
+    Packed8<T> x8 = ahead8<SHORT>(x + row * a.x.ld, col, a.cols), base8 = {};
+    if (base) base8 = ahead8<SHORT>(base + row * a.base.ld, col, a.cols);
+    const uint32_t kept = drop_kept(a.drop, call, row, block);
+    trim8(x8, col, a.cols);
+    Values8 v = widen(x8);
+    drop_apply(a.drop, kept, v);
     if (base) {
-      const Values8 r = read8(base + row * a.base.ld + col, left);
+      trim8(base8, col, a.cols);
+      const Values8 r = widen(base8);
 #pragma unroll
       for (int h = 0; h < 8; ++h) v.v[h] += r.v[h];
     }
@@ -33,9 +38,14 @@ template <typename T> __global__ __launch_bounds__(256) void k_dropout(DropoutAr
 void launch_dropout(const DropoutArgs &a, int dtype, int cus, hipStream_t s) {
   const uint64_t total = (uint64_t)a.rows * (((uint64_t)a.cols + 7) / 8);
   const dim3 grid((unsigned)std::min<uint64_t>((total + 255) / 256, (uint64_t)cus * 16));
-  if (dtype == RPU_F32) hipLaunchKernelGGL(k_dropout<float>, grid, dim3(256), 0, s, a);
-  else if (dtype == RPU_F16) hipLaunchKernelGGL(k_dropout<_Float16>, grid, dim3(256), 0, s, a);
-  else hipLaunchKernelGGL(k_dropout<__bf16>, grid, dim3(256), 0, s, a);
+  const auto launch = [&](auto x) {
+    using T = decltype(x);
+    if (a.cols < 8) hipLaunchKernelGGL((k_dropout<T, true>), grid, dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((k_dropout<T, false>), grid, dim3(256), 0, s, a);
+  };
+  if (dtype == RPU_F32) launch(float{});
+  else if (dtype == RPU_F16) launch(_Float16{});
+  else launch(__bf16{});
 }
 
 } // namespace rpu_amd

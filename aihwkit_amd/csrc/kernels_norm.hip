@@ -25,16 +25,16 @@ template <int TPR> __device__ __forceinline__ float row_sum(float v, float *room
   return v;
 }
 
-template <typename T> __device__ __forceinline__ Values8 parameter8(const T *p, long at, int left, float otherwise) {
-  if (p) return read8(p + at, left);
+template <bool SHORT, typename T> __device__ __forceinline__ Values8 parameter8(const T *p, long col, long cols, float otherwise) {
+  if (p) return read8<SHORT>(p, col, cols);
   Values8 r;
 #pragma unroll
   for (int h = 0; h < 8; ++h) r.v[h] = otherwise;
   return r;
 }
 
-// Rows of up to 8 * TPR * V columns, TPR threads to a row.
-template <typename T, typename TW, int TPR, int V> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_layer_norm(NormArgs a) {
+// Rows of up to 8 * TPR * V columns, TPR threads to a row; SHORT: of fewer than 8.
+template <typename T, typename TW, int TPR, int V, bool SHORT = false> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_layer_norm(NormArgs a) {
   constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
   __shared__ float room[THREADS / 64];
   const int t = (int)threadIdx.x % TPR;
@@ -44,17 +44,20 @@ template <typename T, typename TW, int TPR, int V> __global__ __launch_bounds__(
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int col = (t + k * TPR) * 8;
-    w[k] = parameter8(static_cast<const TW *>(a.w), col, a.cols - col, 1.0f);
-    b[k] = parameter8(static_cast<const TW *>(a.b), col, a.cols - col, 0.0f);
+    w[k] = parameter8<SHORT>(static_cast<const TW *>(a.w), col, a.cols, 1.0f);
+    b[k] = parameter8<SHORT>(static_cast<const TW *>(a.b), col, a.cols, 0.0f);
   }
   const float n = (float)a.cols;
   for (long row = (long)blockIdx.x * ROWS + threadIdx.x / TPR; row < a.rows; row += (long)gridDim.x * ROWS) {
+    Packed8<T> p[V];
     Values8 v[V];
     float sum = 0.0f;
 #pragma unroll
+    for (int k = 0; k < V; ++k) p[k] = ahead8<SHORT>(x + row * a.x.ld, (t + k * TPR) * 8, a.cols);
+#pragma unroll
     for (int k = 0; k < V; ++k) {
-      const int col = (t + k * TPR) * 8;
-      v[k] = read8(x + row * a.x.ld + col, a.cols - col);
+      trim8(p[k], (t + k * TPR) * 8, a.cols);
+      v[k] = widen(p[k]);
 #pragma unroll
       for (int h = 0; h < 8; ++h) sum += v[k].v[h];
     }
@@ -94,7 +97,7 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
     T *out = static_cast<T *>(a.out.p) + row * a.out.ld;
     float sum = 0.0f;
     for (long col = (long)threadIdx.x * 8; col < a.cols; col += LONG * 8) {
-      const Values8 v = read8(x + col, (int)(a.cols - col));
+      const Values8 v = read8<false>(x, col, a.cols);
 #pragma unroll
       for (int h = 0; h < 8; ++h) sum += v.v[h];
     }
@@ -102,7 +105,7 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
     float squares = 0.0f;
     for (long col = (long)threadIdx.x * 8; col < a.cols; col += LONG * 8) {
       const int left = (int)(a.cols - col);
-      const Values8 v = read8(x + col, left);
+      const Values8 v = read8<false>(x, col, a.cols);
 #pragma unroll
       for (int h = 0; h < 8; ++h) {
         const float c = h < left ? v.v[h] - mean : 0.0f;
@@ -112,8 +115,8 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
     const float rstd = 1.0f / sqrtf(row_sum<LONG>(squares, room) / n + a.eps);
     for (long col = (long)threadIdx.x * 8; col < a.cols; col += LONG * 8) {
       const int left = (int)(a.cols - col);
-      Values8 v = read8(x + col, left);
-      const Values8 w = parameter8(static_cast<const TW *>(a.w), col, left, 1.0f), b = parameter8(static_cast<const TW *>(a.b), col, left, 0.0f);
+      Values8 v = read8<false>(x, col, a.cols);
+      const Values8 w = parameter8<false>(static_cast<const TW *>(a.w), col, a.cols, 1.0f), b = parameter8<false>(static_cast<const TW *>(a.b), col, a.cols, 0.0f);
 #pragma unroll
       for (int h = 0; h < 8; ++h) v.v[h] = fmaf((v.v[h] - mean) * rstd, w.v[h], b.v[h]);
       write8(out + col, v, left);
@@ -128,9 +131,10 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
 constexpr int backward_threads(int threads_of_a_row) { return threads_of_a_row == 64 ? 512 : threads_of_a_row; }
 // Backward pass of rows of up to 8 * TPR * V columns.  A workgroup adds d and d h of its rows up in registers and leaves the
 // sums in part[workgroup]; k_layer_norm_join adds those.
-template <typename T, typename TW, int TPR, int V>
+template <typename T, typename TW, int TPR, int V, bool SHORT = false>
 __global__ __launch_bounds__(backward_threads(TPR)) void k_layer_norm_backward(NormBackwardArgs a) {
   constexpr int THREADS = backward_threads(TPR), ROWS = THREADS / TPR;
+  constexpr bool EARLY = TPR < 1024; // base under way with d and x, where the registers suffice
   __shared__ float room[THREADS / 64];
   __shared__ Values8 sums[ROWS > 1 ? 2 * TPR * V : 1];
   const int t = (int)threadIdx.x % TPR, group = (int)threadIdx.x / TPR;
@@ -140,18 +144,28 @@ __global__ __launch_bounds__(backward_threads(TPR)) void k_layer_norm_backward(N
 #pragma unroll
   for (int k = 0; k < V; ++k) {
     const int col = (t + k * TPR) * 8;
-    w[k] = parameter8(static_cast<const TW *>(a.w), col, a.cols - col, 1.0f);
+    w[k] = parameter8<SHORT>(static_cast<const TW *>(a.w), col, a.cols, 1.0f);
   }
   const float n = (float)a.cols;
   for (long row = (long)blockIdx.x * ROWS + group; row < a.rows; row += (long)gridDim.x * ROWS) {
+    Packed8<T> p[V], q[V], more[V];
     Values8 g[V], h[V];
     const float mean = a.mean[row], rstd = a.rstd[row];
     float sum_g = 0.0f, sum_gh = 0.0f;
 #pragma unroll
     for (int k = 0; k < V; ++k) {
+      const int col = (t + k * TPR) * 8;
+      p[k] = ahead8<SHORT>(d + row * a.d.ld, col, a.cols);
+      q[k] = ahead8<SHORT>(x + row * a.x.ld, col, a.cols);
+      if (EARLY && base) more[k] = ahead8<SHORT>(base + row * a.base.ld, col, a.cols);
+    }
+#pragma unroll
+    for (int k = 0; k < V; ++k) {
       const int col = (t + k * TPR) * 8, left = a.cols - col;
-      g[k] = read8(d + row * a.d.ld + col, left);
-      h[k] = read8(x + row * a.x.ld + col, left);
+      trim8(p[k], col, a.cols);
+      trim8(q[k], col, a.cols);
+      g[k] = widen(p[k]);
+      h[k] = widen(q[k]);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         const float hat = i < left ? (h[k].v[i] - mean) * rstd : 0.0f;
@@ -171,7 +185,9 @@ __global__ __launch_bounds__(backward_threads(TPR)) void k_layer_norm_backward(N
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.v[i] = rstd * (g[k].v[i] - mean_g - h[k].v[i] * mean_gh);
       if (base) {
-        const Values8 add = read8(base + row * a.base.ld + col, left);
+        if (!EARLY) more[k] = ahead8<SHORT>(base + row * a.base.ld, col, a.cols);
+        trim8(more[k], col, a.cols);
+        const Values8 add = widen(more[k]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] += add.v[i];
       }
@@ -219,11 +235,11 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
     float sum_g = 0.0f, sum_gh = 0.0f;
     for (long col = (long)threadIdx.x * 8; col < a.cols; col += LONG * 8) {
       const int left = (int)(a.cols - col);
-      const Values8 g = read8(d + col, left), v = read8(x + col, left), w = parameter8(static_cast<const TW *>(a.w), col, left, 1.0f);
+      const Values8 g = read8<false>(d, col, a.cols), v = read8<false>(x, col, a.cols), w = parameter8<false>(static_cast<const TW *>(a.w), col, a.cols, 1.0f);
       Values8 dw = {}, db = {};
       if (a.dw && row != (long)blockIdx.x) {
-        dw = read8(part + col, left);
-        db = read8(part + a.cols + col, left);
+        dw = read8<false>(part, col, a.cols);
+        db = read8<false>(part + a.cols, col, a.cols);
       }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
@@ -241,12 +257,12 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
     const float mean_g = row_sum<LONG>(sum_g, room) / n, mean_gh = row_sum<LONG>(sum_gh, room) / n;
     for (long col = (long)threadIdx.x * 8; col < a.cols; col += LONG * 8) {
       const int left = (int)(a.cols - col);
-      const Values8 g = read8(d + col, left), v = read8(x + col, left), w = parameter8(static_cast<const TW *>(a.w), col, left, 1.0f);
+      const Values8 g = read8<false>(d, col, a.cols), v = read8<false>(x, col, a.cols), w = parameter8<false>(static_cast<const TW *>(a.w), col, a.cols, 1.0f);
       Values8 r;
 #pragma unroll
       for (int i = 0; i < 8; ++i) r.v[i] = rstd * (g.v[i] * w.v[i] - mean_g - (v.v[i] - mean) * rstd * mean_gh);
       if (base) {
-        const Values8 add = read8(base + col, left);
+        const Values8 add = read8<false>(base, col, a.cols);
 #pragma unroll
         for (int i = 0; i < 8; ++i) r.v[i] += add.v[i];
       }
@@ -300,7 +316,8 @@ void launch_layer_norm(const NormArgs &a, int dtype, int w_dtype, int cus, hipSt
     using T = decltype(x);
     using TW = decltype(w);
     const auto grid = [&](int rows_each, int per_cu) { return dim3((unsigned)std::min(((long)a.rows + rows_each - 1) / rows_each, (long)cus * per_cu)); };
-    if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm<T, TW, 64, 1>), grid(4, 8), dim3(256), 0, s, a);
+    if (a.cols < 8) hipLaunchKernelGGL((k_layer_norm<T, TW, 64, 1, true>), grid(4, 8), dim3(256), 0, s, a);
+    else if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm<T, TW, 64, 1>), grid(4, 8), dim3(256), 0, s, a);
     else if (a.cols <= 1024) hipLaunchKernelGGL((k_layer_norm<T, TW, 64, 2>), grid(4, 6), dim3(256), 0, s, a);
     else if (a.cols <= 2048) hipLaunchKernelGGL((k_layer_norm<T, TW, 256, 1>), grid(1, 8), dim3(256), 0, s, a);
     else if (a.cols <= 4096) hipLaunchKernelGGL((k_layer_norm<T, TW, 256, 2>), grid(1, 6), dim3(256), 0, s, a);
@@ -321,7 +338,8 @@ void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtyp
     using TW = decltype(w);
     const dim3 grid((unsigned)a.parts);
     if (a.parts) {
-      if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 1>), grid, dim3(512), 0, s, a);
+      if (a.cols < 8) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 1, true>), grid, dim3(512), 0, s, a);
+      else if (a.cols <= 512) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 1>), grid, dim3(512), 0, s, a);
       else if (a.cols <= 1024) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 64, 2>), grid, dim3(512), 0, s, a);
       else if (a.cols <= 2048) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 256, 1>), grid, dim3(256), 0, s, a);
       else if (a.cols <= 4096) hipLaunchKernelGGL((k_layer_norm_backward<T, TW, 256, 2>), grid, dim3(256), 0, s, a);

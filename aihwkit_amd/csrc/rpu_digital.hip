@@ -285,6 +285,7 @@ int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_
     if (hidden_dev) apart(y, written[1]);
     const DropDev d = drop_dev(drop);
     if (!rows) return;
+    if (plan_dev && !hidden_dev) throw RpuError("hidden is null.");
     const Gpu gpu(device_id);
     AdapterRowsArgs a{};
     a.in = {const_cast<void *>(x_dev), x_ld};

@@ -545,7 +545,8 @@ PyObject *adapter_forward_checked(PyObject *const *a, Py_ssize_t n) {
   c10::SmallVector<int64_t, 6> dims(c.x.t->sizes().begin(), c.x.t->sizes().end());
   dims.back() = c.w.out_size;
   if (!take_beside(a[6], c.x, dims, base) || !take_out(a[7], c.x, dims, y, out)) Py_RETURN_NONE;
-  if (truth(a[8])) hidden = per_row(c.x, c.w.rank);
+  const bool wanted = truth(a[8]);
+  if (wanted || g.plan.defined()) hidden = per_row(c.x, c.w.rank);
   const hipStream_t s = stream_of(*c.x.t);
   const int rows = (int)c.x.rows, device = c.x.t->device().index();
   const int32_t *ip = g.index ? static_cast<const int32_t *>(g.index->const_data_ptr()) : nullptr;
@@ -560,7 +561,7 @@ PyObject *adapter_forward_checked(PyObject *const *a, Py_ssize_t n) {
         return rpu_adapter_forward(&c.w, xp, c.x.ld, ip, pp, bytes, &d, bp, base.ld, yp, out.ld, hp, c.x.type, rows, device, s);
       },
       s, truth(a[12]));
-  return ok ? tuple_of(std::move(y), std::move(hidden), {}, 2) : nullptr;
+  return ok ? tuple_of(std::move(y), wanted ? std::move(hidden) : at::Tensor(), {}, 2) : nullptr;
 }
 PyObject *adapter_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&] { return adapter_forward_checked(a, n); });

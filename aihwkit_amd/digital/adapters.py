@@ -145,12 +145,13 @@ class LowRankAdapters:
         if out is None:
             out = torch.empty(shape, dtype=x_input.dtype, device=x_input.device)
         y = like(out, x_input, shape, "out", written=True)
-        hidden = torch.empty((*x_input.shape[:-1], self.rank), dtype=torch.float32, device=x_input.device) if return_hidden else None
+        hidden = torch.empty((*x_input.shape[:-1], self.rank), dtype=torch.float32, device=x_input.device) \
+            if return_hidden or plan else None
         launch(x_input.device, non_blocking,
                lambda device, stream: lib().rpu_adapter_forward(
                    C.byref(adapters), x.ptr, x.ld, None if plan else index.data_ptr(), plan._plan.data_ptr() if plan else None,
                    plan._bytes if plan else 0, C.byref(drop), add.ptr if add else None, add.ld if add else 0, y.ptr, y.ld,
-                   hidden.data_ptr() if return_hidden else None, DTYPES[x_input.dtype], x.rows, device, stream))
+                   hidden.data_ptr() if hidden is not None else None, DTYPES[x_input.dtype], x.rows, device, stream))
         return (out, hidden) if return_hidden else out
 
     def backward(self, d_input: torch.Tensor, x_input: torch.Tensor, rows: Union[torch.Tensor, AdapterRows], hidden: torch.Tensor,

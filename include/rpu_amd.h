@@ -793,7 +793,7 @@ int rpu_adapter_plan(const int32_t *index_dev, int rows, int n, void *plan_dev, 
 
 /* Rows up to which rpu_adapter_forward takes the index alone (plan_dev null): few rows are grouped within the call. */
 #define RPU_ADAPTER_FEW_ROWS 64
-/* hidden_dev [rows][rank], float, dense (null: not wanted).  y may be base, but no other operand. */
+/* hidden_dev [rows][rank], float, dense; without a plan it may be null (not wanted).  y may be base, but no other operand. */
 int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_ld, const int32_t *index_dev,
                         const void *plan_dev, size_t plan_bytes, const rpu_dropout_params *drop, const void *base_dev,
                         long base_ld, void *y_dev, long y_ld, float *hidden_dev, int dtype, int rows, int device_id,
