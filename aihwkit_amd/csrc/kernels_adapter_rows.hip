@@ -186,7 +186,7 @@ template <int NW, int PITCH> __device__ __forceinline__ f32x4 add_shares(const f
 
 // What a workgroup makes: the columns `piece` of the rows `group` of a tile.  Workgroups b, b + 8, b + 16, .. meet the same XCD: they take the
 // pieces of a group, one after another, then the groups of a tile.  (All rows of a piece first: 33.6 us instead of 32.4 for 8192 rows of
-// 2304 floats, 26.5 instead of 25.0 for 4608 rows of 4096 bf16.)
+// 2304 floats, 26.5 instead of 25.0 for 4096 rows of 4096 bf16.)
 struct Place {
   int4 tile;
   int group, piece;
@@ -211,8 +211,8 @@ template <typename T> __device__ __forceinline__ void read8_lds(Packed8<T> &v, c
 // that they fall out of step and some always load.  x and A are read along their rows and turned into the operands' order in
 // LDS of the wave's own: read in that order, 16 rows to every 16 lanes, they would take the address units four times as long.
 // The workgroups begin at different segments: all those of an adapter read the same A.
-// Bound by the reads of x, and the chain of loads before the first of them (tile, its rows, x).  9216 rows of 768 floats, rank 16: 11.2 us
-// (28 MB); 8192 rows of 2304 floats: 21.0 us (75 MB, 3.6 TB/s); 4608 rows of 4096 bf16, rank 64: 14.9 us, where every 16 rows read all
+// Bound by the reads of x, and the chain of loads before the first of them (tile, its rows, x).  8192 rows of 768 floats, rank 16: 11.2 us
+// (28 MB); 8192 rows of 2304 floats: 21.0 us (75 MB, 3.6 TB/s); 4096 rows of 4096 bf16, rank 64: 14.9 us, where every 16 rows read all
 // 0.5 MB of A from the L2, 150 MB.  With the stages of all waves in step (barriers around x in LDS) 15.5, 28 and 25 us; with 4 waves
 // 13.6, 33 and 25 us, with 16 17.7, 30 and 16.4 us, both before loads went out together.  Registers: three or four waves of a SIMD without
 // spills; six spill and take twice the time.
@@ -361,7 +361,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
 // UP_ROWS rows x UP_COLS columns of y.  Everything comes and goes along the rows of its matrix and through LDS: hidden, in the form
 // of the matrix instructions, for all waves; B, 16 columns of the wave at a time; the products, to which base is added as they are
 // stored.  Loads in the lanes' order of the products, 16 rows to every 16 lanes, take the address units four times as long.
-// Bound by base and y: 8192 rows of 2304 floats, rank 16, in 30.3 us (151 MB, 5.0 TB/s; a copy of that size 5.4), 4608 rows of 4096
+// Bound by base and y: 8192 rows of 2304 floats, rank 16, in 30.3 us (151 MB, 5.0 TB/s; a copy of that size 5.4), 4096 rows of 4096
 // bf16, rank 64, in 24.7 us.  16 x 256 took 32.0 and 25.0 us, 32 x 128 34.5 and 27.7 us where 16 x 128 took 32.4 and 25.0.
 constexpr int UP_ROWS = 16, UP_COLS = 128, UP_MT = UP_ROWS / 16, UP_PITCH = UP_COLS + 4, UP_T = UP_COLS / 16 / UP_WAVES;
 template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __global__ __launch_bounds__(64 * UP_WAVES) void k_adapter_up(AdapterRowsArgs a) {

@@ -438,6 +438,34 @@ def test_adapters_forward_and_backward(rows, x, d, rank, n, dtype, w_dtype):
     assert all(torch.equal(p, q) for p, q in zip(s.step(), again))            # sums in a fixed order
 
 
+@pytest.mark.parametrize("dtype, w_dtype", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("rows, x, d, rank, n", [
+    (70, 7, 300, 128, 2), (70, 300, 5, 64, 3), (90, 3, 2, 20, 2), (66, 1, 8, 16, 1), (80, 8, 1, 33, 2), (64, 6, 700, 16, 2),  # fewer than 8 columns
+    (40, 5003, 4100, 16, 2), (20, 4099, 2050, 128, 1), (65, 2050, 1111, 40, 2),                                            # many segments
+    (70000, 9, 10, 3, 3), (66000, 12, 5, 17, 400),                                                                         # long lists of rows
+])
+def test_adapters_of_extreme_sizes(rows, x, d, rank, n, dtype, w_dtype):
+    s = Set(rows, x, d, rank, n, dtype, w_dtype, p=0.0 if x % 2 else 0.3)
+    results = s.step()
+    s.check(results)
+    if rows <= 64:
+        close(s.forward(), *(t[0] for t in s.reference()))
+    assert all(torch.equal(p, q) for p, q in zip(s.step(), results))
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("rows", [9, 200])
+@pytest.mark.parametrize("d", [5, 200])
+def test_base_goes_through_rows_without_adapter_bit_by_bit(dtype, rows, d):
+    s = Set(rows, 24, d, 4, 2, dtype, dtype, index=(torch.arange(rows, device="cuda") % 3).to(torch.int32))
+    none = s.index == 2
+    s.base[none] = torch.tensor([-0.0, 0.0, float("inf"), -1.5], dtype=dtype, device="cuda").repeat(d)[:d]
+    bits = {2: torch.int16, 4: torch.int32}[dtype.itemsize]
+    for rows_of in (s.index, digital.AdapterRows(s.index, 2)):
+        y = s.forward(rows_of)
+        assert torch.equal(y[none].view(bits), s.base[none].view(bits))
+
+
 @pytest.mark.parametrize("rows", [1, 15, 64, 65, 500])
 def test_rows_without_adapter(rows):
     """Numbers outside of 0 .. n - 1 mean none: base goes through, and nothing of such a row reaches a gradient."""
