@@ -328,6 +328,44 @@ template <typename T> __device__ __forceinline__ void write8(T *p, const Values8
     if (i < count) p[i] = (T)r.v[i];
 }
 
+// ---- products of 16-bit operands with floats ----------------------------------------------------------------------------
+// 32 terms of 16 x 16 results
+template <typename T> __device__ __forceinline__ f32x4 multiply32(u32x4 a, u32x4 b, f32x4 c) {
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// what a part leaves of a value; nothing of an infinity
+__device__ __forceinline__ float rest_of(float v, float part) { return __builtin_isfinite(v) ? v - part : 0.0f; }
+// Two floats as three bf16 each, all of their 24 bits.  Cut off, not rounded: the largest float stays finite.
+__device__ __forceinline__ void parts_of(float a, float b, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    part[k] = (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u);
+    a = rest_of(a, __uint_as_float(part[k] << 16));
+    b = rest_of(b, __uint_as_float(part[k] & 0xffff0000u));
+  }
+}
+// as two halves each, 22 bits
+__device__ __forceinline__ void halves_of(float a, float b, uint32_t (&part)[2]) {
+  part[0] = pack2(a, b, _Float16{});
+  const f16x2 r = __builtin_bit_cast(f16x2, part[0]);
+  part[1] = pack2(rest_of(a, (float)r.x), rest_of(b, (float)r.y), _Float16{});
+}
+// Power of two that floats are multiplied by before halves_of, from their largest finite magnitude: they may leave the range of halves, the
+// largest becomes 2^14 .. 2^15.  (Numbers of less than 2^-97 in steps of 2^-135.)
+__device__ __forceinline__ float lift_of(float most) {
+  const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased
+  return __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);
+}
+// the largest finite magnitude
+__device__ __forceinline__ float most_of(f32x4 v, float most = 0.0f) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) most = __builtin_isfinite(v[i]) ? fmaxf(most, fabsf(v[i])) : most;
+  return most;
+}
+// 1 over a power of two
+__device__ __forceinline__ float inverse_of(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 // the first `count` of 4 or 8 values
 template <typename T, int N> __device__ __forceinline__ void store_first(T *p, const float (&v)[N], int count) {
   static_assert(N == 4 || N == 8);

@@ -40,8 +40,8 @@ __device__ __forceinline__ int4 plan_piece(int i, const int *firsts, const int *
 }
 
 // Few adapters (a byte holds a key) and rows that LDS holds the keys of: one trip to memory for the index, everything else in
-// LDS.
-constexpr int PLAN_LDS_ROWS = 65536, PLAN_LDS_KEYS = 256;
+// LDS.  A chain of latencies in one workgroup: 6 us for 256 rows, 9 for 8192, 75 for 100000, for which the other kernel takes 206.
+constexpr int PLAN_LDS_ROWS = 131072, PLAN_LDS_KEYS = 256;
 __global__ __launch_bounds__(PLAN_THREADS) void k_adapter_plan_lds(const int *index, int *plan, AdapterPlan p) {
   __shared__ uint8_t key_of[PLAN_LDS_ROWS];
   __shared__ int hist[PLAN_WAVES][PLAN_LDS_KEYS], sums[4][4], firsts[4][PLAN_LDS_KEYS + 1]; // of rows, tiles, chunks, slots
@@ -277,10 +277,11 @@ constexpr int GRAD_WAVES = 4;
 
 // 128 columns of dA (of x, against up) or of dB (of d, against scale hidden).  A wave takes 16 rows of its chunk at a time; lane
 // % 16 reads eight columns of four rows, 16 bytes beside those of its neighbours at a time, and product j of a row takes its column j.
-// Bound by the reads of x and d, which no other workgroup reads, and the products on the fp32 instructions: 8192 rows of 768 and 2304 floats,
-// rank 16, in 25.7 us (101 MB, 3.9 TB/s).  One group at a time, each waited for, 35 us; the next one under way with a branch around
-// every load 33 us.
-template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bounds__(64 * GRAD_WAVES, RT == 1 ? 3 : 1) void k_adapter_grads(AdapterGradArgs a) {
+// Rows of float: products on the fp32 instructions, bound by the reads of x and d up to rank 16 (8192 rows of 768 and 2304 columns in 25.7
+// us, 101 MB, 3.9 TB/s; one group at a time, each waited for, 35 us), by the products beyond: a backward pass of those rows takes 75 us
+// with rank 16, 263 with 64, 475 with 128.  16-bit rows: their numbers as they are on the 16-bit instructions, the factors in parts.  The
+// same backward pass in bf16 takes 48.6 us with rank 16, 102 with 64, 186 with 128; on the fp32 instructions 53.8, 193 and 348.
+template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bounds__(64 * GRAD_WAVES, RT == 1 ? 3 : sizeof(T) == 2 ? 2 : 1) void k_adapter_grads(AdapterGradArgs a) {
   __shared__ float sums[32 * RT][64];
   const int4 chunk = reinterpret_cast<const int4 *>(a.plan + a.p.chunks)[blockIdx.x];
   const int adapter = chunk.x, count = chunk.z;
@@ -299,27 +300,90 @@ template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bound
   const int col = c0 + EACH * lm, rank0 = 16 * RT * (int)blockIdx.z;
   f32x4 acc[8][RT] = {};
   // the next group is under way, and the rows of the one after it
+  constexpr bool NARROW = sizeof(T) == 2;
+  constexpr int OWN = NARROW ? 8 : 4, GROUP = 4 * OWN; // rows of a lane, of a group
   struct Group {
-    Packed16<T> x[4][PIECES];
-    float u[4][RT];
+    Packed16<T> x[OWN][PIECES];
+    float u[OWN][RT];
   };
-  const auto find = [&](int (&row)[4], int g) {
+  const auto find = [&](int (&row)[OWN], int g) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) row[i] = order[min(16 * g + 4 * kg + i, count - 1)]; // rows beyond the last repeat it
+    for (int i = 0; i < OWN; ++i) row[i] = order[min(GROUP * g + OWN * kg + i, count - 1)]; // rows beyond the last repeat it
   };
-  const auto fetch = [&](Group &next, const int (&row)[4]) {
+  const auto fetch = [&](Group &next, const int (&row)[OWN]) {
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
+    for (int i = 0; i < OWN; ++i) {
 #pragma unroll
       for (int h = 0; h < PIECES; ++h) next.x[i][h] = ahead16<SHORT>(static_cast<const T *>(m.p) + (long)row[i] * m.ld, col + STEP * h, width);
 #pragma unroll
       for (int q = 0; q < RT; ++q) next.u[i][q] = factor[(long)row[i] * a.rank + min(rank0 + 16 * q + lm, a.rank - 1)];
     }
   };
-  const auto multiply = [&](Group &here, const int (&row)[4], int g) {
+  // 16-bit rows: 32 terms to a product, the lane's 8 rows x 8 columns turned in its registers; the factors in parts of the rows' type
+  const auto multiply_narrow = [&](Group &here, const int (&row)[OWN], int g) {
+    u32x4 v[8];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const bool valid = 16 * g + 4 * kg + i < count;
+    for (int i = 0; i < 8; i += 2) {
+#pragma unroll
+      for (int h = i; h < i + 2; ++h) {
+        trim16(here.x[h][0], col, width);
+        uint32_t kept = drop ? drop_kept(a.drop, call, (uint32_t)row[h], (uint32_t)col / 8u) : 0xffu;
+        kept = GROUP * g + OWN * kg + h < count ? kept : 0u;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) here.x[h][0].q[w] &= (kept & (1u << 2 * w) ? 0xffffu : 0u) | (kept & (2u << 2 * w) ? 0xffff0000u : 0u);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const uint32_t x0 = here.x[i][0].q[j / 2], x1 = here.x[i + 1][0].q[j / 2];
+        v[j][i / 2] = j & 1 ? x0 >> 16 | (x1 & 0xffff0000u) : (x0 & 0xffffu) | x1 << 16;
+      }
+    }
+    const float factors = drop ? a.drop.scale : scale;
+#pragma unroll
+    for (int q = 0; q < RT; ++q) {
+      float u[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) u[i] = GROUP * g + OWN * kg + i < count && rank0 + 16 * q + lm < a.rank ? here.u[i][q] * factors : 0.0f;
+      u32x4 part[3];
+      if constexpr (__is_same(T, __bf16)) {
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t p[3];
+          parts_of(u[2 * w], u[2 * w + 1], p);
+#pragma unroll
+          for (int k = 0; k < 3; ++k) part[k][w] = p[k];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+          for (int k = 0; k < 3; ++k) acc[j][q] = multiply32<T>(v[j], part[k], acc[j][q]);
+      } else {
+        float most = 0.0f; // of the rank's factors in this group
+#pragma unroll
+        for (int i = 0; i < 8; ++i) most = __builtin_isfinite(u[i]) ? fmaxf(most, fabsf(u[i])) : most;
+        most = fmaxf(most, __shfl_xor(most, 16));
+        most = fmaxf(most, __shfl_xor(most, 32));
+        const float lift = lift_of(most), back = inverse_of(lift);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          uint32_t p[2];
+          halves_of(u[2 * w] * lift, u[2 * w + 1] * lift, p);
+          part[0][w] = p[0];
+          part[1][w] = p[1];
+        }
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const f32x4 sum = multiply32<T>(v[j], part[1], multiply32<T>(v[j], part[0], f32x4{}));
+#pragma unroll
+          for (int i = 0; i < 4; ++i) acc[j][q][i] = fmaf(sum[i], back, acc[j][q][i]);
+        }
+      }
+    }
+  };
+  const auto multiply = [&](Group &here, const int (&row)[OWN], int g) {
+#pragma unroll
+    for (int i = 0; i < OWN; ++i) {
+      const bool valid = GROUP * g + OWN * kg + i < count;
       Values8 x;
 #pragma unroll
       for (int h = 0; h < PIECES; ++h) {
@@ -350,24 +414,38 @@ template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bound
       }
     }
   };
-  const int groups = (count + 15) / 16;
-  int rows[2][4], last[4];
-  Group group[2];
-  if (wave < groups) {
-    find(rows[0], wave);
-    fetch(group[0], rows[0]);
-    find(rows[1], wave + GRAD_WAVES);
-  }
-  const auto step = [&](Group &here, Group &next, int (&row)[4], int (&ahead)[4], int g) {
-    if (g + GRAD_WAVES < groups) fetch(next, ahead);
+  const int groups = (count + GROUP - 1) / GROUP;
+  if constexpr (NARROW) { // twice the rows to a group: the next one's would leave the registers
+    int row[OWN];
+    if (wave < groups) find(row, wave);
+    for (int g = wave; g < groups; g += GRAD_WAVES) {
+      Group here;
+      fetch(here, row);
+      int last[OWN];
 #pragma unroll
-    for (int i = 0; i < 4; ++i) last[i] = row[i];
-    if (g + 2 * GRAD_WAVES < groups) find(row, g + 2 * GRAD_WAVES);
-    multiply(here, last, g);
-  };
-  for (int g = wave; g < groups; g += 2 * GRAD_WAVES) {
-    step(group[0], group[1], rows[0], rows[1], g);
-    if (g + GRAD_WAVES < groups) step(group[1], group[0], rows[1], rows[0], g + GRAD_WAVES);
+      for (int i = 0; i < OWN; ++i) last[i] = row[i];
+      if (g + GRAD_WAVES < groups) find(row, g + GRAD_WAVES);
+      multiply_narrow(here, last, g);
+    }
+  } else {
+    int rows[2][OWN], last[OWN];
+    Group group[2];
+    if (wave < groups) {
+      find(rows[0], wave);
+      fetch(group[0], rows[0]);
+      find(rows[1], wave + GRAD_WAVES);
+    }
+    const auto step = [&](Group &here, Group &next, int (&row)[OWN], int (&ahead)[OWN], int g) {
+      if (g + GRAD_WAVES < groups) fetch(next, ahead);
+#pragma unroll
+      for (int i = 0; i < OWN; ++i) last[i] = row[i];
+      if (g + 2 * GRAD_WAVES < groups) find(row, g + 2 * GRAD_WAVES);
+      multiply(here, last, g);
+    };
+    for (int g = wave; g < groups; g += 2 * GRAD_WAVES) {
+      step(group[0], group[1], rows[0], rows[1], g);
+      if (g + GRAD_WAVES < groups) step(group[1], group[0], rows[1], rows[0], g + GRAD_WAVES);
+    }
   }
   for (int from = 0; from < GRAD_WAVES; ++from) { // the waves' sums, added in their order
     if (wave == from) {
@@ -497,7 +575,7 @@ void launch_adapter_grads(const AdapterGradArgs &a, int dtype, int w_dtype, int 
       hipLaunchKernelGGL((k_adapter_grads<T, TW, 1, true>), dim3((unsigned)a.p.max_chunks, slices, (unsigned)(a.rank + 15) / 16), dim3(64 * GRAD_WAVES), 0, s, a);
     else if (a.rows)
       with_rank_tiles(a.rank, [&](auto rt) {
-        constexpr int RT = decltype(rt)::value, AT_ONCE = RT < 4 ? RT : 4; // more sums than that of 64 ranks leave the registers
+        constexpr int RT = decltype(rt)::value, MOST = sizeof(T) == 2 ? 2 : 4, AT_ONCE = RT < MOST ? RT : MOST; // more sums, or rows under way, leave the registers
         hipLaunchKernelGGL((k_adapter_grads<T, TW, AT_ONCE, false>), dim3((unsigned)a.p.max_chunks, slices, RT / AT_ONCE), dim3(64 * GRAD_WAVES), 0, s, a);
       });
     hipLaunchKernelGGL(k_adapter_join<TW>, join, dim3(256), 0, s, a);

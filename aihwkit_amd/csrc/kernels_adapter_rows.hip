@@ -11,7 +11,6 @@ namespace rpu_amd {
 namespace {
 
 // ---- eight terms, or four ranks, of both operands of a product, as the matrix instructions take them ------------------
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // rows of float: products on the fp32 instructions, whatever the weights are stored as
 template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) == 2> struct Pipe {
@@ -68,41 +67,28 @@ template <typename T> struct Pipe<T, T, true> {
     u32x4 upper; // the first two parts
     u32x2 third;
   };
-  static __device__ __forceinline__ f32x4 multiply(u32x4 a, u32x4 b, f32x4 c) {
-    if constexpr (__is_same(T, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-    else return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-  }
-  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) { return multiply(w.q, x.q, c); }
+  static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) { return multiply32<T>(w.q, x.q, c); }
   static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x.q[i] &= (kept & (1u << 2 * i) ? 0xffffu : 0u) | (kept & (2u << 2 * i) ? 0xffff0000u : 0u);
   }
-  static __device__ __forceinline__ uint32_t cut(float a, float b) { return (__float_as_uint(a) >> 16) | (__float_as_uint(b) & 0xffff0000u); }
-  static __device__ __forceinline__ float rest(float v, float part) { return __builtin_isfinite(v) ? v - part : 0.0f; }
-  // Power of two that hidden of a row is multiplied by, from its largest finite magnitude: hidden may leave the range of halves, the largest
-  // becomes 2^14 .. 2^15.  (Rows of less than 2^-97 in steps of 2^-135.)
-  static __device__ __forceinline__ float lift(float most) {
-    if constexpr (__is_same(T, __bf16)) return 1.0f;
-    const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased
-    return __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);
-  }
+  static __device__ __forceinline__ float lift(float most) { return __is_same(T, __bf16) ? 1.0f : lift_of(most); }
   static __device__ __forceinline__ V split(f32x4 v, float lift) {
     V to = {};
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const float a = v[2 * h] * lift, b = v[2 * h + 1] * lift;
-      if constexpr (__is_same(T, __bf16)) { // cut off, not rounded: the largest float stays finite
-        const uint32_t high = cut(a, b);
-        const float a1 = rest(a, __uint_as_float(high << 16)), b1 = rest(b, __uint_as_float(high & 0xffff0000u));
-        const uint32_t mid = cut(a1, b1);
-        to.upper[h] = high;
-        to.upper[2 + h] = mid;
-        to.third[h] = cut(a1 - __uint_as_float(mid << 16), b1 - __uint_as_float(mid & 0xffff0000u)); // eight bits are left
+      if constexpr (__is_same(T, __bf16)) {
+        uint32_t part[3];
+        parts_of(a, b, part);
+        to.upper[h] = part[0];
+        to.upper[2 + h] = part[1];
+        to.third[h] = part[2];
       } else {
-        const uint32_t high = pack2(a, b, T{});
-        const f16x2 r = __builtin_bit_cast(f16x2, high);
-        to.upper[h] = high;
-        to.upper[2 + h] = pack2(rest(a, (float)r.x), rest(b, (float)r.y), T{});
+        uint32_t part[2];
+        halves_of(a, b, part);
+        to.upper[h] = part[0];
+        to.upper[2 + h] = part[1];
       }
     }
     return to;
@@ -116,13 +102,13 @@ template <typename T> struct Pipe<T, T, true> {
   }
   template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT], const V (&v)[RT], f32x4 c) {
 #pragma unroll
-    for (int q = 0; q < RT; ++q) c = multiply(u32x4{w[q][0], w[q][1], w[q][0], w[q][1]}, v[q].upper, c);
+    for (int q = 0; q < RT; ++q) c = multiply32<T>(u32x4{w[q][0], w[q][1], w[q][0], w[q][1]}, v[q].upper, c);
     if constexpr (__is_same(T, __bf16)) { // the third parts of two tiles of ranks at a time
 #pragma unroll
       for (int q = 0; q < RT; q += 2) {
         const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q] : R{};
         const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
-        c = multiply(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
+        c = multiply32<T>(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
       }
     }
     return c;
@@ -140,14 +126,6 @@ template <typename P, typename W> __device__ __forceinline__ typename P::R load_
   for (int i = 0; i < 4; ++i) P::put(r, i, v[i], (uint32_t)((rank + i - ranks) >> 31));
   return r;
 }
-// the largest finite magnitude
-__device__ __forceinline__ float most_of(f32x4 v, float most = 0.0f) {
-#pragma unroll
-  for (int i = 0; i < 4; ++i) most = __builtin_isfinite(v[i]) ? fmaxf(most, fabsf(v[i])) : most;
-  return most;
-}
-// 1 over a power of two
-__device__ __forceinline__ float inverse_of(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 template <typename T> __device__ __forceinline__ void clear_unless(Packed8<T> &r, bool kept) {
   const uint32_t mask = kept ? ~0u : 0u;
   if constexpr (sizeof(T) == 4) {
@@ -372,7 +350,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   __shared__ float products[UP_ROWS][UP_PITCH];
   __shared__ typename P::V hidden_of[UP_ROWS][QUADS + 1];
   __shared__ float back_of[UP_ROWS];
-  constexpr bool STAGED = RT > 1; // the 16 columns of a rank tile lie side by side anyway
+  constexpr bool STAGED = RT > 1 || !FULL; // the 16 columns of one full tile of ranks lie side by side anyway
   __shared__ __align__(16) char weights[STAGED ? UP_WAVES : 1][STAGED ? 16 * (W_PITCH + 16) : 16];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, lm = lane & 15, kg = lane >> 4;
   const auto [tile, group, piece] = place_of(a, ADAPTER_TILE_ROWS / UP_ROWS, (a.out_size + UP_COLS - 1) / UP_COLS);
@@ -494,7 +472,8 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   }
 }
 
-// Up to ADAPTER_FEW_ROWS rows by their index alone: workgroup (i, s) makes the columns of slice s for all rows of the adapter of row
+// Up to ADAPTER_FEW_ROWS rows by their index alone (64 rows of 4096 bf16 for 8 adapters of rank 16 in 12.4 us; a plan and the two kernels
+// above take 16.6): workgroup (i, s) makes the columns of slice s for all rows of the adapter of row
 // i, unless an earlier row has it, and the hidden that it needs for them.
 template <typename T, typename TW, int RT, bool FULL, bool SHORT> __global__ __launch_bounds__(64 * WAVES) void k_adapter_few(AdapterRowsArgs a) {
   using P = Pipe<T, TW>;
@@ -615,7 +594,8 @@ void launch_adapter_rows(const AdapterRowsArgs &args, int dtype, int w_dtype, in
     with_sizes(a.rank, std::min(a.in_size, a.out_size), [&](auto rt, auto full, auto small) {
       constexpr int RT = decltype(rt)::value, FULL = decltype(full)::value, SHORT = decltype(small)::value;
       if (!a.plan) {
-        // rows that leave CUs idle share their columns among several workgroups, each of which makes hidden for itself
+        // rows that leave CUs idle share their columns among several workgroups, each of which makes hidden for itself: 8 rows of 768
+        // and 2304 columns take 6.3 us, with a workgroup to an adapter 11.3; 64 rows 7.7 and 11.9
         const int units = (a.out_size + 31) / 32, pieces = std::max(1, cus / std::max(a.rows, 1));
         a.units_each = ((units + pieces - 1) / pieces + WAVES - 1) / WAVES * WAVES;
         const dim3 grid((unsigned)a.rows, (unsigned)((units + a.units_each - 1) / a.units_each));

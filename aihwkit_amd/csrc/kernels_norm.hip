@@ -33,7 +33,8 @@ template <bool SHORT, typename T> __device__ __forceinline__ Values8 parameter8(
   return r;
 }
 
-// Rows of up to 8 * TPR * V columns, TPR threads to a row; SHORT: of fewer than 8.
+// Rows of up to 8 * TPR * V columns, TPR threads to a row; SHORT: of fewer than 8.  Bound by memory: 16384 x 1024 bf16 in 11.7 us (67 MB,
+// 5.7 TB/s); one row of 768 floats in 6.7 us, a launch.
 template <typename T, typename TW, int TPR, int V, bool SHORT = false> __global__ __launch_bounds__(TPR > 256 ? TPR : 256) void k_layer_norm(NormArgs a) {
   constexpr int THREADS = TPR > 256 ? TPR : 256, ROWS = THREADS / TPR;
   __shared__ float room[THREADS / 64];
@@ -130,7 +131,8 @@ template <typename T, typename TW> __global__ __launch_bounds__(LONG) void k_lay
 
 constexpr int backward_threads(int threads_of_a_row) { return threads_of_a_row == 64 ? 512 : threads_of_a_row; }
 // Backward pass of rows of up to 8 * TPR * V columns.  A workgroup adds d and d h of its rows up in registers and leaves the
-// sums in part[workgroup]; k_layer_norm_join adds those.
+// sums in part[workgroup]; k_layer_norm_join adds those.  Bound by memory: 8192 x 768 floats with a base in 20.9 us (101 MB, 4.8 TB/s), and
+// 3.9 for the join, 23.5 in a row.  The next row's loads under way while one is worked on took 21.4: the waves of a CU suffice.
 template <typename T, typename TW, int TPR, int V, bool SHORT = false>
 __global__ __launch_bounds__(backward_threads(TPR)) void k_layer_norm_backward(NormBackwardArgs a) {
   constexpr int THREADS = backward_threads(TPR), ROWS = THREADS / TPR;
@@ -327,11 +329,16 @@ void launch_layer_norm(const NormArgs &a, int dtype, int w_dtype, int cus, hipSt
   });
 }
 
+constexpr long MOST_PARTS = 1024; // that scratch sizes are for
+
 int layer_norm_parts(int rows, int cols, int cus) {
-  // A workgroup to a CU, two where a workgroup is but four waves: 1037 rows of 1537 halves take 12.1 us with one, 10.2 with two, 8192 rows
-  // of 768 floats, in workgroups of eight waves, 20.8 and 23.7.  Two rows at least, so that the sums' parts stay the lesser traffic.
+  // Workgroups of a CU.  Four waves each (1025 .. 4096 columns): 8192 rows of 1537 halves take 53 us with one, 33 with two, 28 with three,
+  // 27 with four; of 4096 bf16 68, 46, 43 and 52.  Eight waves with rows of 513 .. 1024 columns in many registers: 16384 rows of 768
+  // bf16 22.8 with one, 26.8 with two; shorter rows: 50000 of 64 floats 33.6 and 25.6, 16384 of 512 bf16 16.0 and 15.5.  Sixteen waves:
+  // 4096 rows of 5000 halves 49.3 and 54.2.  Two rows each at least, so that the sums' parts stay the lesser traffic.
+  const int per_cu = cols <= 512 ? 2 : cols <= 1024 ? 1 : cols <= 4096 ? 3 : 1;
   const long groups = ((long)rows + backward_rows(cols) - 1) / backward_rows(cols);
-  return (int)std::min((groups + 1) / 2, (long)cus * (cols > 1024 && cols <= 4096 ? 2 : 1));
+  return (int)std::min((groups + 1) / 2, std::min((long)cus * per_cu, MOST_PARTS));
 }
 
 void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtype, hipStream_t s) {

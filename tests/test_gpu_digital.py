@@ -442,7 +442,7 @@ def test_adapters_forward_and_backward(rows, x, d, rank, n, dtype, w_dtype):
 @pytest.mark.parametrize("rows, x, d, rank, n", [
     (70, 7, 300, 128, 2), (70, 300, 5, 64, 3), (90, 3, 2, 20, 2), (66, 1, 8, 16, 1), (80, 8, 1, 33, 2), (64, 6, 700, 16, 2),  # fewer than 8 columns
     (40, 5003, 4100, 16, 2), (20, 4099, 2050, 128, 1), (65, 2050, 1111, 40, 2),                                            # many segments
-    (70000, 9, 10, 3, 3), (66000, 12, 5, 17, 400),                                                                         # long lists of rows
+    (70000, 9, 10, 3, 3), (140000, 4, 3, 2, 2), (66000, 12, 5, 17, 400),                                                   # long lists of rows
 ])
 def test_adapters_of_extreme_sizes(rows, x, d, rank, n, dtype, w_dtype):
     s = Set(rows, x, d, rank, n, dtype, w_dtype, p=0.0 if x % 2 else 0.3)
