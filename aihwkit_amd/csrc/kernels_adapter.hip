@@ -535,7 +535,9 @@ AdapterPlan adapter_plan(int rows, int n) {
   AdapterPlan p{};
   p.rows = rows;
   p.n = n;
-  p.chunk_rows = 64;
+  // A group of rows for every wave of the gradients' workgroups at least (128 rows; with 64 the backward pass of 1024 bf16 rows, rank 64, takes
+  // 44.8 us instead of 38.0, of 512 rows of floats 29.7 and 27.8), and few enough chunks that their sums stay the lesser traffic.
+  p.chunk_rows = 128;
   while (p.chunk_rows < 1024 && rows / p.chunk_rows > 32) p.chunk_rows *= 2;
   // every group of rows but for one may end with a piece that is not full
   p.max_tiles = (int)std::min<long>(rows, ((long)rows + ADAPTER_TILE_ROWS - 1) / ADAPTER_TILE_ROWS + std::min(n, rows));
