@@ -32,18 +32,6 @@ struct DropoutArgs {
   int rows, cols;
   DropDev drop;
 };
-// types of rows and adapter weights, and a number, as arguments of a generic function
-template <typename F> void with_adapter_types(int dtype, int w_dtype, F &&f) {
-  if (dtype == RPU_BF16) f(__bf16{}, __bf16{});
-  else if (dtype == RPU_F16) f(_Float16{}, _Float16{});
-  else if (w_dtype == RPU_F32) f(float{}, float{});
-  else if (w_dtype == RPU_F16) f(float{}, _Float16{});
-  else f(float{}, __bf16{});
-}
-template <int V> struct Int {
-  static constexpr int value = V;
-};
-
 void launch_dropout(const DropoutArgs &a, int dtype, int cus, hipStream_t s);
 
 struct NormArgs {
@@ -327,6 +315,18 @@ template <typename T> __device__ __forceinline__ void write8(T *p, const Values8
   for (int i = 0; i < 8; ++i)
     if (i < count) p[i] = (T)r.v[i];
 }
+
+// types of rows and adapter weights, and a number, as arguments of a generic function
+template <typename F> void with_adapter_types(int dtype, int w_dtype, F &&f) {
+  if (dtype == RPU_BF16) f(__bf16{}, __bf16{});
+  else if (dtype == RPU_F16) f(_Float16{}, _Float16{});
+  else if (w_dtype == RPU_F32) f(float{}, float{});
+  else if (w_dtype == RPU_F16) f(float{}, _Float16{});
+  else f(float{}, __bf16{});
+}
+template <int V> struct Int {
+  static constexpr int value = V;
+};
 
 // ---- products of 16-bit operands with floats ----------------------------------------------------------------------------
 // 32 terms of 16 x 16 results

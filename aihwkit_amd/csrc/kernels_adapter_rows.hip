@@ -1,6 +1,6 @@
 // The rows of low-rank adapters through their two thin products (kernels_adapter.hip says what is computed):
 //   k_adapter_down  hidden = A x of 16 rows, the terms shared by the waves of a workgroup
-//   k_adapter_up    y = base + s B hidden of up to 64 rows, every wave on columns of its own
+//   k_adapter_up    y = base + s B hidden of 16 rows and 128 columns, every wave on columns of its own
 //   k_adapter_few   both in one launch, for few rows
 // The backward pass is the same with d for x, and the matrices turned (k_adapter_turn).
 #include "digital.h"

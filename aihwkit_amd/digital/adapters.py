@@ -48,7 +48,8 @@ class LowRankAdapters:
     ``a`` [n, rank, in_size], ``b`` [n, out_size, rank] (float32, float16 or bfloat16) and ``scale`` [n] (float32; None: ones)
     are the caller's tensors, dense and on one GPU, and are used as they are at every call: an optimizer may write them, or they may be replaced
     by others of their shape.  Beside 16-bit rows the matrices are of the rows' type.  An adapter of a smaller rank than the
-    others has zeros in the rest."""
+    others has zeros in the rest.  Infinities and NaN of a row stay with it, and in gradients with its adapter; beside 16-bit
+    rows a product with an infinity may be NaN where the formula has an infinity."""
 
     def __init__(self, a: torch.Tensor, b: torch.Tensor, scale: Optional[torch.Tensor] = None):
         for tensor, what in ((a, "a"), (b, "b")):
