@@ -346,24 +346,53 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&part)[3]) 
     b = rest_of(b, __uint_as_float(part[k] & 0xffff0000u));
   }
 }
-// as two halves each, 22 bits
-__device__ __forceinline__ void halves_of(float a, float b, uint32_t (&part)[2]) {
-  part[0] = pack2(a, b, _Float16{});
-  const f16x2 r = __builtin_bit_cast(f16x2, part[0]);
-  part[1] = pack2(rest_of(a, (float)r.x), rest_of(b, (float)r.y), _Float16{});
+// As three halves each, cut off too: of floats that lift_of was found from all bits of those down to 2^-16 of the largest.  a and b become what is
+// left of the others.  (An infinity leaves some finite number: where that is added, the infinity decides.)
+__device__ __forceinline__ void halves_of(float &a, float &b, uint32_t (&part)[3]) {
+#pragma unroll
+  for (int k = 0; k < 3; ++k) {
+    part[k] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+    const f16x2 r = __builtin_bit_cast(f16x2, part[k]);
+    a -= (float)r.x;
+    b -= (float)r.y;
+    if (!k) { // less than the 2^5 of the last bit, or a NaN
+      a = fmaxf(a, -32.0f);
+      b = fmaxf(b, -32.0f);
+    }
+  }
 }
-// Power of two that floats are multiplied by before halves_of, from their largest finite magnitude: they may leave the range of halves, the
+// Power of two that floats are multiplied by before halves_of, from their largest magnitude: they may leave the range of halves, the
 // largest becomes 2^14 .. 2^15.  (Numbers of less than 2^-97 in steps of 2^-135.)
+// What halves_of leaves is multiplied in another round, with a lift of its own, until nothing is left: a small value beside a large one that
+// meets a zero keeps its 24 bits.  A round leaves less than 2^-38 of the largest value, so that there are at most seven; of values of like
+// size there is one.
+constexpr int HALF_ROUNDS = 8;
 __device__ __forceinline__ float lift_of(float most) {
   const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased
   return __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);
 }
-// the largest finite magnitude
+// the largest magnitude; of an infinity or a NaN, beside which nothing else counts, the largest number's
 __device__ __forceinline__ float most_of(f32x4 v, float most = 0.0f) {
 #pragma unroll
-  for (int i = 0; i < 4; ++i) most = __builtin_isfinite(v[i]) ? fmaxf(most, fabsf(v[i])) : most;
+  for (int i = 0; i < 4; ++i) most = fmaxf(most, fminf(fabsf(v[i]), 0x1.fffffep127f));
   return most;
 }
+// the largest of N = 4, 8, 16, 32 neighbouring lanes, in all of them; up to 16 without a trip through LDS
+template <int N> __device__ __forceinline__ float most_of_lanes(float most) {
+  static_assert(N == 4 || N == 8 || N == 16 || N == 32);
+  const auto with = [&](auto ctrl) { // lanes of a row of 16 exchanged
+    const int v = __float_as_int(most);
+    most = fmaxf(most, __int_as_float(__builtin_amdgcn_update_dpp(v, v, decltype(ctrl)::value, 0xf, 0xf, true)));
+  };
+  with(Int<0xb1>{});                   // 1 0 3 2 of every four
+  with(Int<0x4e>{});                   // 2 3 0 1
+  if (N > 4) with(Int<0x141>{});       // eight from behind
+  if (N > 8) with(Int<0x140>{});       // sixteen from behind
+  if (N > 16) most = fmaxf(most, __shfl_xor(most, 16));
+  return most;
+}
+// something is left that a further round can take (less than 2^-120 is not)
+__device__ __forceinline__ bool is_left(float most) { return most >= 0x1p-120f; }
 // 1 over a power of two
 __device__ __forceinline__ float inverse_of(float power) { return __uint_as_float((254u << 23) - __float_as_uint(power)); }
 // the first `count` of 4 or 8 values

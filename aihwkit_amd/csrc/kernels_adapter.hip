@@ -319,7 +319,8 @@ template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bound
       for (int q = 0; q < RT; ++q) next.u[i][q] = factor[(long)row[i] * a.rank + min(rank0 + 16 * q + lm, a.rank - 1)];
     }
   };
-  // 16-bit rows: 32 terms to a product, the lane's 8 rows x 8 columns turned in its registers; the factors in parts of the rows' type
+  // 16-bit rows: 32 terms to a product, the lane's 8 rows x 8 columns turned in its registers; the factors in three parts of the rows'
+  // type, halves in as many rounds as they take
   const auto multiply_narrow = [&](Group &here, const int (&row)[OWN], int g) {
     u32x4 v[8];
 #pragma unroll
@@ -358,24 +359,33 @@ template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bound
 #pragma unroll
           for (int k = 0; k < 3; ++k) acc[j][q] = multiply32<T>(v[j], part[k], acc[j][q]);
       } else {
-        float most = 0.0f; // of the rank's factors in this group
+        for (int round = 0; round < HALF_ROUNDS; ++round) {
+          float most = 0.0f; // of the rank's factors in this group
 #pragma unroll
-        for (int i = 0; i < 8; ++i) most = __builtin_isfinite(u[i]) ? fmaxf(most, fabsf(u[i])) : most;
-        most = fmaxf(most, __shfl_xor(most, 16));
-        most = fmaxf(most, __shfl_xor(most, 32));
-        const float lift = lift_of(most), back = inverse_of(lift);
+          for (int i = 0; i < 8; i += 4) most = most_of(f32x4{u[i], u[i + 1], u[i + 2], u[i + 3]}, most);
+          most = fmaxf(most, __shfl_xor(most, 16));
+          most = fmaxf(most, __shfl_xor(most, 32));
+          if (round && !__ballot(is_left(most))) break;
+          const float lift = lift_of(most), back = inverse_of(lift);
+          bool left = false;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          uint32_t p[2];
-          halves_of(u[2 * w] * lift, u[2 * w + 1] * lift, p);
-          part[0][w] = p[0];
-          part[1][w] = p[1];
-        }
+          for (int w = 0; w < 4; ++w) {
+            uint32_t p[3];
+            float u0 = u[2 * w] * lift, u1 = u[2 * w + 1] * lift;
+            halves_of(u0, u1, p);
+            u[2 * w] = u0 * back;
+            u[2 * w + 1] = u1 * back;
+            left |= u0 != 0.0f || u1 != 0.0f;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const f32x4 sum = multiply32<T>(v[j], part[1], multiply32<T>(v[j], part[0], f32x4{}));
+            for (int k = 0; k < 3; ++k) part[k][w] = p[k];
+          }
 #pragma unroll
-          for (int i = 0; i < 4; ++i) acc[j][q][i] = fmaf(sum[i], back, acc[j][q][i]);
+          for (int j = 0; j < 8; ++j) {
+            const f32x4 sum = multiply32<T>(v[j], part[2], multiply32<T>(v[j], part[1], multiply32<T>(v[j], part[0], f32x4{})));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) acc[j][q][i] = fmaf(sum[i], back, acc[j][q][i]);
+          }
+          if (!__ballot(left)) break;
         }
       }
     }

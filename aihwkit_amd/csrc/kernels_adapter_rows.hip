@@ -31,8 +31,9 @@ template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) =
 #pragma unroll
     for (int i = 0; i < 8; ++i) x.q[i >> 2][i & 3] = kept & (1u << i) ? x.q[i >> 2][i & 3] : 0u;
   }
+  static constexpr bool ROUNDS = false;
   static __device__ __forceinline__ float lift(float) { return 1.0f; }
-  static __device__ __forceinline__ V split(f32x4 v, float) { return v; }
+  static __device__ __forceinline__ V split(const f32x4 &v, float) { return v; }
   using R = f32x4; // four ranks of a weight row
   static __device__ __forceinline__ R four(const float *p) { return *reinterpret_cast<const f32x4_unaligned *>(p); }
   template <typename H> static __device__ __forceinline__ R four(const H *p) {
@@ -58,8 +59,8 @@ template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) =
 };
 
 // 16-bit rows with weights of their type: exact products, sums in 32 bits.  hidden, which is not one of their numbers, goes into the
-// second product as the sum of some that are, against the same weights again: three bf16 parts, which are all of its 24 bits; two
-// halves, 22 bits (an error of 2^-23, twice that of a float, far below the 2^-11 of what is stored in the end).
+// second product as the sum of three that are, against the same weights again: all of its 24 bits.  Three bf16 always are; three halves
+// are of the larger values, and what they leave of others takes another round.
 template <typename T> struct Pipe<T, T, true> {
   using X = Packed8<T>;
   using W = Packed8<T>;
@@ -67,31 +68,48 @@ template <typename T> struct Pipe<T, T, true> {
     u32x4 upper; // the first two parts
     u32x2 third;
   };
+  static constexpr bool ROUNDS = __is_same(T, _Float16);
   static __device__ __forceinline__ f32x4 terms(const W &w, const X &x, f32x4 c) { return multiply32<T>(w.q, x.q, c); }
   static __device__ __forceinline__ void keep(X &x, uint32_t kept) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) x.q[i] &= (kept & (1u << 2 * i) ? 0xffffu : 0u) | (kept & (2u << 2 * i) ? 0xffff0000u : 0u);
   }
   static __device__ __forceinline__ float lift(float most) { return __is_same(T, __bf16) ? 1.0f : lift_of(most); }
-  static __device__ __forceinline__ V split(f32x4 v, float lift) {
-    V to = {};
+  static __device__ __forceinline__ V split(f32x4 &v, float lift) { // v: what is left
+    V to;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const float a = v[2 * h] * lift, b = v[2 * h + 1] * lift;
-      if constexpr (__is_same(T, __bf16)) {
-        uint32_t part[3];
-        parts_of(a, b, part);
-        to.upper[h] = part[0];
-        to.upper[2 + h] = part[1];
-        to.third[h] = part[2];
-      } else {
-        uint32_t part[2];
+      uint32_t part[3];
+      if constexpr (ROUNDS) {
+        const float back = inverse_of(lift);
+        float a = v[2 * h] * lift, b = v[2 * h + 1] * lift;
         halves_of(a, b, part);
-        to.upper[h] = part[0];
-        to.upper[2 + h] = part[1];
+        v[2 * h] = a * back;
+        v[2 * h + 1] = b * back;
+      } else {
+        parts_of(v[2 * h], v[2 * h + 1], part);
       }
+      to.upper[h] = part[0];
+      to.upper[2 + h] = part[1];
+      to.third[h] = part[2];
     }
     return to;
+  }
+  // what an earlier round left of four ranks of a lane, those of lanes that are 16 apart together, against N tiles of weights
+  template <int N> static __device__ __forceinline__ void add_left(const u32x2 (&w)[N], f32x4 left, f32x4 (&c)[N]) {
+    for (int round = 1; round < HALF_ROUNDS; ++round) {
+      float most = most_of(left);
+      most = fmaxf(most, __shfl_xor(most, 16));
+      most = fmaxf(most, __shfl_xor(most, 32));
+      if (!__ballot(is_left(most))) break;
+      const float lift = lift_of(most), back = inverse_of(lift);
+      const V v[1] = {split(left, lift)};
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+        const u32x2 w1[1] = {w[t]};
+        c[t] += ranks(w1, v, f32x4{}) * back;
+      }
+    }
   }
   using R = u32x2;
   static __device__ __forceinline__ R four(const T *p) { return *reinterpret_cast<const u32x2_from2 *>(p); }
@@ -103,13 +121,11 @@ template <typename T> struct Pipe<T, T, true> {
   template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT], const V (&v)[RT], f32x4 c) {
 #pragma unroll
     for (int q = 0; q < RT; ++q) c = multiply32<T>(u32x4{w[q][0], w[q][1], w[q][0], w[q][1]}, v[q].upper, c);
-    if constexpr (__is_same(T, __bf16)) { // the third parts of two tiles of ranks at a time
 #pragma unroll
-      for (int q = 0; q < RT; q += 2) {
-        const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q] : R{};
-        const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
-        c = multiply32<T>(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
-      }
+    for (int q = 0; q < RT; q += 2) { // the third parts of two tiles of ranks at a time
+      const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q] : R{};
+      const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
+      c = multiply32<T>(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
     }
     return c;
   }
@@ -350,6 +366,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   __shared__ float products[UP_ROWS][UP_PITCH];
   __shared__ typename P::V hidden_of[UP_ROWS][QUADS + 1];
   __shared__ float back_of[UP_ROWS];
+  __shared__ int left_of[UP_WAVES]; // whether the wave's values leave something for another round
   constexpr bool STAGED = RT > 1 || !FULL; // the 16 columns of one full tile of ranks lie side by side anyway
   __shared__ __align__(16) char weights[STAGED ? UP_WAVES : 1][STAGED ? 16 * (W_PITCH + 16) : 16];
   const int tid = (int)threadIdx.x, lane = tid & 63, wave = tid >> 6, lm = lane & 15, kg = lane >> 4;
@@ -403,18 +420,21 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   }
   if (some) {
     const float scale = a.back ? 1.0f : a.scale[adapter];
+    bool left = false;
 #pragma unroll
     for (int k = 0; k < H_SHARE; ++k) {
       h[k] *= scale;
-      float most = most_of(h[k]);
-#pragma unroll
-      for (int m = 1; m < QUADS; m *= 2) most = fmaxf(most, __shfl_xor(most, m));
-      const float lift = P::lift(most);
+      const float lift = P::lift(most_of_lanes<QUADS>(most_of(h[k])));
       const int r = (tid + 64 * UP_WAVES * k) / QUADS;
       if (r < UP_ROWS) {
         hidden_of[r][tid % QUADS] = P::split(h[k], lift);
-        if (tid % QUADS == 0) back_of[r] = inverse_of(lift) * (DROP ? a.drop.scale : 1.0f);
+        if (tid % QUADS == 0) back_of[r] = inverse_of(lift);
+        left |= P::ROUNDS && is_left(most_of(h[k]));
       }
+    }
+    if (P::ROUNDS) {
+      const uint64_t of_wave = __ballot(left);
+      if (lane == 0) left_of[wave] = of_wave != 0;
     }
     __syncthreads();
     typename P::V hidden[UP_MT][RT];
@@ -446,6 +466,28 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
 #pragma unroll
       for (int mt = 0; mt < UP_MT; ++mt) *reinterpret_cast<f32x4 *>(&products[16 * mt + lm][16 * (UP_T * wave + t) + 4 * kg]) = P::ranks(r, hidden[mt], f32x4{});
     }
+    if constexpr (P::ROUNDS) { // rare: what the first round left, on operands that are read again rather than kept
+      static_assert(UP_MT == 1);
+      int more = 0;
+#pragma unroll
+      for (int w = 0; w < UP_WAVES; ++w) more |= left_of[w];
+      if (more) {
+        const float *from = a.hidden + (long)order[min(lm, count - 1)] * a.rank;
+        const float lift = inverse_of(back_of[lm]);
+        f32x4 c[UP_T] = {};
+#pragma unroll 1
+        for (int rank = 4 * kg; rank < 16 * RT; rank += 16) {
+          typename P::R r[UP_T];
+#pragma unroll
+          for (int t = 0; t < UP_T; ++t) r[t] = load_ranks<P>(w_out + (long)min(mine + 16 * t + lm, a.out_size - 1) * a.rank, rank, a.rank);
+          f32x4 v = load_ranks<Pipe<float, float>>(from, rank, a.rank) * scale;
+          P::split(v, lift);
+          P::add_left(r, v, c);
+        }
+#pragma unroll
+        for (int t = 0; t < UP_T; ++t) *reinterpret_cast<f32x4 *>(&products[lm][16 * (UP_T * wave + t) + 4 * kg]) += c[t] * lift;
+      }
+    }
     __syncthreads();
   }
   const uint32_t call = DROP ? drop_call(a.drop) : 0;
@@ -458,7 +500,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
     if (!some) { // rows without adapter: base goes through, zeros without it
       if (base) widen16(v, add[k]);
     } else {
-      const float factor = back_of[m];
+      const float factor = back_of[m] * (DROP ? a.drop.scale : 1.0f);
 #pragma unroll
       for (int i = 0; i < EACH; ++i) v[i] = products[m][my_col + i] * factor;
       if (DROP) {
@@ -545,8 +587,13 @@ template <typename T, typename TW, int RT, bool FULL, bool SHORT> __global__ __l
     most = fmaxf(most, __shfl_xor(most, 16));
     most = fmaxf(most, __shfl_xor(most, 32));
     const float lift = P::lift(most), back = inverse_of(lift);
+    bool left = false;
 #pragma unroll
-    for (int q = 0; q < RT; ++q) hidden[q] = P::split(sum[q], lift);
+    for (int q = 0; q < RT; ++q) {
+      hidden[q] = P::split(sum[q], lift);
+      left |= P::ROUNDS && is_left(most_of(sum[q]));
+    }
+    const bool more = P::ROUNDS && __ballot(left) != 0;
     for (int unit = unit0 + wave; unit < unit1; unit += WAVES) {
       const int col = unit * 32 + 8 * kg; // the lane's results
       Packed8<T> add = {};
@@ -561,6 +608,21 @@ template <typename T, typename TW, int RT, bool FULL, bool SHORT> __global__ __l
 #pragma unroll
           for (int q = 0; q < RT; ++q) w[q] = FULL ? P::four(at + 16 * q + 4 * kg) : load_ranks<P>(at, 16 * q + 4 * kg, a.rank);
           acc[j] = P::ranks(w, hidden, acc[j]);
+          if constexpr (P::ROUNDS) {
+            if (__builtin_expect(more, 0)) { // what the first round left, found from the shares again, not kept
+              f32x4 c[1] = {};
+#pragma unroll 1
+              for (int q = 0; q < RT; ++q) {
+                f32x4 v = add_shares<WAVES, PITCH>(red, q) * kept_scale;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] = FULL || 16 * q + 4 * kg + i < a.rank ? v[i] * scale : 0.0f;
+                P::split(v, lift);
+                const typename P::R of_tile[1] = {load_ranks<P>(at, 16 * q + 4 * kg, a.rank)};
+                P::add_left(of_tile, v, c);
+              }
+              acc[j] += c[0] * lift;
+            }
+          }
         }
       }
       if (m0 + lm >= count) continue;
