@@ -5,7 +5,7 @@ leaves what a small one beside it gives with 24 bits.  The bounds are those of `
 import pytest
 import torch
 
-from test_gpu_digital import BF16, F16, IDS, PAIR_IDS, PAIRS, TYPES, Set, close, rand
+from test_gpu_digital import BF16, F16, F32, IDS, PAIR_IDS, PAIRS, TYPES, Set, close, rand
 
 pytestmark = pytest.mark.gpu
 
@@ -112,3 +112,21 @@ def test_infinite_rows_give_infinities_beside_ones(rows, rank, dtype):
     assert (da[0][:, sound] == float("-inf")).all()            # of row 6; column 2 adds an infinity of the other sign
     sound = torch.arange(24, device="cuda") != 4
     assert (db[0][sound] == float("inf")).all()
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [20, 90])
+def test_hidden_values_near_the_smallest_floats(rows, dtype):
+    """hidden of 2^-120 and about: of the parts that such a number is taken apart into the second and third are subnormal."""
+    s = Set(rows, 48, 40, 16, 2, dtype, dtype, seed=930)
+    s.x.mul_(2.0 ** -60)
+    s.a.mul_(2.0 ** -60)
+    s.base.zero_()
+    y, hidden = s.adapters.forward(s.x, s.index, return_hidden=True)
+    values, bounds = s.reference()                       # y is of the order of hidden
+    assert 2.0 ** -124 < values[1].abs().max() < 2.0 ** -112
+    close(hidden, values[1], bounds[1])
+    # The parts of scale * hidden are cut to multiples of the smallest bf16 number, 2^-133, so that together they are less than that short of
+    # it: on top of the sums' bound y may be off by 2^-133 for every rank, times its weight.
+    cut = 2.0 ** -133 * s.b.double().abs().sum(2).amax(0).cpu() if dtype == BF16 else 0.0
+    close(y, values[0], bounds[0] + cut)
