@@ -7,6 +7,7 @@ import torch
 from .._cabi import Adapters, check, lib, torch_calls
 from ._operands import DTYPES, Matrix, check_rows, drop_params, launch, like
 
+MOST_SIZE = 1 << 21   # inputs or outputs of an adapter, as the C entry points take them
 FEW_ROWS = 64   # RPU_ADAPTER_FEW_ROWS: a forward call groups so many rows by itself
 
 
@@ -62,8 +63,8 @@ class LowRankAdapters:
             raise RuntimeError("The number of adapters must be in 1 .. 65535.")
         if self.rank < 1 or self.rank > 128:
             raise RuntimeError("The rank of the adapters must be in 1 .. 128.")
-        if self.out_size < 1:
-            raise RuntimeError("The sizes of the adapters must be positive.")
+        if not 1 <= self.out_size <= MOST_SIZE or self.in_size > MOST_SIZE:
+            raise RuntimeError("The sizes of the adapters must be in 1 .. 2^21.")
         self.a, self.b = a, b
         self._a_shape, self._b_shape = a.shape, torch.Size((self.n_adapters, self.out_size, self.rank))
         self.scale = torch.ones(self.n_adapters, dtype=torch.float32, device=a.device) if scale is None else scale
@@ -86,14 +87,18 @@ class LowRankAdapters:
         return Adapters(a_dev=a.data_ptr(), b_dev=b.data_ptr(), scale_dev=scale.data_ptr(), n=self.n_adapters,
                         in_size=self.in_size, out_size=self.out_size, rank=self.rank, w_dtype=DTYPES[a.dtype])
 
-    def _rows(self, tensor: torch.Tensor, size: int, what: str) -> Matrix:
+    @staticmethod
+    def _checked_rows(tensor: torch.Tensor, size: int, what: str) -> torch.Tensor:
         check_rows(tensor, what)
         if tensor.size(-1) != size:
             raise RuntimeError(f"Invalid {what} dimensions: expected {size} columns, got {tensor.size(-1)}")
-        return Matrix(tensor, what)
+        return tensor
 
-    def _grouped(self, rows: Union[torch.Tensor, AdapterRows], x: Matrix, few: int):
-        """(index, plan) of a call: an index of more than ``few`` rows is grouped first."""
+    def _rows(self, tensor: torch.Tensor, size: int, what: str) -> Matrix:
+        return Matrix(self._checked_rows(tensor, size, what), what)
+
+    def _chosen(self, rows: Union[torch.Tensor, AdapterRows], x_input: torch.Tensor):
+        """(index, plan) as given, one of them None."""
         if isinstance(rows, AdapterRows):
             if rows.n_adapters != self.n_adapters:
                 raise RuntimeError("The rows were grouped for %d adapters, not %d" % (rows.n_adapters, self.n_adapters))
@@ -102,13 +107,30 @@ class LowRankAdapters:
         else:
             index, plan = _check_index(rows), None
             count, device = index.numel(), index.device
-        if count != x.rows:
-            raise RuntimeError("Invalid index dimensions: expected %d rows, got %d" % (x.rows, count))
-        if device != x.tensor.device:
-            raise RuntimeError(f"The index must be on {x.tensor.device}")
-        if plan is None and count > few:
+        expected = x_input.numel() // x_input.size(-1)
+        if count != expected:
+            raise RuntimeError("Invalid index dimensions: expected %d rows, got %d" % (expected, count))
+        if device != x_input.device:
+            raise RuntimeError(f"The index must be on {x_input.device}")
+        return index, plan
+
+    def _grouped(self, rows: Union[torch.Tensor, AdapterRows], x: Matrix, few: int):
+        """(index, plan) of a call: an index of more than ``few`` rows is grouped first."""
+        index, plan = self._chosen(rows, x.tensor)
+        if plan is None and index.numel() > few:
             plan = AdapterRows(index, self.n_adapters)
         return index, plan
+
+    def check_forward(self, x_input: torch.Tensor, rows: Union[torch.Tensor, AdapterRows], out_size: int) -> None:
+        """Raises what ``forward`` would raise for rows beside a projection of ``out_size`` outputs, without computing anything: for a
+        projection that is not to run in vain."""
+        self._checked_rows(x_input, self.in_size, "x_input")
+        self._operand(x_input)
+        if x_input.dtype != torch.float32 and x_input.dtype != self.a.dtype:
+            raise RuntimeError("Adapters beside 16-bit rows must be of the rows' type.")
+        if out_size != self.out_size:
+            raise RuntimeError("The adapters have %d outputs, the projection %d" % (self.out_size, out_size))
+        self._chosen(rows, x_input)
 
     def _native(self, rows, x_input):
         """(index, plan) for the native calls, (None, None) for what the general path has to look at."""

@@ -174,7 +174,10 @@ class InferenceTile:
         compensated output, each row's by ``rows`` (see ``LowRankAdapters.forward``); the reference has no counterpart."""
         if (adapters is None) != (rows is None):
             raise RuntimeError("adapters and the rows' choice of them (rows) come together")
-        out = self._gpu().forward(x_input, bias, False, False, is_test, adapters is not None)
+        tile = self._gpu()
+        if adapters is not None:   # before the tile computes: its pass draws, and a refused call is to leave it as it was
+            adapters.check_forward(x_input, rows, tile.get_d_size())
+        out = tile.forward(x_input, bias, False, False, is_test, adapters is not None)
         if is_test and self.drift_compensation is not None and self.alpha != 1.0 and not self._alpha_in_tile:
             out = out * self.alpha
         return out if adapters is None else adapters.forward(x_input, rows, base=out, out=out)
