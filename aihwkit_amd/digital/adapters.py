@@ -23,11 +23,15 @@ class AdapterRows:
     """Rows grouped by adapter, for any number of calls on as many rows: a step's layers share one.
 
     ``index``: int32 CUDA tensor, the adapter of every row; a row whose number is not in ``0 .. n_adapters - 1`` has none.  The
-    grouping is made on the current stream when the object is; it is of the numbers that ``index`` holds then."""
+    grouping is made on the current stream when the object is, of the numbers that ``index`` holds then, and nothing waits for it on the
+    host.  Calls on other streams wait for it on the GPU, and its memory is kept until they are done.  A capture on another stream
+    cannot wait for what is not captured: by then the grouping has to be done (``torch.cuda.graph`` waits for the GPU before it
+    begins), and the object lives as long as the graph.  Made within a capture, it is made by each replay, and not before the first."""
 
     def __init__(self, index: torch.Tensor, n_adapters: int):
         index = _check_index(index)
         self.n_adapters, self.rows, self.device = int(n_adapters), index.numel(), index.device
+        self._stream = torch._C._cuda_getCurrentRawStream(index.device.index)
         self._plan = torch_calls().adapter_plan(index, self.n_adapters)
         if self._plan is not None:
             self._bytes = self._plan.numel()
@@ -38,9 +42,19 @@ class AdapterRows:
         if not self._bytes:
             raise RuntimeError("The number of adapters must be in 1 .. 65535, that of rows at most 2^28.")
         self._plan = torch.empty(self._bytes, dtype=torch.uint8, device=index.device)
-        stream = torch.cuda.current_stream(index.device)
         check(lib().rpu_adapter_plan(index.data_ptr(), self.rows, self.n_adapters, self._plan.data_ptr(), self._bytes,
-                                     index.device.index, C.c_void_p(stream.cuda_stream)))
+                                     index.device.index, C.c_void_p(self._stream)))
+
+    def _plan_here(self) -> torch.Tensor:
+        """The plan, for work on the current stream: on another one than its own, after it has been made."""
+        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
+            with torch.cuda.device(self.device):
+                captured = torch.cuda.is_current_stream_capturing()
+            if not captured:
+                here = torch.cuda.current_stream(self.device)
+                here.wait_stream(torch.cuda.ExternalStream(self._stream, device=self.device))
+                self._plan.record_stream(here)
+        return self._plan
 
 
 class LowRankAdapters:
@@ -142,7 +156,7 @@ class LowRankAdapters:
             return rows, None
         if rows.n_adapters != self.n_adapters or rows.rows * self.in_size != x_input.numel():
             return None, None
-        return None, rows._plan
+        return None, rows._plan_here()
 
     def forward(self, x_input: torch.Tensor, rows: Union[torch.Tensor, AdapterRows], base: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None, return_hidden: bool = False, p: float = 0.0, seed: int = 0,
@@ -172,7 +186,7 @@ class LowRankAdapters:
             if return_hidden or plan else None
         launch(x_input.device, non_blocking,
                lambda device, stream: lib().rpu_adapter_forward(
-                   C.byref(adapters), x.ptr, x.ld, None if plan else index.data_ptr(), plan._plan.data_ptr() if plan else None,
+                   C.byref(adapters), x.ptr, x.ld, None if plan else index.data_ptr(), plan._plan_here().data_ptr() if plan else None,
                    plan._bytes if plan else 0, C.byref(drop), add.ptr if add else None, add.ld if add else 0, y.ptr, y.ld,
                    hidden.data_ptr() if hidden is not None else None, DTYPES[x_input.dtype], x.rows, device, stream))
         return (out, hidden) if return_hidden else out
@@ -207,7 +221,7 @@ class LowRankAdapters:
         scratch = torch.empty(scratch_bytes // 4, dtype=torch.float32, device=x_input.device)
         launch(x_input.device, non_blocking,
                lambda device, stream: lib().rpu_adapter_backward(
-                   C.byref(adapters), d.ptr, d.ld, x.ptr, x.ld, hidden.data_ptr(), plan._plan.data_ptr(), plan._bytes,
+                   C.byref(adapters), d.ptr, d.ld, x.ptr, x.ld, hidden.data_ptr(), plan._plan_here().data_ptr(), plan._bytes,
                    C.byref(drop), add.ptr if add else None, add.ld if add else 0, dx.ptr, dx.ld, da.data_ptr(), db.data_ptr(),
                    DTYPES[x_input.dtype], x.rows, scratch.data_ptr(), scratch_bytes, device, stream))
         return out, da, db
