@@ -329,16 +329,15 @@ void launch_layer_norm(const NormArgs &a, int dtype, int w_dtype, int cus, hipSt
   });
 }
 
-constexpr long MOST_PARTS = 1024; // that scratch sizes are for
-
 int layer_norm_parts(int rows, int cols, int cus) {
   // Workgroups of a CU.  Four waves each (1025 .. 4096 columns): 8192 rows of 1537 halves take 53 us with one, 33 with two, 28 with three,
   // 27 with four; of 4096 bf16 68, 46, 43 and 52.  Eight waves with rows of 513 .. 1024 columns in many registers: 16384 rows of 768
   // bf16 22.8 with one, 26.8 with two; shorter rows: 50000 of 64 floats 33.6 and 25.6, 16384 of 512 bf16 16.0 and 15.5.  Sixteen waves:
-  // 4096 rows of 5000 halves 49.3 and 54.2.  Two rows each at least, so that the sums' parts stay the lesser traffic.
+  // 4096 rows of 5000 halves 49.3 and 54.2.  Two rows each at least: of a column they read and write 12 bytes (16-bit rows without a base) to 32
+  // (floats with one), their sums, written and read again, take 16.
   const int per_cu = cols <= 512 ? 2 : cols <= 1024 ? 1 : cols <= 4096 ? 3 : 1;
   const long groups = ((long)rows + backward_rows(cols) - 1) / backward_rows(cols);
-  return (int)std::min((groups + 1) / 2, std::min((long)cus * per_cu, MOST_PARTS));
+  return (int)std::min((groups + 1) / 2, (long)cus * per_cu);
 }
 
 void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtype, hipStream_t s) {
