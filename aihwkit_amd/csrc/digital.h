@@ -72,6 +72,10 @@ struct AdapterPlan {
 };
 AdapterPlan adapter_plan(int rows, int n);
 void launch_adapter_plan(const int *index, int *plan, const AdapterPlan &p, hipStream_t s);
+// Turned matrices are made of adapters with rows.  Of fewer rows than adapters there are at most as many as rows: their matrices lie by the
+// number of the adapter's first chunk, which is below `rows` then, the others' by the adapter.
+inline bool adapter_listed(const AdapterPlan &p) { return p.n > p.rows; }
+inline int adapter_turned(const AdapterPlan &p) { return p.n > p.rows ? p.rows : p.n; } // matrices that there is room for
 constexpr int ADAPTER_FEW_ROWS = 64; // up to so many rows a forward call groups them by itself
 constexpr int ADAPTER_MAX_RANK = 128;
 constexpr int ADAPTER_MAX = 65535;
@@ -86,6 +90,7 @@ struct AdapterRowsArgs {
   AdapterPlan p;
   int rows, n, rank, in_size, out_size;
   int back;
+  int listed;                  // the matrices lie by the adapters' first chunks (adapter_listed)
   int units_each;              // few rows: 32 columns of the output each, of a workgroup (set by the launch)
   DropDev drop;                // of the input (forward) or of the output (backward)
 };
@@ -93,10 +98,11 @@ void launch_adapter_rows(const AdapterRowsArgs &a, int dtype, int w_dtype, int c
 
 struct AdapterTurnArgs {
   const void *a, *b;
-  void *a_turned, *b_turned;   // [n][in][rank], [n][rank][out], of adapters with rows
+  void *a_turned, *b_turned;   // [in][rank], [rank][out] of adapters with rows
   const int *plan;
   AdapterPlan p;
   int n, rank, in_size, out_size;
+  int listed;                  // as in AdapterRowsArgs
 };
 void launch_adapter_turn(const AdapterTurnArgs &a, int w_dtype, int cus, hipStream_t s);
 

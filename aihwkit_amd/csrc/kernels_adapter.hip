@@ -245,15 +245,16 @@ template <typename TW> __global__ __launch_bounds__(256) void k_adapter_turn(Ada
   const int a_tiles = (a.in_size + 63) / 64, b_tiles = (a.out_size + 63) / 64, rank_tiles = (a.rank + 63) / 64;
   for (int adapter = (int)blockIdx.y; adapter < a.n; adapter += (int)gridDim.y) {
     if (seg[adapter + 1] == seg[adapter]) continue;
+    const int turned = a.listed ? a.plan[a.p.first + adapter] : adapter;
     for (int k = (int)blockIdx.x; k < (a_tiles + b_tiles) * rank_tiles; k += (int)gridDim.x) {
       const int c = k / rank_tiles, r0 = k % rank_tiles * 64;
       const bool of_a = c < a_tiles;
       // a: [rank][in] -> [in][rank], b: [out][rank] -> [rank][out]
       const int rows = of_a ? a.rank : a.out_size, cols = of_a ? a.in_size : a.rank;
       const int row0 = of_a ? r0 : (c - a_tiles) * 64, col0 = of_a ? c * 64 : r0;
-      const long at = (long)adapter * rows * cols;
-      const TW *from = static_cast<const TW *>(of_a ? a.a : a.b) + at;
-      TW *to = static_cast<TW *>(of_a ? a.a_turned : a.b_turned) + at;
+      const long size = (long)rows * cols;
+      const TW *from = static_cast<const TW *>(of_a ? a.a : a.b) + adapter * size;
+      TW *to = static_cast<TW *>(of_a ? a.a_turned : a.b_turned) + turned * size;
       __syncthreads();
       TW v[16];
 #pragma unroll

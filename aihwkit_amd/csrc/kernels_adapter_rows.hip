@@ -192,6 +192,8 @@ __device__ __forceinline__ Place place_of(const AdapterRowsArgs &a, uint32_t gro
   return at;
 }
 
+__device__ __forceinline__ int matrix_of(const AdapterRowsArgs &a, int adapter) { return a.listed ? a.plan[a.p.first + adapter] : adapter; }
+
 template <typename T> __device__ __forceinline__ void read8_lds(Packed8<T> &v, const uint32_t *at) {
   if constexpr (sizeof(T) == 4) {
     v.q[0] = *reinterpret_cast<const u32x4 *>(at);
@@ -234,7 +236,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   const T *x_at[X_LOADS];
 #pragma unroll
   for (int j = 0; j < X_LOADS; ++j) x_at[j] = static_cast<const T *>(a.in.p) + (long)__shfl(row, 4 * j + kg) * a.in.ld;
-  const TW *w_in = static_cast<const TW *>(a.w_in) + (long)adapter * a.rank * a.in_size;
+  const TW *w_in = static_cast<const TW *>(a.w_in) + (long)matrix_of(a, adapter) * a.rank * a.in_size;
   const uint32_t call = DROP ? drop_call(a.drop) : 0;
   const int segments = (a.in_size + SEG - 1) / SEG, n = (segments - wave + NW - 1) / NW; // n of the wave
   const int first = n > 0 ? (int)(blockIdx.x / 8 % (unsigned)n) : 0;
@@ -378,7 +380,7 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   const bool some = adapter >= 0;
   // B: 16 columns of ranks lie side by side
   const int mine = col0 + 16 * UP_T * wave; // the wave's first column
-  const TW *w_out = static_cast<const TW *>(a.w_out) + (some ? (long)adapter * a.rank * a.out_size : 0);
+  const TW *w_out = static_cast<const TW *>(a.w_out) + (some ? (long)matrix_of(a, adapter) * a.rank * a.out_size : 0);
   const long w_all = (long)a.rank * a.out_size;
   Packed16<TW> w[UP_T][W_LOADS];
   typename P::R direct[UP_T];

@@ -124,8 +124,8 @@ struct BackwardScratch { // offsets in bytes
     bytes = 0;
     up = take(4 * (size_t)rows * a->rank);
     part = take(4 * (size_t)p.max_slots * a->rank * ((size_t)a->in_size + a->out_size));
-    a_turned = take(rows ? e * a->n * a->rank * a->in_size : 0);
-    b_turned = take(rows ? e * a->n * a->rank * a->out_size : 0);
+    a_turned = take(e * adapter_turned(p) * a->rank * a->in_size);
+    b_turned = take(e * adapter_turned(p) * a->rank * a->out_size);
   }
   size_t take(size_t n) {
     const size_t from = bytes;
@@ -363,7 +363,7 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
     g.out_size = w.out_size;
     g.drop = drop_of_x;
     if (rows) {
-      AdapterTurnArgs turn{w.a_dev, w.b_dev, (char *)scratch_dev + s.a_turned, (char *)scratch_dev + s.b_turned, g.plan, p, w.n, w.rank, w.in_size, w.out_size};
+      AdapterTurnArgs turn{w.a_dev, w.b_dev, (char *)scratch_dev + s.a_turned, (char *)scratch_dev + s.b_turned, g.plan, p, w.n, w.rank, w.in_size, w.out_size, adapter_listed(p)};
       launch_adapter_turn(turn, w.w_dtype, gpu.cus(), (hipStream_t)stream);
       AdapterRowsArgs a{};
       a.in = g.d;
@@ -382,6 +382,7 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
       a.out_size = w.in_size;
       a.drop = drop_of_x;
       a.back = 1;
+      a.listed = adapter_listed(p);
       launch_adapter_rows(a, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
     }
     launch_adapter_grads(g, dtype, w.w_dtype, gpu.cus(), (hipStream_t)stream);
