@@ -12,7 +12,7 @@ namespace {
 template <typename T, bool SHORT> __global__ __launch_bounds__(256) void k_dropout(DropoutArgs a) {
   const T *x = static_cast<const T *>(a.x.p), *base = static_cast<const T *>(a.base.p);
   T *out = static_cast<T *>(a.out.p);
-  const uint32_t blocks = ((uint32_t)a.cols + 7u) / 8u, call = drop_call(a.drop);
+  const uint32_t blocks = ((uint32_t)a.cols + 7u) / 8u, call = a.drop.on ? drop_call(a.drop) : 0;
   const uint64_t total = (uint64_t)a.rows * blocks;
   for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (uint64_t)gridDim.x * 256) {
     const uint32_t row = (uint32_t)(i / blocks), block = (uint32_t)(i % blocks);
@@ -20,7 +20,7 @@ template <typename T, bool SHORT> __global__ __launch_bounds__(256) void k_dropo
     const long col = (long)block * 8;
     Packed8<T> x8 = ahead8<SHORT>(x + row * a.x.ld, col, a.cols), base8 = {};
     if (base) base8 = ahead8<SHORT>(base + row * a.base.ld, col, a.cols);
-    const uint32_t kept = drop_kept(a.drop, call, row, block);
+    const uint32_t kept = a.drop.on ? drop_kept(a.drop, call, row, block) : 0xffu;
     trim8(x8, col, a.cols);
     Values8 v = widen(x8);
     drop_apply(a.drop, kept, v);

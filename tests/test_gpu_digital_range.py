@@ -5,6 +5,7 @@ leaves what a small one beside it gives with 24 bits.  The bounds are those of `
 import pytest
 import torch
 
+from aihwkit_amd import digital
 from test_gpu_digital import BF16, F16, F32, IDS, PAIR_IDS, PAIRS, TYPES, Set, close, rand
 
 pytestmark = pytest.mark.gpu
@@ -130,3 +131,17 @@ def test_hidden_values_near_the_smallest_floats(rows, dtype):
     # it: on top of the sums' bound y may be off by 2^-133 for every rank, times its weight.
     cut = 2.0 ** -133 * s.b.double().abs().sum(2).amax(0).cpu() if dtype == BF16 else 0.0
     close(y, values[0], bounds[0] + cut)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("cols", [5, 64, 785])
+def test_dropout_of_nothing_is_the_input_bit_by_bit(cols, dtype):
+    """At p = 0 nothing is drawn and every element kept, whatever it holds; a probability that rounds to no limit at all drops as little."""
+    x = rand(950, 70, cols, dtype=dtype)
+    x[3], x[4], x[5] = -0.0, float("inf"), torch.finfo(dtype).smallest_normal / 2
+    bits = {2: torch.int16, 4: torch.int32}[dtype.itemsize]
+    count = torch.tensor([7], device="cuda")
+    for p, call in ((0.0, 3), (0.0, count), (2.0 ** -34, 3)):
+        assert torch.equal(digital.dropout(x, p, 9, call).view(bits), x.view(bits))
+    x[6] = float("nan")
+    assert torch.equal(torch.isnan(digital.dropout(x, 0.0, 9)), torch.isnan(x))
