@@ -53,10 +53,12 @@ float *out_data(const at::Tensor &t) { return static_cast<float *>(t.data_ptr())
 
 hipStream_t stream_of(const at::Tensor &t) { return c10::hip::getCurrentHIPStream(t.device().index()).stream(); }
 
-// an entry point of the module: a C++ exception becomes a Python one
+// an entry point of the module: a C++ exception becomes a Python one, and an error of a flag without a truth value is raised
 template <typename F> PyObject *guarded(F &&f) {
   try {
-    return f();
+    PyObject *result = f();
+    if (result && PyErr_Occurred()) Py_CLEAR(result);
+    return result;
   } catch (const c10::Error &e) {
     PyErr_SetString(PyExc_RuntimeError, e.what_without_backtrace());
   } catch (const std::exception &e) {
@@ -497,6 +499,7 @@ PyObject *adapter_plan_checked(PyObject *const *a, Py_ssize_t n) {
   const at::Tensor *index = index_of(a[0]);
   if (!index) Py_RETURN_NONE;
   const long adapters = integer(a[1]);
+  if (adapters < 0) PyErr_Clear(); // beyond a long: the caller words it
   at::Tensor plan = plan_for(*index, adapters);
   if (!plan.defined()) Py_RETURN_NONE;
   const hipStream_t s = stream_of(*index);
