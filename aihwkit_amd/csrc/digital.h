@@ -352,8 +352,10 @@ __device__ __forceinline__ void parts_of(float a, float b, uint32_t (&part)[3]) 
     b = rest_of(b, __uint_as_float(part[k] & 0xffff0000u));
   }
 }
-// As three halves each, cut off too: of floats that lift_of was found from all bits of those down to 2^-16 of the largest.  a and b become what is
-// left of the others.  (An infinity leaves some finite number: where that is added, the infinity decides.)
+// As three halves each, cut off too, the third 1 / HALF_THIRD times what it stands for: of floats that lift_of was found from all bits of those
+// down to 2^-26 of the largest.  a and b become what is left of the others.  (An infinity leaves some finite number: where that is added, the
+// infinity decides.)
+constexpr float HALF_THIRD = 0x1p-11f;
 __device__ __forceinline__ void halves_of(float &a, float &b, uint32_t (&part)[3]) {
 #pragma unroll
   for (int k = 0; k < 3; ++k) {
@@ -361,18 +363,21 @@ __device__ __forceinline__ void halves_of(float &a, float &b, uint32_t (&part)[3
     const f16x2 r = __builtin_bit_cast(f16x2, part[k]);
     a -= (float)r.x;
     b -= (float)r.y;
-    if (!k) { // less than the 2^5 of the last bit, or a NaN
+    if (k == 0) { // less than the 2^5 of the last bit, or a NaN
       a = fmaxf(a, -32.0f);
       b = fmaxf(b, -32.0f);
     }
+    const float next = k == 1 ? 1.0f / HALF_THIRD : k == 2 ? HALF_THIRD : 1.0f;
+    a *= next;
+    b *= next;
   }
 }
 // Power of two that floats are multiplied by before halves_of, from their largest magnitude: they may leave the range of halves, the
 // largest becomes 2^14 .. 2^15.  (Numbers of less than 2^-97 in steps of 2^-135.)
 // What halves_of leaves is multiplied in another round, with a lift of its own, until nothing is left: a small value beside a large one that
-// meets a zero keeps its 24 bits.  A round leaves less than 2^-38 of the largest value, so that there are at most seven; of values of like
+// meets a zero keeps its 24 bits.  A round leaves less than 2^-48 of the largest value, so that there are at most six; of values of like
 // size there is one.
-constexpr int HALF_ROUNDS = 8;
+constexpr int HALF_ROUNDS = 7;
 __device__ __forceinline__ float lift_of(float most) {
   const int exponent = max((int)(__float_as_uint(most) >> 23), 30); // biased
   return __uint_as_float((uint32_t)(127 + 14 + 127 - exponent) << 23);

@@ -382,9 +382,9 @@ template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bound
           }
 #pragma unroll
           for (int j = 0; j < 8; ++j) {
-            const f32x4 sum = multiply32<T>(v[j], part[2], multiply32<T>(v[j], part[1], multiply32<T>(v[j], part[0], f32x4{})));
+            const f32x4 sum = multiply32<T>(v[j], part[1], multiply32<T>(v[j], part[0], f32x4{})), third = multiply32<T>(v[j], part[2], f32x4{});
 #pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][q][i] = fmaf(sum[i], back, acc[j][q][i]);
+            for (int i = 0; i < 4; ++i) acc[j][q][i] = fmaf(fmaf(third[i], HALF_THIRD, sum[i]), back, acc[j][q][i]);
           }
           if (!__ballot(left)) break;
         }

@@ -59,8 +59,8 @@ template <typename T, typename TW, bool NARROW = __is_same(T, TW) && sizeof(T) =
 };
 
 // 16-bit rows with weights of their type: exact products, sums in 32 bits.  hidden, which is not one of their numbers, goes into the
-// second product as the sum of three that are, against the same weights again: all of its 24 bits.  Three bf16 always are; three halves
-// are of the larger values, and what they leave of others takes another round.
+// second product as the sum of three that are, against the same weights again: all of its 24 bits.  Three bf16 always are; three halves,
+// of which the third has a sum of its own, are of values down to 2^-26 of the largest, and what they leave of others takes another round.
 template <typename T> struct Pipe<T, T, true> {
   using X = Packed8<T>;
   using W = Packed8<T>;
@@ -121,13 +121,14 @@ template <typename T> struct Pipe<T, T, true> {
   template <int RT> static __device__ __forceinline__ f32x4 ranks(const R (&w)[RT], const V (&v)[RT], f32x4 c) {
 #pragma unroll
     for (int q = 0; q < RT; ++q) c = multiply32<T>(u32x4{w[q][0], w[q][1], w[q][0], w[q][1]}, v[q].upper, c);
+    f32x4 third = ROUNDS ? f32x4{} : c;
 #pragma unroll
     for (int q = 0; q < RT; q += 2) { // the third parts of two tiles of ranks at a time
       const R next = q + 1 < RT ? w[q + 1 < RT ? q + 1 : q] : R{};
       const u32x2 more = q + 1 < RT ? v[q + 1 < RT ? q + 1 : q].third : u32x2{};
-      c = multiply32<T>(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, c);
+      third = multiply32<T>(u32x4{w[q][0], w[q][1], next[0], next[1]}, u32x4{v[q].third[0], v[q].third[1], more[0], more[1]}, third);
     }
-    return c;
+    return ROUNDS ? c + third * HALF_THIRD : third;
   }
 };
 
@@ -359,8 +360,10 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
 // stored.  Loads in the lanes' order of the products, 16 rows to every 16 lanes, take the address units four times as long.
 // Bound by base and y: 8192 rows of 2304 floats, rank 16, in 30.3 us (151 MB, 5.0 TB/s; a copy of that size 5.4), 4096 rows of 4096
 // bf16, rank 64, in 24.7 us.  16 x 256 took 32.0 and 25.0 us, 32 x 128 34.5 and 27.7 us where 16 x 128 took 32.4 and 25.0.
+// Halves: registers for what is rare would leave a SIMD fewer waves, where no spill comes of it (rank 64 without a bound 41.0 us, with 39.0).
+constexpr int up_waves_of_rounds(int rank_tiles, bool full) { return rank_tiles == 1 ? 8 : rank_tiles == 2 ? 7 : rank_tiles == 4 ? 5 + full : 1; }
 constexpr int UP_ROWS = 16, UP_COLS = 128, UP_MT = UP_ROWS / 16, UP_PITCH = UP_COLS + 4, UP_T = UP_COLS / 16 / UP_WAVES;
-template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __global__ __launch_bounds__(64 * UP_WAVES) void k_adapter_up(AdapterRowsArgs a) {
+template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __global__ __launch_bounds__(64 * UP_WAVES, (Pipe<T, TW>::ROUNDS ? up_waves_of_rounds(RT, FULL) : 1)) void k_adapter_up(AdapterRowsArgs a) {
   using P = Pipe<T, TW>;
   constexpr int EACH = CHUNK<T>, SHARE = UP_ROWS * UP_COLS / EACH / (64 * UP_WAVES); // values of a load; loads of a thread
   constexpr int QUADS = 4 * RT, H_SHARE = (UP_ROWS * QUADS + 64 * UP_WAVES - 1) / (64 * UP_WAVES);

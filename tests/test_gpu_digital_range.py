@@ -145,3 +145,28 @@ def test_dropout_of_nothing_is_the_input_bit_by_bit(cols, dtype):
         assert torch.equal(digital.dropout(x, p, 9, call).view(bits), x.view(bits))
     x[6] = float("nan")
     assert torch.equal(torch.isnan(digital.dropout(x, 0.0, 9)), torch.isnan(x))
+
+
+@pytest.mark.parametrize("rows", [30, 100])
+@pytest.mark.parametrize("rank", [12, 16, 64])
+@pytest.mark.parametrize("level", [30, 0, -34])
+def test_three_levels_of_hidden_values(level, rank, rows):
+    """Half precision: ranks of 2^30, 1 and 2^-34, each of which alone makes a share of the columns.  The scale brings those of one level into
+    the type's range."""
+    s = Set(rows, 48, 45, rank, 2, F16, F16, seed=960)
+    s.a.zero_()
+    s.b.zero_()
+    for k, exponent in enumerate((30, 0, -34)):
+        x, r, d = slice(16 * k, 16 * k + 16), slice(k, None, 3), slice(k, None, 3)
+        s.x[:, x] = rand(961 + k, rows, 16, dtype=F16, std=2.0 ** (exponent // 2 - 1))
+        s.a[:, r, x] = rand(964 + k, *s.a[:, r, x].shape, dtype=F16, std=2.0 ** (exponent // 2 - 1))
+        s.b[:, d, r] = rand(967 + k, *s.b[:, d, r].shape, dtype=F16)
+    s.scale.fill_(2.0 ** -level)
+    s.base.zero_()
+    y, few = s.adapters.forward(s.x, digital.AdapterRows(s.index, 2), base=s.base), s.forward()
+    values, bounds = s.reference()
+    some = s.index.cpu() >= 0
+    part = values[0][:, {30: 0, 0: 1, -34: 2}[level]::3][some].abs()
+    assert 2.0 ** -4 < part.median() < 2.0 ** 8
+    for got in (y, few):
+        close(got, values[0], bounds[0])
