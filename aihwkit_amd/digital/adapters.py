@@ -24,14 +24,15 @@ class AdapterRows:
 
     ``index``: int32 CUDA tensor, the adapter of every row; a row whose number is not in ``0 .. n_adapters - 1`` has none.  The
     grouping is made on the current stream when the object is, of the numbers that ``index`` holds then, and nothing waits for it on the
-    host.  Calls on other streams wait for it on the GPU, and its memory is kept until they are done.  A capture on another stream
-    cannot wait for what is not captured: by then the grouping has to be done (``torch.cuda.graph`` waits for the GPU before it
-    begins), and the object lives as long as the graph.  Made within a capture, it is made by each replay, and not before the first."""
+    host.  Calls on other streams wait for it on the GPU, and its memory is kept until they are done.  A capture cannot wait for what is
+    not captured: by then the grouping has to be done (``torch.cuda.graph`` waits for the GPU before it begins), and the object lives
+    as long as the graph.  Made within a capture, the grouping is done by each replay, and not before the first."""
 
     def __init__(self, index: torch.Tensor, n_adapters: int):
         index = _check_index(index)
         self.n_adapters, self.rows, self.device = int(n_adapters), index.numel(), index.device
-        self._stream = torch._C._cuda_getCurrentRawStream(index.device.index)
+        self._device = self.device.index
+        self._stream = torch._C._cuda_getCurrentRawStream(self._device)
         self._plan = torch_calls().adapter_plan(index, self.n_adapters)
         if self._plan is not None:
             self._bytes = self._plan.numel()
@@ -43,18 +44,29 @@ class AdapterRows:
             raise RuntimeError("The number of adapters must be in 1 .. 65535, that of rows at most 2^28.")
         self._plan = torch.empty(self._bytes, dtype=torch.uint8, device=index.device)
         check(lib().rpu_adapter_plan(index.data_ptr(), self.rows, self.n_adapters, self._plan.data_ptr(), self._bytes,
-                                     index.device.index, C.c_void_p(self._stream)))
+                                     self._device, C.c_void_p(self._stream)))
 
     def _plan_here(self) -> torch.Tensor:
         """The plan, for work on the current stream: on another one than its own, after it has been made."""
-        if torch._C._cuda_getCurrentRawStream(self.device.index) != self._stream:
-            with torch.cuda.device(self.device):
-                captured = torch.cuda.is_current_stream_capturing()
-            if not captured:
-                here = torch.cuda.current_stream(self.device)
-                here.wait_stream(torch.cuda.ExternalStream(self._stream, device=self.device))
-                self._plan.record_stream(here)
+        if torch._C._cuda_getCurrentRawStream(self._device) != self._stream:
+            self._order_after(torch.cuda.current_stream(self.device))
         return self._plan
+
+    def _order_after(self, here: torch.cuda.Stream) -> None:
+        made = torch.cuda.ExternalStream(self._stream, device=self.device)
+
+        def captured(stream):      # the default stream never is
+            with torch.cuda.stream(stream):
+                return stream.cuda_stream != 0 and torch.cuda.is_current_stream_capturing()
+
+        if captured(made):
+            if not captured(here):
+                raise RuntimeError("The stream that the rows were grouped on is being captured, the current one is not.")
+        elif captured(here):
+            return                 # done by now, as the class's description asks for
+        else:
+            self._plan.record_stream(here)
+        here.wait_stream(made)
 
 
 class LowRankAdapters:

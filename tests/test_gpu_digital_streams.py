@@ -61,3 +61,44 @@ def test_rows_grouped_before_a_capture():
         eager = step(s, rows)
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) and torch.equal(r, q) for p, q, r in zip(results, expected, eager))
+
+
+def test_rows_grouped_within_a_capture_and_used_on_a_stream_of_it():
+    """Two streams of one capture: the second, which joined before the rows were grouped, comes after that all the same."""
+    s = Set(300, 64, 80, 8, 4, p=0.1)
+    index = s.index.clone()
+    second = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        first = torch.cuda.current_stream()
+        second.wait_stream(first)
+        rows = digital.AdapterRows(index, s.n)
+        with torch.cuda.stream(second):
+            results = step(s, rows)
+        first.wait_stream(second)
+    for k in range(4):
+        s.index.copy_((s.index + 1) % 4)
+        index.copy_(s.index)
+        for t in results:
+            t.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(results, s.step())), k
+
+
+def test_rows_whose_stream_is_being_captured_are_refused_elsewhere():
+    s = Set(300, 64, 80, 8, 4)
+    first, second = torch.cuda.Stream(), torch.cuda.Stream()
+    with torch.cuda.stream(first):
+        rows = digital.AdapterRows(s.index, s.n)
+    torch.cuda.synchronize()
+    x = torch.ones(64, 64, device="cuda")
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=first):
+        y = digital.dropout(x, 0.5, 1, non_blocking=True)
+        with torch.cuda.stream(second), pytest.raises(RuntimeError, match="captured"):
+            s.adapters.forward(s.x, rows, non_blocking=True)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, digital.dropout(x, 0.5, 1))
