@@ -61,8 +61,8 @@ void launch_layer_norm_backward(const NormBackwardArgs &a, int dtype, int w_dtyp
 //   chunks [4 * chunks]  the same in longer pieces for the gradients, of adapters only; the last number is the slot for the
 //                      chunk's sums, -1 if it holds all rows of its adapter
 //   first [n + 1]      first[a]: the first chunk of adapter a
-//   tile_first [n + 2], slot_first [n + 1]  the same of the tiles and of the slots
-//   other [rows]       scratch
+//   slot_first [n + 1]  the same of the slots
+//   tile_first [n + 2], other [rows]  scratch of k_adapter_plan
 constexpr int ADAPTER_TILE_ROWS = 64;
 struct AdapterPlan {
   int rows, n;

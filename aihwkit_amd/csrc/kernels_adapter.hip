@@ -278,10 +278,12 @@ constexpr int GRAD_WAVES = 4;
 
 // 128 columns of dA (of x, against up) or of dB (of d, against scale hidden).  A wave takes 16 rows of its chunk at a time; lane
 // % 16 reads eight columns of four rows, 16 bytes beside those of its neighbours at a time, and product j of a row takes its column j.
-// Rows of float: products on the fp32 instructions, bound by the reads of x and d up to rank 16 (8192 rows of 768 and 2304 columns in 25.7
-// us, 101 MB, 3.9 TB/s; one group at a time, each waited for, 35 us), by the products beyond: a backward pass of those rows takes 75 us
-// with rank 16, 263 with 64, 475 with 128.  16-bit rows: their numbers as they are on the 16-bit instructions, the factors in parts.  The
-// same backward pass in bf16 takes 48.6 us with rank 16, 102 with 64, 186 with 128; on the fp32 instructions 53.8, 193 and 348.
+// Rows of float: products on the fp32 instructions, bound by the reads of x and d up to rank 16 (8192 rows of 768 and 2304 columns in 25.1
+// us, 101 MB, 4.0 TB/s; one group at a time, each waited for, 35 us).  Beyond, by too few waves: with rank 64 160 us, in which the matrix pipes
+// are busy for 13 %; 256 registers leave less than one wave to a SIMD, and it waits for 45 % of its time, for loads and, at the end, for the
+// waves before it to add 128 sums each in LDS.  A backward pass of those rows takes 79 us with rank 16, 256 with 64, 458 with 128.  16-bit
+// rows: their numbers as they are on the 16-bit instructions, the factors in parts.  The same backward pass in bf16 takes 48 us with rank 16,
+// 103 with 64, 188 with 128; on the fp32 instructions 53.8, 193 and 348; in f16 51, 114 and 205.
 template <typename T, typename TW, int RT, bool SHORT> __global__ __launch_bounds__(64 * GRAD_WAVES, RT == 1 ? 3 : sizeof(T) == 2 ? 2 : 1) void k_adapter_grads(AdapterGradArgs a) {
   __shared__ float sums[32 * RT][64];
   const int4 chunk = reinterpret_cast<const int4 *>(a.plan + a.p.chunks)[blockIdx.x];

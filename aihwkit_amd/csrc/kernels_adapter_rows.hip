@@ -210,7 +210,7 @@ template <typename T> __device__ __forceinline__ void read8_lds(Packed8<T> &v, c
 // The workgroups begin at different segments: all those of an adapter read the same A.
 // Bound by the reads of x, and the chain of loads before the first of them (tile, its rows, x).  8192 rows of 768 floats, rank 16: 11.2 us
 // (28 MB); 8192 rows of 2304 floats: 21.0 us (75 MB, 3.6 TB/s); 4096 rows of 4096 bf16, rank 64: 14.9 us, where every 16 rows read all
-// 0.5 MB of A from the L2, 150 MB.  With the stages of all waves in step (barriers around x in LDS) 15.5, 28 and 25 us; with 4 waves
+// 0.5 MB of A from the L2, 134 MB.  With the stages of all waves in step (barriers around x in LDS) 15.5, 28 and 25 us; with 4 waves
 // 13.6, 33 and 25 us, with 16 17.7, 30 and 16.4 us, both before loads went out together.  Registers: three or four waves of a SIMD without
 // spills; six spill and take twice the time.
 constexpr int DOWN_WAVES = 8;
@@ -358,8 +358,9 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
 // UP_ROWS rows x UP_COLS columns of y.  Everything comes and goes along the rows of its matrix and through LDS: hidden, in the form
 // of the matrix instructions, for all waves; B, 16 columns of the wave at a time; the products, to which base is added as they are
 // stored.  Loads in the lanes' order of the products, 16 rows to every 16 lanes, take the address units four times as long.
-// Bound by base and y: 8192 rows of 2304 floats, rank 16, in 30.3 us (151 MB, 5.0 TB/s; a copy of that size 5.4), 4096 rows of 4096
-// bf16, rank 64, in 24.7 us.  16 x 256 took 32.0 and 25.0 us, 32 x 128 34.5 and 27.7 us where 16 x 128 took 32.4 and 25.0.
+// Bound by base and y with small ranks: 8192 rows of 2304 floats, rank 16, in 30.5 us (151 MB, 4.9 TB/s; a copy of that size 5.4).  With larger
+// ones by what comes from the L2: 4096 rows of 4096 bf16, rank 64, in 24.8 us, 67 MB of base and y (2.7 TB/s), and for every 8 KB of them 16
+// of B and 4 of hidden.  16 x 256 took 32.0 and 25.0 us, 32 x 128 34.5 and 27.7 us where 16 x 128 took 32.4 and 25.0.
 // Halves: registers for what is rare would leave a SIMD fewer waves, where no spill comes of it (rank 64 without a bound 41.0 us, with 39.0).
 constexpr int up_waves_of_rounds(int rank_tiles, bool full) { return rank_tiles == 1 ? 8 : rank_tiles == 2 ? 7 : rank_tiles == 4 ? 5 + full : 1; }
 constexpr int UP_ROWS = 16, UP_COLS = 128, UP_MT = UP_ROWS / 16, UP_PITCH = UP_COLS + 4, UP_T = UP_COLS / 16 / UP_WAVES;
@@ -519,8 +520,10 @@ template <typename T, typename TW, int RT, bool FULL, bool DROP, bool SHORT> __g
   }
 }
 
-// Up to ADAPTER_FEW_ROWS rows by their index alone (64 rows of 4096 bf16 for 8 adapters of rank 16 in 12.4 us; a plan and the two kernels
-// above take 16.6): workgroup (i, s) makes the columns of slice s for all rows of the adapter of row
+// Up to ADAPTER_FEW_ROWS rows by their index alone.  4096 -> 4096 bf16, and a plan (6 us) with the two kernels above: 64 rows, rank 16, of 8
+// adapters 12.1 and 17.4 us, of two 21.7 and 17.9, of one 47.7 and 18.5; rank 64 29.8 and 22.2, 56.7 and 22.6, 114.6 and 24.0; 16 rows of one
+// adapter 11.3 and 17.5, rank 64 24.9 and 21.3.  (Rows of an adapter go through a workgroup 16 at a time, one group after another.)  Workgroup
+// (i, s) makes the columns of slice s for all rows of the adapter of row
 // i, unless an earlier row has it, and the hidden that it needs for them.
 template <typename T, typename TW, int RT, bool FULL, bool SHORT> __global__ __launch_bounds__(64 * WAVES) void k_adapter_few(AdapterRowsArgs a) {
   using P = Pipe<T, TW>;
@@ -641,7 +644,9 @@ template <typename T, typename TW, int RT, bool FULL, bool SHORT> __global__ __l
   }
 }
 
-// tiles of 16 ranks, whether the rank fills them, and whether a matrix has rows of fewer than eight columns
+// tiles of 16 ranks, whether the rank fills them, and whether a matrix has rows of fewer than eight columns.  Those are rare, and take the
+// kernels of eight tiles whatever the rank, so that there is one more set of kernels and not four: 4096 rows, 4096 -> 7, rank 4, in 34 us
+// (bf16) and 91 (floats), where 4096 -> 8 takes 14 and 20.
 template <typename F> void with_sizes(int rank, int least, F &&f) {
   const auto full = [&](auto rt) { rank == 16 * decltype(rt)::value ? f(rt, Int<1>{}, Int<0>{}) : f(rt, Int<0>{}, Int<0>{}); };
   if (least < 8) f(Int<8>{}, Int<0>{}, Int<1>{});

@@ -8,7 +8,8 @@ differs from request to request is digital: low-rank adapters of a tile's projec
 Tensors are on the GPU, float32, float16 or bfloat16; the last dimension holds the columns, the others together are the rows.
 Matrices whose rows are apart (column slices) are read and written in place; other layouts of inputs are copied first.
 Everything is computed in 32 bits and rounded once.  As with the tiles, calls go to the current stream of the tensors' GPU and
-wait for it unless ``non_blocking`` is set, and nothing takes part in autograd: forward and backward are calls of their own.
+wait for it unless ``non_blocking`` is set (``AdapterRows`` never waits: calls that use it come after it on whatever stream), and nothing
+takes part in autograd: forward and backward are calls of their own.
 """
 from .adapters import AdapterRows, LowRankAdapters
 from .elementwise import dropout

@@ -763,7 +763,7 @@ int rpu_layer_norm(const void *x_dev, long x_ld, const void *w_dev, const void *
 
 /* Its gradients: with h = (x - mean) rstd and g = d w, dx = base + rstd (g - mean(g) - h mean(g h)), dw = sum over rows d h,
  * db = sum over rows d (of `w_dtype`, both or neither; zeros for no rows).  dx may be d or x.  Sums over rows are added in a
- * fixed order.  scratch: rpu_layer_norm_backward_scratch bytes (no less for other GPUs), used until the call's work is done. */
+ * fixed order.  scratch: rpu_layer_norm_backward_scratch bytes, used until the call's work is done. */
 size_t rpu_layer_norm_backward_scratch(int rows, int cols);
 int rpu_layer_norm_backward(const void *d_dev, long d_ld, const void *x_dev, long x_ld, const float *mean_dev,
                             const float *rstd_dev, const void *w_dev, int w_dtype, const void *base_dev, long base_ld,
@@ -787,7 +787,8 @@ typedef struct rpu_adapters {
 /* index_dev [rows]: the adapter of every row; a row whose number is not in 0 .. n - 1 has none (y = base, hidden = 0, dx =
  * base, no part in da and db).  Groups the rows by adapter into plan_dev, rpu_adapter_plan_bytes(rows, n) bytes, for any
  * number of forward and backward calls on as many rows and adapters, of whatever sizes; the order of the rows of an adapter is kept, so that the
- * sums over them do not depend on the run. */
+ * sums over them do not depend on the run.  (The order of a row's own sum begins at a place that depends on where the row comes to lie: its last bits may
+ * depend on the rows beside it.)  The plan is read by the calls it is given to: on other streams they are the caller's to order after it. */
 size_t rpu_adapter_plan_bytes(int rows, int n);
 int rpu_adapter_plan(const int32_t *index_dev, int rows, int n, void *plan_dev, size_t plan_bytes, int device_id, void *stream);
 
@@ -800,7 +801,7 @@ int rpu_adapter_forward(const rpu_adapters *adapters, const void *x_dev, long x_
                         void *stream);
 
 /* da_dev, db_dev: laid out and typed like a and b, zeros for adapters without rows.  dx may be base, but no other operand.
- * scratch: rpu_adapter_backward_scratch bytes, used until the call's work is done. */
+ * scratch: rpu_adapter_backward_scratch bytes, used until the call's work is done: room for the matrices of min(n, rows) adapters. */
 size_t rpu_adapter_backward_scratch(const rpu_adapters *adapters, int rows);
 int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d_ld, const void *x_dev, long x_ld,
                          const float *hidden_dev, const void *plan_dev, size_t plan_bytes, const rpu_dropout_params *drop,
