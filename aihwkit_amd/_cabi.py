@@ -55,6 +55,18 @@ class Adapters(C.Structure):
                 ("out_size", i32), ("rank", i32), ("w_dtype", i32), ("reserved", i32)]
 
 
+class Cache(C.Structure):
+    """``rpu_cache``."""
+    _fields_ = [("k_dev", C.c_void_p), ("v_dev", C.c_void_p), ("turns_dev", C.c_void_p), ("pages", i32), ("page_size", i32), ("heads", i32),
+                ("head_size", i32), ("dtype", i32), ("pairs", i32), ("neighbours", i32), ("reserved", i32)]
+
+
+class CacheRows(C.Structure):
+    """``rpu_cache_rows``."""
+    _fields_ = [("tables_dev", C.c_void_p), ("lengths_dev", C.c_void_p), ("starts_dev", C.c_void_p), ("table_ld", C.c_long), ("n", i32),
+                ("table_width", i32), ("rows", i32), ("reserved", i32)]
+
+
 class DeviceParams(C.Structure):
     """``rpu_device_params``."""
 
@@ -240,6 +252,11 @@ SYMBOLS = {
     "rpu_adapter_backward": (C.c_int, [C.POINTER(Adapters), _P, C.c_long, _P, C.c_long, _P, _P, C.c_size_t,
                                        C.POINTER(DropoutParams), _P, C.c_long, _P, C.c_long, _P, _P, C.c_int, C.c_int, _P,
                                        C.c_size_t, C.c_int, _P]),
+    "rpu_cache_append": (C.c_int, [C.POINTER(Cache), C.POINTER(CacheRows), _P, C.c_long, _P, C.c_long, _P, C.c_long, _P, C.c_long, C.c_int,
+                                   C.c_int, C.c_int, _P]),
+    "rpu_cache_attend_scratch": (C.c_size_t, [C.POINTER(Cache), C.POINTER(CacheRows), C.c_int, C.c_int, C.c_int, C.c_int, C.c_int]),
+    "rpu_cache_attend": (C.c_int, [C.POINTER(Cache), C.POINTER(CacheRows), _P, C.c_long, _P, C.c_long, C.c_int, C.c_int, C.c_float, C.c_int,
+                                   C.c_int, C.c_int, _P, C.c_size_t, C.c_int, _P]),
     "rpu_device_allocation_count": (C.c_long, []),
     "rpu_last_error": (C.c_char_p, []),
     "rpu_abi_version": (C.c_int, []),

@@ -1,0 +1,83 @@
+// Attention over a paged cache: argument blocks, launches, and what the kernels share: where rows and positions lie.
+#pragma once
+#include "digital.h"
+
+namespace rpu_amd {
+
+struct CacheDev {
+  void *k, *v;         // [pages][heads][page_size][head]
+  const double *turns; // [pairs]
+  int pages, page_shift, heads, head, pairs, neighbours;
+};
+struct CacheRowsDev {
+  const int *tables, *lengths, *starts; // starts null: rows / n each
+  long table_ld;
+  int n, places, rows; // places: positions that a table holds
+};
+
+struct AppendArgs {
+  CacheDev c;
+  CacheRowsDev r;
+  MatrixDev k, v, q, out; // q.p null: none
+  int q_heads;
+};
+void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cus, hipStream_t s);
+
+struct AttendArgs {
+  CacheDev c;
+  CacheRowsDev r;
+  MatrixDev q, out;
+  int group;           // heads of a row that share one of the cache
+  float scale;
+  int window, sinks;   // window 0: none
+};
+void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, int cus, hipStream_t s);
+
+#if defined(__HIPCC__)
+// The rows of a sequence, and the position of the first.  Numbers on the GPU that are out of range leave it without rows or positions: nothing
+// outside of the operands is touched.
+struct Sequence {
+  int which, begin, end;
+  long first; // position of row `begin`
+};
+__device__ __forceinline__ Sequence sequence_at(const CacheRowsDev &r, int which) {
+  Sequence s;
+  s.which = which;
+  if (r.starts) {
+    s.begin = min(max(r.starts[which], 0), r.rows);
+    s.end = min(max(r.starts[which + 1], s.begin), r.rows);
+  } else {
+    const int each = r.rows / r.n;
+    s.begin = which * each;
+    s.end = s.begin + each;
+  }
+  s.first = (long)r.lengths[which] - (s.end - s.begin);
+  return s;
+}
+// the sequence that a row belongs to; which < 0: none
+__device__ __forceinline__ Sequence sequence_of(const CacheRowsDev &r, int row) {
+  if (!r.starts) return sequence_at(r, row / (r.rows / r.n));
+  int low = -1, high = r.n; // starts[low] <= row < starts[high]
+  while (high - low > 1) {
+    const int middle = (low + high) / 2;
+    if (r.starts[middle] <= row) low = middle;
+    else high = middle;
+  }
+  if (low < 0) return {-1, 0, 0, 0};
+  Sequence s = sequence_at(r, low);
+  if (row < s.begin || row >= s.end) s.which = -1;
+  return s;
+}
+// the page of a position of a sequence; -1: none
+__device__ __forceinline__ int page_of(const CacheDev &c, const CacheRowsDev &r, const int *table, long position) {
+  if (position < 0 || position >= r.places) return -1;
+  const int page = table[position >> c.page_shift];
+  return page >= 0 && page < c.pages ? page : -1;
+}
+// value 0 of a head at a position
+__device__ __forceinline__ long place_of(const CacheDev &c, int page, int head, long position) {
+  return ((((long)page * c.heads + head) << c.page_shift) + (position & ((1 << c.page_shift) - 1))) * c.head;
+}
+#endif
+
+} // namespace rpu_amd

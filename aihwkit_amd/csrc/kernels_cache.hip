@@ -1,0 +1,114 @@
+// New keys and values into a paged cache; keys and queries are rotated by their positions on the way.
+//   t = p f (turns; f: turns per position), (a, b) -> (a cos 2 pi t - b sin 2 pi t, a sin 2 pi t + b cos 2 pi t) of each pair
+// t is taken in 64 bits and only what it has beyond whole turns goes on: far positions lose nothing.
+#include "cache.h"
+
+#include <algorithm>
+
+namespace rpu_amd {
+namespace {
+
+// cosine and sine of a number of turns.  The fraction as a float and what that leaves, d: cos(x + d) = cos x - d sin x, d < 2^-24.
+__device__ __forceinline__ float2 turned(double turns) {
+  const double rest = turns - rint(turns);
+  const float f = (float)rest;
+  const float d = 6.2831853f * (float)(rest - (double)f);
+  float sine, cosine;
+  sincospif(2.0f * f, &sine, &cosine);
+  return {cosine - d * sine, sine + d * cosine};
+}
+
+constexpr int THREADS = 256, MOST_ROWS_EACH = 8;
+
+// A workgroup takes `each` rows: their places and angles go to LDS, once for all heads, then every thread moves groups of eight values (of
+// both halves, where pairs lie apart).  SHORT: some part of a head is no row of eight columns and more.
+// Bound by memory.
+template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THREADS) void k_cache_append(AppendArgs a, int each) {
+  __shared__ int page[MOST_ROWS_EACH];
+  __shared__ long at[MOST_ROWS_EACH];
+  __shared__ float2 angles[MOST_ROWS_EACH * (RPU_CACHE_MAX_HEAD / 2)];
+  const int first = blockIdx.x * each, count = min(each, a.r.rows - first), tid = threadIdx.x;
+  const int pairs = a.c.pairs, head = a.c.head, rest = head - 2 * pairs;
+  if (tid < count) {
+    const Sequence s = sequence_of(a.r, first + tid);
+    const long position = s.first + (first + tid - s.begin);
+    at[tid] = position;
+    page[tid] = s.which < 0 ? -2 : page_of(a.c, a.r, a.r.tables + s.which * a.r.table_ld, position); // -2: no sequence
+  }
+  __syncthreads();
+  for (int i = tid; i < count * pairs; i += THREADS) angles[i] = turned((double)at[i / pairs] * a.c.turns[i % pairs]);
+  __syncthreads();
+  // groups of a head: of its pairs, then of what is not rotated; values go over whole
+  const int of_pairs = ((a.c.neighbours ? 2 * pairs : pairs) + 7) / 8, of_head = of_pairs + (rest + 7) / 8, of_value = head / 8;
+  const int q_heads = a.q.p ? a.q_heads : 0;
+  const int of_row = (q_heads + a.c.heads) * of_head + a.c.heads * of_value;
+  for (int i = tid; i < count * of_row; i += THREADS) {
+    const int r = i / of_row;
+    int g = i % of_row;
+    if (page[r] == -2) continue;
+    const long row = first + r;
+    if (g >= (q_heads + a.c.heads) * of_head) {
+      if (page[r] < 0) continue;
+      g -= (q_heads + a.c.heads) * of_head;
+      const int h = g / of_value, col = g % of_value * 8;
+      const Values8 v = widen(load8(static_cast<const T *>(a.v.p) + row * a.v.ld + h * head + col));
+      store8(static_cast<TC *>(a.c.v) + place_of(a.c, page[r], h, at[r]) + col, v);
+      continue;
+    }
+    const int h = g / of_head;
+    const bool query = h < q_heads;
+    if (!query && page[r] < 0) continue;
+    g %= of_head;
+    const T *in = query ? static_cast<const T *>(a.q.p) + row * a.q.ld + h * head : static_cast<const T *>(a.k.p) + row * a.k.ld + (h - q_heads) * head;
+    T *out = static_cast<T *>(a.out.p) + row * a.out.ld + h * head;
+    TC *key = static_cast<TC *>(a.c.k) + (query ? 0 : place_of(a.c, page[r], h - q_heads, at[r]));
+    const auto write = [&](int col, const Values8 &v, int n) {
+      if (query) write8(out + col, v, n);
+      else write8(key + col, v, n);
+    };
+    if (g >= of_pairs) {
+      const int col = (g - of_pairs) * 8;
+      write(2 * pairs + col, read8<SHORT>(in + 2 * pairs, col, rest), rest - col);
+    } else if (a.c.neighbours) {
+      const int col = g * 8;
+      Values8 v = read8<SHORT>(in, col, 2 * pairs);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 t = angles[r * pairs + min(col / 2 + k, pairs - 1)];
+        const float x = v.v[2 * k], y = v.v[2 * k + 1];
+        v.v[2 * k] = fmaf(x, t.x, -(y * t.y));
+        v.v[2 * k + 1] = fmaf(x, t.y, y * t.x);
+      }
+      write(col, v, 2 * pairs - col);
+    } else {
+      const int col = g * 8;
+      Values8 x = read8<SHORT>(in, col, pairs), y = read8<SHORT>(in + pairs, col, pairs);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const float2 t = angles[r * pairs + min(col + k, pairs - 1)];
+        const float u = fmaf(x.v[k], t.x, -(y.v[k] * t.y));
+        y.v[k] = fmaf(x.v[k], t.y, y.v[k] * t.x);
+        x.v[k] = u;
+      }
+      write(col, x, pairs - col);
+      write(pairs + col, y, pairs - col);
+    }
+  }
+}
+
+} // namespace
+
+void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cus, hipStream_t s) {
+  const int rotated = a.c.neighbours ? 2 * a.c.pairs : a.c.pairs, rest = a.c.head - 2 * a.c.pairs;
+  const bool is_short = (rotated && rotated < 8) || (rest && rest < 8);
+  const int each = (int)std::min<long>(MOST_ROWS_EACH, std::max<long>(1, a.r.rows / (8l * cus)));
+  const dim3 grid((unsigned)((a.r.rows + each - 1) / each));
+  with_adapter_types(dtype, cache_dtype, [&](auto x, auto c) {
+    using T = decltype(x);
+    using TC = decltype(c);
+    if (is_short) hipLaunchKernelGGL((k_cache_append<T, TC, true>), grid, dim3(THREADS), 0, s, a, each);
+    else hipLaunchKernelGGL((k_cache_append<T, TC, false>), grid, dim3(THREADS), 0, s, a, each);
+  });
+}
+
+} // namespace rpu_amd

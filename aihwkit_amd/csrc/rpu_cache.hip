@@ -1,0 +1,142 @@
+// C entry points of attention over a paged cache: what they check on the host before anything is launched.
+#include "cache.h"
+#include "operand_checks.h"
+
+#include <cmath>
+#include <vector>
+
+namespace rpu_amd {
+namespace {
+
+constexpr int MOST_PLACES = 1 << 30, MOST_HEADS = 1 << 16;
+
+CacheDev cache_dev(const rpu_cache *cache, int dtype) {
+  if (!cache) throw RpuError("The cache is null.");
+  const rpu_cache &c = *cache;
+  check_dtype(dtype);
+  check_dtype(c.dtype);
+  if (c.reserved) throw RpuError("A reserved field of the cache is not 0.");
+  if (dtype != RPU_F32 && c.dtype != dtype) throw RpuError("A cache beside 16-bit rows must be of the rows' type.");
+  if (c.pages < 1 || c.heads < 1 || c.heads > MOST_HEADS) throw RpuError("A cache has pages, and 1 .. 65536 heads.");
+  if (c.page_size < 1 || c.page_size > RPU_CACHE_MAX_PAGE || (c.page_size & (c.page_size - 1)))
+    throw RpuError("The size of a page must be a power of two up to 65536.");
+  if (c.head_size < 8 || c.head_size > RPU_CACHE_MAX_HEAD || c.head_size % 8) throw RpuError("The size of a head must be a multiple of 8 up to 256.");
+  if (c.pairs < 0 || 2 * (long)c.pairs > c.head_size) throw RpuError("A head cannot have so many pairs.");
+  if (c.pairs && !c.turns_dev) throw RpuError("The rotation's turns are null.");
+  if (!c.k_dev || !c.v_dev) throw RpuError("The cache's keys or values are null.");
+  if ((uintptr_t)c.k_dev % 16 || (uintptr_t)c.v_dev % 16) throw RpuError("The cache's keys and values must be aligned to 16 bytes.");
+  return {c.k_dev, c.v_dev, c.turns_dev, c.pages, __builtin_ctz((unsigned)c.page_size), c.heads, c.head_size, c.pairs, c.neighbours != 0};
+}
+CacheRowsDev rows_dev(const rpu_cache &c, const rpu_cache_rows *rows) {
+  if (!rows) throw RpuError("The rows' sequences are null.");
+  const rpu_cache_rows &r = *rows;
+  if (r.reserved) throw RpuError("A reserved field of the rows' sequences is not 0.");
+  check_rows(r.rows);
+  if (r.n < 1 || r.n > MOST_ROWS) throw RpuError("The number of sequences must be in 1 .. 2^28.");
+  if (!r.starts_dev && r.rows % r.n) throw RpuError("Without starts, the sequences have as many rows each.");
+  if (r.table_width < 1 || (long)r.table_width * c.page_size > MOST_PLACES) throw RpuError("A table must hold 1 .. 2^30 positions.");
+  if (!r.tables_dev || !r.lengths_dev) throw RpuError("The tables or lengths are null.");
+  if (r.n > 1 && (r.table_ld < r.table_width || r.table_ld > LONG_MAX / 8 / MOST_ROWS)) throw RpuError("The tables overlap or lie too far apart.");
+  return {r.tables_dev, r.lengths_dev, r.starts_dev, r.n > 1 ? r.table_ld : r.table_width, r.n, r.table_width * c.page_size, r.rows};
+}
+std::vector<Span> numbers(const rpu_cache &c, const rpu_cache_rows &r) { // what the kernels are steered by
+  std::vector<Span> all{matrix("the tables", r.tables_dev, r.table_ld, r.n, r.table_width, 4), dense("the lengths", r.lengths_dev, 4 * (size_t)r.n)};
+  if (r.starts_dev) all.push_back(dense("the starts", r.starts_dev, 4 * ((size_t)r.n + 1)));
+  if (c.pairs) all.push_back(dense("the turns", c.turns_dev, 8 * (size_t)c.pairs));
+  return all;
+}
+size_t cache_bytes(const rpu_cache &c) { return value_size(c.dtype) * (size_t)c.pages * c.heads * c.page_size * c.head_size; }
+int width_of(int heads, const rpu_cache &c) {
+  const long width = (long)heads * c.head_size;
+  if (heads < 1 || width > MOST_COLS) throw RpuError("A row must have at least one head, and at most 2^24 values.");
+  return (int)width;
+}
+
+} // namespace
+} // namespace rpu_amd
+
+using namespace rpu_amd;
+
+extern "C" {
+
+int rpu_cache_append(const rpu_cache *cache, const rpu_cache_rows *rows, const void *k_dev, long k_ld, const void *v_dev, long v_ld,
+                     const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads, int dtype, int device_id, void *stream) {
+  return guarded([&] {
+    AppendArgs a{};
+    a.c = cache_dev(cache, dtype);
+    a.r = rows_dev(*cache, rows);
+    const size_t e = value_size(dtype), bytes = cache_bytes(*cache);
+    const int width = width_of(cache->heads, *cache);
+    std::vector<Span> read = numbers(*cache, *rows), written{dense("the cache's keys", cache->k_dev, bytes), dense("the cache's values", cache->v_dev, bytes)};
+    read.push_back(matrix("k", k_dev, k_ld, a.r.rows, width, e));
+    read.push_back(matrix("v", v_dev, v_ld, a.r.rows, width, e));
+    apart(written[0], written[1]);
+    if (q_dev) {
+      const int q_width = width_of(q_heads, *cache);
+      const Span q = matrix("q", q_dev, q_ld, a.r.rows, q_width, e), out = matrix("the output", out_dev, out_ld, a.r.rows, q_width, e);
+      apart(out, q, true);
+      for (const Span &w : written) {
+        apart(w, q);
+        apart(out, w);
+      }
+      for (const Span &r : read) apart(out, r);
+    }
+    for (const Span &w : written)
+      for (const Span &r : read) apart(w, r);
+    if (!a.r.rows) return;
+    a.k = {const_cast<void *>(k_dev), k_ld};
+    a.v = {const_cast<void *>(v_dev), v_ld};
+    a.q = {const_cast<void *>(q_dev), q_ld};
+    a.out = {out_dev, out_ld};
+    a.q_heads = q_heads;
+    const Gpu gpu(device_id);
+    launch_cache_append(a, dtype, cache->dtype, gpu.cus(), (hipStream_t)stream);
+    check_launch();
+  });
+}
+
+size_t rpu_cache_attend_scratch(const rpu_cache *, const rpu_cache_rows *, int, int, int, int, int) { return 0; }
+
+int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads,
+                     int dtype, float scale, int window, int sinks, int longest, void *scratch_dev, size_t scratch_bytes, int device_id,
+                     void *stream) {
+  return guarded([&] {
+    AttendArgs a{};
+    a.c = cache_dev(cache, dtype);
+    a.r = rows_dev(*cache, rows);
+    const size_t e = value_size(dtype), bytes = cache_bytes(*cache);
+    const int width = width_of(q_heads, *cache);
+    if (q_heads % cache->heads) throw RpuError("The heads of a row must be a multiple of the cache's.");
+    if (!std::isfinite(scale)) throw RpuError("The scale must be finite.");
+    if (window < 0 || sinks < 0) throw RpuError("window and sinks must not be negative.");
+    if (sinks && !window) throw RpuError("Only a window has first tokens that stay visible.");
+    if (longest < 0) throw RpuError("longest must not be negative.");
+    const size_t need = rpu_cache_attend_scratch(cache, rows, q_heads, dtype, window, sinks, longest);
+    if (scratch_bytes < need) throw RpuError("The scratch memory is too small.");
+    const Span q = matrix("q", q_dev, q_ld, a.r.rows, width, e), out = matrix("the output", out_dev, out_ld, a.r.rows, width, e),
+               scratch = dense("the scratch memory", scratch_dev, need);
+    if (need && (uintptr_t)scratch_dev % 16) throw RpuError("The scratch memory is not aligned to 16 bytes.");
+    std::vector<Span> read = numbers(*cache, *rows);
+    read.push_back(dense("the cache's keys", cache->k_dev, bytes));
+    read.push_back(dense("the cache's values", cache->v_dev, bytes));
+    for (const Span &r : read) {
+      apart(out, r);
+      apart(scratch, r);
+    }
+    apart(out, q, true);
+    apart(scratch, q);
+    apart(scratch, out);
+    if (!a.r.rows) return;
+    a.q = {const_cast<void *>(q_dev), q_ld};
+    a.out = {out_dev, out_ld};
+    a.group = q_heads / cache->heads;
+    a.scale = scale;
+    a.window = window;
+    a.sinks = sinks;
+    const Gpu gpu(device_id);
+    launch_cache_attend(a, dtype, cache->dtype, gpu.cus(), (hipStream_t)stream);
+    check_launch();
+  });
+}
+
+} // extern "C"

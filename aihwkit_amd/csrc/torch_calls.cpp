@@ -17,6 +17,7 @@
 #include <c10/hip/HIPStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <vector>
 
 #include "../../include/rpu_amd.h"
@@ -610,6 +611,166 @@ PyObject *adapter_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
   return guarded([&] { return adapter_backward_checked(a, n); });
 }
 
+// Rows of heads, [rows][heads][head], the values of a row in a row.
+struct Heads {
+  const at::Tensor *t = nullptr;
+  int type = -1;
+  int64_t rows = 0, heads = 0;
+  long ld = 0;
+  bool take(PyObject *o, int64_t head) {
+    t = stored(o);
+    if (!t || !t->is_cuda() || t->dim() != 3 || (type = rpu_type(*t)) < 0) return false;
+    rows = t->size(0);
+    heads = t->size(1);
+    if (t->size(2) != head || heads < 1 || heads > 0x7fffffff || rows > 0x7fffffff || t->stride(2) != 1 || (heads > 1 && t->stride(1) != head)) return false;
+    ld = (long)(rows > 1 ? t->stride(0) : heads * head);
+    return ld >= heads * head;
+  }
+  bool like(const Heads &o) const { return type == o.type && t->device() == o.t->device(); }
+  const void *in() const { return t ? t->const_data_ptr() : nullptr; }
+};
+
+const at::Tensor *numbers_of(PyObject *o, const c10::Device &device, int64_t dims) {
+  const at::Tensor *t = stored(o);
+  return t && t->is_cuda() && t->device() == device && t->scalar_type() == at::kInt && t->dim() == dims ? t : nullptr;
+}
+
+// A paged cache and the sequences of a call's rows.
+struct CacheCall {
+  rpu_cache c{};
+  rpu_cache_rows r{};
+  // keys, values [pages][heads][page size][head size] of the shape that they had, turns or None
+  bool take(PyObject *keys, PyObject *values, PyObject *shape, PyObject *turns, PyObject *neighbours, c10::Device &device) {
+    const at::Tensor *k = stored(keys), *v = stored(values), *f = nullptr;
+    if (!k || !v || !k->is_cuda() || k->device() != v->device() || k->dim() != 4 || k->sizes() != v->sizes() || !k->is_contiguous() || !v->is_contiguous())
+      return false;
+    if (!PyTuple_Check(shape) || PyTuple_GET_SIZE(shape) != 4) return false;
+    for (int i = 0; i < 4; ++i) {
+      const long n = integer(PyTuple_GET_ITEM(shape, i));
+      if (n < 0 && PyErr_Occurred()) PyErr_Clear();
+      if (n != k->size(i) || n > 0x7fffffff) return false;
+    }
+    device = k->device();
+    if ((c.dtype = rpu_type(*k)) < 0 || rpu_type(*v) != c.dtype) return false;
+    if (turns != Py_None) {
+      f = stored(turns);
+      if (!f || f->device() != device || f->scalar_type() != at::kDouble || !f->is_contiguous()) return false;
+      c.turns_dev = static_cast<const double *>(f->const_data_ptr());
+      c.pairs = (int)f->numel();
+    }
+    c.k_dev = k->data_ptr();
+    c.v_dev = v->data_ptr();
+    c.pages = (int)k->size(0);
+    c.heads = (int)k->size(1);
+    c.page_size = (int)k->size(2);
+    c.head_size = (int)k->size(3);
+    c.neighbours = neighbours && truth(neighbours);
+    return true;
+  }
+  bool take_rows(PyObject *tables, PyObject *lengths, PyObject *starts, const c10::Device &device, int64_t rows) {
+    const at::Tensor *t = numbers_of(tables, device, 2), *l = numbers_of(lengths, device, 1), *s = nullptr;
+    if (!t || !l || !l->is_contiguous()) return false;
+    const int64_t n = t->size(0), width = t->size(1);
+    if (n < 1 || n > 0x7fffffff || width < 1 || width > 0x7fffffff || l->numel() != n || (width > 1 && t->stride(1) != 1)) return false;
+    if (n > 1 && t->stride(0) < width) return false;
+    if (starts != Py_None) {
+      s = numbers_of(starts, device, 1);
+      if (!s || !s->is_contiguous() || s->numel() != n + 1) return false;
+      r.starts_dev = static_cast<const int32_t *>(s->const_data_ptr());
+    }
+    r.tables_dev = static_cast<const int32_t *>(t->const_data_ptr());
+    r.lengths_dev = static_cast<const int32_t *>(l->const_data_ptr());
+    r.table_ld = (long)(n > 1 ? t->stride(0) : width);
+    r.n = (int)n;
+    r.table_width = (int)width;
+    r.rows = (int)rows;
+    return true;
+  }
+};
+
+// the given output, or a new one (zeros where rows may belong to no sequence); false: not the plain case
+bool take_heads_out(PyObject *o, const Heads &x, bool zeros, at::Tensor &keep, long &ld) {
+  if (o != Py_None) {
+    Heads y;
+    if (!y.take(o, x.t->size(2)) || !y.like(x) || y.t->sizes() != x.t->sizes()) return false;
+    keep = *y.t;
+    ld = y.ld;
+    return true;
+  }
+  const auto options = x.t->options().requires_grad(false);
+  keep = zeros ? at::zeros(x.t->sizes(), options) : at::empty(x.t->sizes(), options);
+  ld = (long)(x.heads * x.t->size(2));
+  return true;
+}
+
+// a number of 0 .. 2^31 - 1
+bool take_count(PyObject *o, int &value) {
+  if (!PyLong_CheckExact(o)) return false;
+  const long v = integer(o);
+  if (v == -1 && PyErr_Occurred()) PyErr_Clear();
+  value = (int)v;
+  return v >= 0 && v <= 0x7fffffff;
+}
+
+// (cache keys, values, shape, turns, neighbours, keys, values, tables, lengths, starts, queries, out, non_blocking) -> (rotated queries or None,),
+// or None
+PyObject *cache_append_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments expected"), nullptr;
+  CacheCall c;
+  Heads k, v, q;
+  at::Tensor y;
+  long y_ld = 0;
+  c10::Device device(c10::kCPU);
+  if (!c.take(a[0], a[1], a[2], a[3], a[4], device) || !k.take(a[5], c.c.head_size) || k.t->device() != device || k.heads != c.c.heads) Py_RETURN_NONE;
+  if (!v.take(a[6], c.c.head_size) || !v.like(k) || v.t->sizes() != k.t->sizes() || !c.take_rows(a[7], a[8], a[9], device, k.rows)) Py_RETURN_NONE;
+  if (k.type != RPU_F32 && k.type != c.c.dtype) Py_RETURN_NONE;
+  if (a[10] != Py_None) {
+    if (!q.take(a[10], c.c.head_size) || !q.like(k) || q.rows != k.rows || !take_heads_out(a[11], q, c.r.starts_dev, y, y_ld)) Py_RETURN_NONE;
+  } else if (a[11] != Py_None) {
+    Py_RETURN_NONE;
+  }
+  const hipStream_t s = stream_of(*k.t);
+  void *yp = y.defined() ? y.data_ptr() : nullptr;
+  const void *kp = k.in(), *vp = v.in(), *qp = q.in();
+  const bool ok = call(
+      [&] { return rpu_cache_append(&c.c, &c.r, kp, k.ld, vp, v.ld, qp, q.ld, yp, y_ld, (int)q.heads, k.type, device.index(), s); }, s, truth(a[12]));
+  return ok ? tuple_of(std::move(y), {}, {}, 1) : nullptr;
+}
+PyObject *cache_append(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return cache_append_checked(a, n); });
+}
+
+// (cache keys, values, shape, queries, tables, lengths, starts, scale, window, sinks, longest, out, non_blocking) -> out, or None
+PyObject *cache_attend_checked(PyObject *const *a, Py_ssize_t n) {
+  if (n != 13) return PyErr_Format(PyExc_TypeError, "13 arguments expected"), nullptr;
+  CacheCall c;
+  Heads q;
+  at::Tensor y, scratch;
+  long y_ld = 0;
+  int window = 0, sinks = 0, longest = 0;
+  c10::Device device(c10::kCPU);
+  if (!c.take(a[0], a[1], a[2], Py_None, nullptr, device) || !q.take(a[3], c.c.head_size) || q.t->device() != device) Py_RETURN_NONE;
+  if (!c.take_rows(a[4], a[5], a[6], device, q.rows) || (q.type != RPU_F32 && q.type != c.c.dtype)) Py_RETURN_NONE;
+  if ((a[7] != Py_None && !PyFloat_CheckExact(a[7])) || !take_count(a[8], window) || !take_count(a[9], sinks)) Py_RETURN_NONE;
+  if (a[10] != Py_None && !take_count(a[10], longest)) Py_RETURN_NONE;
+  if (!take_heads_out(a[11], q, c.r.starts_dev, y, y_ld)) Py_RETURN_NONE;
+  const float scale = a[7] == Py_None ? (float)(1.0 / std::sqrt((double)c.c.head_size)) : (float)PyFloat_AS_DOUBLE(a[7]);
+  const size_t bytes = rpu_cache_attend_scratch(&c.c, &c.r, (int)q.heads, q.type, window, sinks, longest);
+  if (bytes) scratch = at::empty({(int64_t)bytes}, q.t->options().dtype(at::kByte).requires_grad(false));
+  const hipStream_t s = stream_of(*q.t);
+  void *yp = y.data_ptr(), *sp = bytes ? scratch.data_ptr() : nullptr;
+  const void *qp = q.in();
+  const bool ok = call(
+      [&] {
+        return rpu_cache_attend(&c.c, &c.r, qp, q.ld, yp, y_ld, (int)q.heads, q.type, scale, window, sinks, longest, sp, bytes, device.index(), s);
+      },
+      s, truth(a[12]));
+  return ok ? THPVariable_Wrap(std::move(y)) : nullptr;
+}
+PyObject *cache_attend(PyObject *, PyObject *const *a, Py_ssize_t n) {
+  return guarded([&] { return cache_attend_checked(a, n); });
+}
+
 PyMethodDef methods[] = {
     {"forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(forward)), METH_FASTCALL, nullptr},
     {"backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(backward)), METH_FASTCALL, nullptr},
@@ -623,6 +784,8 @@ PyMethodDef methods[] = {
     {"adapter_plan", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_plan)), METH_FASTCALL, nullptr},
     {"adapter_forward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_forward)), METH_FASTCALL, nullptr},
     {"adapter_backward", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(adapter_backward)), METH_FASTCALL, nullptr},
+    {"cache_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_append)), METH_FASTCALL, nullptr},
+    {"cache_attend", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(cache_attend)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "rpu_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -808,6 +808,46 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
                          const void *base_dev, long base_ld, void *dx_dev, long dx_ld, void *da_dev, void *db_dev, int dtype,
                          int rows, void *scratch_dev, size_t scratch_bytes, int device_id, void *stream);
 
+/* Attention between tiles over a paged cache.  k_dev, v_dev [pages][heads][page_size][head_size]: dense, aligned to 16 bytes, of `dtype`.
+ * turns_dev [pairs], doubles: rotation of each pair of a head per position, in turns (radians / 2 pi); pairs = 0: no rotation.  Pair i is
+ * columns (i, i + pairs), with `neighbours` (2 i, 2 i + 1); the columns from 2 pairs on are not rotated.  page_size: a power of two
+ * up to RPU_CACHE_MAX_PAGE; head_size: a multiple of 8 up to RPU_CACHE_MAX_HEAD. */
+#define RPU_CACHE_MAX_PAGE 65536
+#define RPU_CACHE_MAX_HEAD 256
+typedef struct rpu_cache {
+  void *k_dev, *v_dev;
+  const double *turns_dev;
+  int32_t pages, page_size, heads, head_size, dtype, pairs, neighbours, reserved;
+} rpu_cache;
+
+/* The new rows of n sequences: those of sequence s are starts[s] .. starts[s + 1] - 1 (starts_dev [n + 1], not decreasing), without
+ * starts_dev rows / n each.  lengths_dev [n]: positions of a sequence, its new rows included, so that the i-th of its m rows is at
+ * lengths[s] - m + i.  Position j lies on page tables[s][j / page_size] (tables_dev [n][table_width], rows table_ld apart) in slot
+ * j % page_size.  What has no page -- a page number outside 0 .. pages - 1, a position below 0 or beyond the table -- is not written and not
+ * seen.  table_width * page_size is at most 2^30.  All three are read when the kernels run, so that captured calls follow them. */
+typedef struct rpu_cache_rows {
+  const int32_t *tables_dev, *lengths_dev, *starts_dev;
+  long table_ld;
+  int32_t n, table_width, rows, reserved;
+} rpu_cache_rows;
+
+/* Writes the new rows' keys (rotated by their positions) and values into the cache.  k_dev, v_dev: rows of heads * head_size values; q_dev
+ * (null: none): rows of q_heads * head_size values, whose rotation goes to out_dev, which may be q_dev.  `dtype` of k, v, q and out: RPU_F32
+ * beside any cache, otherwise the cache's.  Rows of no sequence are left as they are.  Two rows for one place of the cache: either's. */
+int rpu_cache_append(const rpu_cache *cache, const rpu_cache_rows *rows, const void *k_dev, long k_ld, const void *v_dev, long v_ld,
+                     const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads, int dtype, int device_id, void *stream);
+
+/* Attention of the new rows over the cache, which holds them by then: out = sum_j w_j v_j / sum_j w_j with w_j = exp(scale q k_j - max)
+ * over the positions j that the row at position p sees: 0 <= j <= p and, with a window > 0, j > p - window or j < sinks.  A row that sees
+ * nothing, or whose weights are all zero, becomes zeros.  q_heads: a multiple of the cache's heads, each of which serves as many neighbouring ones.
+ * out_dev may be q_dev; rows of no sequence are left as they are.  longest: what no length exceeds (0: what the tables hold); how the
+ * work is shared goes by it, results are right without it.  Values of places that a row does not see do not reach it, infinities and NaN
+ * included.  scratch: rpu_cache_attend_scratch bytes (0: may be null), aligned to 16, used until the call's work is done. */
+size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *rows, int q_heads, int dtype, int window, int sinks, int longest);
+int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads,
+                     int dtype, float scale, int window, int sinks, int longest, void *scratch_dev, size_t scratch_bytes, int device_id,
+                     void *stream);
+
 /* ---- inspection hooks (mirror the reference's debug hooks) ------------------------------ */
 
 /* After rpu_tile_update with a stochastic pulse type: copies the packed pulse words of that call
