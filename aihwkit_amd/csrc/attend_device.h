@@ -1,0 +1,517 @@
+// Attention of new rows over a paged cache: out = sum_j w_j v_j / sum_j w_j, w_j = exp(scale q k_j - max), over the positions that a row sees.
+//
+// The heads of a row that share one of the cache count as rows of their own beside each other ("lines": line = token * group + head of the group),
+// so that keys and values are read once for all of them.  A wave has 32 lines, one to a lane and the lane 32 further on, and goes over tiles of
+// positions with a running maximum and sum: scores S^T = K Q^T and sums O^T = V^T W^T in matrix instructions of 32 x 32 results, whose
+// columns are the lines -- maximum, sum and rescaling stay in the lane, and the weights are the second product's operand as the first leaves
+// them: its terms may come in any order, so that values are read (transposed, from LDS) in the order that the lanes have.
+//
+// Matrix operands are 16-bit.  Of 16-bit rows and caches they are the numbers themselves, weights are rounded to that type (half a step of it,
+// relative to each weight, in a mean of values).  Floats go in parts: beside bf16 and floats three bf16 each, beside halves two halves, lifted
+// by a power of two; products of parts that add up to less than 2^-24 of the largest are left out.
+#pragma once
+#include "cache.h"
+
+#include <type_traits>
+
+namespace rpu_amd {
+namespace attend {
+
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+constexpr float NONE = -__builtin_inff(), LOG2E = 1.44269504088896340736f;
+
+// How rows of T beside a cache of TC, heads of up to 32 D32 values, are worked on.
+template <typename T, typename TC, int D32, bool FEW> struct Shape {
+  static constexpr bool HALF = __is_same(TC, _Float16);
+  using M = std::conditional_t<__is_same(TC, float), __bf16, TC>; // of matrix operands
+  static constexpr int KP = sizeof(TC) == 4 ? 3 : 1;                         // parts of keys and values
+  static constexpr int QP = sizeof(T) == 2 ? 1 : HALF ? 2 : 3;               // of queries and weights
+  static constexpr int DP = D32 <= 2 ? 64 : D32 <= 4 ? 128 : 256, CHUNKS = DP / 8; // a head in LDS, and its pieces of 16 bytes
+  static constexpr int TILE = FEW || KP == 3 || DP == 256 ? 32 : 64;         // positions
+  static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
+  static constexpr int PLANE = TILE * DP, TILE_VALUES = 2 * KP * PLANE;      // of one part, of all parts of keys and values
+  static constexpr int KEY_WAVES = !FEW ? 1 : KP == 1 || DP == 64 ? 4 : DP == 128 ? 2 : 1; // that share a line's positions
+  static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
+  static constexpr int LOADS = TILE * CHUNKS / LOADERS;
+  static constexpr int STAGES = FEW || (KP == 3 && DP == 256) ? 1 : 2;
+  static constexpr int PER_SIMD = D32 <= 4 && KP == 1 && (QP == 1 || D32 <= 2) ? 2 : 1; // waves, as the registers allow
+  static constexpr int LDS = (FEW ? KEY_WAVES : STAGES) * TILE_VALUES * 2;
+  static_assert(!FEW || TILE_VALUES * 2 >= 32 * DP * 4, "the sums of a wave fit where its tile was");
+};
+
+// 16 bytes of a row in LDS lie at chunk ^ turn: 16 rows that read the same chunk, and four neighbouring ones that read four, touch all banks
+template <int CHUNKS> __device__ __forceinline__ int turn_of(int row) {
+  return CHUNKS == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
+}
+
+template <typename M> __device__ __forceinline__ floatx16 multiply(u32x4 a, u32x4 b, floatx16 c) {
+  if constexpr (__is_same(M, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// two floats as PARTS of type M each (rounded, what is left goes on); the largest floats stay finite, an infinity is in the second part
+template <typename M, int PARTS> __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[PARTS]) {
+#pragma unroll
+  for (int k = 0; k < PARTS; ++k) {
+    if constexpr (__is_same(M, __bf16)) {
+      constexpr float MOST = 0x1.fep127f;
+      part[k] = PARTS == 1 || k ? pack2(a, b, __bf16{}) : pack2(__builtin_amdgcn_fmed3f(a, -MOST, MOST), __builtin_amdgcn_fmed3f(b, -MOST, MOST), __bf16{});
+      if (k + 1 < PARTS) {
+        a -= __uint_as_float(part[k] << 16);
+        b -= __uint_as_float(part[k] & 0xffff0000u);
+      }
+    } else {
+      part[k] = pack2(a, b, _Float16{});
+      if (k + 1 < PARTS) {
+        const f16x2 r = __builtin_bit_cast(f16x2, part[k]);
+        a -= (float)r.x;
+        b -= (float)r.y;
+      }
+    }
+  }
+}
+template <typename M> __device__ __forceinline__ float value_of(uint16_t v) { return to_float(__builtin_bit_cast(M, v)); }
+// one of two 16-bit values is infinite or NaN
+template <typename M> __device__ __forceinline__ bool not_finite2(uint32_t v) {
+  constexpr uint32_t FIELD = __is_same(M, __bf16) ? 0x7f807f80u : 0x7c007c00u, STEP = __is_same(M, __bf16) ? 0x00800080u : 0x04000400u;
+  return ((v & FIELD) + STEP) & 0x80008000u;
+}
+__device__ __forceinline__ float most(float a, float b) { return __builtin_elementwise_maximum(a, b); } // NaN if one is: no quieting before it
+__device__ __forceinline__ float half_and_half(float v, float &other) { // of the lanes below 32, and of the others
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  other = __uint_as_float(r[1]);
+  return __uint_as_float(r[0]);
+}
+
+// Lines of a sequence, some of its heads and positions: what a workgroup does.
+struct Job {
+  Sequence s;
+  int head, line, lines, split; // head of the cache; first line, lines of the sequence
+};
+__device__ __forceinline__ int lines_of(const Sequence &s, int group) { return (s.end - s.begin) * group; }
+
+// number `at` of launch_units: the parts of one head of a sequence beside each other, and on one of the eight L2 caches
+__device__ __forceinline__ bool job_few(const AttendArgs &a, long at, Job &job) {
+  const long units = (long)a.r.n * a.c.heads;
+  if (at >= units * a.few_splits) return false;
+  job.split = (int)(at % a.few_splits);
+  at /= a.few_splits;
+  job.head = (int)(at % a.c.heads);
+  job.s = sequence_at(a.r, (int)(at / a.c.heads));
+  job.line = 0;
+  job.lines = lines_of(job.s, a.group);
+  return job.lines > 0 && job.lines <= a.few;
+}
+// Tiles of LINES lines: sequence s has those from (starts[s] * group) / LINES + s on, one more than it can need at most.
+template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &a, long at, Job &job) {
+  if (at >= (long)a.tiles * a.c.heads * a.splits) return false;
+  job.split = (int)(at % a.splits);
+  at /= a.splits;
+  const int tile = a.tiles - 1 - (int)(at % a.tiles); // long ones first
+  job.head = (int)(at / a.tiles);
+  int which, first;
+  if (a.r.starts) {
+    int low = 0, high = a.r.n;
+    const auto base = [&](int s) { return (long)min(max(a.r.starts[s], 0), a.r.rows) * a.group / LINES + s; };
+    while (high - low > 1) {
+      const int middle = (low + high) / 2;
+      if (base(middle) <= tile) low = middle;
+      else high = middle;
+    }
+    which = low;
+    first = (int)max(tile - base(low), 0l);
+  } else {
+    const int each = a.tiles / a.r.n;
+    which = tile / each;
+    first = tile % each;
+  }
+  job.s = sequence_at(a.r, which);
+  job.lines = lines_of(job.s, a.group);
+  if ((long)first * LINES >= job.lines || job.lines <= a.few) return false;
+  job.line = first * LINES;
+  return true;
+}
+
+template <typename T, typename TC, int D32, bool FEW>
+__global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a) {
+  using S = Shape<T, TC, D32, FEW>;
+  using M = typename S::M;
+  constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
+  extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int loader = FEW ? lane : tid;
+  // neighbouring workgroups run on different L2 caches: a run of jobs to each
+  const long per_cache = (gridDim.x + 7) / 8, at = (blockIdx.x % 8) * per_cache + blockIdx.x / 8;
+  Job job;
+  if (FEW ? !job_few(a, at, job) : !job_many<S::LINES>(a, at, job)) return;
+  const int group = a.group, head = a.c.head;
+
+  // the line of this lane
+  const int line = job.line + (FEW ? 0 : 32 * wave) + (lane & 31);
+  const bool live = line < job.lines;
+  const int token = live ? line / group : 0, row = job.s.begin + token, q_head = job.head * group + (live ? line % group : 0);
+  const auto place = [](long p) { return (int)min(max(p, -1l), 1l << 30); };
+  const int last_seen = live ? place(job.s.first + token) : -1;                                     // positions <= last_seen
+  const int before = a.window ? place(job.s.first + token - a.window) : -1;                         // and > before, or < sinks
+  // positions that some line of the workgroup sees, and those that all of them do
+  const int token0 = job.line / group, token1 = (min(job.line + S::LINES, job.lines) - 1) / group;
+  const int end = min(place(job.s.first + token1) + 1, a.r.places), low = a.window ? min(place(job.s.first + token0 - a.window) + 1, end) : 0;
+  const int all_last = place(job.s.first + token0), all_before = a.window ? place(job.s.first + token1 - a.window) : -1;
+  const int sink_end = low > 0 ? min(a.sinks, end) : 0;
+  const int sink_tiles = (sink_end + TILE - 1) / TILE, first_tile = max(low / TILE, sink_tiles), tiles = sink_tiles + max((end + TILE - 1) / TILE - first_tile, 0);
+  const int splits = FEW ? a.few_splits : a.splits, each = max((tiles + splits - 1) / splits, FEW ? ATTEND_FEW_LEAST : 1);
+  const int from = min(job.split * each, tiles), to = min(from + each, tiles), step = S::KEY_WAVES;
+  const auto base_of = [&](int t) { return (t < sink_tiles ? t : first_tile + t - sink_tiles) * TILE; };
+
+  // queries: 8 values of each 16 to a lane
+  u32x4 q[QP][STEPS];
+  float c = a.scale * LOG2E; // of the exponents, in powers of two
+  {
+    const T *at_q = static_cast<const T *>(a.q.p) + (live ? row * a.q.ld + q_head * head : 0l);
+    Packed8<T> p[STEPS];
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const int d = 16 * i + 8 * half;
+      p[i] = load8(at_q + (d < head ? d : 0));
+    }
+    const bool none = a.scale == 0.0f;
+    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
+    float lift = 1.0f;
+    if constexpr (QP == 2) {
+      float m = 0.0f;
+#pragma unroll
+      for (int i = 0; i < STEPS; ++i) {
+        const Values8 v = widen(p[i]);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) m = 16 * i + 8 * half < head ? fmaxf(m, fminf(fabsf(v.v[k]), 0x1.fffffep127f)) : m;
+      }
+      m = fmaxf(m, __shfl_xor(m, 32));
+      lift = lift_of(m);
+    }
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) {
+      const bool there = live && 16 * i + 8 * half < head && !none;
+      if constexpr (QP == 1) {
+        q[0][i] = p[i].q;
+        if (a.scale < 0.0f) q[0][i] ^= 0x80008000u;
+        q[0][i] = there ? q[0][i] : u32x4{};
+      } else {
+        const Values8 v = widen(p[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          uint32_t part[QP];
+          split2<M>(there ? v.v[2 * k] * sign * lift : 0.0f, there ? v.v[2 * k + 1] * sign * lift : 0.0f, part);
+#pragma unroll
+          for (int j = 0; j < QP; ++j) q[j][i][k] = part[j];
+        }
+      }
+    }
+    c = none ? LOG2E : fabsf(c) * inverse_of(lift);
+  }
+
+  // Tiles: page numbers are under way two tiles ahead, keys and values one.
+  const int *table = a.r.tables + job.s.which * a.r.table_ld;
+  const auto page_at = [&](int t) { // of position `lane` of a tile; -1: not wanted, or not there
+    const int j = base_of(t) + lane;
+    const bool wanted = t < to && lane < TILE && j < end && (j >= low || j < sink_end);
+    const int page = table[wanted ? j >> a.c.page_shift : 0];
+    return wanted && page >= 0 && page < a.c.pages ? page : -1;
+  };
+  Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
+  uint32_t loaded = 0;
+  const auto load = [&](int t, int page) {
+    const int base = base_of(t);
+    loaded = 0;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int piece = i * S::LOADERS + loader, r = piece / CHUNKS, chunk = piece % CHUNKS, mine = __shfl(page, r);
+      const bool ok = mine >= 0 && chunk * 8 < head;
+      const long offset = ok ? place_of(a.c, mine, job.head, base + r) + chunk * 8 : 0l;
+      k_ahead[i] = load8(static_cast<const TC *>(a.c.k) + offset);
+      v_ahead[i] = load8(static_cast<const TC *>(a.c.v) + offset);
+      loaded |= ok ? 1u << i : 0u;
+    }
+  };
+  // keys and values into LDS, zeros where there are none; whether some value is not finite
+  const auto put = [&](uint16_t *tile) {
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int piece = i * S::LOADERS + loader, r = piece / CHUNKS, chunk = piece % CHUNKS;
+      const bool ok = (loaded >> i) & 1;
+      uint16_t *to_k = tile + r * DP + (chunk ^ turn_of<CHUNKS>(r)) * 8, *to_v = to_k + KP * S::PLANE;
+      if constexpr (KP == 1) {
+        const u32x4 k = ok ? (u32x4)k_ahead[i].q : u32x4{}, v = ok ? (u32x4)v_ahead[i].q : u32x4{};
+        *reinterpret_cast<u32x4 *>(to_k) = k;
+        *reinterpret_cast<u32x4 *>(to_v) = v;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) bad |= not_finite2<M>(v[n]);
+      } else {
+        const Values8 k = widen(k_ahead[i]), v = widen(v_ahead[i]);
+        u32x4 out[2][KP];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          uint32_t part[KP];
+          split2<M>(ok ? k.v[2 * n] : 0.0f, ok ? k.v[2 * n + 1] : 0.0f, part);
+#pragma unroll
+          for (int j = 0; j < KP; ++j) out[0][j][n] = part[j];
+          split2<M>(ok ? v.v[2 * n] : 0.0f, ok ? v.v[2 * n + 1] : 0.0f, part);
+#pragma unroll
+          for (int j = 0; j < KP; ++j) {
+            out[1][j][n] = part[j];
+            bad |= not_finite2<M>(part[j]);
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < KP; ++j) {
+          *reinterpret_cast<u32x4 *>(to_k + j * S::PLANE) = out[0][j];
+          *reinterpret_cast<u32x4 *>(to_v + j * S::PLANE) = out[1][j];
+        }
+      }
+    }
+    return bad;
+  };
+  const auto all_there = [&] {
+    if constexpr (FEW) wave_sync();
+    else __syncthreads();
+  };
+
+  float m = NONE, power = NONE, total = 0.0f; // largest score, as a power of two, sum of the weights (of this lane's positions)
+  floatx16 sums[D32] = {};
+  uint16_t *const lds = attend_lds + (FEW ? wave * S::TILE_VALUES : 0);
+  int t = from + (FEW ? wave : 0), page = -1, next_page = -1;
+  uint64_t there = 0;
+  if (t < to) {
+    page = page_at(t);
+    next_page = page_at(t + step);
+    load(t, page);
+    there = __ballot(page >= 0);
+  }
+  for (int turn = 0; t < to; t += step, turn ^= 1) {
+    uint16_t *const tile = lds + (S::STAGES == 2 ? turn * S::TILE_VALUES : 0);
+    const int base = base_of(t);
+    constexpr uint64_t ALL = TILE == 64 ? ~0ull : (1ull << TILE % 64) - 1;
+    const uint64_t here = there;
+    const bool masked = here != ALL || base + TILE - 1 > all_last || (a.window && base <= all_before && base + TILE > a.sinks);
+    if (S::STAGES == 1) all_there(); // the tile before has been read
+    bool bad = put(tile);
+    if (masked) { // values that are not finite and not seen by all lines must not meet their weights of zero
+      if constexpr (FEW) {
+        bad = __any(bad);
+        wave_sync();
+      } else {
+        bad = __syncthreads_or(bad);
+      }
+    } else {
+      bad = false;
+      all_there();
+    }
+    if (t + step < to) {
+      load(t + step, next_page);
+      there = __ballot(next_page >= 0);
+      next_page = page_at(t + 2 * step);
+    }
+
+    // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
+    floatx16 score[BLOCKS] = {};
+    const int row_k = lane & 31;
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i)
+#pragma unroll
+      for (int n = 0; n < BLOCKS; ++n)
+#pragma unroll
+        for (int j = 0; j < KP; ++j) {
+          const int r = 32 * n + row_k;
+          const u32x4 k = *reinterpret_cast<const u32x4 *>(tile + j * S::PLANE + r * DP + ((2 * i + half) ^ turn_of<CHUNKS>(r)) * 8);
+#pragma unroll
+          for (int l = 0; l < QP; ++l)
+            if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
+        }
+    const auto seen = [&](int n) { // position n of the tile
+      return base + n <= last_seen && (base + n > before || base + n < a.sinks) && ((here >> n) & 1);
+    };
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < BLOCKS; ++n)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) score[n][i] = seen(32 * n + 8 * (i / 4) + 4 * half + i % 4) ? score[n][i] : NONE;
+    }
+    float now = score[0][0], other;
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) now = most(now, score[n][i]);
+    now = half_and_half(now, other);
+    now = most(most(now, other), m);
+    const float less = now == NONE ? 0.0f : now * c;
+    if (!__all(now == m)) {
+      const float shrink = __builtin_amdgcn_exp2f(power - less);
+      total *= shrink;
+#pragma unroll
+      for (int n = 0; n < D32; ++n) sums[n] *= shrink;
+      m = now;
+      power = now == NONE ? NONE : less;
+    }
+    // weights, as operands of 16 positions each: 4 half + 8 (e / 4) + e % 4
+    u32x4 weights[QP][2 * BLOCKS];
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n)
+#pragma unroll
+      for (int i = 0; i < 16; i += 2) {
+        float w0 = __builtin_amdgcn_exp2f(fmaf(score[n][i], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[n][i + 1], c, -less));
+        total += w0 + w1;
+        if constexpr (S::HALF) { // up to 2^15, so that small ones keep their bits; `total` is of the others
+          w0 *= 0x1p15f;
+          w1 *= 0x1p15f;
+        }
+        uint32_t part[QP];
+        split2<M>(w0, w1, part);
+#pragma unroll
+        for (int l = 0; l < QP; ++l) weights[l][2 * n + i / 8][i % 8 / 2] = part[l];
+      }
+    uint16_t *const values = tile + KP * S::PLANE;
+    if (bad) { // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
+#pragma unroll 1
+      for (int r = 0; r < TILE; ++r) {
+        const bool mine = seen(r);
+#pragma unroll
+        for (int n = 0; n < D32; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            float v = 0.0f;
+#pragma unroll
+            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::PLANE + r * DP + ((4 * n + i / 4) ^ turn_of<CHUNKS>(r)) * 8 + 4 * half + i % 4]);
+            if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
+          }
+      }
+      all_there();
+      for (int i = loader; i < KP * S::PLANE / 2; i += S::LOADERS) {
+        uint32_t *const two = reinterpret_cast<uint32_t *>(values) + i;
+        const uint32_t v = *two;
+        if (not_finite2<M>(v)) *two = (not_finite2<M>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite2<M>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
+      }
+      all_there();
+    }
+    const int li = lane & 15, row_v = 4 * half + (li >> 2), chunk_v = 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
+#pragma unroll
+    for (int b = 0; b < 2 * BLOCKS; ++b)
+#pragma unroll
+      for (int n = 0; n < D32; ++n)
+#pragma unroll
+        for (int j = 0; j < KP; ++j) {
+          s16x4 v[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int r = 16 * b + 8 * e + row_v;
+            uint16_t *p = values + j * S::PLANE + r * DP + ((4 * n + chunk_v) ^ turn_of<CHUNKS>(r)) * 8 + (li & 1) * 4;
+            v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
+          }
+          const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
+          const u32x4 both = {v0[0], v0[1], v1[0], v1[1]};
+#pragma unroll
+          for (int l = 0; l < QP; ++l)
+            if (j + l < 3) sums[n] = multiply<M>(both, weights[l][b], sums[n]);
+        }
+  }
+  {
+    float other;
+    const float mine = half_and_half(total, other);
+    total = mine + other;
+  }
+  if constexpr (S::HALF) total *= 0x1p15f;
+  if constexpr (!FEW) {
+    if (!live) return;
+    const long unit = (long)row * (a.c.heads * group) + q_head;
+    if (a.splits > 1) {
+      const long part = (long)job.split * a.r.rows * (a.c.heads * group) + unit;
+      if (!half) a.stats[part] = float2{power, total};
+#pragma unroll
+      for (int n = 0; n < D32; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int d = 32 * n + 8 * i + 4 * half;
+          if (d < head) *reinterpret_cast<f32x4 *>(a.part + part * head + d) = f32x4{sums[n][4 * i], sums[n][4 * i + 1], sums[n][4 * i + 2], sums[n][4 * i + 3]};
+        }
+      return;
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    T *out = static_cast<T *>(a.out.p) + row * a.out.ld + q_head * head;
+#pragma unroll
+    for (int n = 0; n < D32; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * n + 8 * i + 4 * half;
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : sums[n][4 * i + k] * inverse;
+        if (d < head) store_first(out + d, v, 4);
+      }
+  } else {
+    // the waves' parts meet in LDS, each where its tile was
+    __shared__ float2 stats[S::KEY_WAVES][32];
+    __shared__ float2 joined[32];
+    if (!half) stats[wave][lane & 31] = float2{power, total};
+    __syncthreads();
+    float top = NONE, sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < S::KEY_WAVES; ++w) top = most(top, stats[w][lane & 31].x);
+    const auto shrink_of = [&](float p) { return p == NONE ? 0.0f : __builtin_amdgcn_exp2f(p - top); };
+#pragma unroll
+    for (int w = 0; w < S::KEY_WAVES; ++w) sum = fmaf(stats[w][lane & 31].y, shrink_of(stats[w][lane & 31].x), sum);
+    if (wave == 0 && !half) joined[lane & 31] = float2{top, sum};
+    const float shrink = shrink_of(power);
+    float *const mine = reinterpret_cast<float *>(lds) + (lane & 31) * DP;
+    if (live)
+#pragma unroll
+      for (int n = 0; n < D32; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int piece = 8 * n + 2 * i + half; // of four values
+          *reinterpret_cast<f32x4 *>(mine + (piece ^ (lane & (DP / 4 - 1) & 31)) * 4) =
+              f32x4{sums[n][4 * i], sums[n][4 * i + 1], sums[n][4 * i + 2], sums[n][4 * i + 3]} * shrink;
+        }
+    __syncthreads();
+    const int pieces = head / 4, count = job.lines * pieces;
+    for (int i = tid; i < count; i += S::WAVES * 64) {
+      const int l = i / pieces, piece = i % pieces;
+      f32x4 v = {};
+#pragma unroll
+      for (int w = 0; w < S::KEY_WAVES; ++w)
+        v += *reinterpret_cast<const f32x4 *>(reinterpret_cast<const float *>(attend_lds + w * S::TILE_VALUES) + l * DP + (piece ^ (l & (DP / 4 - 1) & 31)) * 4);
+      const float2 both = joined[l];
+      if (a.few_splits > 1) {
+        const long part = (((long)job.split * a.r.n + job.s.which) * a.c.heads + job.head) * a.few + l;
+        *reinterpret_cast<f32x4 *>(a.few_part + part * head + piece * 4) = v;
+        if (piece == 0) a.few_stats[part] = both;
+      } else {
+        const float inverse = both.y == 0.0f ? 0.0f : 1.0f / both.y;
+        float r[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) r[k] = both.y == 0.0f ? 0.0f : v[k] * inverse;
+        store_first(static_cast<T *>(a.out.p) + (job.s.begin + l / group) * a.out.ld + (job.head * group + l % group) * head + piece * 4, r, 4);
+      }
+    }
+  }
+}
+
+template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t s) {
+  const auto with = [&](auto d32) {
+    constexpr int D32 = decltype(d32)::value;
+    const auto go = [&](auto few, long jobs) {
+      constexpr bool FEW = decltype(few)::value;
+      using Sh = Shape<T, TC, D32, FEW>;
+      if (!jobs) return;
+      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)((jobs + 7) / 8 * 8)), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
+    };
+    go(Int<1>{}, a.few_jobs);
+    go(Int<0>{}, a.jobs);
+  };
+  if (a.c.head <= 64) with(Int<2>{});
+  else if (a.c.head <= 96) with(Int<3>{});
+  else if (a.c.head <= 128) with(Int<4>{});
+  else with(Int<8>{});
+}
+
+} // namespace attend
+} // namespace rpu_amd

@@ -23,6 +23,17 @@ struct AppendArgs {
 };
 void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cus, hipStream_t s);
 
+// How a call's work is shared among workgroups: sequences of few lines (a row's heads that share one of the cache count as lines of their own)
+// have their positions shared by the waves of a workgroup, others have tiles of lines.  Of both, the positions may go in parts to several
+// workgroups, whose sums are joined.
+constexpr int ATTEND_FEW = 32, ATTEND_LINES = 128; // lines of a sequence that are few; of a tile
+constexpr int ATTEND_FEW_LEAST = 8;                // tiles of 32 positions that a part has at least
+struct AttendPlan {
+  int few, few_splits, splits, tiles;              // few: the most lines of a sequence that goes that way, 0: none
+  long few_jobs, jobs;                             // workgroups
+  size_t few_part, few_stats, part, stats, bytes;  // offsets in the scratch memory, its size
+};
+
 struct AttendArgs {
   CacheDev c;
   CacheRowsDev r;
@@ -30,8 +41,15 @@ struct AttendArgs {
   int group;           // heads of a row that share one of the cache
   float scale;
   int window, sinks;   // window 0: none
+  int few, few_splits, splits, tiles;
+  long few_jobs, jobs;
+  float *few_part, *part;      // sums of a part of the positions: [few_splits][n][heads][few][head], [splits][rows][q heads][head]
+  float2 *few_stats, *stats;   // maximum (as a power of two) and sum of the weights
 };
-void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, int cus, hipStream_t s);
+namespace attend {
+template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t s);
+}
+void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, hipStream_t s);
 
 #if defined(__HIPCC__)
 // The rows of a sequence, and the position of the first.  Numbers on the GPU that are out of range leave it without rows or positions: nothing

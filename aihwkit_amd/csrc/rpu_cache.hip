@@ -52,6 +52,43 @@ int width_of(int heads, const rpu_cache &c) {
   return (int)width;
 }
 
+// Workgroups for `units` of work that each go over up to `longest` positions: parts so that the GPU is filled, of at least `least` positions.
+int splits_for(long units, long longest, long least, long wanted) {
+  const long most = std::min((longest + least - 1) / least, 64l);
+  return (int)std::max(1l, std::min(most, wanted / std::max(units, 1l)));
+}
+AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
+  AttendPlan p{};
+  const long group = q_heads / c.heads, places = (long)r.table_width * c.page_size;
+  long seen = longest && longest < places ? longest : places;
+  const long lines = r.starts_dev ? 0 : r.rows / r.n * group; // of every sequence
+  if (window) seen = std::min(seen, (long)window + sinks + (r.starts_dev ? r.rows : r.rows / r.n) + 64);
+  if (r.starts_dev || lines <= ATTEND_FEW) {
+    p.few = ATTEND_FEW;
+    p.few_splits = splits_for((long)r.n * c.heads, seen, 32 * ATTEND_FEW_LEAST, 2048);
+    p.few_jobs = (long)r.n * c.heads * p.few_splits;
+  }
+  if (r.starts_dev || lines > ATTEND_FEW) {
+    const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
+    if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
+    p.tiles = (int)tiles;
+    p.splits = splits_for(tiles * c.heads, seen, 512, 512);
+    p.jobs = tiles * c.heads * p.splits;
+  }
+  if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
+  const auto take = [&](size_t n) {
+    const size_t at = p.bytes;
+    p.bytes += (n + 15) / 16 * 16;
+    return at;
+  };
+  const size_t few = p.few_splits > 1 ? (size_t)p.few_jobs * p.few : 0, many = p.splits > 1 ? (size_t)p.splits * r.rows * q_heads : 0;
+  p.few_part = take(few * 4 * c.head_size);
+  p.few_stats = take(few * 8);
+  p.part = take(many * 4 * c.head_size);
+  p.stats = take(many * 8);
+  return p;
+}
+
 } // namespace
 } // namespace rpu_amd
 
@@ -95,7 +132,15 @@ int rpu_cache_append(const rpu_cache *cache, const rpu_cache_rows *rows, const v
   });
 }
 
-size_t rpu_cache_attend_scratch(const rpu_cache *, const rpu_cache_rows *, int, int, int, int, int) { return 0; }
+size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *rows, int q_heads, int dtype, int window, int sinks, int longest) {
+  size_t bytes = 0; // of operands that the call refuses: none
+  (void)guarded([&] {
+    (void)cache_dev(cache, dtype);
+    if (rows_dev(*cache, rows).rows && width_of(q_heads, *cache) && q_heads % cache->heads == 0 && window >= 0 && sinks >= 0 && longest >= 0)
+      bytes = attend_plan(*cache, *rows, q_heads, window, sinks, longest).bytes;
+  });
+  return bytes;
+}
 
 int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads,
                      int dtype, float scale, int window, int sinks, int longest, void *scratch_dev, size_t scratch_bytes, int device_id,
@@ -111,7 +156,8 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     if (window < 0 || sinks < 0) throw RpuError("window and sinks must not be negative.");
     if (sinks && !window) throw RpuError("Only a window has first tokens that stay visible.");
     if (longest < 0) throw RpuError("longest must not be negative.");
-    const size_t need = rpu_cache_attend_scratch(cache, rows, q_heads, dtype, window, sinks, longest);
+    const AttendPlan p = a.r.rows ? attend_plan(*cache, *rows, q_heads, window, sinks, longest) : AttendPlan{};
+    const size_t need = p.bytes;
     if (scratch_bytes < need) throw RpuError("The scratch memory is too small.");
     const Span q = matrix("q", q_dev, q_ld, a.r.rows, width, e), out = matrix("the output", out_dev, out_ld, a.r.rows, width, e),
                scratch = dense("the scratch memory", scratch_dev, need);
@@ -133,8 +179,19 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     a.scale = scale;
     a.window = window;
     a.sinks = sinks;
+    a.few = p.few;
+    a.few_splits = p.few_splits;
+    a.splits = p.splits;
+    a.tiles = p.tiles;
+    a.few_jobs = p.few_jobs;
+    a.jobs = p.jobs;
+    char *const at = (char *)scratch_dev;
+    a.few_part = (float *)(at + p.few_part);
+    a.few_stats = (float2 *)(at + p.few_stats);
+    a.part = (float *)(at + p.part);
+    a.stats = (float2 *)(at + p.stats);
     const Gpu gpu(device_id);
-    launch_cache_attend(a, dtype, cache->dtype, gpu.cus(), (hipStream_t)stream);
+    launch_cache_attend(a, dtype, cache->dtype, (hipStream_t)stream);
     check_launch();
   });
 }
