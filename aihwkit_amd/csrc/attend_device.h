@@ -30,7 +30,10 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int DP = D32 <= 2 ? 64 : D32 <= 4 ? 128 : 256, CHUNKS = DP / 8; // a head in LDS, and its pieces of 16 bytes
   static constexpr int TILE = FEW || KP == 3 || DP == 256 ? 32 : 64;         // positions
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
-  static constexpr int PLANE = TILE * DP, TILE_VALUES = 2 * KP * PLANE;      // of one part, of all parts of keys and values
+  // Rows in LDS lie 16 bytes (keys) and 64 bytes (values) more than their length apart: 16 rows that read the same 16 bytes, and four neighbouring
+  // ones that read 64, touch every bank once, at distances that instructions have as a constant.
+  static constexpr int K_ROW = DP + 8, V_ROW = DP + 32, K_PLANE = TILE * K_ROW, V_PLANE = TILE * V_ROW; // of one part
+  static constexpr int TILE_VALUES = KP * (K_PLANE + V_PLANE);
   static constexpr int KEY_WAVES = !FEW ? 1 : KP == 1 || DP == 64 ? 4 : DP == 128 ? 2 : 1; // that share a line's positions
   static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
@@ -39,11 +42,6 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int LDS = (FEW ? KEY_WAVES : STAGES) * TILE_VALUES * 2;
   static_assert(!FEW || TILE_VALUES * 2 >= 32 * DP * 4, "the sums of a wave fit where its tile was");
 };
-
-// 16 bytes of a row in LDS lie at chunk ^ turn: 16 rows that read the same chunk, and four neighbouring ones that read four, touch all banks
-template <int CHUNKS> __device__ __forceinline__ int turn_of(int row) {
-  return CHUNKS == 8 ? (((row >> 1) & 1) << 2) | ((row >> 2) & 3) : ((row & 3) << 2) | ((row >> 2) & 3);
-}
 
 template <typename M> __device__ __forceinline__ floatx16 multiply(u32x4 a, u32x4 b, floatx16 c) {
   if constexpr (__is_same(M, __bf16)) return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
@@ -91,10 +89,10 @@ struct Job {
 };
 __device__ __forceinline__ int lines_of(const Sequence &s, int group) { return (s.end - s.begin) * group; }
 
-// number `at` of launch_units: the parts of one head of a sequence beside each other, and on one of the eight L2 caches
+// The parts of one head of a sequence beside each other: of unlike sequences every L2 cache (neighbouring workgroups run on different ones) gets
+// like shares.
 __device__ __forceinline__ bool job_few(const AttendArgs &a, long at, Job &job) {
-  const long units = (long)a.r.n * a.c.heads;
-  if (at >= units * a.few_splits) return false;
+  if (at >= a.few_jobs) return false;
   job.split = (int)(at % a.few_splits);
   at /= a.few_splits;
   job.head = (int)(at % a.c.heads);
@@ -103,14 +101,29 @@ __device__ __forceinline__ bool job_few(const AttendArgs &a, long at, Job &job) 
   job.lines = lines_of(job.s, a.group);
   return job.lines > 0 && job.lines <= a.few;
 }
-// Tiles of LINES lines: sequence s has those from (starts[s] * group) / LINES + s on, one more than it can need at most.
+// Tiles of LINES lines, the last of the sequences first: they see most.  Where heads (of all sequences, if these have as many rows each) divide
+// by the eight L2 caches, each cache has some of them; otherwise all go in turn.  Sequences of unlike rows have the tiles from
+// (starts[s] * group) / LINES + s on, one more than they can need at most.
 template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &a, long at, Job &job) {
-  if (at >= (long)a.tiles * a.c.heads * a.splits) return false;
-  job.split = (int)(at % a.splits);
-  at /= a.splits;
-  const int tile = a.tiles - 1 - (int)(at % a.tiles); // long ones first
-  job.head = (int)(at / a.tiles);
-  int which, first;
+  if (at >= a.jobs) return false;
+  const int each = a.r.starts ? a.tiles : a.tiles / a.r.n, sets = a.r.starts ? a.c.heads : a.c.heads * a.r.n; // tiles of a set
+  int set, tile;
+  if (sets % 8 == 0) {
+    const int cache = (int)(at % 8), of_cache = sets / 8;
+    at /= 8;
+    job.split = (int)(at % a.splits);
+    at /= a.splits;
+    set = cache * of_cache + (int)(at % of_cache);
+    tile = (int)(at / of_cache);
+  } else {
+    job.split = (int)(at % a.splits);
+    at /= a.splits;
+    set = (int)(at % sets);
+    tile = (int)(at / sets);
+  }
+  tile = each - 1 - tile;
+  job.head = set % a.c.heads;
+  int which = set / a.c.heads;
   if (a.r.starts) {
     int low = 0, high = a.r.n;
     const auto base = [&](int s) { return (long)min(max(a.r.starts[s], 0), a.r.rows) * a.group / LINES + s; };
@@ -120,16 +133,12 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
       else high = middle;
     }
     which = low;
-    first = (int)max(tile - base(low), 0l);
-  } else {
-    const int each = a.tiles / a.r.n;
-    which = tile / each;
-    first = tile % each;
+    tile = (int)max(tile - base(low), 0l);
   }
   job.s = sequence_at(a.r, which);
   job.lines = lines_of(job.s, a.group);
-  if ((long)first * LINES >= job.lines || job.lines <= a.few) return false;
-  job.line = first * LINES;
+  if ((long)tile * LINES >= job.lines || job.lines <= a.few) return false;
+  job.line = tile * LINES;
   return true;
 }
 
@@ -141,10 +150,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
   const int loader = FEW ? lane : tid;
-  // neighbouring workgroups run on different L2 caches: a run of jobs to each
-  const long per_cache = (gridDim.x + 7) / 8, at = (blockIdx.x % 8) * per_cache + blockIdx.x / 8;
   Job job;
-  if (FEW ? !job_few(a, at, job) : !job_many<S::LINES>(a, at, job)) return;
+  if (FEW ? !job_few(a, blockIdx.x, job) : !job_many<S::LINES>(a, blockIdx.x, job)) return;
   const int group = a.group, head = a.c.head;
 
   // the line of this lane
@@ -158,6 +165,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   const int token0 = job.line / group, token1 = (min(job.line + S::LINES, job.lines) - 1) / group;
   const int end = min(place(job.s.first + token1) + 1, a.r.places), low = a.window ? min(place(job.s.first + token0 - a.window) + 1, end) : 0;
   const int all_last = place(job.s.first + token0), all_before = a.window ? place(job.s.first + token1 - a.window) : -1;
+  const int wave_last = FEW ? 0 : place(job.s.first + (min(job.line + 32 * (tid >> 6) + 32, job.lines) - 1) / group); // of the lines of this wave
   const int sink_end = low > 0 ? min(a.sinks, end) : 0;
   const int sink_tiles = (sink_end + TILE - 1) / TILE, first_tile = max(low / TILE, sink_tiles), tiles = sink_tiles + max((end + TILE - 1) / TILE - first_tile, 0);
   const int splits = FEW ? a.few_splits : a.splits, each = max((tiles + splits - 1) / splits, FEW ? ATTEND_FEW_LEAST : 1);
@@ -240,7 +248,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     for (int i = 0; i < LOADS; ++i) {
       const int piece = i * S::LOADERS + loader, r = piece / CHUNKS, chunk = piece % CHUNKS;
       const bool ok = (loaded >> i) & 1;
-      uint16_t *to_k = tile + r * DP + (chunk ^ turn_of<CHUNKS>(r)) * 8, *to_v = to_k + KP * S::PLANE;
+      uint16_t *to_k = tile + r * S::K_ROW + chunk * 8, *to_v = tile + KP * S::K_PLANE + r * S::V_ROW + chunk * 8;
       if constexpr (KP == 1) {
         const u32x4 k = ok ? (u32x4)k_ahead[i].q : u32x4{}, v = ok ? (u32x4)v_ahead[i].q : u32x4{};
         *reinterpret_cast<u32x4 *>(to_k) = k;
@@ -265,8 +273,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         }
 #pragma unroll
         for (int j = 0; j < KP; ++j) {
-          *reinterpret_cast<u32x4 *>(to_k + j * S::PLANE) = out[0][j];
-          *reinterpret_cast<u32x4 *>(to_v + j * S::PLANE) = out[1][j];
+          *reinterpret_cast<u32x4 *>(to_k + j * S::K_PLANE) = out[0][j];
+          *reinterpret_cast<u32x4 *>(to_v + j * S::V_PLANE) = out[1][j];
         }
       }
     }
@@ -313,17 +321,19 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       next_page = page_at(t + 2 * step);
     }
 
+    // (the first lines of a tile do not see its last positions)
+    if (!FEW && !bad && base > wave_last) continue;
+
     // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
     floatx16 score[BLOCKS] = {};
-    const int row_k = lane & 31;
+    const uint16_t *const keys = tile + (lane & 31) * S::K_ROW + half * 8;
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
       for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
         for (int j = 0; j < KP; ++j) {
-          const int r = 32 * n + row_k;
-          const u32x4 k = *reinterpret_cast<const u32x4 *>(tile + j * S::PLANE + r * DP + ((2 * i + half) ^ turn_of<CHUNKS>(r)) * 8);
+          const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + j * S::K_PLANE + 32 * n * S::K_ROW + 16 * i);
 #pragma unroll
           for (int l = 0; l < QP; ++l)
             if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
@@ -370,7 +380,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 #pragma unroll
         for (int l = 0; l < QP; ++l) weights[l][2 * n + i / 8][i % 8 / 2] = part[l];
       }
-    uint16_t *const values = tile + KP * S::PLANE;
+    uint16_t *const values = tile + KP * S::K_PLANE;
     if (bad) { // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
 #pragma unroll 1
       for (int r = 0; r < TILE; ++r) {
@@ -381,19 +391,20 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           for (int i = 0; i < 16; ++i) {
             float v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::PLANE + r * DP + ((4 * n + i / 4) ^ turn_of<CHUNKS>(r)) * 8 + 4 * half + i % 4]);
+            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + r * S::V_ROW + 32 * n + 8 * (i / 4) + 4 * half + i % 4]);
             if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
           }
       }
       all_there();
-      for (int i = loader; i < KP * S::PLANE / 2; i += S::LOADERS) {
+      for (int i = loader; i < KP * S::V_PLANE / 2; i += S::LOADERS) { // (what lies between rows is never used)
         uint32_t *const two = reinterpret_cast<uint32_t *>(values) + i;
         const uint32_t v = *two;
         if (not_finite2<M>(v)) *two = (not_finite2<M>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite2<M>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
       }
       all_there();
     }
-    const int li = lane & 15, row_v = 4 * half + (li >> 2), chunk_v = 2 * ((lane >> 4) & 1) + ((li & 3) >> 1);
+    // four positions of 16 columns to 16 lanes
+    uint16_t *const columns = values + (4 * half + ((lane & 15) >> 2)) * S::V_ROW + 16 * ((lane >> 4) & 1) + (lane & 3) * 4;
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b)
 #pragma unroll
@@ -403,8 +414,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           s16x4 v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const int r = 16 * b + 8 * e + row_v;
-            uint16_t *p = values + j * S::PLANE + r * DP + ((4 * n + chunk_v) ^ turn_of<CHUNKS>(r)) * 8 + (li & 1) * 4;
+            uint16_t *p = columns + j * S::V_PLANE + (16 * b + 8 * e) * S::V_ROW + 32 * n;
             v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
           }
           const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
@@ -502,7 +512,7 @@ template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t 
       constexpr bool FEW = decltype(few)::value;
       using Sh = Shape<T, TC, D32, FEW>;
       if (!jobs) return;
-      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)((jobs + 7) / 8 * 8)), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
+      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
     };
     go(Int<1>{}, a.few_jobs);
     go(Int<0>{}, a.jobs);

@@ -6,35 +6,54 @@ namespace {
 
 constexpr float NONE = -__builtin_inff();
 
-// out = sum over the parts 2^(m_p - m) sums_p / sum over the parts 2^(m_p - m) total_p.  A wave for a line; parts are shared by the lanes for
-// their factors, columns for the sums.
-__device__ __forceinline__ void join_line(const float *sums, const float2 *stats, long unit, long stride, int parts, int head, int lane, float (&v)[4], float &total) {
+// out = sum over the parts 2^(m_p - m) sums_p / sum over the parts 2^(m_p - m) total_p.  A workgroup for a line: the parts' factors to the lanes
+// of every wave, their sums to the waves, four columns to a lane (and two parts to a wave, of heads of up to 128 columns).
+constexpr int JOIN_WAVES = 4;
+__device__ __forceinline__ bool join_line(const float *sums, const float2 *stats, long unit, long stride, int parts, int head, f32x4 &v) {
+  __shared__ f32x4 room[JOIN_WAVES][64];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float2 mine = lane < parts ? stats[lane * stride + unit] : float2{NONE, 0.0f};
   float top = mine.x;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
   const float factor = mine.x == NONE ? 0.0f : __builtin_amdgcn_exp2f(mine.x - top);
-  total = mine.x == NONE ? 0.0f : mine.y * factor;
+  float total = mine.x == NONE ? 0.0f : mine.y * factor;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) total += __shfl_xor(total, m);
+  const int width = head <= 128 ? 32 : 64, d = lane % width * 4, columns = min(d, head - 4);
+  const int first = wave * (64 / width) + lane / width, step = JOIN_WAVES * (64 / width);
   f32x4 r = {};
-  const int d = lane * 4;
-  for (int p = 0; p < parts; ++p) {
-    const float f = __shfl(factor, p);
-    if (f == 0.0f) continue; // nothing seen, or nothing left of it
-    if (d < head) r += *reinterpret_cast<const f32x4 *>(sums + (p * stride + unit) * head + d) * f;
+  for (int from = 0; from < parts; from += 4 * step) { // four loads under way together
+    f32x4 part[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) part[u] = *reinterpret_cast<const f32x4 *>(sums + (min(from + first + u * step, parts - 1) * stride + unit) * head + columns);
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int p = from + first + u * step;
+      const float f = __shfl(factor, min(p, parts - 1));
+      if (p < parts && f != 0.0f) r += part[u] * f; // 0: nothing seen, nothing left of it, or never written
+    }
   }
+  room[wave][lane] = r;
+  __syncthreads();
+  if ((int)threadIdx.x >= width || d >= head) return false;
+  r = f32x4{};
+  for (int w = 0; w < JOIN_WAVES; ++w)
+    for (int k = lane; k < 64; k += width) r += room[w][k];
   const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
 #pragma unroll
   for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : r[k] * inverse;
+  return true;
 }
 
 // Lines of sequences of few lines first, then those of rows.
-template <typename T> __global__ __launch_bounds__(256) void k_attend_join(AttendArgs a, long few_units, long units) {
-  const int lane = threadIdx.x & 63, q_heads = a.c.heads * a.group;
-  long unit = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  float v[4], total;
+template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attend_join(AttendArgs a, long few_units) {
+  const int q_heads = a.c.heads * a.group;
+  long unit = blockIdx.x;
+  const long units = gridDim.x - few_units;
+  f32x4 v;
   int row, h;
+  bool mine;
   if (unit < few_units) {
     const int l = (int)(unit % a.few), head = (int)(unit / a.few % a.c.heads), which = (int)(unit / a.few / a.c.heads);
     const Sequence s = sequence_at(a.r, which);
@@ -42,17 +61,17 @@ template <typename T> __global__ __launch_bounds__(256) void k_attend_join(Atten
     if (lines > a.few || l >= lines) return;
     row = s.begin + l / a.group;
     h = head * a.group + l % a.group;
-    join_line(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, lane, v, total);
+    mine = join_line(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, v);
   } else {
     unit -= few_units;
-    if (unit >= units) return;
     row = (int)(unit / q_heads);
     h = (int)(unit % q_heads);
     const Sequence s = sequence_of(a.r, row);
     if (s.which < 0 || (long)(s.end - s.begin) * a.group <= a.few) return;
-    join_line(a.part, a.stats, unit, units, a.splits, a.c.head, lane, v, total);
+    mine = join_line(a.part, a.stats, unit, units, a.splits, a.c.head, v);
   }
-  if (lane * 4 < a.c.head) store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * a.c.head + lane * 4, v, 4);
+  const float r[4] = {v[0], v[1], v[2], v[3]};
+  if (mine) store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * a.c.head + threadIdx.x * 4, r, 4);
 }
 
 } // namespace
@@ -62,7 +81,7 @@ void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, hipStr
     using T = decltype(x);
     attend::launch<T, decltype(c)>(a, s);
     const long few = a.few_jobs && a.few_splits > 1 ? (long)a.r.n * a.c.heads * a.few : 0, rows = a.jobs && a.splits > 1 ? (long)a.r.rows * a.c.heads * a.group : 0;
-    if (few + rows) hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)((few + rows + 3) / 4)), dim3(256), 0, s, a, few, rows);
+    if (few + rows) hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(few + rows)), dim3(64 * JOIN_WAVES), 0, s, a, few);
   });
 }
 

@@ -64,7 +64,7 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
   const long lines = r.starts_dev ? 0 : r.rows / r.n * group; // of every sequence
   if (window) seen = std::min(seen, (long)window + sinks + (r.starts_dev ? r.rows : r.rows / r.n) + 64);
   if (r.starts_dev || lines <= ATTEND_FEW) {
-    p.few = ATTEND_FEW;
+    p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
     p.few_splits = splits_for((long)r.n * c.heads, seen, 32 * ATTEND_FEW_LEAST, 2048);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
