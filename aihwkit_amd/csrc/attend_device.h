@@ -28,16 +28,31 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int KP = sizeof(TC) == 4 ? 3 : 1;                         // parts of keys and values
   static constexpr int QP = sizeof(T) == 2 ? 1 : HALF ? 2 : 3;               // of queries and weights
   static constexpr int DP = D32 <= 2 ? 64 : D32 <= 4 ? 128 : 256, CHUNKS = DP / 8; // a head in LDS, and its pieces of 16 bytes
-  static constexpr int TILE = FEW || KP == 3 || DP == 256 ? 32 : 64;         // positions
+  static constexpr int TILE = FEW || KP == 3 ? 32 : 64;                      // positions
+  // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
+  static constexpr bool DIRECT = !FEW && KP == 1;
+  static constexpr int GROUP = 64 / CHUNKS;
+  static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
-  // Rows in LDS lie 16 bytes (keys) and 64 bytes (values) more than their length apart: 16 rows that read the same 16 bytes, and four neighbouring
-  // ones that read 64, touch every bank once, at distances that instructions have as a constant.
-  static constexpr int K_ROW = DP + 8, V_ROW = DP + 32, K_PLANE = TILE * K_ROW, V_PLANE = TILE * V_ROW; // of one part
+  // Where 16 bytes of a row lie in LDS: 16 rows that read the same chunk of keys, and four neighbouring rows that read four chunks of values,
+  // touch every bank once, at distances that instructions mostly have as constants.  Through registers: rows 16 (keys) and 64 (values) bytes
+  // more than their length apart.  DIRECT: chunk ^ turn of the row in its group, and groups at distances of more than 1 KB.
+  static constexpr int K_ROW = DP + 8, V_ROW = DP + 32;
+  static constexpr int K_GROUP = 512 + (DP == 256 ? 16 : 32), V_GROUP = 512 + (DP == 256 ? 64 : 0);
+  static constexpr int K_PLANE = DIRECT ? TILE / GROUP * K_GROUP : TILE * K_ROW, V_PLANE = DIRECT ? TILE / GROUP * V_GROUP : TILE * V_ROW; // of one part
+  static __device__ __forceinline__ int k_turn(int row) { return DP == 64 ? (row >> 1) & 3 : row & (GROUP - 1); }
+  static __device__ __forceinline__ int v_turn(int row) { return (DP == 64 ? (row >> 1) & 1 : row & (GROUP - 1)) << 2; }
+  static __device__ __forceinline__ int k_at(int row, int chunk) {
+    return DIRECT ? row / GROUP * K_GROUP + row % GROUP * DP + (chunk ^ k_turn(row)) * 8 : row * K_ROW + chunk * 8;
+  }
+  static __device__ __forceinline__ int v_at(int row, int chunk) {
+    return DIRECT ? row / GROUP * V_GROUP + row % GROUP * DP + (chunk ^ v_turn(row)) * 8 : row * V_ROW + chunk * 8;
+  }
   static constexpr int TILE_VALUES = KP * (K_PLANE + V_PLANE);
   static constexpr int KEY_WAVES = !FEW ? 1 : KP == 1 || DP == 64 ? 4 : DP == 128 ? 2 : 1; // that share a line's positions
   static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
-  static constexpr int STAGES = FEW || (KP == 3 && DP == 256) ? 1 : 2;
+  static constexpr int STAGES = FEW || (KP == 3 && DP == 256) ? 1 : 2; // tiles that there is room for
   static constexpr int PER_SIMD = D32 <= 4 && KP == 1 && (QP == 1 || D32 <= 2) ? 2 : 1; // waves, as the registers allow
   static constexpr int LDS = (FEW ? KEY_WAVES : STAGES) * TILE_VALUES * 2;
   static_assert(!FEW || TILE_VALUES * 2 >= 32 * DP * 4, "the sums of a wave fit where its tile was");
@@ -149,7 +164,6 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
-  const int loader = FEW ? lane : tid;
   Job job;
   if (FEW ? !job_few(a, blockIdx.x, job) : !job_many<S::LINES>(a, blockIdx.x, job)) return;
   const int group = a.group, head = a.c.head;
@@ -220,56 +234,106 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 
   // Tiles: page numbers are under way two tiles ahead, keys and values one.
   const int *table = a.r.tables + job.s.which * a.r.table_ld;
-  const auto page_at = [&](int t) { // of position `lane` of a tile; -1: not wanted, or not there
+  const auto page_at = [&](int t) { // of position `lane` of a tile; -1: not there
     const int j = base_of(t) + lane;
-    const bool wanted = t < to && lane < TILE && j < end && (j >= low || j < sink_end);
-    const int page = table[wanted ? j >> a.c.page_shift : 0];
-    return wanted && page >= 0 && page < a.c.pages ? page : -1;
+    const bool inside = t < to && lane < TILE && j < end;
+    const int page = table[inside ? j >> a.c.page_shift : 0];
+    return inside && page >= 0 && page < a.c.pages ? page : -1;
   };
-  Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
-  uint32_t loaded = 0;
-  const auto load = [&](int t, int page) {
+  const auto wanted = [&](int t, int page) { // positions of a tile that are there and that some line sees
+    const int j = base_of(t) + lane;
+    return __ballot(page >= 0 && (j >= low || j < sink_end));
+  };
+  // The rows of a group are of one page: their address is the wave's, each lane has its place from there.  DIRECT: from global memory to LDS, 16
+  // bytes to a lane; columns beyond a head are zeros from the start.
+  const int uniform_wave = __builtin_amdgcn_readfirstlane(wave), r_lane = lane / CHUNKS;
+  const int k_lane = (lane % CHUNKS) ^ S::k_turn(r_lane), v_lane = (lane % CHUNKS) ^ S::v_turn(r_lane);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)attend_lds;
+  const auto fetch = [&](int t, int page, int stage) {
     const int base = base_of(t);
-    loaded = 0;
+    const uint32_t to = lds_at + stage * S::TILE_VALUES * 2;
+    const bool k_there = k_lane * 8 < head, v_there = v_lane * 8 < head;
+    const uint32_t k_off = (r_lane * head + k_lane * 8) * 2, v_off = (r_lane * head + v_lane * 8) * 2;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int piece = i * S::LOADERS + loader, r = piece / CHUNKS, chunk = piece % CHUNKS, mine = __shfl(page, r);
-      const bool ok = mine >= 0 && chunk * 8 < head;
-      const long offset = ok ? place_of(a.c, mine, job.head, base + r) + chunk * 8 : 0l;
-      k_ahead[i] = load8(static_cast<const TC *>(a.c.k) + offset);
-      v_ahead[i] = load8(static_cast<const TC *>(a.c.v) + offset);
-      loaded |= ok ? 1u << i : 0u;
+    for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
+      const int g = 4 * i + uniform_wave, r = g * S::GROUP;
+      const uint32_t to_k = to + g * S::K_GROUP * 2, to_v = to + (S::K_PLANE + g * S::V_GROUP) * 2;
+      const long first = place_of(a.c, max(__builtin_amdgcn_readlane(page, r), 0), job.head, base + r);
+      const TC *const k = static_cast<const TC *>(a.c.k) + first, *const v = static_cast<const TC *>(a.c.v) + first;
+      if (k_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(k_off), "s"(k), "s"(to_k) : "memory");
+      if (v_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(v_off), "s"(v), "s"(to_v) : "memory");
     }
   };
-  // keys and values into LDS, zeros where there are none; whether some value is not finite
-  const auto put = [&](uint16_t *tile) {
+  // what this thread fetched: zeros where there is nothing; whether some value is not finite
+  const auto clean = [&](uint16_t *tile, uint64_t here) {
     bool bad = false;
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int piece = i * S::LOADERS + loader, r = piece / CHUNKS, chunk = piece % CHUNKS;
-      const bool ok = (loaded >> i) & 1;
-      uint16_t *to_k = tile + r * S::K_ROW + chunk * 8, *to_v = tile + KP * S::K_PLANE + r * S::V_ROW + chunk * 8;
-      if constexpr (KP == 1) {
-        const u32x4 k = ok ? (u32x4)k_ahead[i].q : u32x4{}, v = ok ? (u32x4)v_ahead[i].q : u32x4{};
-        *reinterpret_cast<u32x4 *>(to_k) = k;
-        *reinterpret_cast<u32x4 *>(to_v) = v;
+    for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
+      const int g = 4 * i + wave;
+      u32x4 *const v = reinterpret_cast<u32x4 *>(tile + S::K_PLANE + g * S::V_GROUP + lane * 8);
+      if (!((here >> (g * S::GROUP + r_lane)) & 1)) *v = u32x4{};
+      else {
+        const u32x4 w = *v;
 #pragma unroll
-        for (int n = 0; n < 4; ++n) bad |= not_finite2<M>(v[n]);
+        for (int n = 0; n < 4; ++n) bad |= not_finite2<M>(w[n]);
+      }
+    }
+    return bad;
+  };
+  // Through registers otherwise, by the same groups of rows.
+  Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
+  const int chunk = lane % CHUNKS, first_group = FEW ? 0 : uniform_wave;
+  const uint32_t lane_at = (r_lane * head + (chunk * 8 < head ? chunk * 8 : 0)) * (uint32_t)sizeof(TC);
+  const auto load = [&](int t, int page) {
+    const int base = base_of(t);
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP;
+      const long first = place_of(a.c, max(__builtin_amdgcn_readlane(page, r), 0), job.head, base + r) * (long)sizeof(TC);
+      k_ahead[i] = load8(reinterpret_cast<const TC *>(static_cast<const char *>(a.c.k) + first + lane_at));
+      v_ahead[i] = load8(reinterpret_cast<const TC *>(static_cast<const char *>(a.c.v) + first + lane_at));
+    }
+  };
+  // keys and values into LDS, zeros where there are none; whether some value is not finite (looked at where it matters)
+  const auto put = [&](uint16_t *tile, uint64_t here, bool whole, bool look) {
+    bool bad = false;
+    if (!whole) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i)
+        if (!((here >> ((S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane)) & 1) || chunk * 8 >= head) k_ahead[i] = v_ahead[i] = {};
+    }
+    if (look) {
+#pragma unroll
+      for (int i = 0; i < LOADS; ++i) {
+        if constexpr (KP == 1) {
+#pragma unroll
+          for (int n = 0; n < 4; ++n) bad |= not_finite2<M>(v_ahead[i].q[n]);
+        } else {
+          const Values8 v = widen(v_ahead[i]);
+#pragma unroll
+          for (int n = 0; n < 8; ++n) bad |= !__builtin_isfinite(v.v[n]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane;
+      uint16_t *to_k = tile + S::k_at(r, chunk), *to_v = tile + KP * S::K_PLANE + S::v_at(r, chunk);
+      if constexpr (KP == 1) {
+        *reinterpret_cast<u32x4 *>(to_k) = k_ahead[i].q;
+        *reinterpret_cast<u32x4 *>(to_v) = v_ahead[i].q;
       } else {
         const Values8 k = widen(k_ahead[i]), v = widen(v_ahead[i]);
         u32x4 out[2][KP];
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
           uint32_t part[KP];
-          split2<M>(ok ? k.v[2 * n] : 0.0f, ok ? k.v[2 * n + 1] : 0.0f, part);
+          split2<M>(k.v[2 * n], k.v[2 * n + 1], part);
 #pragma unroll
           for (int j = 0; j < KP; ++j) out[0][j][n] = part[j];
-          split2<M>(ok ? v.v[2 * n] : 0.0f, ok ? v.v[2 * n + 1] : 0.0f, part);
+          split2<M>(v.v[2 * n], v.v[2 * n + 1], part);
 #pragma unroll
-          for (int j = 0; j < KP; ++j) {
-            out[1][j][n] = part[j];
-            bad |= not_finite2<M>(part[j]);
-          }
+          for (int j = 0; j < KP; ++j) out[1][j][n] = part[j];
         }
 #pragma unroll
         for (int j = 0; j < KP; ++j) {
@@ -292,9 +356,17 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   uint64_t there = 0;
   if (t < to) {
     page = page_at(t);
+    there = wanted(t, page);
     next_page = page_at(t + step);
-    load(t, page);
-    there = __ballot(page >= 0);
+    if constexpr (S::DIRECT) {
+      if (head < DP) {
+        for (int i = tid * 8; i < S::STAGES * S::TILE_VALUES; i += S::WAVES * 64 * 8) *reinterpret_cast<u32x4 *>(attend_lds + i) = u32x4{};
+        __syncthreads();
+      }
+      fetch(t, page, 0);
+    } else {
+      load(t, page);
+    }
   }
   for (int turn = 0; t < to; t += step, turn ^= 1) {
     uint16_t *const tile = lds + (S::STAGES == 2 ? turn * S::TILE_VALUES : 0);
@@ -303,7 +375,13 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     const uint64_t here = there;
     const bool masked = here != ALL || base + TILE - 1 > all_last || (a.window && base <= all_before && base + TILE > a.sinks);
     if (S::STAGES == 1) all_there(); // the tile before has been read
-    bool bad = put(tile);
+    bool bad = false;
+    if constexpr (S::DIRECT) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      if (masked) bad = clean(tile, here);
+    } else {
+      bad = put(tile, here, here == ALL && head == DP, masked);
+    }
     if (masked) { // values that are not finite and not seen by all lines must not meet their weights of zero
       if constexpr (FEW) {
         bad = __any(bad);
@@ -316,8 +394,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       all_there();
     }
     if (t + step < to) {
-      load(t + step, next_page);
-      there = __ballot(next_page >= 0);
+      there = wanted(t + step, next_page);
+      if constexpr (S::DIRECT) fetch(t + step, next_page, turn ^ 1);
+      else load(t + step, next_page);
       next_page = page_at(t + 2 * step);
     }
 
@@ -326,14 +405,17 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 
     // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
     floatx16 score[BLOCKS] = {};
-    const uint16_t *const keys = tile + (lane & 31) * S::K_ROW + half * 8;
+    const uint16_t *keys[2]; // of even and odd steps
+#pragma unroll
+    for (int i = 0; i < 2; ++i) keys[i] = tile + S::k_at(lane & 31, 2 * i + half) - (S::DIRECT ? 0 : 16 * i);
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
       for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
         for (int j = 0; j < KP; ++j) {
-          const u32x4 k = *reinterpret_cast<const u32x4 *>(keys + j * S::K_PLANE + 32 * n * S::K_ROW + 16 * i);
+          const u32x4 k = *reinterpret_cast<const u32x4 *>(S::DIRECT ? keys[i & 1] + 32 / S::GROUP * n * S::K_GROUP + i / 2 * 32
+                                                                     : keys[0] + j * S::K_PLANE + 32 * n * S::K_ROW + 16 * i);
 #pragma unroll
           for (int l = 0; l < QP; ++l)
             if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
@@ -391,12 +473,12 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           for (int i = 0; i < 16; ++i) {
             float v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + r * S::V_ROW + 32 * n + 8 * (i / 4) + 4 * half + i % 4]);
+            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + S::v_at(r, 4 * n + i / 4) + 4 * half + i % 4]);
             if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
           }
       }
       all_there();
-      for (int i = loader; i < KP * S::V_PLANE / 2; i += S::LOADERS) { // (what lies between rows is never used)
+      for (int i = FEW ? lane : tid; i < KP * S::V_PLANE / 2; i += S::LOADERS) { // (what lies between rows is never used)
         uint32_t *const two = reinterpret_cast<uint32_t *>(values) + i;
         const uint32_t v = *two;
         if (not_finite2<M>(v)) *two = (not_finite2<M>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite2<M>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
@@ -404,7 +486,10 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       all_there();
     }
     // four positions of 16 columns to 16 lanes
-    uint16_t *const columns = values + (4 * half + ((lane & 15) >> 2)) * S::V_ROW + 16 * ((lane >> 4) & 1) + (lane & 3) * 4;
+    constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
+    uint16_t *columns[COLUMNS];
+#pragma unroll
+    for (int n = 0; n < COLUMNS; ++n) columns[n] = values + S::v_at(4 * half + ((lane & 15) >> 2), 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b)
 #pragma unroll
@@ -414,7 +499,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           s16x4 v[2];
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            uint16_t *p = columns + j * S::V_PLANE + (16 * b + 8 * e) * S::V_ROW + 32 * n;
+            uint16_t *p = S::DIRECT ? columns[n % COLUMNS] + (16 * b + 8 * e) / S::GROUP * S::V_GROUP + n / 4 * 128
+                                    : columns[0] + j * S::V_PLANE + (16 * b + 8 * e) * S::V_ROW + 32 * n;
             v[e] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4 *)p);
           }
           const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);

@@ -18,8 +18,8 @@ CacheDev cache_dev(const rpu_cache *cache, int dtype) {
   if (c.reserved) throw RpuError("A reserved field of the cache is not 0.");
   if (dtype != RPU_F32 && c.dtype != dtype) throw RpuError("A cache beside 16-bit rows must be of the rows' type.");
   if (c.pages < 1 || c.heads < 1 || c.heads > MOST_HEADS) throw RpuError("A cache has pages, and 1 .. 65536 heads.");
-  if (c.page_size < 1 || c.page_size > RPU_CACHE_MAX_PAGE || (c.page_size & (c.page_size - 1)))
-    throw RpuError("The size of a page must be a power of two up to 65536.");
+  if (c.page_size < RPU_CACHE_MIN_PAGE || c.page_size > RPU_CACHE_MAX_PAGE || (c.page_size & (c.page_size - 1)))
+    throw RpuError("The size of a page must be a power of two, 8 to 65536.");
   if (c.head_size < 8 || c.head_size > RPU_CACHE_MAX_HEAD || c.head_size % 8) throw RpuError("The size of a head must be a multiple of 8 up to 256.");
   if (c.pairs < 0 || 2 * (long)c.pairs > c.head_size) throw RpuError("A head cannot have so many pairs.");
   if (c.pairs && !c.turns_dev) throw RpuError("The rotation's turns are null.");

@@ -60,7 +60,7 @@ class PagedCache:
     """Keys and values of the tokens of many sequences, in pages that sequences take as they grow.
 
     ``keys`` and ``values`` [pages, heads, page_size, head_size] (float32, float16 or bfloat16) are the caller's tensors, dense and on one
-    GPU, and are used as they are at every call.  ``page_size`` is a power of two up to 65536, ``head_size`` a multiple of 8 up to 256.
+    GPU, and are used as they are at every call.  ``page_size`` is a power of two, 8 to 65536, ``head_size`` a multiple of 8 up to 256.
     ``frequencies`` (None: no rotation): the angles, in radians, by which the pairs of a head turn from a position to the next, at most
     ``head_size / 2`` of them (``rotation_frequencies``); they are copied, as float64.  Pair ``i`` is columns ``(i, i + pairs)`` or, with
     ``neighbours``, ``(2 i, 2 i + 1)``; columns from ``2 pairs`` on are not rotated.
@@ -82,8 +82,8 @@ class PagedCache:
             if tensor.dim() != 4 or tensor.numel() == 0:
                 raise RuntimeError(f"{what} must be of four dimensions: pages, heads, positions of a page, values of a head")
         self.pages, self.n_heads, self.page_size, self.head_size = keys.shape
-        if self.page_size & (self.page_size - 1) or self.page_size > 65536:
-            raise RuntimeError("The size of a page must be a power of two up to 65536.")
+        if self.page_size & (self.page_size - 1) or not 8 <= self.page_size <= 65536:
+            raise RuntimeError("The size of a page must be a power of two, 8 to 65536.")
         if self.head_size % 8 or self.head_size > 256:
             raise RuntimeError("The size of a head must be a multiple of 8 up to 256.")
         if self.n_heads > 65536 or self.pages >= NUMBER:

@@ -50,7 +50,7 @@ def attend(c=None, r=None, q=place(7), q_ld=256, out=place(8), out_ld=256, heads
 
 @pytest.mark.parametrize("kw, text", [
     (dict(pages=0), "has pages"), (dict(heads=0), "has pages"), (dict(heads=65537), "has pages"), (dict(pages=-1), "has pages"),
-    (dict(page_size=0), "power of two"), (dict(page_size=24), "power of two"), (dict(page_size=131072), "power of two"),
+    (dict(page_size=0), "power of two"), (dict(page_size=4), "power of two"), (dict(page_size=24), "power of two"), (dict(page_size=131072), "power of two"),
     (dict(page_size=-16), "power of two"),
     (dict(head_size=0), "multiple of 8"), (dict(head_size=60), "multiple of 8"), (dict(head_size=264), "multiple of 8"),
     (dict(pairs=-1), "pairs"), (dict(pairs=33), "pairs"), (dict(turns_dev=None), "turns"), (dict(k_dev=None), "null"), (dict(v_dev=None), "null"),

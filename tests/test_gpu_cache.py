@@ -92,7 +92,7 @@ def test_windows_and_first_tokens(window, sinks, heads, kv, head, dtype, cache_d
         batch.check(batch.attend(window=window, sinks=sinks), window=window, sinks=sinks)
 
 
-@pytest.mark.parametrize("page", [1, 2, 8, 64, 128, 1024])
+@pytest.mark.parametrize("page", [8, 16, 64, 128, 1024])
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 def test_sizes_of_pages(page, dtype, cache_dtype):
     batch = Batch(LAYOUTS["mixed"], 4, 2, 64, page, dtype, cache_dtype, seed=6, before=3, behind=5).gpu()
@@ -357,7 +357,7 @@ def test_append_of_slices_and_in_place(dtype, cache_dtype):
 
 
 def test_values_beyond_a_half_become_infinite_and_nan_stays():
-    cache = digital.PagedCache(*torch.zeros(2, 2, 1, 4, 8, dtype=F16, device="cuda"))
+    cache = digital.PagedCache(*torch.zeros(2, 2, 1, 8, 8, dtype=F16, device="cuda"))
     k = torch.tensor([[1e6, -1e6, NAN, 65519.0, 65520.0, 1e-9, -0.0, INF]], device="cuda").view(1, 1, 8)
     cache.append(k, k, numbers([[1]]), numbers([2]))
     for t in (cache.keys, cache.values):
