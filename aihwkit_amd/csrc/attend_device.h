@@ -97,6 +97,10 @@ __device__ __forceinline__ float half_and_half(float v, float &other) { // of th
   return __uint_as_float(r[0]);
 }
 
+// the next instructions that the compiler's scheduler puts: COUNT of a kind
+enum { VECTOR = 0x2, PRODUCT = 0x8, READ = 0x100 };
+template <int KIND, int COUNT> __device__ __forceinline__ void order(Int<COUNT>) { __builtin_amdgcn_sched_group_barrier(KIND, COUNT, 0); }
+
 // Lines of a sequence, some of its heads and positions: what a workgroup does.
 struct Job {
   Sequence s;
@@ -244,13 +248,21 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     const int j = base_of(t) + lane;
     return __ballot(page >= 0 && (j >= low || j < sink_end));
   };
-  // The rows of a group are of one page: their address is the wave's, each lane has its place from there.  DIRECT: from global memory to LDS, 16
+  // Row `lane` of a tile, in bytes from the first of the cache.  The rows of a group are of one page: their address is the wave's, read from the
+  // lane of the first, and each lane has its place from there.
+  const auto rows_at = [&](int t, int page) { return (uint64_t)place_of(a.c, max(page, 0), job.head, base_of(t) + lane) * sizeof(TC); };
+  const auto address = [&](const void *from, uint64_t at, int r) {
+    const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)at, r), high = __builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), r);
+    const char *p = static_cast<const char *>(from) + ((uint64_t)high << 32 | low);
+    asm("" : "+s"(p));
+    return p;
+  };
+  // DIRECT: from global memory to LDS, 16
   // bytes to a lane; columns beyond a head are zeros from the start.
   const int uniform_wave = __builtin_amdgcn_readfirstlane(wave), r_lane = lane / CHUNKS;
   const int k_lane = (lane % CHUNKS) ^ S::k_turn(r_lane), v_lane = (lane % CHUNKS) ^ S::v_turn(r_lane);
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)attend_lds;
-  const auto fetch = [&](int t, int page, int stage) {
-    const int base = base_of(t);
+  const auto fetch = [&](uint64_t at, int stage) {
     const uint32_t to = lds_at + stage * S::TILE_VALUES * 2;
     const bool k_there = k_lane * 8 < head, v_there = v_lane * 8 < head;
     const uint32_t k_off = (r_lane * head + k_lane * 8) * 2, v_off = (r_lane * head + v_lane * 8) * 2;
@@ -258,8 +270,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
       const int g = 4 * i + uniform_wave, r = g * S::GROUP;
       const uint32_t to_k = to + g * S::K_GROUP * 2, to_v = to + (S::K_PLANE + g * S::V_GROUP) * 2;
-      const long first = place_of(a.c, max(__builtin_amdgcn_readlane(page, r), 0), job.head, base + r);
-      const TC *const k = static_cast<const TC *>(a.c.k) + first, *const v = static_cast<const TC *>(a.c.v) + first;
+      const char *const k = address(a.c.k, at, r), *const v = address(a.c.v, at, r);
       if (k_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(k_off), "s"(k), "s"(to_k) : "memory");
       if (v_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(v_off), "s"(v), "s"(to_v) : "memory");
     }
@@ -284,14 +295,12 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
   const int chunk = lane % CHUNKS, first_group = FEW ? 0 : uniform_wave;
   const uint32_t lane_at = (r_lane * head + (chunk * 8 < head ? chunk * 8 : 0)) * (uint32_t)sizeof(TC);
-  const auto load = [&](int t, int page) {
-    const int base = base_of(t);
+  const auto load = [&](uint64_t at) {
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP;
-      const long first = place_of(a.c, max(__builtin_amdgcn_readlane(page, r), 0), job.head, base + r) * (long)sizeof(TC);
-      k_ahead[i] = load8(reinterpret_cast<const TC *>(static_cast<const char *>(a.c.k) + first + lane_at));
-      v_ahead[i] = load8(reinterpret_cast<const TC *>(static_cast<const char *>(a.c.v) + first + lane_at));
+      k_ahead[i] = load8(reinterpret_cast<const TC *>(address(a.c.k, at, r) + lane_at));
+      v_ahead[i] = load8(reinterpret_cast<const TC *>(address(a.c.v, at, r) + lane_at));
     }
   };
   // keys and values into LDS, zeros where there are none; whether some value is not finite (looked at where it matters)
@@ -363,9 +372,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         for (int i = tid * 8; i < S::STAGES * S::TILE_VALUES; i += S::WAVES * 64 * 8) *reinterpret_cast<u32x4 *>(attend_lds + i) = u32x4{};
         __syncthreads();
       }
-      fetch(t, page, 0);
+      fetch(rows_at(t, page), 0);
     } else {
-      load(t, page);
+      load(rows_at(t, page));
     }
   }
   for (int turn = 0; t < to; t += step, turn ^= 1) {
@@ -395,8 +404,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     }
     if (t + step < to) {
       there = wanted(t + step, next_page);
-      if constexpr (S::DIRECT) fetch(t + step, next_page, turn ^ 1);
-      else load(t + step, next_page);
+      if constexpr (S::DIRECT) fetch(rows_at(t + step, next_page), turn ^ 1);
+      else load(rows_at(t + step, next_page));
       next_page = page_at(t + 2 * step);
     }
 
@@ -420,14 +429,27 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           for (int l = 0; l < QP; ++l)
             if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
         }
-    const auto seen = [&](int n) { // position n of the tile
-      return base + n <= last_seen && (base + n > before || base + n < a.sinks) && ((here >> n) & 1);
-    };
+    // reads of LDS stay ahead of the products
+    constexpr int PRODUCTS = KP == 3 ? 6 : QP; // of a piece of keys or values, all parts
+    order<READ>(Int<4 * KP>{});
+#pragma unroll
+    for (int i = 0; i < STEPS * BLOCKS - 4; ++i) {
+      order<PRODUCT>(Int<PRODUCTS>{});
+      order<READ>(Int<KP>{});
+    }
+    order<PRODUCT>(Int<4 * PRODUCTS>{});
+    // bit n: this lane's line sees position n of 32
+    uint32_t seen[BLOCKS] = {};
     if (masked) {
 #pragma unroll
-      for (int n = 0; n < BLOCKS; ++n)
+      for (int n = 0; n < BLOCKS; ++n) {
+        const int first = base + 32 * n;
+        const auto below = [](int count) { return count >= 32 ? ~0u : (1u << max(count, 0)) - 1; };
+        seen[n] = (uint32_t)(here >> (32 * n)) & below(last_seen - first + 1) & (~below(before - first + 1) | below(a.sinks - first));
+        const uint32_t mine = seen[n] >> (4 * half);
 #pragma unroll
-        for (int i = 0; i < 16; ++i) score[n][i] = seen(32 * n + 8 * (i / 4) + 4 * half + i % 4) ? score[n][i] : NONE;
+        for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
+      }
     }
     float now = score[0][0], other;
 #pragma unroll
@@ -445,28 +467,11 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       m = now;
       power = now == NONE ? NONE : less;
     }
-    // weights, as operands of 16 positions each: 4 half + 8 (e / 4) + e % 4
-    u32x4 weights[QP][2 * BLOCKS];
-#pragma unroll
-    for (int n = 0; n < BLOCKS; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; i += 2) {
-        float w0 = __builtin_amdgcn_exp2f(fmaf(score[n][i], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[n][i + 1], c, -less));
-        total += w0 + w1;
-        if constexpr (S::HALF) { // up to 2^15, so that small ones keep their bits; `total` is of the others
-          w0 *= 0x1p15f;
-          w1 *= 0x1p15f;
-        }
-        uint32_t part[QP];
-        split2<M>(w0, w1, part);
-#pragma unroll
-        for (int l = 0; l < QP; ++l) weights[l][2 * n + i / 8][i % 8 / 2] = part[l];
-      }
     uint16_t *const values = tile + KP * S::K_PLANE;
     if (bad) { // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
 #pragma unroll 1
       for (int r = 0; r < TILE; ++r) {
-        const bool mine = seen(r);
+        const bool mine = (seen[BLOCKS - 1 ? r >> 5 : 0] >> (r & 31)) & 1;
 #pragma unroll
         for (int n = 0; n < D32; ++n)
 #pragma unroll
@@ -490,8 +495,24 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     uint16_t *columns[COLUMNS];
 #pragma unroll
     for (int n = 0; n < COLUMNS; ++n) columns[n] = values + S::v_at(4 * half + ((lane & 15) >> 2), 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
+    // Weights of 16 positions (4 half + 8 (e / 4) + e % 4), then their products, among which those of the next 16 are made.
 #pragma unroll
-    for (int b = 0; b < 2 * BLOCKS; ++b)
+    for (int b = 0; b < 2 * BLOCKS; ++b) {
+      u32x4 weights[QP];
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const int at = 8 * (b & 1) + i;
+        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -less));
+        total += w0 + w1;
+        if constexpr (S::HALF) { // up to 2^15, so that small ones keep their bits; `total` is of the others
+          w0 *= 0x1p15f;
+          w1 *= 0x1p15f;
+        }
+        uint32_t part[QP];
+        split2<M>(w0, w1, part);
+#pragma unroll
+        for (int l = 0; l < QP; ++l) weights[l][i / 2] = part[l];
+      }
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
@@ -507,8 +528,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           const u32x4 both = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
           for (int l = 0; l < QP; ++l)
-            if (j + l < 3) sums[n] = multiply<M>(both, weights[l][b], sums[n]);
+            if (j + l < 3) sums[n] = multiply<M>(both, weights[l], sums[n]);
         }
+    }
   }
   {
     float other;
