@@ -31,6 +31,7 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int TILE = FEW || KP == 3 ? 32 : 64;                      // positions
   // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
   static constexpr bool DIRECT = !FEW && KP == 1;
+  static constexpr bool AHEAD = DIRECT && DP > 64; // the next tile's scores among this one's weights: where a third wave to a SIMD has no registers
   static constexpr int GROUP = 64 / CHUNKS;
   static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
@@ -52,9 +53,9 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int KEY_WAVES = !FEW ? 1 : KP == 1 || DP == 64 ? 4 : DP == 128 ? 2 : 1; // that share a line's positions
   static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
-  static constexpr int STAGES = FEW || (KP == 3 && DP == 256) ? 1 : 2; // tiles that there is room for
-  static constexpr int PER_SIMD = D32 <= 4 && KP == 1 && (QP == 1 || D32 <= 2) ? 2 : 1; // waves, as the registers allow
-  static constexpr int LDS = (FEW ? KEY_WAVES : STAGES) * TILE_VALUES * 2;
+  static constexpr int STAGES = FEW || KP == 3 ? 1 : 2; // tiles that there is room for
+  static constexpr int PER_SIMD = D32 <= 4 && (KP == 1 ? QP == 1 || D32 <= 2 : !FEW) ? 2 : 1; // waves, as the registers allow
+  static constexpr int TILES = FEW ? KEY_WAVES : STAGES, LDS = TILES * TILE_VALUES * 2;
   static_assert(!FEW || TILE_VALUES * 2 >= 32 * DP * 4, "the sums of a wave fit where its tile was");
 };
 
@@ -167,10 +168,16 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   using M = typename S::M;
   constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, half = lane >> 5;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   Job job;
   if (FEW ? !job_few(a, blockIdx.x, job) : !job_many<S::LINES>(a, blockIdx.x, job)) return;
   const int group = a.group, head = a.c.head;
+  // (the same in all lanes, which the compiler does not see of what comes from memory)
+  job.s.begin = __builtin_amdgcn_readfirstlane(job.s.begin);
+  job.s.which = __builtin_amdgcn_readfirstlane(job.s.which);
+  job.s.first = (long)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(job.s.first >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)job.s.first));
+  job.line = __builtin_amdgcn_readfirstlane(job.line);
+  job.lines = __builtin_amdgcn_readfirstlane(job.lines);
 
   // the line of this lane
   const int line = job.line + (FEW ? 0 : 32 * wave) + (lane & 31);
@@ -183,7 +190,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   const int token0 = job.line / group, token1 = (min(job.line + S::LINES, job.lines) - 1) / group;
   const int end = min(place(job.s.first + token1) + 1, a.r.places), low = a.window ? min(place(job.s.first + token0 - a.window) + 1, end) : 0;
   const int all_last = place(job.s.first + token0), all_before = a.window ? place(job.s.first + token1 - a.window) : -1;
-  const int wave_last = FEW ? 0 : place(job.s.first + (min(job.line + 32 * (tid >> 6) + 32, job.lines) - 1) / group); // of the lines of this wave
+  // what the lines of this wave see at most
+  const int wave_line = job.line + 32 * wave, wave_last = FEW || wave_line >= job.lines ? -1 : place(job.s.first + (min(wave_line + 32, job.lines) - 1) / group);
   const int sink_end = low > 0 ? min(a.sinks, end) : 0;
   const int sink_tiles = (sink_end + TILE - 1) / TILE, first_tile = max(low / TILE, sink_tiles), tiles = sink_tiles + max((end + TILE - 1) / TILE - first_tile, 0);
   const int splits = FEW ? a.few_splits : a.splits, each = max((tiles + splits - 1) / splits, FEW ? ATTEND_FEW_LEAST : 1);
@@ -250,38 +258,42 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   };
   // Row `lane` of a tile, in bytes from the first of the cache.  The rows of a group are of one page: their address is the wave's, read from the
   // lane of the first, and each lane has its place from there.
-  const auto rows_at = [&](int t, int page) { return (uint64_t)place_of(a.c, max(page, 0), job.head, base_of(t) + lane) * sizeof(TC); };
+  const auto rows_at = [&](int t, int page) {
+    uint64_t at = (uint64_t)place_of(a.c, max(page, 0), job.head, base_of(t) + lane) * sizeof(TC);
+    asm volatile("" : "+v"(at)); // made here, by all lanes: not in a branch that only some take, where others' are read from
+    return at;
+  };
   const auto address = [&](const void *from, uint64_t at, int r) {
     const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)at, r), high = __builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), r);
     const char *p = static_cast<const char *>(from) + ((uint64_t)high << 32 | low);
-    asm("" : "+s"(p));
+    asm volatile("" : "+s"(p)); // (in scalar registers)
     return p;
   };
-  // DIRECT: from global memory to LDS, 16
-  // bytes to a lane; columns beyond a head are zeros from the start.
-  const int uniform_wave = __builtin_amdgcn_readfirstlane(wave), r_lane = lane / CHUNKS;
+  // DIRECT: from global memory to LDS, 16 bytes to a lane; columns beyond a head are zeros from the start.
+  const int r_lane = lane / CHUNKS;
   const int k_lane = (lane % CHUNKS) ^ S::k_turn(r_lane), v_lane = (lane % CHUNKS) ^ S::v_turn(r_lane);
   const uint32_t lds_at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint16_t *)attend_lds;
-  const auto fetch = [&](uint64_t at, int stage) {
-    const uint32_t to = lds_at + stage * S::TILE_VALUES * 2;
-    const bool k_there = k_lane * 8 < head, v_there = v_lane * 8 < head;
-    const uint32_t k_off = (r_lane * head + k_lane * 8) * 2, v_off = (r_lane * head + v_lane * 8) * 2;
+  const auto fetch = [&](const void *from, uint64_t at, int turned, int group_bytes, uint32_t to) {
+    const uint32_t off = (r_lane * head + turned * 8) * 2;
+    const char *p[TILE / S::GROUP / 4];
 #pragma unroll
-    for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
-      const int g = 4 * i + uniform_wave, r = g * S::GROUP;
-      const uint32_t to_k = to + g * S::K_GROUP * 2, to_v = to + (S::K_PLANE + g * S::V_GROUP) * 2;
-      const char *const k = address(a.c.k, at, r), *const v = address(a.c.v, at, r);
-      if (k_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(k_off), "s"(k), "s"(to_k) : "memory");
-      if (v_there) asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(v_off), "s"(v), "s"(to_v) : "memory");
-    }
+    for (int i = 0; i < TILE / S::GROUP / 4; ++i) p[i] = address(from, at, (4 * i + wave) * S::GROUP);
+    if (turned * 8 < head)
+#pragma unroll
+      for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
+        const int to_group = __builtin_amdgcn_readfirstlane(to + (4 * i + wave) * group_bytes);
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p[i]), "s"(to_group) : "memory");
+      }
   };
+  const auto fetch_keys = [&](uint64_t at, int stage) { fetch(a.c.k, at, k_lane, S::K_GROUP * 2, lds_at + stage * S::K_PLANE * 2); };
+  const auto fetch_values = [&](uint64_t at, int stage) { fetch(a.c.v, at, v_lane, S::V_GROUP * 2, lds_at + (S::STAGES * S::K_PLANE + stage * S::V_PLANE) * 2); };
   // what this thread fetched: zeros where there is nothing; whether some value is not finite
-  const auto clean = [&](uint16_t *tile, uint64_t here) {
+  const auto clean = [&](uint16_t *values, uint64_t here) {
     bool bad = false;
 #pragma unroll
     for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
       const int g = 4 * i + wave;
-      u32x4 *const v = reinterpret_cast<u32x4 *>(tile + S::K_PLANE + g * S::V_GROUP + lane * 8);
+      u32x4 *const v = reinterpret_cast<u32x4 *>(values + g * S::V_GROUP + lane * 8);
       if (!((here >> (g * S::GROUP + r_lane)) & 1)) *v = u32x4{};
       else {
         const u32x4 w = *v;
@@ -293,7 +305,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   };
   // Through registers otherwise, by the same groups of rows.
   Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
-  const int chunk = lane % CHUNKS, first_group = FEW ? 0 : uniform_wave;
+  const int chunk = lane % CHUNKS, first_group = FEW ? 0 : wave;
   const uint32_t lane_at = (r_lane * head + (chunk * 8 < head ? chunk * 8 : 0)) * (uint32_t)sizeof(TC);
   const auto load = [&](uint64_t at) {
 #pragma unroll
@@ -304,7 +316,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     }
   };
   // keys and values into LDS, zeros where there are none; whether some value is not finite (looked at where it matters)
-  const auto put = [&](uint16_t *tile, uint64_t here, bool whole, bool look) {
+  const auto put = [&](uint16_t *keys, uint16_t *values, uint64_t here, bool whole, bool look) {
     bool bad = false;
     if (!whole) {
 #pragma unroll
@@ -327,7 +339,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 #pragma unroll
     for (int i = 0; i < LOADS; ++i) {
       const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane;
-      uint16_t *to_k = tile + S::k_at(r, chunk), *to_v = tile + KP * S::K_PLANE + S::v_at(r, chunk);
+      uint16_t *to_k = keys + S::k_at(r, chunk), *to_v = values + S::v_at(r, chunk);
       if constexpr (KP == 1) {
         *reinterpret_cast<u32x4 *>(to_k) = k_ahead[i].q;
         *reinterpret_cast<u32x4 *>(to_v) = v_ahead[i].q;
@@ -358,65 +370,15 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     else __syncthreads();
   };
 
-  float m = NONE, power = NONE, total = 0.0f; // largest score, as a power of two, sum of the weights (of this lane's positions)
-  floatx16 sums[D32] = {};
-  uint16_t *const lds = attend_lds + (FEW ? wave * S::TILE_VALUES : 0);
-  int t = from + (FEW ? wave : 0), page = -1, next_page = -1;
-  uint64_t there = 0;
-  if (t < to) {
-    page = page_at(t);
-    there = wanted(t, page);
-    next_page = page_at(t + step);
-    if constexpr (S::DIRECT) {
-      if (head < DP) {
-        for (int i = tid * 8; i < S::STAGES * S::TILE_VALUES; i += S::WAVES * 64 * 8) *reinterpret_cast<u32x4 *>(attend_lds + i) = u32x4{};
-        __syncthreads();
-      }
-      fetch(rows_at(t, page), 0);
-    } else {
-      load(rows_at(t, page));
-    }
-  }
-  for (int turn = 0; t < to; t += step, turn ^= 1) {
-    uint16_t *const tile = lds + (S::STAGES == 2 ? turn * S::TILE_VALUES : 0);
-    const int base = base_of(t);
-    constexpr uint64_t ALL = TILE == 64 ? ~0ull : (1ull << TILE % 64) - 1;
-    const uint64_t here = there;
-    const bool masked = here != ALL || base + TILE - 1 > all_last || (a.window && base <= all_before && base + TILE > a.sinks);
-    if (S::STAGES == 1) all_there(); // the tile before has been read
-    bool bad = false;
-    if constexpr (S::DIRECT) {
-      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      if (masked) bad = clean(tile, here);
-    } else {
-      bad = put(tile, here, here == ALL && head == DP, masked);
-    }
-    if (masked) { // values that are not finite and not seen by all lines must not meet their weights of zero
-      if constexpr (FEW) {
-        bad = __any(bad);
-        wave_sync();
-      } else {
-        bad = __syncthreads_or(bad);
-      }
-    } else {
-      bad = false;
-      all_there();
-    }
-    if (t + step < to) {
-      there = wanted(t + step, next_page);
-      if constexpr (S::DIRECT) fetch(rows_at(t + step, next_page), turn ^ 1);
-      else load(rows_at(t + step, next_page));
-      next_page = page_at(t + 2 * step);
-    }
-
-    // (the first lines of a tile do not see its last positions)
-    if (!FEW && !bad && base > wave_last) continue;
-
-    // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
-    floatx16 score[BLOCKS] = {};
+  // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
+  typedef floatx16 Scores[BLOCKS];
+  constexpr int PRODUCTS = KP == 3 ? 6 : QP; // of a piece of keys or values, all parts
+  const auto scores_of = [&](const uint16_t *tile, Scores &score) {
     const uint16_t *keys[2]; // of even and odd steps
 #pragma unroll
     for (int i = 0; i < 2; ++i) keys[i] = tile + S::k_at(lane & 31, 2 * i + half) - (S::DIRECT ? 0 : 16 * i);
+#pragma unroll
+    for (int n = 0; n < BLOCKS; ++n) score[n] = floatx16{};
 #pragma unroll
     for (int i = 0; i < STEPS; ++i)
 #pragma unroll
@@ -429,28 +391,24 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           for (int l = 0; l < QP; ++l)
             if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
         }
-    // reads of LDS stay ahead of the products
-    constexpr int PRODUCTS = KP == 3 ? 6 : QP; // of a piece of keys or values, all parts
-    order<READ>(Int<4 * KP>{});
+  };
+  // bit n: this lane's line sees position n of 32; the scores of the others leave
+  typedef uint32_t Seen[BLOCKS];
+  const auto mask = [&](int base, uint64_t here, Scores &score, Seen &seen) {
 #pragma unroll
-    for (int i = 0; i < STEPS * BLOCKS - 4; ++i) {
-      order<PRODUCT>(Int<PRODUCTS>{});
-      order<READ>(Int<KP>{});
+    for (int n = 0; n < BLOCKS; ++n) {
+      const int first = base + 32 * n;
+      const auto below = [](int count) { return count >= 32 ? ~0u : (1u << max(count, 0)) - 1; };
+      seen[n] = (uint32_t)(here >> (32 * n)) & below(last_seen - first + 1) & (~below(before - first + 1) | below(a.sinks - first));
+      const uint32_t mine = seen[n] >> (4 * half);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
     }
-    order<PRODUCT>(Int<4 * PRODUCTS>{});
-    // bit n: this lane's line sees position n of 32
-    uint32_t seen[BLOCKS] = {};
-    if (masked) {
-#pragma unroll
-      for (int n = 0; n < BLOCKS; ++n) {
-        const int first = base + 32 * n;
-        const auto below = [](int count) { return count >= 32 ? ~0u : (1u << max(count, 0)) - 1; };
-        seen[n] = (uint32_t)(here >> (32 * n)) & below(last_seen - first + 1) & (~below(before - first + 1) | below(a.sinks - first));
-        const uint32_t mine = seen[n] >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
-      }
-    }
+  };
+  float m = NONE, power = NONE, total = 0.0f; // largest score, as a power of two, sum of the weights (of this lane's positions)
+  floatx16 sums[D32] = {};
+  // the maximum with these scores, as a power of two
+  const auto raise = [&](const Scores &score) {
     float now = score[0][0], other;
 #pragma unroll
     for (int n = 0; n < BLOCKS; ++n)
@@ -467,35 +425,37 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       m = now;
       power = now == NONE ? NONE : less;
     }
-    uint16_t *const values = tile + KP * S::K_PLANE;
-    if (bad) { // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
+    return less;
+  };
+  // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
+  const auto repair = [&](uint16_t *values, const Seen &seen) {
 #pragma unroll 1
-      for (int r = 0; r < TILE; ++r) {
-        const bool mine = (seen[BLOCKS - 1 ? r >> 5 : 0] >> (r & 31)) & 1;
+    for (int r = 0; r < TILE; ++r) {
+      const bool mine = (seen[BLOCKS - 1 ? r >> 5 : 0] >> (r & 31)) & 1;
 #pragma unroll
-        for (int n = 0; n < D32; ++n)
+      for (int n = 0; n < D32; ++n)
 #pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            float v = 0.0f;
+        for (int i = 0; i < 16; ++i) {
+          float v = 0.0f;
 #pragma unroll
-            for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + S::v_at(r, 4 * n + i / 4) + 4 * half + i % 4]);
-            if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
-          }
-      }
-      all_there();
-      for (int i = FEW ? lane : tid; i < KP * S::V_PLANE / 2; i += S::LOADERS) { // (what lies between rows is never used)
-        uint32_t *const two = reinterpret_cast<uint32_t *>(values) + i;
-        const uint32_t v = *two;
-        if (not_finite2<M>(v)) *two = (not_finite2<M>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite2<M>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
-      }
-      all_there();
+          for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + S::v_at(r, 4 * n + i / 4) + 4 * half + i % 4]);
+          if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
+        }
     }
-    // four positions of 16 columns to 16 lanes
+    all_there();
+    for (int i = FEW ? lane : tid; i < KP * S::V_PLANE / 2; i += S::LOADERS) { // (what lies between rows is never used)
+      uint32_t *const two = reinterpret_cast<uint32_t *>(values) + i;
+      const uint32_t v = *two;
+      if (not_finite2<M>(v)) *two = (not_finite2<M>(v & 0xffffu) ? 0u : v & 0xffffu) | (not_finite2<M>(v & 0xffff0000u) ? 0u : v & 0xffff0000u);
+    }
+    all_there();
+  };
+  // Weights of 16 positions each (4 half + 8 (e / 4) + e % 4), and their products with four positions of 16 columns to 16 lanes.
+  const auto add = [&](uint16_t *values, const Scores &score, float less) {
     constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
     uint16_t *columns[COLUMNS];
 #pragma unroll
     for (int n = 0; n < COLUMNS; ++n) columns[n] = values + S::v_at(4 * half + ((lane & 15) >> 2), 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
-    // Weights of 16 positions (4 half + 8 (e / 4) + e % 4), then their products, among which those of the next 16 are made.
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b) {
       u32x4 weights[QP];
@@ -530,6 +490,149 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           for (int l = 0; l < QP; ++l)
             if (j + l < 3) sums[n] = multiply<M>(both, weights[l], sums[n]);
         }
+    }
+  };
+  const auto zero_columns = [&] { // of DIRECT, beyond a head
+    if (head == DP) return;
+    for (int i = tid * 8; i < S::TILES * S::TILE_VALUES; i += S::WAVES * 64 * 8) *reinterpret_cast<u32x4 *>(attend_lds + i) = u32x4{};
+    __syncthreads();
+  };
+  constexpr uint64_t ALL = TILE == 64 ? ~0ull : (1ull << TILE % 64) - 1;
+  const auto is_masked = [&](int base, uint64_t here) { // some line does not see some position
+    return here != ALL || base + TILE - 1 > all_last || (a.window && base <= all_before && base + TILE > a.sinks);
+  };
+  // what is not finite and not seen by all lines must not meet their weights of zero
+  const auto everybody = [&](bool masked, bool bad) {
+    if (!masked) {
+      all_there();
+      return false;
+    }
+    if constexpr (FEW) {
+      bad = __any(bad);
+      wave_sync();
+      return bad;
+    } else {
+      return __syncthreads_or(bad) != 0;
+    }
+  };
+
+  if constexpr (S::AHEAD) {
+    // The scores of the next tile are multiplied among the weights of this one: keys are fetched two tiles ahead, values one.
+    uint16_t *const all_keys = attend_lds, *const all_values = attend_lds + S::STAGES * S::K_PLANE;
+    if (from < to) {
+      zero_columns();
+      int page = page_at(from);
+      uint64_t here = wanted(from, page), at = rows_at(from, page);
+      fetch_keys(at, 0);
+      fetch_values(at, 0);
+      page = page_at(from + 1);
+      uint64_t next_here = wanted(from + 1, page);
+      at = rows_at(from + 1, page);
+      if (from + 1 < to) fetch_keys(at, 1);
+      page = page_at(from + 2);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      __syncthreads();
+      Scores even, odd;
+      scores_of(all_keys, even);
+      // one tile, whose scores are in `now`; those of the next come into `then` (of the last one there is nothing that needs them)
+      const auto one = [&](int t, auto parity, Scores &now, Scores &then) {
+        constexpr int turn = decltype(parity)::value;
+        const int base = base_of(t);
+        uint16_t *const values = all_values + turn * S::V_PLANE;
+        const bool masked = is_masked(base, here);
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        const bool bad = everybody(masked, masked && clean(values, here));
+        const uint64_t here_now = here;
+        if (t + 1 < to) {
+          fetch_values(at, turn ^ 1);
+          here = next_here;
+          next_here = wanted(t + 2, page);
+          at = rows_at(t + 2, page);
+          if (t + 2 < to) fetch_keys(at, turn);
+          page = page_at(t + 3);
+        }
+        if (!bad && base > wave_last) return; // (the first lines of a workgroup do not see its last positions)
+        Seen seen = {};
+        if (masked) mask(base, here_now, now, seen);
+        const float less = raise(now);
+        if (bad) repair(values, seen);
+        scores_of(all_keys + (turn ^ 1) * S::K_PLANE, then);
+        add(values, now, less);
+        order<READ>(Int<4>{});
+#pragma unroll
+        for (int i = 0; i < STEPS * BLOCKS; ++i) {
+          order<PRODUCT>(Int<PRODUCTS>{});
+          order<VECTOR>(Int<(112 * BLOCKS / 2) / (STEPS * BLOCKS)>{});
+          order<READ>(Int<1>{});
+        }
+#pragma unroll
+        for (int i = 0; i < 2 * BLOCKS * D32; ++i) {
+          order<READ>(Int<2>{});
+          order<PRODUCT>(Int<PRODUCTS>{});
+        }
+      };
+      for (int t = from; t < to; t += 2) {
+        one(t, Int<0>{}, even, odd);
+        if (t + 1 < to) one(t + 1, Int<1>{}, odd, even);
+      }
+    }
+  } else {
+    int t = from + (FEW ? wave : 0), page = -1, next_page = -1;
+    uint64_t there = 0;
+    if (t < to) {
+      page = page_at(t);
+      there = wanted(t, page);
+      next_page = page_at(t + step);
+      if constexpr (S::DIRECT) {
+        zero_columns();
+        fetch_keys(rows_at(t, page), 0);
+        fetch_values(rows_at(t, page), 0);
+      } else {
+        load(rows_at(t, page));
+      }
+    }
+    for (int turn = 0; t < to; t += step, turn ^= 1) {
+      const int stage = FEW ? wave : S::STAGES == 2 ? turn : 0;
+      uint16_t *const keys = attend_lds + stage * KP * S::K_PLANE, *const values = attend_lds + S::TILES * KP * S::K_PLANE + stage * KP * S::V_PLANE;
+      const int base = base_of(t);
+      const uint64_t here = there;
+      const bool masked = is_masked(base, here);
+      if (S::STAGES == 1) all_there(); // the tile before has been read
+      bool bad = false;
+      if constexpr (S::DIRECT) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        bad = masked && clean(values, here);
+      } else {
+        bad = put(keys, values, here, here == ALL && head == DP, masked);
+      }
+      bad = everybody(masked, bad);
+      if (t + step < to) {
+        there = wanted(t + step, next_page);
+        const uint64_t at = rows_at(t + step, next_page);
+        if constexpr (S::DIRECT) {
+          fetch_keys(at, turn ^ 1);
+          fetch_values(at, turn ^ 1);
+        } else {
+          load(at);
+        }
+        next_page = page_at(t + 2 * step);
+      }
+      if (!FEW && !bad && base > wave_last) continue; // (the first lines of a workgroup do not see its last positions)
+      Scores score;
+      scores_of(keys, score);
+      // reads of LDS stay ahead of the products
+      order<READ>(Int<4 * KP>{});
+#pragma unroll
+      for (int i = 0; i < STEPS * BLOCKS - 4; ++i) {
+        order<PRODUCT>(Int<PRODUCTS>{});
+        order<READ>(Int<KP>{});
+      }
+      order<PRODUCT>(Int<4 * PRODUCTS>{});
+      Seen seen = {};
+      if (masked) mask(base, here, score, seen);
+      const float less = raise(score);
+      if (bad) repair(values, seen);
+      add(values, score, less);
     }
   }
   {
@@ -579,7 +682,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     for (int w = 0; w < S::KEY_WAVES; ++w) sum = fmaf(stats[w][lane & 31].y, shrink_of(stats[w][lane & 31].x), sum);
     if (wave == 0 && !half) joined[lane & 31] = float2{top, sum};
     const float shrink = shrink_of(power);
-    float *const mine = reinterpret_cast<float *>(lds) + (lane & 31) * DP;
+    float *const mine = reinterpret_cast<float *>(attend_lds + wave * S::TILE_VALUES) + (lane & 31) * DP;
     if (live)
 #pragma unroll
       for (int n = 0; n < D32; ++n)

@@ -60,19 +60,22 @@ int splits_for(long units, long longest, long least, long wanted) {
 AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
   AttendPlan p{};
   const long group = q_heads / c.heads, places = (long)r.table_width * c.page_size;
-  long seen = longest && longest < places ? longest : places;
   const long lines = r.starts_dev ? 0 : r.rows / r.n * group; // of every sequence
-  if (window) seen = std::min(seen, (long)window + sinks + (r.starts_dev ? r.rows : r.rows / r.n) + 64);
+  // positions that a workgroup goes over, whose lines are of up to so many neighbouring tokens
+  const auto seen = [&](long tokens) {
+    const long all = longest && longest < places ? longest : places;
+    return window ? std::min(all, (long)window + sinks + tokens + 64) : all;
+  };
   if (r.starts_dev || lines <= ATTEND_FEW) {
     p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
-    p.few_splits = splits_for((long)r.n * c.heads, seen, 32 * ATTEND_FEW_LEAST, 2048);
+    p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 2048);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
   if (r.starts_dev || lines > ATTEND_FEW) {
     const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
-    p.splits = splits_for(tiles * c.heads, seen, 512, 512);
+    p.splits = splits_for(tiles * c.heads, seen(ATTEND_LINES / group + 1), 512, 512);
     p.jobs = tiles * c.heads * p.splits;
   }
   if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
