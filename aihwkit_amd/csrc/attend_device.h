@@ -246,12 +246,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 
   // Tiles: page numbers are under way two tiles ahead, keys and values one.
   const int *table = a.r.tables + job.s.which * a.r.table_ld;
-  const auto page_at = [&](int t) { // of position `lane` of a tile; -1: not there
-    const int j = base_of(t) + lane;
-    const bool inside = t < to && lane < TILE && j < end;
-    const int page = table[inside ? j >> a.c.page_shift : 0];
-    return inside && page >= 0 && page < a.c.pages ? page : -1;
-  };
+  const auto inside = [&](int t) { return t < to && lane < TILE && base_of(t) + lane < end; };
+  const auto entry_at = [&](int t) { return table[inside(t) ? (base_of(t) + lane) >> a.c.page_shift : 0]; }; // (looked at later: not waited for)
+  const auto page_at = [&](int t, int entry) { return inside(t) && entry >= 0 && entry < a.c.pages ? entry : -1; }; // of position `lane`; -1: not there
   const auto wanted = [&](int t, int page) { // positions of a tile that are there and that some line sees
     const int j = base_of(t) + lane;
     return __ballot(page >= 0 && (j >= low || j < sink_end));
@@ -521,15 +518,15 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     uint16_t *const all_keys = attend_lds, *const all_values = attend_lds + S::STAGES * S::K_PLANE;
     if (from < to) {
       zero_columns();
-      int page = page_at(from);
+      const int entry0 = entry_at(from), entry1 = entry_at(from + 1);
+      int entry = entry_at(from + 2), page = page_at(from, entry0);
       uint64_t here = wanted(from, page), at = rows_at(from, page);
       fetch_keys(at, 0);
       fetch_values(at, 0);
-      page = page_at(from + 1);
+      page = page_at(from + 1, entry1);
       uint64_t next_here = wanted(from + 1, page);
       at = rows_at(from + 1, page);
       if (from + 1 < to) fetch_keys(at, 1);
-      page = page_at(from + 2);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       __syncthreads();
       Scores even, odd;
@@ -546,10 +543,11 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         if (t + 1 < to) {
           fetch_values(at, turn ^ 1);
           here = next_here;
+          const int page = page_at(t + 2, entry);
           next_here = wanted(t + 2, page);
           at = rows_at(t + 2, page);
           if (t + 2 < to) fetch_keys(at, turn);
-          page = page_at(t + 3);
+          entry = entry_at(t + 3);
         }
         if (!bad && base > wave_last) return; // (the first lines of a workgroup do not see its last positions)
         Seen seen = {};
@@ -577,12 +575,13 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       }
     }
   } else {
-    int t = from + (FEW ? wave : 0), page = -1, next_page = -1;
+    int t = from + (FEW ? wave : 0), next_entry = 0;
     uint64_t there = 0;
     if (t < to) {
-      page = page_at(t);
+      const int entry = entry_at(t);
+      next_entry = entry_at(t + step);
+      const int page = page_at(t, entry);
       there = wanted(t, page);
-      next_page = page_at(t + step);
       if constexpr (S::DIRECT) {
         zero_columns();
         fetch_keys(rows_at(t, page), 0);
@@ -607,15 +606,16 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       }
       bad = everybody(masked, bad);
       if (t + step < to) {
-        there = wanted(t + step, next_page);
-        const uint64_t at = rows_at(t + step, next_page);
+        const int page = page_at(t + step, next_entry);
+        there = wanted(t + step, page);
+        const uint64_t at = rows_at(t + step, page);
         if constexpr (S::DIRECT) {
           fetch_keys(at, turn ^ 1);
           fetch_values(at, turn ^ 1);
         } else {
           load(at);
         }
-        next_page = page_at(t + 2 * step);
+        next_entry = entry_at(t + 2 * step);
       }
       if (!FEW && !bad && base > wave_last) continue; // (the first lines of a workgroup do not see its last positions)
       Scores score;

@@ -52,10 +52,12 @@ int width_of(int heads, const rpu_cache &c) {
   return (int)width;
 }
 
-// Workgroups for `units` of work that each go over up to `longest` positions: parts so that the GPU is filled, of at least `least` positions.
-int splits_for(long units, long longest, long least, long wanted) {
-  const long most = std::min((longest + least - 1) / least, 64l);
-  return (int)std::max(1l, std::min(most, wanted / std::max(units, 1l)));
+// Parts that `units` of work are split into, over up to `longest` positions: as long as there are fewer workgroups than the GPU runs together, of
+// at least `least` positions; beyond that, so that units of unlike length do not wait for the longest, of at least 1024.  (64 sequences, 8 heads of 128
+// bf16: lengths up to 8192, in 512, 2048 and 4096 workgroups 251, 248 and 244 us; a window of 1024 in 512, 1024 and 2048 57, 67 and 71 us.)
+int splits_for(long units, long longest, long least, long together, long many) {
+  const long fill = std::min(together / units, (longest + least - 1) / least), more = std::min(many / units, longest / 1024);
+  return (int)std::max(1l, std::min(64l, std::max(fill, more)));
 }
 AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
   AttendPlan p{};
@@ -68,14 +70,14 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
   };
   if (r.starts_dev || lines <= ATTEND_FEW) {
     p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
-    p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 2048);
+    p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 512, 4096);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
   if (r.starts_dev || lines > ATTEND_FEW) {
     const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
-    p.splits = splits_for(tiles * c.heads, seen(ATTEND_LINES / group + 1), 512, 512);
+    p.splits = splits_for(tiles * c.heads, seen(ATTEND_LINES / group + 1), 512, 512, 0);
     p.jobs = tiles * c.heads * p.splits;
   }
   if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
