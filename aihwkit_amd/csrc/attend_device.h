@@ -86,6 +86,11 @@ template <typename M, int PARTS> __device__ __forceinline__ void split2(float a,
   }
 }
 template <typename M> __device__ __forceinline__ float value_of(uint16_t v) { return to_float(__builtin_bit_cast(M, v)); }
+// a sum and two 16-bit values
+template <typename M> __device__ __forceinline__ float add2(uint32_t two, float sum) {
+  if constexpr (__is_same(M, __bf16)) return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, two), __builtin_bit_cast(bf16x2, 0x3f803f80u), sum, false);
+  else return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), __builtin_bit_cast(f16x2, 0x3c003c00u), sum, false);
+}
 // one of two 16-bit values is infinite or NaN
 template <typename M> __device__ __forceinline__ bool not_finite2(uint32_t v) {
   constexpr uint32_t FIELD = __is_same(M, __bf16) ? 0x7f807f80u : 0x7c007c00u, STEP = __is_same(M, __bf16) ? 0x00800080u : 0x04000400u;
@@ -448,7 +453,10 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     all_there();
   };
   // Weights of 16 positions each (4 half + 8 (e / 4) + e % 4), and their products with four positions of 16 columns to 16 lanes.
+  // Halves are up to 2^15, so that small ones keep their bits: of half rows by the exponent, of floats, whose `total` is of the weights, by a product.
+  constexpr float LIFT = 0x1p15f;
   const auto add = [&](uint16_t *values, const Scores &score, float less) {
+    const float exponent = S::HALF && QP == 1 ? less - 15.0f : less;
     constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
     uint16_t *columns[COLUMNS];
 #pragma unroll
@@ -459,14 +467,15 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const int at = 8 * (b & 1) + i;
-        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -less));
-        total += w0 + w1;
-        if constexpr (S::HALF) { // up to 2^15, so that small ones keep their bits; `total` is of the others
-          w0 *= 0x1p15f;
-          w1 *= 0x1p15f;
+        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -exponent)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -exponent));
+        if constexpr (QP > 1) total += w0 + w1;
+        if constexpr (S::HALF && QP > 1) {
+          w0 *= LIFT;
+          w1 *= LIFT;
         }
         uint32_t part[QP];
         split2<M>(w0, w1, part);
+        if constexpr (QP == 1) total = add2<M>(part[0], total); // of the rounded ones: those that the values are multiplied with
 #pragma unroll
         for (int l = 0; l < QP; ++l) weights[l][i / 2] = part[l];
       }
@@ -640,7 +649,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     const float mine = half_and_half(total, other);
     total = mine + other;
   }
-  if constexpr (S::HALF) total *= 0x1p15f;
+  if constexpr (S::HALF && QP > 1) total *= LIFT;
   if constexpr (!FEW) {
     if (!live) return;
     const long unit = (long)row * (a.c.heads * group) + q_head;
