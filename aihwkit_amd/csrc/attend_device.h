@@ -260,12 +260,17 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   };
   // Row `lane` of a tile, in bytes from the first of the cache.  The rows of a group are of one page: their address is the wave's, read from the
   // lane of the first, and each lane has its place from there.
+  const uint32_t row_bytes = head * (uint32_t)sizeof(TC), head_bytes = row_bytes << a.c.page_shift, page_bytes = head_bytes * a.c.heads, of_head = head_bytes * job.head;
   const auto rows_at = [&](int t, int page) {
-    uint64_t at = (uint64_t)place_of(a.c, max(page, 0), job.head, base_of(t) + lane) * sizeof(TC);
+    uint64_t at = (uint64_t)(uint32_t)max(page, 0) * page_bytes + of_head + ((base_of(t) + lane) & ((1 << a.c.page_shift) - 1)) * row_bytes;
     asm volatile("" : "+v"(at)); // made here, by all lanes: not in a branch that only some take, where others' are read from
     return at;
   };
   const auto address = [&](const void *from, uint64_t at, int r) {
+    if (a.c.page_shift >= __builtin_ctz(TILE)) { // of one page
+      from = static_cast<const char *>(from) + r * row_bytes;
+      r = 0;
+    }
     const uint32_t low = __builtin_amdgcn_readlane((int)(uint32_t)at, r), high = __builtin_amdgcn_readlane((int)(uint32_t)(at >> 32), r);
     const char *p = static_cast<const char *>(from) + ((uint64_t)high << 32 | low);
     asm volatile("" : "+s"(p)); // (in scalar registers)
@@ -407,9 +412,11 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
     }
   };
-  float m = NONE, power = NONE, total = 0.0f; // largest score, as a power of two, sum of the weights (of this lane's positions)
+  // The score that weights are relative to, as a power of two too, and their sum (of this lane's positions).  It follows the maximum where that is
+  // more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.
+  constexpr float SLACK = 8.0f;
+  float m = NONE, power = NONE, total = 0.0f;
   floatx16 sums[D32] = {};
-  // the maximum with these scores, as a power of two
   const auto raise = [&](const Scores &score) {
     float now = score[0][0], other;
 #pragma unroll
@@ -417,17 +424,18 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 #pragma unroll
       for (int i = 0; i < 16; ++i) now = most(now, score[n][i]);
     now = half_and_half(now, other);
-    now = most(most(now, other), m);
-    const float less = now == NONE ? 0.0f : now * c;
-    if (!__all(now == m)) {
-      const float shrink = __builtin_amdgcn_exp2f(power - less);
+    now = most(now, other);
+    const bool far = !(now * c <= power + SLACK) && now != NONE; // (NaN is)
+    if (__any(far)) {
+      now = far ? most(now, m) : m;
+      const float next = now == NONE ? NONE : now * c, shrink = far ? __builtin_amdgcn_exp2f(power - next) : 1.0f;
       total *= shrink;
 #pragma unroll
       for (int n = 0; n < D32; ++n) sums[n] *= shrink;
       m = now;
-      power = now == NONE ? NONE : less;
+      power = next;
     }
-    return less;
+    return power == NONE ? 0.0f : power;
   };
   // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
   const auto repair = [&](uint16_t *values, const Seen &seen) {
@@ -454,9 +462,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   };
   // Weights of 16 positions each (4 half + 8 (e / 4) + e % 4), and their products with four positions of 16 columns to 16 lanes.
   // Halves are up to 2^15, so that small ones keep their bits: of half rows by the exponent, of floats, whose `total` is of the weights, by a product.
-  constexpr float LIFT = 0x1p15f;
+  constexpr float LIFT = 0x1p7f;
   const auto add = [&](uint16_t *values, const Scores &score, float less) {
-    const float exponent = S::HALF && QP == 1 ? less - 15.0f : less;
+    const float exponent = S::HALF && QP == 1 ? less - (15.0f - SLACK) : less;
     constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
     uint16_t *columns[COLUMNS];
 #pragma unroll

@@ -21,6 +21,7 @@ CacheDev cache_dev(const rpu_cache *cache, int dtype) {
   if (c.page_size < RPU_CACHE_MIN_PAGE || c.page_size > RPU_CACHE_MAX_PAGE || (c.page_size & (c.page_size - 1)))
     throw RpuError("The size of a page must be a power of two, 8 to 65536.");
   if (c.head_size < 8 || c.head_size > RPU_CACHE_MAX_HEAD || c.head_size % 8) throw RpuError("The size of a head must be a multiple of 8 up to 256.");
+  if (value_size(c.dtype) * c.head_size * c.page_size * (size_t)c.heads > INT_MAX) throw RpuError("The keys of a page must take less than 2 GB.");
   if (c.pairs < 0 || 2 * (long)c.pairs > c.head_size) throw RpuError("A head cannot have so many pairs.");
   if (c.pairs && !c.turns_dev) throw RpuError("The rotation's turns are null.");
   if (!c.k_dev || !c.v_dev) throw RpuError("The cache's keys or values are null.");

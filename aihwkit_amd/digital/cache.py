@@ -88,6 +88,8 @@ class PagedCache:
             raise RuntimeError("The size of a head must be a multiple of 8 up to 256.")
         if self.n_heads > 65536 or self.pages >= NUMBER:
             raise RuntimeError("A cache has at most 65536 heads and 2^31 - 1 pages.")
+        if keys[0].numel() * keys.element_size() >= NUMBER:
+            raise RuntimeError("The keys of a page must take less than 2 GB.")
         self._shape = keys.shape
         self.keys, self.values = keys, values
         self.neighbours = bool(neighbours)

@@ -811,7 +811,8 @@ int rpu_adapter_backward(const rpu_adapters *adapters, const void *d_dev, long d
 /* Attention between tiles over a paged cache.  k_dev, v_dev [pages][heads][page_size][head_size]: dense, aligned to 16 bytes, of `dtype`.
  * turns_dev [pairs], doubles: rotation of each pair of a head per position, in turns (radians / 2 pi); pairs = 0: no rotation.  Pair i is
  * columns (i, i + pairs), with `neighbours` (2 i, 2 i + 1); the columns from 2 pairs on are not rotated.  page_size: a power of two,
- * RPU_CACHE_MIN_PAGE to RPU_CACHE_MAX_PAGE; head_size: a multiple of 8 up to RPU_CACHE_MAX_HEAD. */
+ * RPU_CACHE_MIN_PAGE to RPU_CACHE_MAX_PAGE; head_size: a multiple of 8 up to RPU_CACHE_MAX_HEAD; the keys of a page, of all heads, take
+ * less than 2 GB. */
 #define RPU_CACHE_MIN_PAGE 8
 #define RPU_CACHE_MAX_PAGE 65536
 #define RPU_CACHE_MAX_HEAD 256

@@ -62,12 +62,12 @@ def attended(q, keys, values, tables, lengths, starts, scale, window=0, sinks=0,
 
 def bound_of(parts, head, dtype, compute=None):
     """How far the result may be from ``out`` before it is stored: scores off by (head + 6) U of their terms' magnitude (sums in any order, the
-    scale, the exponent's argument), exponentials by 4 U (of halves by 12 U: weights lifted by 2^15 have exponents of up to 16, half a step of which is 2^-21,
-    times log 2), sums over the places by U each -- in both the weighted values and the weights, which
+    scale, the exponent's argument), exponentials by 4 U (of 16-bit rows by 12 U: weights relative to another score than the largest, or lifted, have exponents of
+    up to 16, half a step of which is 2^-21, times log 2), sums over the places by U each -- in both the weighted values and the weights, which
     are divided by -- and weights rounded to ``compute`` before they meet values of that type (half a step of theirs; of halves at least
     2^-25 of the largest weight)."""
     compute = dtype if compute is None else compute
-    each = (head + 6) * U * parts["magnitude"] + (12 if compute == torch.float16 else 4) * U + parts["count"] * U
+    each = (head + 6) * U * parts["magnitude"] + (4 if compute == torch.float32 else 12) * U + parts["count"] * U
     step = 0.0 if compute == torch.float32 else torch.finfo(compute).eps / 2
     limit = (2 * each + step) * parts["plain"] * (1 + 2 * each + step)
     if compute != torch.float32:

@@ -55,6 +55,7 @@ def attend(c=None, r=None, q=place(7), q_ld=256, out=place(8), out_ld=256, heads
     (dict(head_size=0), "multiple of 8"), (dict(head_size=60), "multiple of 8"), (dict(head_size=264), "multiple of 8"),
     (dict(pairs=-1), "pairs"), (dict(pairs=33), "pairs"), (dict(turns_dev=None), "turns"), (dict(k_dev=None), "null"), (dict(v_dev=None), "null"),
     (dict(k_dev=place(0) + 8), "aligned"), (dict(v_dev=place(1) + 2), "aligned"), (dict(dtype=3), "Unknown data type"), (dict(reserved=1), "reserved"),
+    (dict(heads=1024, page_size=65536), "2 GB"),
 ])
 def test_caches_that_are_refused(kw, text):
     refused(append(c=cache(**kw)), text)
