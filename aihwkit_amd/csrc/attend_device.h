@@ -28,16 +28,19 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int KP = sizeof(TC) == 4 ? 3 : 1;                         // parts of keys and values
   static constexpr int QP = sizeof(T) == 2 ? 1 : HALF ? 2 : 3;               // of queries and weights
   static constexpr int DP = D32 <= 2 ? 64 : D32 <= 4 ? 128 : 256, CHUNKS = DP / 8; // a head in LDS, and its pieces of 16 bytes
-  static constexpr int TILE = FEW || KP == 3 ? 32 : 64;                      // positions
+  static constexpr int TILE = FEW || KP == 3 || (DP == 256 && QP > 1) ? 32 : 64; // positions
   // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
   static constexpr bool DIRECT = !FEW && KP == 1;
-  static constexpr bool AHEAD = DIRECT && DP > 64; // the next tile's scores among this one's weights: where a third wave to a SIMD has no registers
+  static constexpr bool AHEAD = DIRECT && (DP == 128 || (DP == 256 && QP == 1)); // the next tile's scores among this one's weights: where a third wave to a SIMD has no registers
   static constexpr int GROUP = 64 / CHUNKS;
   static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
   // Where 16 bytes of a row lie in LDS: 16 rows that read the same chunk of keys, and four neighbouring rows that read four chunks of values,
   // touch every bank once, at distances that instructions mostly have as constants.  Through registers: rows 16 (keys) and 64 (values) bytes
   // more than their length apart.  DIRECT: chunk ^ turn of the row in its group, and groups at distances of more than 1 KB.
+  // Registers are short: none for a tile that is under way, and queries are read and split again for every tile.  (No kernel may spill: this compiler
+  // has stored and reloaded three registers of a spilled four.)
+  static constexpr bool LATE = KP == 3 && D32 > 2 && !FEW, QUERIES_AGAIN = QP == 3 && DP == 256;
   static constexpr int K_ROW = DP + 8, V_ROW = DP + 32;
   static constexpr int K_GROUP = 512 + (DP == 256 ? 16 : 32), V_GROUP = 512 + (DP == 256 ? 64 : 0);
   static constexpr int K_PLANE = DIRECT ? TILE / GROUP * K_GROUP : TILE * K_ROW, V_PLANE = DIRECT ? TILE / GROUP * V_GROUP : TILE * V_ROW; // of one part
@@ -150,15 +153,9 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
   job.head = set % a.c.heads;
   int which = set / a.c.heads;
   if (a.r.starts) {
-    int low = 0, high = a.r.n;
-    const auto base = [&](int s) { return (long)min(max(a.r.starts[s], 0), a.r.rows) * a.group / LINES + s; };
-    while (high - low > 1) {
-      const int middle = (low + high) / 2;
-      if (base(middle) <= tile) low = middle;
-      else high = middle;
-    }
-    which = low;
-    tile = (int)max(tile - base(low), 0l);
+    const auto base = [&](int start, int s) { return (long)min(max(start, 0), a.r.rows) * a.group / LINES + s; };
+    which = max(last_of(a.r.starts, a.r.n, [&](int start, int s) { return base(start, s) <= tile; }), 0);
+    tile = (int)max(tile - base(a.r.starts[which], which), 0l);
   }
   job.s = sequence_at(a.r, which);
   job.lines = lines_of(job.s, a.group);
@@ -204,19 +201,36 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   const auto base_of = [&](int t) { return (t < sink_tiles ? t : first_tile + t - sink_tiles) * TILE; };
 
   // queries: 8 values of each 16 to a lane
-  u32x4 q[QP][STEPS];
-  float c = a.scale * LOG2E; // of the exponents, in powers of two
-  {
-    const T *at_q = static_cast<const T *>(a.q.p) + (live ? row * a.q.ld + q_head * head : 0l);
+  const T *const at_q = static_cast<const T *>(a.q.p) + (live ? row * a.q.ld + q_head * head : 0l);
+  const auto query_at = [&](int i) { return load8(at_q + (16 * i + 8 * half < head ? 16 * i + 8 * half : 0)); };
+  const bool none = a.scale == 0.0f;
+  float lift = 1.0f;
+  const auto parts_of_query = [&](const Packed8<T> &p, int i, auto &&put) { // (the scale's sign goes with them)
+    const bool there = live && 16 * i + 8 * half < head && !none;
+    if constexpr (QP == 1) {
+      u32x4 v = p.q;
+      if (a.scale < 0.0f) v ^= 0x80008000u;
+      put(0, there ? v : u32x4{});
+    } else {
+      const Values8 v = widen(p);
+      const float factor = a.scale < 0.0f ? -lift : lift;
+      u32x4 out[QP];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        uint32_t part[QP];
+        split2<M>(there ? v.v[2 * k] * factor : 0.0f, there ? v.v[2 * k + 1] * factor : 0.0f, part);
+#pragma unroll
+        for (int j = 0; j < QP; ++j) out[j][k] = part[j];
+      }
+#pragma unroll
+      for (int j = 0; j < QP; ++j) put(j, out[j]);
+    }
+  };
+  u32x4 q[QP][S::QUERIES_AGAIN ? 1 : STEPS];
+  if constexpr (!S::QUERIES_AGAIN) {
     Packed8<T> p[STEPS];
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const int d = 16 * i + 8 * half;
-      p[i] = load8(at_q + (d < head ? d : 0));
-    }
-    const bool none = a.scale == 0.0f;
-    const float sign = a.scale < 0.0f ? -1.0f : 1.0f;
-    float lift = 1.0f;
+    for (int i = 0; i < STEPS; ++i) p[i] = query_at(i);
     if constexpr (QP == 2) {
       float m = 0.0f;
 #pragma unroll
@@ -229,25 +243,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       lift = lift_of(m);
     }
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i) {
-      const bool there = live && 16 * i + 8 * half < head && !none;
-      if constexpr (QP == 1) {
-        q[0][i] = p[i].q;
-        if (a.scale < 0.0f) q[0][i] ^= 0x80008000u;
-        q[0][i] = there ? q[0][i] : u32x4{};
-      } else {
-        const Values8 v = widen(p[i]);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          uint32_t part[QP];
-          split2<M>(there ? v.v[2 * k] * sign * lift : 0.0f, there ? v.v[2 * k + 1] * sign * lift : 0.0f, part);
-#pragma unroll
-          for (int j = 0; j < QP; ++j) q[j][i][k] = part[j];
-        }
-      }
-    }
-    c = none ? LOG2E : fabsf(c) * inverse_of(lift);
+    for (int i = 0; i < STEPS; ++i) parts_of_query(p[i], i, [&](int j, u32x4 v) { q[j][i] = v; });
   }
+  const float c = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift); // of the exponents, in powers of two
 
   // Tiles: page numbers are under way two tiles ahead, keys and values one.
   const int *table = a.r.tables + job.s.which * a.r.table_ld;
@@ -267,7 +265,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     return at;
   };
   const auto address = [&](const void *from, uint64_t at, int r) {
-    if (a.c.page_shift >= __builtin_ctz(TILE)) { // of one page
+    if (S::DIRECT && a.c.page_shift >= __builtin_ctz(TILE)) { // of one page
       from = static_cast<const char *>(from) + r * row_bytes;
       r = 0;
     }
@@ -387,7 +385,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
 #pragma unroll
     for (int n = 0; n < BLOCKS; ++n) score[n] = floatx16{};
 #pragma unroll
-    for (int i = 0; i < STEPS; ++i)
+    for (int i = 0; i < STEPS; ++i) {
+      const int slot = S::QUERIES_AGAIN ? 0 : i;
+      if constexpr (S::QUERIES_AGAIN) parts_of_query(query_at(i), i, [&](int j, u32x4 v) { q[j][0] = v; });
 #pragma unroll
       for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
@@ -396,8 +396,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
                                                                      : keys[0] + j * S::K_PLANE + 32 * n * S::K_ROW + 16 * i);
 #pragma unroll
           for (int l = 0; l < QP; ++l)
-            if (j + l < 3) score[n] = multiply<M>(k, q[l][i], score[n]);
+            if (j + l < 3) score[n] = multiply<M>(k, q[l][slot], score[n]);
         }
+    }
   };
   // bit n: this lane's line sees position n of 32; the scores of the others leave
   typedef uint32_t Seen[BLOCKS];
@@ -593,18 +594,19 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     }
   } else {
     int t = from + (FEW ? wave : 0), next_entry = 0;
-    uint64_t there = 0;
+    uint64_t there = 0, at_now = 0;
     if (t < to) {
       const int entry = entry_at(t);
       next_entry = entry_at(t + step);
       const int page = page_at(t, entry);
       there = wanted(t, page);
+      at_now = rows_at(t, page);
       if constexpr (S::DIRECT) {
         zero_columns();
-        fetch_keys(rows_at(t, page), 0);
-        fetch_values(rows_at(t, page), 0);
-      } else {
-        load(rows_at(t, page));
+        fetch_keys(at_now, 0);
+        fetch_values(at_now, 0);
+      } else if constexpr (!S::LATE) {
+        load(at_now);
       }
     }
     for (int turn = 0; t < to; t += step, turn ^= 1) {
@@ -619,6 +621,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         bad = masked && clean(values, here);
       } else {
+        if constexpr (S::LATE) load(at_now);
         bad = put(keys, values, here, here == ALL && head == DP, masked);
       }
       bad = everybody(masked, bad);
@@ -629,6 +632,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         if constexpr (S::DIRECT) {
           fetch_keys(at, turn ^ 1);
           fetch_values(at, turn ^ 1);
+        } else if constexpr (S::LATE) {
+          at_now = at;
         } else {
           load(at);
         }
@@ -742,7 +747,7 @@ template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t 
       if (!jobs) return;
       hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
     };
-    go(Int<1>{}, a.few_jobs);
+    if constexpr (D32 <= 4) go(Int<1>{}, a.few_jobs); // (longer heads have no few lines)
     go(Int<0>{}, a.jobs);
   };
   if (a.c.head <= 64) with(Int<2>{});

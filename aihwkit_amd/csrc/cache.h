@@ -27,7 +27,8 @@ void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cu
 // have their positions shared by the waves of a workgroup, others have tiles of lines.  Of both, the positions may go in parts to several
 // workgroups, whose sums are joined.
 constexpr int ATTEND_FEW = 32, ATTEND_LINES = 128; // lines of a sequence that are few; of a tile
-constexpr int ATTEND_FEW_LEAST = 8;                // tiles of 32 positions that a part has at least
+constexpr int ATTEND_FEW_HEAD = 128;               // of heads up to so many values; of longer ones all go in tiles of lines
+constexpr int ATTEND_FEW_LEAST = 4;                // tiles of 32 positions that a part has at least
 struct AttendPlan {
   int few, few_splits, splits, tiles;              // few: the most lines of a sequence that goes that way, 0: none
   long few_jobs, jobs;                             // workgroups
@@ -72,15 +73,24 @@ __device__ __forceinline__ Sequence sequence_at(const CacheRowsDev &r, int which
   s.first = (long)r.lengths[which] - (s.end - s.begin);
   return s;
 }
-// the sequence that a row belongs to; which < 0: none
+// The last of n numbers that `at_most` holds for, of numbers for which it holds up to some and then not; -1: none.  By a whole wave, 64 numbers at
+// a time: two trips to memory for up to 4096 of them.
+template <typename F> __device__ __forceinline__ int last_of(const int *numbers, int n, F &&at_most) {
+  const int lane = threadIdx.x & 63;
+  int low = -1, high = n; // holds for low, not for high
+  while (high - low > 1) {
+    const int step = max((high - low - 1 + 63) / 64, 1), i = low + 1 + lane * step;
+    const int held = __popcll(__ballot(i < high && at_most(numbers[min(i, n - 1)], i)));
+    const int from = low;
+    if (held) low = from + 1 + (held - 1) * step;
+    high = min(high, from + 1 + held * step);
+  }
+  return low;
+}
+// the sequence that a row belongs to (by a whole wave); which < 0: none
 __device__ __forceinline__ Sequence sequence_of(const CacheRowsDev &r, int row) {
   if (!r.starts) return sequence_at(r, row / (r.rows / r.n));
-  int low = -1, high = r.n; // starts[low] <= row < starts[high]
-  while (high - low > 1) {
-    const int middle = (low + high) / 2;
-    if (r.starts[middle] <= row) low = middle;
-    else high = middle;
-  }
+  const int low = last_of(r.starts, r.n, [&](int start, int) { return start <= row; });
   if (low < 0) return {-1, 0, 0, 0};
   Sequence s = sequence_at(r, low);
   if (row < s.begin || row >= s.end) s.which = -1;

@@ -21,45 +21,63 @@ __device__ __forceinline__ float2 turned(double turns) {
 constexpr int THREADS = 256, MOST_ROWS_EACH = 8;
 
 // A workgroup takes `each` rows: their places and angles go to LDS, once for all heads, then every thread moves groups of eight values (of
-// both halves, where pairs lie apart).  SHORT: some part of a head is no row of eight columns and more.
-// Bound by memory.
+// both halves, where pairs lie apart).  Of few rows a
+// thread's first group is under way while places and angles, a chain of four trips to memory, are found.
+// SHORT: some part of a head is no row of eight columns and more.
 template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THREADS) void k_cache_append(AppendArgs a, int each) {
   __shared__ int page[MOST_ROWS_EACH];
   __shared__ long at[MOST_ROWS_EACH];
   __shared__ float2 angles[MOST_ROWS_EACH * (RPU_CACHE_MAX_HEAD / 2)];
   const int first = blockIdx.x * each, count = min(each, a.r.rows - first), tid = threadIdx.x;
   const int pairs = a.c.pairs, head = a.c.head, rest = head - 2 * pairs;
-  if (tid < count) {
-    const Sequence s = sequence_of(a.r, first + tid);
-    const long position = s.first + (first + tid - s.begin);
-    at[tid] = position;
-    page[tid] = s.which < 0 ? -2 : page_of(a.c, a.r, a.r.tables + s.which * a.r.table_ld, position); // -2: no sequence
-  }
-  __syncthreads();
-  for (int i = tid; i < count * pairs; i += THREADS) angles[i] = turned((double)at[i / pairs] * a.c.turns[i % pairs]);
-  __syncthreads();
   // groups of a head: of its pairs, then of what is not rotated; values go over whole
   const int of_pairs = ((a.c.neighbours ? 2 * pairs : pairs) + 7) / 8, of_head = of_pairs + (rest + 7) / 8, of_value = head / 8;
-  const int q_heads = a.q.p ? a.q_heads : 0;
-  const int of_row = (q_heads + a.c.heads) * of_head + a.c.heads * of_value;
-  for (int i = tid; i < count * of_row; i += THREADS) {
+  const int q_heads = a.q.p ? a.q_heads : 0, of_keys = (q_heads + a.c.heads) * of_head;
+  const int of_row = of_keys + a.c.heads * of_value, groups = count * of_row;
+
+  struct Group {
+    Packed8<T> one, two;
+  };
+  const auto take = [&](int i) { // only loads
+    const long row = first + i / of_row;
+    int g = i % of_row;
+    const T *in;
+    int col, cols;
+    bool both = false;
+    if (g >= of_keys) {
+      g -= of_keys;
+      in = static_cast<const T *>(a.v.p) + row * a.v.ld + g / of_value * head;
+      col = g % of_value * 8;
+      cols = head;
+    } else {
+      const int h = g / of_head;
+      g %= of_head;
+      in = h < q_heads ? static_cast<const T *>(a.q.p) + row * a.q.ld + h * head : static_cast<const T *>(a.k.p) + row * a.k.ld + (h - q_heads) * head;
+      both = g < of_pairs && !a.c.neighbours;
+      if (g >= of_pairs) in += 2 * pairs;
+      col = (g >= of_pairs ? g - of_pairs : g) * 8;
+      cols = g >= of_pairs ? rest : both ? pairs : 2 * pairs;
+    }
+    Group p;
+    p.one = ahead8<SHORT>(in, col, cols);
+    if (both) p.two = ahead8<SHORT>(in + pairs, col, cols);
+    return p;
+  };
+  const auto give = [&](int i, Group &p) {
     const int r = i / of_row;
     int g = i % of_row;
-    if (page[r] == -2) continue;
+    if (page[r] == -2) return;
     const long row = first + r;
-    if (g >= (q_heads + a.c.heads) * of_head) {
-      if (page[r] < 0) continue;
-      g -= (q_heads + a.c.heads) * of_head;
-      const int h = g / of_value, col = g % of_value * 8;
-      const Values8 v = widen(load8(static_cast<const T *>(a.v.p) + row * a.v.ld + h * head + col));
-      store8(static_cast<TC *>(a.c.v) + place_of(a.c, page[r], h, at[r]) + col, v);
-      continue;
+    if (g >= of_keys) {
+      g -= of_keys;
+      const int col = g % of_value * 8;
+      if (page[r] >= 0) store8(static_cast<TC *>(a.c.v) + place_of(a.c, page[r], g / of_value, at[r]) + col, widen(p.one));
+      return;
     }
     const int h = g / of_head;
     const bool query = h < q_heads;
-    if (!query && page[r] < 0) continue;
+    if (!query && page[r] < 0) return;
     g %= of_head;
-    const T *in = query ? static_cast<const T *>(a.q.p) + row * a.q.ld + h * head : static_cast<const T *>(a.k.p) + row * a.k.ld + (h - q_heads) * head;
     T *out = static_cast<T *>(a.out.p) + row * a.out.ld + h * head;
     TC *key = static_cast<TC *>(a.c.k) + (query ? 0 : place_of(a.c, page[r], h - q_heads, at[r]));
     const auto write = [&](int col, const Values8 &v, int n) {
@@ -68,10 +86,12 @@ template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THRE
     };
     if (g >= of_pairs) {
       const int col = (g - of_pairs) * 8;
-      write(2 * pairs + col, read8<SHORT>(in + 2 * pairs, col, rest), rest - col);
+      trim8(p.one, col, rest);
+      write(2 * pairs + col, widen(p.one), rest - col);
     } else if (a.c.neighbours) {
       const int col = g * 8;
-      Values8 v = read8<SHORT>(in, col, 2 * pairs);
+      trim8(p.one, col, 2 * pairs);
+      Values8 v = widen(p.one);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const float2 t = angles[r * pairs + min(col / 2 + k, pairs - 1)];
@@ -82,7 +102,9 @@ template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THRE
       write(col, v, 2 * pairs - col);
     } else {
       const int col = g * 8;
-      Values8 x = read8<SHORT>(in, col, pairs), y = read8<SHORT>(in + pairs, col, pairs);
+      trim8(p.one, col, pairs);
+      trim8(p.two, col, pairs);
+      Values8 x = widen(p.one), y = widen(p.two);
 #pragma unroll
       for (int k = 0; k < 8; ++k) {
         const float2 t = angles[r * pairs + min(col + k, pairs - 1)];
@@ -93,6 +115,25 @@ template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THRE
       write(col, x, pairs - col);
       write(pairs + col, y, pairs - col);
     }
+  };
+
+  const bool early = each == 1;
+  Group now;
+  if (early) now = take(min(tid, groups - 1));
+  // (rows whose sequences are searched for by a wave each, others by a thread)
+  const int by = a.r.starts ? 64 : 1;
+  for (int i = tid / by; i < count; i += THREADS / by) {
+    const Sequence s = sequence_of(a.r, first + i);
+    const long position = s.first + (first + i - s.begin);
+    at[i] = position;
+    page[i] = s.which < 0 ? -2 : page_of(a.c, a.r, a.r.tables + s.which * a.r.table_ld, position); // -2: no sequence
+  }
+  __syncthreads();
+  for (int i = tid; i < count * pairs; i += THREADS) angles[i] = turned((double)at[i / pairs] * a.c.turns[i % pairs]);
+  __syncthreads();
+  for (int i = tid; i < groups; i += THREADS) {
+    if (!early || i != tid) now = take(i);
+    give(i, now);
   }
 }
 

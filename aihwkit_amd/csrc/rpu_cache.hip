@@ -69,12 +69,13 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     const long all = longest && longest < places ? longest : places;
     return window ? std::min(all, (long)window + sinks + tokens + 64) : all;
   };
-  if (r.starts_dev || lines <= ATTEND_FEW) {
+  const bool long_head = c.head_size > ATTEND_FEW_HEAD;
+  if (!long_head && (r.starts_dev || lines <= ATTEND_FEW)) {
     p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
     p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 512, 4096);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
-  if (r.starts_dev || lines > ATTEND_FEW) {
+  if (long_head || r.starts_dev || lines > ATTEND_FEW) {
     const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
