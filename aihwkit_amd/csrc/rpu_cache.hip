@@ -79,7 +79,9 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
-    p.splits = splits_for(tiles * c.heads, seen(ATTEND_LINES / group + 1), 512, 512, 0);
+    // (tiles that there are if the rows are of one sequence, at most about as many workgroups without work as with it)
+    const long least = r.starts_dev ? r.rows * group / ATTEND_LINES + 1 : tiles;
+    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, 512, 0), 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
   if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
