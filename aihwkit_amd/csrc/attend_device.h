@@ -52,8 +52,10 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static __device__ __forceinline__ int v_at(int row, int chunk) {
     return DIRECT ? row / GROUP * V_GROUP + row % GROUP * DP + (chunk ^ v_turn(row)) * 8 : row * V_ROW + chunk * 8;
   }
-  static constexpr int TILE_VALUES = KP * (K_PLANE + V_PLANE);
-  static constexpr int KEY_WAVES = !FEW ? 1 : KP == 1 || DP == 64 ? 4 : DP == 128 ? 2 : 1; // that share a line's positions
+  // A wave that has its tile of float parts by itself puts the values where the keys were: four waves have room beside each other.
+  static constexpr bool IN_TURN = FEW && KP == 3;
+  static constexpr int TILE_VALUES = KP * (IN_TURN ? (K_PLANE > V_PLANE ? K_PLANE : V_PLANE) : K_PLANE + V_PLANE);
+  static constexpr int KEY_WAVES = FEW ? 4 : 1; // that share a line's positions
   static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
   static constexpr int STAGES = FEW || KP == 3 ? 1 : 2; // tiles that there is room for
@@ -312,22 +314,44 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   Packed8<TC> k_ahead[LOADS], v_ahead[LOADS];
   const int chunk = lane % CHUNKS, first_group = FEW ? 0 : wave;
   const uint32_t lane_at = (r_lane * head + (chunk * 8 < head ? chunk * 8 : 0)) * (uint32_t)sizeof(TC);
-  const auto load = [&](uint64_t at) {
+  const auto load = [&](Packed8<TC> (&ahead)[LOADS], const void *from, uint64_t at) {
 #pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP;
-      k_ahead[i] = load8(reinterpret_cast<const TC *>(address(a.c.k, at, r) + lane_at));
-      v_ahead[i] = load8(reinterpret_cast<const TC *>(address(a.c.v, at, r) + lane_at));
-    }
+    for (int i = 0; i < LOADS; ++i) ahead[i] = load8(reinterpret_cast<const TC *>(address(from, at, (S::LOADERS / 64 * i + first_group) * S::GROUP) + lane_at));
   };
-  // keys and values into LDS, zeros where there are none; whether some value is not finite (looked at where it matters)
-  const auto put = [&](uint16_t *keys, uint16_t *values, uint64_t here, bool whole, bool look) {
-    bool bad = false;
+  // into LDS, zeros where there is nothing
+  const auto put = [&](Packed8<TC> (&ahead)[LOADS], auto at, int plane, uint16_t *tile, uint64_t here, bool whole) {
     if (!whole) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i)
-        if (!((here >> ((S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane)) & 1) || chunk * 8 >= head) k_ahead[i] = v_ahead[i] = {};
+        if (!((here >> ((S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane)) & 1) || chunk * 8 >= head) ahead[i] = {};
     }
+#pragma unroll
+    for (int i = 0; i < LOADS; ++i) {
+      uint16_t *const to = tile + at((S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane, chunk);
+      if constexpr (KP == 1) {
+        *reinterpret_cast<u32x4 *>(to) = ahead[i].q;
+      } else {
+        const Values8 v = widen(ahead[i]);
+        u32x4 out[KP];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          uint32_t part[KP];
+          split2<M>(v.v[2 * n], v.v[2 * n + 1], part);
+#pragma unroll
+          for (int j = 0; j < KP; ++j) out[j][n] = part[j];
+        }
+#pragma unroll
+        for (int j = 0; j < KP; ++j) *reinterpret_cast<u32x4 *>(to + j * plane) = out[j];
+      }
+    }
+  };
+  const auto put_keys = [&](uint16_t *keys, uint64_t here, bool whole) {
+    put(k_ahead, [](int r, int chunk) { return S::k_at(r, chunk); }, S::K_PLANE, keys, here, whole);
+  };
+  // whether some value is not finite, looked at where it matters
+  const auto put_values = [&](uint16_t *values, uint64_t here, bool whole, bool look) {
+    put(v_ahead, [](int r, int chunk) { return S::v_at(r, chunk); }, S::V_PLANE, values, here, whole);
+    bool bad = false;
     if (look) {
 #pragma unroll
       for (int i = 0; i < LOADS; ++i) {
@@ -338,33 +362,6 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           const Values8 v = widen(v_ahead[i]);
 #pragma unroll
           for (int n = 0; n < 8; ++n) bad |= !__builtin_isfinite(v.v[n]);
-        }
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < LOADS; ++i) {
-      const int r = (S::LOADERS / 64 * i + first_group) * S::GROUP + r_lane;
-      uint16_t *to_k = keys + S::k_at(r, chunk), *to_v = values + S::v_at(r, chunk);
-      if constexpr (KP == 1) {
-        *reinterpret_cast<u32x4 *>(to_k) = k_ahead[i].q;
-        *reinterpret_cast<u32x4 *>(to_v) = v_ahead[i].q;
-      } else {
-        const Values8 k = widen(k_ahead[i]), v = widen(v_ahead[i]);
-        u32x4 out[2][KP];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          uint32_t part[KP];
-          split2<M>(k.v[2 * n], k.v[2 * n + 1], part);
-#pragma unroll
-          for (int j = 0; j < KP; ++j) out[0][j][n] = part[j];
-          split2<M>(v.v[2 * n], v.v[2 * n + 1], part);
-#pragma unroll
-          for (int j = 0; j < KP; ++j) out[1][j][n] = part[j];
-        }
-#pragma unroll
-        for (int j = 0; j < KP; ++j) {
-          *reinterpret_cast<u32x4 *>(to_k + j * S::K_PLANE) = out[0][j];
-          *reinterpret_cast<u32x4 *>(to_v + j * S::V_PLANE) = out[1][j];
         }
       }
     }
@@ -606,42 +603,61 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         fetch_keys(at_now, 0);
         fetch_values(at_now, 0);
       } else if constexpr (!S::LATE) {
-        load(at_now);
+        load(k_ahead, a.c.k, at_now);
+        load(v_ahead, a.c.v, at_now);
       }
     }
     for (int turn = 0; t < to; t += step, turn ^= 1) {
       const int stage = FEW ? wave : S::STAGES == 2 ? turn : 0;
-      uint16_t *const keys = attend_lds + stage * KP * S::K_PLANE, *const values = attend_lds + S::TILES * KP * S::K_PLANE + stage * KP * S::V_PLANE;
+      uint16_t *const keys = attend_lds + stage * (S::IN_TURN ? S::TILE_VALUES : KP * S::K_PLANE);
+      uint16_t *const values = S::IN_TURN ? keys : attend_lds + S::TILES * KP * S::K_PLANE + stage * KP * S::V_PLANE;
       const int base = base_of(t);
       const uint64_t here = there;
-      const bool masked = is_masked(base, here);
+      const bool masked = is_masked(base, here), whole = here == ALL && head == DP, more = t + step < to;
       if (S::STAGES == 1) all_there(); // the tile before has been read
-      bool bad = false;
-      if constexpr (S::DIRECT) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        bad = masked && clean(values, here);
-      } else {
-        if constexpr (S::LATE) load(at_now);
-        bad = put(keys, values, here, here == ALL && head == DP, masked);
-      }
-      bad = everybody(masked, bad);
-      if (t + step < to) {
+      uint64_t at = 0;
+      if (more) {
         const int page = page_at(t + step, next_entry);
         there = wanted(t + step, page);
-        const uint64_t at = rows_at(t + step, page);
-        if constexpr (S::DIRECT) {
-          fetch_keys(at, turn ^ 1);
-          fetch_values(at, turn ^ 1);
-        } else if constexpr (S::LATE) {
-          at_now = at;
-        } else {
-          load(at);
-        }
+        at = rows_at(t + step, page);
         next_entry = entry_at(t + 2 * step);
       }
-      if (!FEW && !bad && base > wave_last) continue; // (the first lines of a workgroup do not see its last positions)
+      bool bad = false;
       Scores score;
-      scores_of(keys, score);
+      if constexpr (S::IN_TURN) {
+        put_keys(keys, here, whole);
+        all_there();
+        if (more) load(k_ahead, a.c.k, at);
+        scores_of(keys, score);
+        all_there();
+        bad = everybody(masked, put_values(values, here, whole, masked));
+        if (more) load(v_ahead, a.c.v, at);
+      } else {
+        if constexpr (S::DIRECT) {
+          asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          bad = masked && clean(values, here);
+        } else {
+          if constexpr (S::LATE) {
+            load(k_ahead, a.c.k, at_now);
+            load(v_ahead, a.c.v, at_now);
+          }
+          put_keys(keys, here, whole);
+          bad = put_values(values, here, whole, masked);
+        }
+        bad = everybody(masked, bad);
+        if (more) {
+          at_now = at;
+          if constexpr (S::DIRECT) {
+            fetch_keys(at, turn ^ 1);
+            fetch_values(at, turn ^ 1);
+          } else if constexpr (!S::LATE) {
+            load(k_ahead, a.c.k, at);
+            load(v_ahead, a.c.v, at);
+          }
+        }
+      }
+      if (!FEW && !bad && base > wave_last) continue; // (the first lines of a workgroup do not see its last positions)
+      if constexpr (!S::IN_TURN) scores_of(keys, score);
       // reads of LDS stay ahead of the products
       order<READ>(Int<4 * KP>{});
 #pragma unroll

@@ -81,7 +81,7 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     p.tiles = (int)tiles;
     // (tiles that there are if the rows are of one sequence, at most about as many workgroups without work as with it)
     const long least = r.starts_dev ? r.rows * group / ATTEND_LINES + 1 : tiles;
-    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, 512, 0), 2048 / (tiles * c.heads)));
+    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0), 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
   if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
