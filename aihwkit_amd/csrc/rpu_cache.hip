@@ -62,6 +62,7 @@ int splits_for(long units, long longest, long least, long together, long many) {
 }
 AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
   AttendPlan p{};
+  if ((long)r.rows * (q_heads / c.heads) > (1 << 30)) throw RpuError("So many rows and heads are too many for a call.");
   const long group = q_heads / c.heads, places = (long)r.table_width * c.page_size;
   const long lines = r.starts_dev ? 0 : r.rows / r.n * group; // of every sequence
   // positions that a workgroup goes over, whose lines are of up to so many neighbouring tokens
@@ -84,6 +85,7 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0), 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
+  // (sequences, tiles and parts are counted in 32 bits)
   if (std::max(p.few_jobs, p.jobs) > (1l << 30)) throw RpuError("So many sequences, rows and heads are too many for a call.");
   const auto take = [&](size_t n) {
     const size_t at = p.bytes;
@@ -161,7 +163,7 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     const size_t e = value_size(dtype), bytes = cache_bytes(*cache);
     const int width = width_of(q_heads, *cache);
     if (q_heads % cache->heads) throw RpuError("The heads of a row must be a multiple of the cache's.");
-    if (!std::isfinite(scale)) throw RpuError("The scale must be finite.");
+    if (!(std::fabs(scale) <= 1e30f)) throw RpuError("The scale must be finite, and at most 1e30.");
     if (window < 0 || sinks < 0) throw RpuError("window and sinks must not be negative.");
     if (sinks && !window) throw RpuError("Only a window has first tokens that stay visible.");
     if (longest < 0) throw RpuError("longest must not be negative.");

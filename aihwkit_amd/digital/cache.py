@@ -193,8 +193,8 @@ class PagedCache:
         """Attention of the new rows [rows, heads, head_size] over what the cache holds, their own keys and values included.
 
         The row at position ``p`` sees positions ``j <= p``; with a ``window`` > 0 those of ``j > p - window`` or ``j < sinks``.  ``heads`` is a
-        multiple of the cache's, each of which serves as many neighbouring ones.  ``scale`` (None: ``head_size ** -0.5``) multiplies the
-        products of queries and keys.  ``longest``: a number that no length exceeds (None: what the tables hold); how the work is
+        multiple of the cache's, each of which serves as many neighbouring ones.  ``scale`` (None: ``head_size ** -0.5``; up to 1e30)
+        multiplies the products of queries and keys.  ``longest``: a number that no length exceeds (None: what the tables hold); how the work is
         shared goes by it, the results are right without it.  A row that sees nothing becomes zeros, and so does one whose weights are all
         zero.  What a row does not see does not reach it, infinities and NaN included.  ``out`` may be ``queries``."""
         done = torch_calls().cache_attend(self.keys, self.values, self._shape, queries, tables, lengths, starts, scale, window, sinks, longest, out,

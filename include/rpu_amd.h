@@ -842,7 +842,7 @@ int rpu_cache_append(const rpu_cache *cache, const rpu_cache_rows *rows, const v
 /* Attention of the new rows over the cache, which holds them by then: out = sum_j w_j v_j / sum_j w_j with w_j = exp(scale q k_j - max)
  * over the positions j that the row at position p sees: 0 <= j <= p and, with a window > 0, j > p - window or j < sinks.  A row that sees
  * nothing, or whose weights are all zero, becomes zeros.  q_heads: a multiple of the cache's heads, each of which serves as many neighbouring ones.
- * out_dev may be q_dev; rows of no sequence are left as they are.  longest: what no length exceeds (0: what the tables hold); how the
+ * scale: up to 1e30 in magnitude.  out_dev may be q_dev; rows of no sequence are left as they are.  longest: what no length exceeds (0: what the tables hold); how the
  * work is shared goes by it, results are right without it.  Values of places that a row does not see do not reach it, infinities and NaN
  * included.  scratch: rpu_cache_attend_scratch bytes (0: may be null), aligned to 16, used until the call's work is done. */
 size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *rows, int q_heads, int dtype, int window, int sinks, int longest);

@@ -89,7 +89,7 @@ def test_append_refusals(kw, text):
 @pytest.mark.parametrize("kw, text", [
     (dict(dtype=4), "Unknown data type"), (dict(dtype=BF16), "16-bit rows"), (dict(q=None), "q is null"), (dict(out=None), "output is null"),
     (dict(heads=3), "multiple of the cache's"), (dict(heads=0), "at least one head"), (dict(q_ld=255), "overlap"), (dict(scale=float("nan")), "scale"),
-    (dict(scale=float("inf")), "scale"), (dict(window=-1), "negative"), (dict(sinks=-1, window=4), "negative"), (dict(sinks=4), "Only a window"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=-2e30), "scale"), (dict(r=rows(rows=1 << 28), c=cache(head_size=8, pairs=0, heads=1), heads=16), "too many"), (dict(window=-1), "negative"), (dict(sinks=-1, window=4), "negative"), (dict(sinks=4), "Only a window"),
     (dict(longest=-1), "longest"), (dict(out=place(7) + 8), "overlaps"), (dict(out=place(0)), "overlaps"), (dict(out=place(1)), "overlaps"),
     (dict(out=place(3)), "overlaps"), (dict(out=place(4)), "overlaps"), (dict(r=rows(starts_dev=place(8))), "overlaps"),
 ])
