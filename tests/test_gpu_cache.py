@@ -113,6 +113,34 @@ def test_long_caches(dtype, cache_dtype):
         batch.check(batch.attend(longest=100))      # too small a number costs time only
 
 
+@pytest.mark.parametrize("dtype", [F16, BF16], ids=["f16", "bf16"])
+@pytest.mark.parametrize("kv, group, head", [(48, 1, 64), (16, 3, 40), (7, 7, 8)])
+def test_batches_of_many_rows(kv, group, head, dtype):
+    """So many rows of short heads that a wave has twice the lines: the same bits as sequence by sequence, and (some rows) the formula."""
+    layout = [(400, 90), (331, 0), (0, 17), (1, 499), (500, 12), (450, 3), (470, 1), (2, 300), (390, 100), (420, 20)]
+    batch = Batch(layout, kv * group, kv, head, 16, dtype, dtype, seed=18, before=1, behind=3)
+    batch.tables_host = batch.tables_host[:, :32].contiguous()      # 512 positions: no parts
+    at = int(batch.tables_host[0, 3])
+    batch.values[at, 0, 5, 2:5] = INF
+    batch.gpu()
+    assert batch.rows * kv * group >= 2 * 128 * 512
+    for kw in (dict(), dict(window=70, sinks=5)):
+        whole = batch.attend(**kw)
+        assert (whole[:1] == 0).all() and (whole[-3:] == 0).all()
+        for s in range(len(layout)):
+            rows = slice(batch.starts_host[s], batch.starts_host[s + 1])
+            if batch.new[s] > 2:       # (few rows go another way)
+                alone = batch.cache.attend(batch.q[rows], batch.tables[s:s + 1], batch.lengths_gpu[s:s + 1], **kw)
+                assert torch.equal(torch.nan_to_num(alone), torch.nan_to_num(whole[rows]))
+        short = Batch.__new__(Batch)
+        short.__dict__.update(batch.__dict__)
+        for s, i in ((1, 0), (1, 330), (4, 255), (4, 256), (5, 100), (8, 389)):     # one row: of as many positions as there are up to it
+            row = batch.starts_host[s] + i
+            short.q, short.rows = batch.q[row:row + 1], 1
+            short.tables_host, short.lengths, short.starts_host = batch.tables_host[s:s + 1], [batch.lengths[s] - batch.new[s] + i + 1], [0, 1]
+            short.check(whole[row:row + 1], **kw)
+
+
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 30.0])
 def test_scales(scale, dtype, cache_dtype):
