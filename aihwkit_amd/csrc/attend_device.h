@@ -22,8 +22,7 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr float NONE = -__builtin_inff(), LOG2E = 1.44269504088896340736f;
 
 // How rows of T beside a cache of TC, heads of up to 32 D32 values, are worked on.
-// SETS: 32 lines each, of a wave.
-template <typename T, typename TC, int D32, bool FEW, int SETS = 1> struct Shape {
+template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr bool HALF = __is_same(TC, _Float16);
   using M = std::conditional_t<__is_same(TC, float), __bf16, TC>; // of matrix operands
   static constexpr int KP = sizeof(TC) == 4 ? 3 : 1;                         // parts of keys and values
@@ -57,7 +56,7 @@ template <typename T, typename TC, int D32, bool FEW, int SETS = 1> struct Shape
   static constexpr bool IN_TURN = FEW && KP == 3;
   static constexpr int TILE_VALUES = KP * (IN_TURN ? (K_PLANE > V_PLANE ? K_PLANE : V_PLANE) : K_PLANE + V_PLANE);
   static constexpr int KEY_WAVES = FEW ? 4 : 1; // that share a line's positions
-  static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128 * SETS, LOADERS = FEW ? 64 : 256;
+  static constexpr int WAVES = FEW ? KEY_WAVES : 4, LINES = FEW ? 32 : 128, LOADERS = FEW ? 64 : 256;
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
   static constexpr int STAGES = FEW || KP == 3 ? 1 : 2; // tiles that there is room for
   static constexpr int PER_SIMD = D32 <= 4 && (KP == 1 ? QP == 1 || D32 <= 2 : !FEW) ? 2 : 1; // waves, as the registers allow
@@ -167,9 +166,9 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
   return true;
 }
 
-template <typename T, typename TC, int D32, bool FEW, int SETS>
-__global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<T, TC, D32, FEW, SETS>::PER_SIMD)) void k_attend(AttendArgs a) {
-  using S = Shape<T, TC, D32, FEW, SETS>;
+template <typename T, typename TC, int D32, bool FEW>
+__global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a) {
+  using S = Shape<T, TC, D32, FEW>;
   using M = typename S::M;
   constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
@@ -184,32 +183,19 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
   job.line = __builtin_amdgcn_readfirstlane(job.line);
   job.lines = __builtin_amdgcn_readfirstlane(job.lines);
 
-  // the lines of this lane, one of each set
-  struct Line {
-    bool live;
-    int token, row, q_head;
-  };
-  const auto line_of = [&](int lane, int g) {
-    const int line = job.line + (FEW ? 0 : 32 * (SETS * wave + g)) + (lane & 31);
-    const bool live = line < job.lines;
-    const int token = live ? line / group : 0;
-    return Line{live, token, job.s.begin + token, job.head * group + (live ? line - token * group : 0)};
-  };
+  // the line of this lane
+  const int line = job.line + (FEW ? 0 : 32 * wave) + (lane & 31);
+  const bool live = line < job.lines;
+  const int token = live ? line / group : 0, row = job.s.begin + token, q_head = job.head * group + (live ? line % group : 0);
   const auto place = [](long p) { return (int)min(max(p, -1l), 1l << 30); };
-  int last_seen[SETS], before[SETS]; // seen are positions <= last_seen, and > before or < sinks
-#pragma unroll
-  for (int g = 0; g < SETS; ++g) {
-    const Line of = line_of(lane, g);
-    last_seen[g] = of.live ? place(job.s.first + of.token) : -1;
-    before[g] = a.window ? place(job.s.first + of.token - a.window) : -1;
-  }
+  const int last_seen = live ? place(job.s.first + token) : -1;                                     // positions <= last_seen
+  const int before = a.window ? place(job.s.first + token - a.window) : -1;                         // and > before, or < sinks
   // positions that some line of the workgroup sees, and those that all of them do
   const int token0 = job.line / group, token1 = (min(job.line + S::LINES, job.lines) - 1) / group;
   const int end = min(place(job.s.first + token1) + 1, a.r.places), low = a.window ? min(place(job.s.first + token0 - a.window) + 1, end) : 0;
   const int all_last = place(job.s.first + token0), all_before = a.window ? place(job.s.first + token1 - a.window) : -1;
   // what the lines of this wave see at most
-  const int wave_line = job.line + 32 * SETS * wave;
-  const int wave_last = FEW || wave_line >= job.lines ? -1 : place(job.s.first + (min(wave_line + 32 * SETS, job.lines) - 1) / group);
+  const int wave_line = job.line + 32 * wave, wave_last = FEW || wave_line >= job.lines ? -1 : place(job.s.first + (min(wave_line + 32, job.lines) - 1) / group);
   const int sink_end = low > 0 ? min(a.sinks, end) : 0;
   const int sink_tiles = (sink_end + TILE - 1) / TILE, first_tile = max(low / TILE, sink_tiles), tiles = sink_tiles + max((end + TILE - 1) / TILE - first_tile, 0);
   const int splits = FEW ? a.few_splits : a.splits, each = max((tiles + splits - 1) / splits, FEW ? ATTEND_FEW_LEAST : 1);
@@ -217,21 +203,19 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
   const auto base_of = [&](int t) { return (t < sink_tiles ? t : first_tile + t - sink_tiles) * TILE; };
 
   // queries: 8 values of each 16 to a lane
+  const T *const at_q = static_cast<const T *>(a.q.p) + (live ? row * a.q.ld + q_head * head : 0l);
+  const auto query_at = [&](int i) { return load8(at_q + (16 * i + 8 * half < head ? 16 * i + 8 * half : 0)); };
   const bool none = a.scale == 0.0f;
-  const T *at_q[SETS];
-  bool live[SETS];
-  float lift[SETS], c[SETS]; // c: of the exponents, in powers of two
-  u32x4 q[SETS][QP][S::QUERIES_AGAIN ? 1 : STEPS];
-  const auto query_at = [&](int g, int i) { return load8(at_q[g] + (16 * i + 8 * half < head ? 16 * i + 8 * half : 0)); };
-  const auto parts_of_query = [&](int g, const Packed8<T> &p, int i, auto &&put) { // (the scale's sign goes with them)
-    const bool there = live[g] && 16 * i + 8 * half < head && !none;
+  float lift = 1.0f;
+  const auto parts_of_query = [&](const Packed8<T> &p, int i, auto &&put) { // (the scale's sign goes with them)
+    const bool there = live && 16 * i + 8 * half < head && !none;
     if constexpr (QP == 1) {
       u32x4 v = p.q;
       if (a.scale < 0.0f) v ^= 0x80008000u;
       put(0, there ? v : u32x4{});
     } else {
       const Values8 v = widen(p);
-      const float factor = a.scale < 0.0f ? -lift[g] : lift[g];
+      const float factor = a.scale < 0.0f ? -lift : lift;
       u32x4 out[QP];
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
@@ -244,32 +228,26 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
       for (int j = 0; j < QP; ++j) put(j, out[j]);
     }
   };
+  u32x4 q[QP][S::QUERIES_AGAIN ? 1 : STEPS];
+  if constexpr (!S::QUERIES_AGAIN) {
+    Packed8<T> p[STEPS];
 #pragma unroll
-  for (int g = 0; g < SETS; ++g) {
-    const Line of = line_of(lane, g);
-    live[g] = of.live;
-    at_q[g] = static_cast<const T *>(a.q.p) + (of.live ? of.row * a.q.ld + of.q_head * head : 0l);
-    lift[g] = 1.0f;
-    if constexpr (!S::QUERIES_AGAIN) {
-      Packed8<T> p[STEPS];
+    for (int i = 0; i < STEPS; ++i) p[i] = query_at(i);
+    if constexpr (QP == 2) {
+      float m = 0.0f;
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) p[i] = query_at(g, i);
-      if constexpr (QP == 2) {
-        float m = 0.0f;
+      for (int i = 0; i < STEPS; ++i) {
+        const Values8 v = widen(p[i]);
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          const Values8 v = widen(p[i]);
-#pragma unroll
-          for (int k = 0; k < 8; ++k) m = 16 * i + 8 * half < head ? fmaxf(m, fminf(fabsf(v.v[k]), 0x1.fffffep127f)) : m;
-        }
-        m = fmaxf(m, __shfl_xor(m, 32));
-        lift[g] = lift_of(m);
+        for (int k = 0; k < 8; ++k) m = 16 * i + 8 * half < head ? fmaxf(m, fminf(fabsf(v.v[k]), 0x1.fffffep127f)) : m;
       }
-#pragma unroll
-      for (int i = 0; i < STEPS; ++i) parts_of_query(g, p[i], i, [&](int j, u32x4 v) { q[g][j][i] = v; });
+      m = fmaxf(m, __shfl_xor(m, 32));
+      lift = lift_of(m);
     }
-    c[g] = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift[g]);
+#pragma unroll
+    for (int i = 0; i < STEPS; ++i) parts_of_query(p[i], i, [&](int j, u32x4 v) { q[j][i] = v; });
   }
+  const float c = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift); // of the exponents, in powers of two
 
   // Tiles: page numbers are under way two tiles ahead, keys and values one.
   const int *table = a.r.tables + job.s.which * a.r.table_ld;
@@ -395,20 +373,18 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
   };
 
   // scores of 32 positions each: 8 (i / 4) + 4 half + i % 4
-  typedef floatx16 Scores[SETS][BLOCKS];
+  typedef floatx16 Scores[BLOCKS];
   constexpr int PRODUCTS = KP == 3 ? 6 : QP; // of a piece of keys or values, all parts
   const auto scores_of = [&](const uint16_t *tile, Scores &score) {
     const uint16_t *keys[2]; // of even and odd steps
 #pragma unroll
     for (int i = 0; i < 2; ++i) keys[i] = tile + S::k_at(lane & 31, 2 * i + half) - (S::DIRECT ? 0 : 16 * i);
 #pragma unroll
-    for (int g = 0; g < SETS; ++g)
-#pragma unroll
-      for (int n = 0; n < BLOCKS; ++n) score[g][n] = floatx16{};
+    for (int n = 0; n < BLOCKS; ++n) score[n] = floatx16{};
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
       const int slot = S::QUERIES_AGAIN ? 0 : i;
-      if constexpr (S::QUERIES_AGAIN) parts_of_query(0, query_at(0, i), i, [&](int j, u32x4 v) { q[0][j][0] = v; });
+      if constexpr (S::QUERIES_AGAIN) parts_of_query(query_at(i), i, [&](int j, u32x4 v) { q[j][0] = v; });
 #pragma unroll
       for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
@@ -416,68 +392,54 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
           const u32x4 k = *reinterpret_cast<const u32x4 *>(S::DIRECT ? keys[i & 1] + 32 / S::GROUP * n * S::K_GROUP + i / 2 * 32
                                                                      : keys[0] + j * S::K_PLANE + 32 * n * S::K_ROW + 16 * i);
 #pragma unroll
-          for (int g = 0; g < SETS; ++g)
-#pragma unroll
-            for (int l = 0; l < QP; ++l)
-              if (j + l < 3) score[g][n] = multiply<M>(k, q[g][l][slot], score[g][n]);
+          for (int l = 0; l < QP; ++l)
+            if (j + l < 3) score[n] = multiply<M>(k, q[l][slot], score[n]);
         }
     }
   };
   // bit n: this lane's line sees position n of 32; the scores of the others leave
-  typedef uint32_t Seen[SETS][BLOCKS];
+  typedef uint32_t Seen[BLOCKS];
   const auto mask = [&](int base, uint64_t here, Scores &score, Seen &seen) {
 #pragma unroll
-    for (int g = 0; g < SETS; ++g)
+    for (int n = 0; n < BLOCKS; ++n) {
+      const int first = base + 32 * n;
+      const auto below = [](int count) { return count >= 32 ? ~0u : (1u << max(count, 0)) - 1; };
+      seen[n] = (uint32_t)(here >> (32 * n)) & below(last_seen - first + 1) & (~below(before - first + 1) | below(a.sinks - first));
+      const uint32_t mine = seen[n] >> (4 * half);
 #pragma unroll
-      for (int n = 0; n < BLOCKS; ++n) {
-        const int first = base + 32 * n;
-        const auto below = [](int count) { return count >= 32 ? ~0u : (1u << max(count, 0)) - 1; };
-        seen[g][n] = (uint32_t)(here >> (32 * n)) & below(last_seen[g] - first + 1) & (~below(before[g] - first + 1) | below(a.sinks - first));
-        const uint32_t mine = seen[g][n] >> (4 * half);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) score[g][n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[g][n][i] : NONE;
-      }
+      for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
+    }
   };
   // The score that weights are relative to, as a power of two too, and their sum (of this lane's positions).  It follows the maximum where that is
   // more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.
   constexpr float SLACK = 8.0f;
-  float m[SETS], power[SETS], total[SETS];
-  floatx16 sums[SETS][D32] = {};
+  float m = NONE, power = NONE, total = 0.0f;
+  floatx16 sums[D32] = {};
+  const auto raise = [&](const Scores &score) {
+    float now = score[0][0], other;
 #pragma unroll
-  for (int g = 0; g < SETS; ++g) {
-    m[g] = power[g] = NONE;
-    total[g] = 0.0f;
-  }
-  const auto raise = [&](const Scores &score, float (&less)[SETS]) {
+    for (int n = 0; n < BLOCKS; ++n)
 #pragma unroll
-    for (int g = 0; g < SETS; ++g) {
-      float now = score[g][0][0], other;
+      for (int i = 0; i < 16; ++i) now = most(now, score[n][i]);
+    now = half_and_half(now, other);
+    now = most(now, other);
+    const bool far = !(now * c <= power + SLACK) && now != NONE; // (NaN is)
+    if (__any(far)) {
+      now = far ? most(now, m) : m;
+      const float next = now == NONE ? NONE : now * c, shrink = far ? __builtin_amdgcn_exp2f(power - next) : 1.0f;
+      total *= shrink;
 #pragma unroll
-      for (int n = 0; n < BLOCKS; ++n)
-#pragma unroll
-        for (int i = 0; i < 16; ++i) now = most(now, score[g][n][i]);
-      now = half_and_half(now, other);
-      now = most(now, other);
-      const bool far = !(now * c[g] <= power[g] + SLACK) && now != NONE; // (NaN is)
-      if (__any(far)) {
-        now = far ? most(now, m[g]) : m[g];
-        const float next = now == NONE ? NONE : now * c[g], shrink = far ? __builtin_amdgcn_exp2f(power[g] - next) : 1.0f;
-        total[g] *= shrink;
-#pragma unroll
-        for (int n = 0; n < D32; ++n) sums[g][n] *= shrink;
-        m[g] = now;
-        power[g] = next;
-      }
-      less[g] = power[g] == NONE ? 0.0f : power[g];
+      for (int n = 0; n < D32; ++n) sums[n] *= shrink;
+      m = now;
+      power = next;
     }
+    return power == NONE ? 0.0f : power;
   };
   // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
   const auto repair = [&](uint16_t *values, const Seen &seen) {
 #pragma unroll 1
     for (int r = 0; r < TILE; ++r) {
-      bool mine[SETS];
-#pragma unroll
-      for (int g = 0; g < SETS; ++g) mine[g] = (seen[g][BLOCKS - 1 ? r >> 5 : 0] >> (r & 31)) & 1;
+      const bool mine = (seen[BLOCKS - 1 ? r >> 5 : 0] >> (r & 31)) & 1;
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
@@ -485,9 +447,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
           float v = 0.0f;
 #pragma unroll
           for (int j = 0; j < KP; ++j) v += value_of<M>(values[j * S::V_PLANE + S::v_at(r, 4 * n + i / 4) + 4 * half + i % 4]);
-#pragma unroll
-          for (int g = 0; g < SETS; ++g)
-            if (mine[g] && !__builtin_isfinite(v)) sums[g][n][i] += v;
+          if (mine && !__builtin_isfinite(v)) sums[n][i] += v;
         }
     }
     all_there();
@@ -501,33 +461,30 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
   // Weights of 16 positions each (4 half + 8 (e / 4) + e % 4), and their products with four positions of 16 columns to 16 lanes.
   // Halves are up to 2^15, so that small ones keep their bits: of half rows by the exponent, of floats, whose `total` is of the weights, by a product.
   constexpr float LIFT = 0x1p7f;
-  const auto add = [&](uint16_t *values, const Scores &score, const float (&less)[SETS]) {
+  const auto add = [&](uint16_t *values, const Scores &score, float less) {
+    const float exponent = S::HALF && QP == 1 ? less - (15.0f - SLACK) : less;
     constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
     uint16_t *columns[COLUMNS];
 #pragma unroll
     for (int n = 0; n < COLUMNS; ++n) columns[n] = values + S::v_at(4 * half + ((lane & 15) >> 2), 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b) {
-      u32x4 weights[SETS][QP];
+      u32x4 weights[QP];
 #pragma unroll
-      for (int g = 0; g < SETS; ++g)
-#pragma unroll
-        for (int i = 0; i < 8; i += 2) {
-          const floatx16 &of = score[g][b / 2];
-          const int at = 8 * (b & 1) + i;
-          const float exponent = S::HALF && QP == 1 ? less[g] - (15.0f - SLACK) : less[g];
-          float w0 = __builtin_amdgcn_exp2f(fmaf(of[at], c[g], -exponent)), w1 = __builtin_amdgcn_exp2f(fmaf(of[at + 1], c[g], -exponent));
-          if constexpr (QP > 1) total[g] += w0 + w1;
-          if constexpr (S::HALF && QP > 1) {
-            w0 *= LIFT;
-            w1 *= LIFT;
-          }
-          uint32_t part[QP];
-          split2<M>(w0, w1, part);
-          if constexpr (QP == 1) total[g] = add2<M>(part[0], total[g]); // of the rounded ones: those that the values are multiplied with
-#pragma unroll
-          for (int l = 0; l < QP; ++l) weights[g][l][i / 2] = part[l];
+      for (int i = 0; i < 8; i += 2) {
+        const int at = 8 * (b & 1) + i;
+        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -exponent)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -exponent));
+        if constexpr (QP > 1) total += w0 + w1;
+        if constexpr (S::HALF && QP > 1) {
+          w0 *= LIFT;
+          w1 *= LIFT;
         }
+        uint32_t part[QP];
+        split2<M>(w0, w1, part);
+        if constexpr (QP == 1) total = add2<M>(part[0], total); // of the rounded ones: those that the values are multiplied with
+#pragma unroll
+        for (int l = 0; l < QP; ++l) weights[l][i / 2] = part[l];
+      }
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
@@ -542,10 +499,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
           const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
           const u32x4 both = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
-          for (int g = 0; g < SETS; ++g)
-#pragma unroll
-            for (int l = 0; l < QP; ++l)
-              if (j + l < 3) sums[g][n] = multiply<M>(both, weights[g][l], sums[g][n]);
+          for (int l = 0; l < QP; ++l)
+            if (j + l < 3) sums[n] = multiply<M>(both, weights[l], sums[n]);
         }
     }
   };
@@ -612,8 +567,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
         if (!bad && base > wave_last) return; // (the first lines of a workgroup do not see its last positions)
         Seen seen = {};
         if (masked) mask(base, here_now, now, seen);
-        float less[SETS];
-        raise(now, less);
+        const float less = raise(now);
         if (bad) repair(values, seen);
         scores_of(all_keys + (turn ^ 1) * S::K_PLANE, then);
         add(values, now, less);
@@ -708,63 +662,55 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
       order<READ>(Int<4 * KP>{});
 #pragma unroll
       for (int i = 0; i < STEPS * BLOCKS - 4; ++i) {
-        order<PRODUCT>(Int<PRODUCTS * SETS>{});
+        order<PRODUCT>(Int<PRODUCTS>{});
         order<READ>(Int<KP>{});
       }
-      order<PRODUCT>(Int<4 * PRODUCTS * SETS>{});
+      order<PRODUCT>(Int<4 * PRODUCTS>{});
       Seen seen = {};
       if (masked) mask(base, here, score, seen);
-      float less[SETS];
-      raise(score, less);
+      const float less = raise(score);
       if (bad) repair(values, seen);
       add(values, score, less);
     }
   }
-#pragma unroll
-  for (int g = 0; g < SETS; ++g) {
+  {
     float other;
-    const float mine = half_and_half(total[g], other);
-    total[g] = mine + other;
-    if constexpr (S::HALF && QP > 1) total[g] *= LIFT;
+    const float mine = half_and_half(total, other);
+    total = mine + other;
   }
-  int lane_again = lane; // places are found again, not kept in registers meanwhile
-  asm volatile("" : "+v"(lane_again));
+  if constexpr (S::HALF && QP > 1) total *= LIFT;
   if constexpr (!FEW) {
-#pragma unroll
-    for (int g = 0; g < SETS; ++g) {
-      const Line of_line = line_of(lane_again, g);
-      if (!of_line.live) continue;
-      if (a.splits > 1) {
-        const long part = ((long)job.split * a.r.rows + of_line.row) * (a.c.heads * group) + of_line.q_head;
-        if (!half) a.stats[part] = float2{power[g], total[g]};
-#pragma unroll
-        for (int n = 0; n < D32; ++n)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = 32 * n + 8 * i + 4 * half;
-            const floatx16 &of = sums[g][n];
-            if (d < head) *reinterpret_cast<f32x4 *>(a.part + part * head + d) = f32x4{of[4 * i], of[4 * i + 1], of[4 * i + 2], of[4 * i + 3]};
-          }
-        continue;
-      }
-      const float inverse = total[g] == 0.0f ? 0.0f : 1.0f / total[g];
-      T *out = static_cast<T *>(a.out.p) + of_line.row * a.out.ld + of_line.q_head * head;
+    if (!live) return;
+    const long unit = (long)row * (a.c.heads * group) + q_head;
+    if (a.splits > 1) {
+      const long part = (long)job.split * a.r.rows * (a.c.heads * group) + unit;
+      if (!half) a.stats[part] = float2{power, total};
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int d = 32 * n + 8 * i + 4 * half;
-          float v[4];
-#pragma unroll
-          for (int k = 0; k < 4; ++k) v[k] = total[g] == 0.0f ? 0.0f : sums[g][n][4 * i + k] * inverse;
-          if (d < head) store_first(out + d, v, 4);
+          if (d < head) *reinterpret_cast<f32x4 *>(a.part + part * head + d) = f32x4{sums[n][4 * i], sums[n][4 * i + 1], sums[n][4 * i + 2], sums[n][4 * i + 3]};
         }
+      return;
     }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    T *out = static_cast<T *>(a.out.p) + row * a.out.ld + q_head * head;
+#pragma unroll
+    for (int n = 0; n < D32; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int d = 32 * n + 8 * i + 4 * half;
+        float v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) v[k] = total == 0.0f ? 0.0f : sums[n][4 * i + k] * inverse;
+        if (d < head) store_first(out + d, v, 4);
+      }
   } else {
     // the waves' parts meet in LDS, each where its tile was
     __shared__ float2 stats[S::KEY_WAVES][32];
     __shared__ float2 joined[32];
-    if (!half) stats[wave][lane & 31] = float2{power[0], total[0]};
+    if (!half) stats[wave][lane & 31] = float2{power, total};
     __syncthreads();
     float top = NONE, sum = 0.0f;
 #pragma unroll
@@ -773,16 +719,16 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
 #pragma unroll
     for (int w = 0; w < S::KEY_WAVES; ++w) sum = fmaf(stats[w][lane & 31].y, shrink_of(stats[w][lane & 31].x), sum);
     if (wave == 0 && !half) joined[lane & 31] = float2{top, sum};
-    const float shrink = shrink_of(power[0]);
+    const float shrink = shrink_of(power);
     float *const mine = reinterpret_cast<float *>(attend_lds + wave * S::TILE_VALUES) + (lane & 31) * DP;
-    if (line_of(lane_again, 0).live)
+    if (live)
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const int piece = 8 * n + 2 * i + half; // of four values
           *reinterpret_cast<f32x4 *>(mine + (piece ^ (lane & (DP / 4 - 1) & 31)) * 4) =
-              f32x4{sums[0][n][4 * i], sums[0][n][4 * i + 1], sums[0][n][4 * i + 2], sums[0][n][4 * i + 3]} * shrink;
+              f32x4{sums[n][4 * i], sums[n][4 * i + 1], sums[n][4 * i + 2], sums[n][4 * i + 3]} * shrink;
         }
     __syncthreads();
     const int pieces = head / 4, count = job.lines * pieces;
@@ -811,21 +757,14 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW, SETS>::WAVES * 64), (Shape<
 template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t s) {
   const auto with = [&](auto d32) {
     constexpr int D32 = decltype(d32)::value;
-    const auto go = [&](auto few, auto sets, long jobs) {
+    const auto go = [&](auto few, long jobs) {
       constexpr bool FEW = decltype(few)::value;
-      constexpr int SETS = decltype(sets)::value;
-      using Sh = Shape<T, TC, D32, FEW, SETS>;
+      using Sh = Shape<T, TC, D32, FEW>;
       if (!jobs) return;
-      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW, SETS>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
+      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
     };
-    if constexpr (D32 <= 4) go(Int<1>{}, Int<1>{}, a.few_jobs); // (longer heads have no few lines)
-    if constexpr (D32 == 2 && sizeof(T) == 2) { // as attend_plan chooses
-      if (a.sets == 2) {
-        go(Int<0>{}, Int<2>{}, a.jobs);
-        return;
-      }
-    }
-    go(Int<0>{}, Int<1>{}, a.jobs);
+    if constexpr (D32 <= 4) go(Int<1>{}, a.few_jobs); // (longer heads have no few lines)
+    go(Int<0>{}, a.jobs);
   };
   if (a.c.head <= 64) with(Int<2>{});
   else if (a.c.head <= 96) with(Int<3>{});

@@ -30,7 +30,7 @@ constexpr int ATTEND_FEW = 32, ATTEND_LINES = 128; // lines of a sequence that a
 constexpr int ATTEND_FEW_HEAD = 128;               // of heads up to so many values; of longer ones all go in tiles of lines
 constexpr int ATTEND_FEW_LEAST = 4;                // tiles of 32 positions that a part has at least
 struct AttendPlan {
-  int few, few_splits, splits, tiles, sets;        // few: the most lines of a sequence that goes that way, 0: none; a tile has ATTEND_LINES * sets lines
+  int few, few_splits, splits, tiles;              // few: the most lines of a sequence that goes that way, 0: none
   long few_jobs, jobs;                             // workgroups
   size_t few_part, few_stats, part, stats, bytes;  // offsets in the scratch memory, its size
 };
@@ -42,7 +42,7 @@ struct AttendArgs {
   int group;           // heads of a row that share one of the cache
   float scale;
   int window, sinks;   // window 0: none
-  int few, few_splits, splits, tiles, sets;
+  int few, few_splits, splits, tiles;
   long few_jobs, jobs;
   float *few_part, *part;      // sums of a part of the positions: [few_splits][n][heads][few][head], [splits][rows][q heads][head]
   float2 *few_stats, *stats;   // maximum (as a power of two) and sum of the weights

@@ -60,7 +60,7 @@ int splits_for(long units, long longest, long least, long together, long many) {
   const long fill = std::min(together / units, (longest + least - 1) / least), more = std::min(many / units, longest / 1024);
   return (int)std::max(1l, std::min(64l, std::max(fill, more)));
 }
-AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int dtype, int window, int sinks, int longest) {
+AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
   AttendPlan p{};
   if ((long)r.rows * (q_heads / c.heads) > (1 << 30)) throw RpuError("So many rows and heads are too many for a call.");
   const long group = q_heads / c.heads, places = (long)r.table_width * c.page_size;
@@ -77,16 +77,12 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
   if (long_head || r.starts_dev || lines > ATTEND_FEW) {
-    const auto tiles_of = [&](long size) { return r.starts_dev ? r.rows * group / size + r.n : (lines + size - 1) / size * r.n; };
-    // 64 lines to a wave read LDS half as often and share a tile's other work, where heads are short enough for their registers and
-    // there are enough of them for the GPU.
-    p.sets = c.head_size <= 64 && dtype != RPU_F32 && r.rows * group / (2 * ATTEND_LINES) * c.heads >= 512 ? 2 : 1;
-    const long tiles = tiles_of(ATTEND_LINES * p.sets);
+    const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
     // (tiles that there are if the rows are of one sequence, at most about as many workgroups without work as with it)
-    const long least = r.starts_dev ? r.rows * group / (ATTEND_LINES * p.sets) + 1 : tiles;
-    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES * p.sets / group + 1), 512, c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0), 2048 / (tiles * c.heads)));
+    const long least = r.starts_dev ? r.rows * group / ATTEND_LINES + 1 : tiles;
+    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0), 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
   // (sequences, tiles and parts are counted in 32 bits)
@@ -152,7 +148,7 @@ size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *ro
   (void)guarded([&] {
     (void)cache_dev(cache, dtype);
     if (rows_dev(*cache, rows).rows && width_of(q_heads, *cache) && q_heads % cache->heads == 0 && window >= 0 && sinks >= 0 && longest >= 0)
-      bytes = attend_plan(*cache, *rows, q_heads, dtype, window, sinks, longest).bytes;
+      bytes = attend_plan(*cache, *rows, q_heads, window, sinks, longest).bytes;
   });
   return bytes;
 }
@@ -171,7 +167,7 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     if (window < 0 || sinks < 0) throw RpuError("window and sinks must not be negative.");
     if (sinks && !window) throw RpuError("Only a window has first tokens that stay visible.");
     if (longest < 0) throw RpuError("longest must not be negative.");
-    const AttendPlan p = a.r.rows ? attend_plan(*cache, *rows, q_heads, dtype, window, sinks, longest) : AttendPlan{};
+    const AttendPlan p = a.r.rows ? attend_plan(*cache, *rows, q_heads, window, sinks, longest) : AttendPlan{};
     const size_t need = p.bytes;
     if (scratch_bytes < need) throw RpuError("The scratch memory is too small.");
     const Span q = matrix("q", q_dev, q_ld, a.r.rows, width, e), out = matrix("the output", out_dev, out_ld, a.r.rows, width, e),
@@ -198,7 +194,6 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     a.few_splits = p.few_splits;
     a.splits = p.splits;
     a.tiles = p.tiles;
-    a.sets = p.sets;
     a.few_jobs = p.few_jobs;
     a.jobs = p.jobs;
     char *const at = (char *)scratch_dev;
