@@ -9,6 +9,18 @@
 // Matrix operands are 16-bit.  Of 16-bit rows and caches they are the numbers themselves, weights are rounded to that type (half a step of it,
 // relative to each weight, in a mean of values).  Floats go in parts: beside bf16 and floats three bf16 each, beside halves two halves, lifted
 // by a power of two; products of parts that add up to less than 2^-24 of the largest are left out.
+//
+// What bounds it, and what it reaches (us; MI355X):
+//   one token a sequence   memory: keys and values are read once.  64 sequences of up to 8192 positions, 8 heads of 128 bf16 (1.3 GB): 242, 5.5 TB/s;
+//                          one of 131072 positions (0.5 GB): 100; a window of 1024 (0.3 GB): 54; one of 1024 positions, 12 heads of 64: 9.7, two launches.
+//                          (One wave for a line, without matrix instructions: 7551, 119976, 1026, 263.)
+//   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 560 us (980 TFLOP/s; a large matrix product 1320), the matrix pipes are
+//                          busy for 45 %, vector instructions take 50 %, LDS 45 %.  Without the loads of keys and values it takes 476, without
+//                          exponentials 541, without barriers 551.  16384 tokens under a window of 2048, 16 heads of 64 halves: 203 (635 TFLOP/s).
+//   float rows             the products of parts: 3 (bf16 cache), 2 (halves), 6 (floats).  8 x 1024 tokens, 12 heads of 64, bf16 cache: 54 (237 TFLOP/s, a matrix
+//                          product of floats 152).
+// Not kept: 64 lines to a wave (half the reads of LDS; heads of 64 211 us for 203, heads of 128 spill), eight waves to a workgroup (618 for 563), the next
+// tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219).
 #pragma once
 #include "cache.h"
 
@@ -31,16 +43,18 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int TILE = FEW || KP == 3 || (DP == 256 && QP > 1) ? 32 : 64; // positions
   // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
   static constexpr bool DIRECT = !FEW && KP == 1;
-  static constexpr bool AHEAD = DIRECT && (DP == 128 || (DP == 256 && QP == 1)); // the next tile's scores among this one's weights: where a third wave to a SIMD has no registers
+  // The scores of the next tile among the weights of this one, where a third wave to a SIMD has no registers anyway.
+  static constexpr bool AHEAD = DIRECT && (DP == 128 || (DP == 256 && QP == 1));
   static constexpr int GROUP = 64 / CHUNKS;
   static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
+  // Registers are short: values are under way while the scores are multiplied, keys while the weights are (KEYS_LATE:
+  // never), not both; and queries are read and split
+  // again for every tile.  (No kernel may spill: this compiler has stored and reloaded three registers of a spilled four.)
+  static constexpr bool LATE = KP == 3 && D32 > 2 && !FEW, KEYS_LATE = LATE && D32 == 4, QUERIES_AGAIN = QP == 3 && DP == 256;
   // Where 16 bytes of a row lie in LDS: 16 rows that read the same chunk of keys, and four neighbouring rows that read four chunks of values,
   // touch every bank once, at distances that instructions mostly have as constants.  Through registers: rows 16 (keys) and 64 (values) bytes
   // more than their length apart.  DIRECT: chunk ^ turn of the row in its group, and groups at distances of more than 1 KB.
-  // Registers are short: none for a tile that is under way, and queries are read and split again for every tile.  (No kernel may spill: this compiler
-  // has stored and reloaded three registers of a spilled four.)
-  static constexpr bool LATE = KP == 3 && D32 > 2 && !FEW, QUERIES_AGAIN = QP == 3 && DP == 256;
   static constexpr int K_ROW = DP + 8, V_ROW = DP + 32;
   static constexpr int K_GROUP = 512 + (DP == 256 ? 16 : 32), V_GROUP = 512 + (DP == 256 ? 64 : 0);
   static constexpr int K_PLANE = DIRECT ? TILE / GROUP * K_GROUP : TILE * K_ROW, V_PLANE = DIRECT ? TILE / GROUP * V_GROUP : TILE * V_ROW; // of one part
@@ -602,9 +616,9 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         zero_columns();
         fetch_keys(at_now, 0);
         fetch_values(at_now, 0);
-      } else if constexpr (!S::LATE) {
-        load(k_ahead, a.c.k, at_now);
-        load(v_ahead, a.c.v, at_now);
+      } else {
+        if constexpr (!S::KEYS_LATE) load(k_ahead, a.c.k, at_now);
+        if constexpr (!S::LATE) load(v_ahead, a.c.v, at_now);
       }
     }
     for (int turn = 0; t < to; t += step, turn ^= 1) {
@@ -614,7 +628,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       const int base = base_of(t);
       const uint64_t here = there;
       const bool masked = is_masked(base, here), whole = here == ALL && head == DP, more = t + step < to;
-      if (S::STAGES == 1) all_there(); // the tile before has been read
+      if (S::STAGES == 1 && !S::LATE) all_there(); // the tile before has been read (LATE: its keys before its values were put)
       uint64_t at = 0;
       if (more) {
         const int page = page_at(t + step, next_entry);
@@ -632,15 +646,20 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         all_there();
         bad = everybody(masked, put_values(values, here, whole, masked));
         if (more) load(v_ahead, a.c.v, at);
+      } else if constexpr (S::LATE) {
+        if constexpr (S::KEYS_LATE) load(k_ahead, a.c.k, at_now);
+        put_keys(keys, here, whole);
+        all_there();
+        load(v_ahead, a.c.v, at_now);
+        if (base <= wave_last) scores_of(keys, score);
+        bad = everybody(masked, put_values(values, here, whole, masked));
+        if (!S::KEYS_LATE && more) load(k_ahead, a.c.k, at);
+        at_now = at;
       } else {
         if constexpr (S::DIRECT) {
           asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
           bad = masked && clean(values, here);
         } else {
-          if constexpr (S::LATE) {
-            load(k_ahead, a.c.k, at_now);
-            load(v_ahead, a.c.v, at_now);
-          }
           put_keys(keys, here, whole);
           bad = put_values(values, here, whole, masked);
         }
@@ -650,14 +669,14 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
           if constexpr (S::DIRECT) {
             fetch_keys(at, turn ^ 1);
             fetch_values(at, turn ^ 1);
-          } else if constexpr (!S::LATE) {
+          } else {
             load(k_ahead, a.c.k, at);
             load(v_ahead, a.c.v, at);
           }
         }
       }
       if (!FEW && !bad && base > wave_last) continue; // (the first lines of a workgroup do not see its last positions)
-      if constexpr (!S::IN_TURN) scores_of(keys, score);
+      if constexpr (!S::IN_TURN && !S::LATE) scores_of(keys, score);
       // reads of LDS stay ahead of the products
       order<READ>(Int<4 * KP>{});
 #pragma unroll

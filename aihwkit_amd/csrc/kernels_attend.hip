@@ -46,7 +46,41 @@ __device__ __forceinline__ bool join_line(const float *sums, const float2 *stats
   return true;
 }
 
-// Lines of sequences of few lines first, then those of rows.
+// Few parts of many lines: a workgroup for a row, four columns to a lane, all of their loads under way together.
+constexpr int JOIN_PARTS = 8;
+template <typename T> __device__ __forceinline__ void join_row(const AttendArgs &a, int row) {
+  const Sequence s = sequence_of(a.r, row);
+  if (s.which < 0 || (long)(s.end - s.begin) * a.group <= a.few) return;
+  const int q_heads = a.c.heads * a.group, head = a.c.head, pieces = head / 4;
+  const long stride = (long)a.r.rows * q_heads;
+  for (int i = threadIdx.x; i < q_heads * pieces; i += 64 * JOIN_WAVES) {
+    const int h = i / pieces, d = i % pieces * 4;
+    const long unit = (long)row * q_heads + h;
+    float2 stats[JOIN_PARTS];
+    f32x4 part[JOIN_PARTS];
+#pragma unroll
+    for (int p = 0; p < JOIN_PARTS; ++p) stats[p] = a.stats[min(p, a.splits - 1) * stride + unit];
+#pragma unroll
+    for (int p = 0; p < JOIN_PARTS; ++p) part[p] = *reinterpret_cast<const f32x4 *>(a.part + (min(p, a.splits - 1) * stride + unit) * head + d);
+    float top = NONE, total = 0.0f;
+#pragma unroll
+    for (int p = 0; p < JOIN_PARTS; ++p) top = fmaxf(top, stats[p].x);
+    f32x4 v = {};
+#pragma unroll
+    for (int p = 0; p < JOIN_PARTS; ++p) {
+      const float f = p < a.splits && stats[p].x != NONE ? __builtin_amdgcn_exp2f(stats[p].x - top) : 0.0f;
+      if (p < a.splits && stats[p].x != NONE) total += stats[p].y * f;
+      if (f != 0.0f) v += part[p] * f;
+    }
+    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+    float r[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) r[k] = total == 0.0f ? 0.0f : v[k] * inverse;
+    store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * head + d, r, 4);
+  }
+}
+
+// Lines of sequences of few lines first, then rows, or the lines of rows.
 template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attend_join(AttendArgs a, long few_units) {
   const int q_heads = a.c.heads * a.group;
   long unit = blockIdx.x;
@@ -64,6 +98,7 @@ template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_atten
     mine = join_line(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, v);
   } else {
     unit -= few_units;
+    if (a.splits <= JOIN_PARTS) return join_row<T>(a, (int)unit);
     row = (int)(unit / q_heads);
     h = (int)(unit % q_heads);
     const Sequence s = sequence_of(a.r, row);
@@ -80,7 +115,7 @@ void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, hipStr
   with_adapter_types(dtype, cache_dtype, [&](auto x, auto c) {
     using T = decltype(x);
     attend::launch<T, decltype(c)>(a, s);
-    const long few = a.few_jobs && a.few_splits > 1 ? (long)a.r.n * a.c.heads * a.few : 0, rows = a.jobs && a.splits > 1 ? (long)a.r.rows * a.c.heads * a.group : 0;
+    const long few = a.few_jobs && a.few_splits > 1 ? (long)a.r.n * a.c.heads * a.few : 0, rows = a.jobs && a.splits > 1 ? (long)a.r.rows * (a.splits > JOIN_PARTS ? a.c.heads * a.group : 1) : 0;
     if (few + rows) hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(few + rows)), dim3(64 * JOIN_WAVES), 0, s, a, few);
   });
 }

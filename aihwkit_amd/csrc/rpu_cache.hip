@@ -82,7 +82,12 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     p.tiles = (int)tiles;
     // (tiles that there are if the rows are of one sequence, at most about as many workgroups without work as with it)
     const long least = r.starts_dev ? r.rows * group / ATTEND_LINES + 1 : tiles;
-    p.splits = (int)std::max(1l, std::min<long>(splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), 512, c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0), 2048 / (tiles * c.heads)));
+    // (Positions of floats cost most, so shorter parts pay: of at least 256 in 768 workgroups 109 and 36 us, of 512 in 256 137 and 49, for 23 sequences
+    // of up to 275 tokens, 15 heads of 80 under a window of 777, and for 760 tokens of one, 14 heads of 72.  Of 16 bits the same parts lose: 84 to 108
+    // and 13.6 to 16.6 us for 2865 tokens of 18 heads of 232 and 2 sequences of 261, 10 heads of 104.)
+    const bool costly = c.dtype == RPU_F32 && !long_head;
+    p.splits = splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), costly ? 256 : 512, costly ? 768 : c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0);
+    p.splits = (int)std::max(1l, std::min<long>(p.splits, 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
   // (sequences, tiles and parts are counted in 32 bits)

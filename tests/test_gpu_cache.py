@@ -141,6 +141,23 @@ def test_batches_of_many_rows(kv, group, head, dtype):
 
 
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("heads, kv, head", [(6, 2, 72), (5, 5, 8), (2, 1, 128), (2, 1, 200)])
+@pytest.mark.parametrize("context", [700, 1300, 5000])
+def test_joins_of_few_and_of_many_parts(context, heads, kv, head, dtype, cache_dtype):
+    """Parts of rows beside parts of few tokens, empty sequences and rows of none; a window leaves most parts nothing."""
+    batch = Batch([(70, context), (1, context - 90), (0, 5), (33, 0), (2, 600), (40, 129)], heads, kv, head, 16, dtype, cache_dtype, seed=21, before=2, behind=3).gpu()
+    for kw in (dict(), dict(window=90, sinks=1)):
+        out = batch.attend(**kw)
+        batch.check(out, **kw)
+        assert (out[:2] == 0).all() and (out[-3:] == 0).all()
+    batch.tables[0, :40] = -1       # the first 640 positions of all of the rows: nothing for the first parts
+    batch.tables_host[0, :40] = -1
+    batch.check(batch.attend())
+    alike = Batch([(70, context), (70, 0)], heads, kv, head, 16, dtype, cache_dtype, seed=22).gpu()
+    alike.check(alike.attend(starts=False))
+
+
+@pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 @pytest.mark.parametrize("scale", [0.0, -0.3, 1.0, 30.0])
 def test_scales(scale, dtype, cache_dtype):
     batch = Batch(LAYOUTS["mixed"], 4, 2, 64, 16, dtype, cache_dtype, seed=9, spread=1.0).gpu()
