@@ -13,12 +13,13 @@
 // What bounds it, and what it reaches (us; MI355X):
 //   one token a sequence   memory: keys and values are read once.  64 sequences of up to 8192 positions, 8 heads of 128 bf16 (1.3 GB): 242, 5.5 TB/s;
 //                          one of 131072 positions (0.5 GB): 100; a window of 1024 (0.3 GB): 54; one of 1024 positions, 12 heads of 64: 9.7, two launches.
-//                          (One wave for a line, without matrix instructions: 7551, 119976, 1026, 263.)
+//                          (One wave for a line, without matrix instructions: 7551, 119976, 1026, 263.)  Heads of 256, 16 sequences of 4096, 8 heads bf16
+//                          (0.3 GB): 78, in tiles of lines 113; one of 1024, 4 heads: 13, in tiles 35.
 //   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 560 us (980 TFLOP/s; a large matrix product 1320), the matrix pipes are
 //                          busy for 45 %, vector instructions take 50 %, LDS 45 %.  Without the loads of keys and values it takes 476, without
 //                          exponentials 541, without barriers 551.  16384 tokens under a window of 2048, 16 heads of 64 halves: 203 (635 TFLOP/s).
 //   float rows             the products of parts: 3 (bf16 cache), 2 (halves), 6 (floats).  8 x 1024 tokens, 12 heads of 64, bf16 cache: 54 (237 TFLOP/s, a matrix
-//                          product of floats 152).
+//                          product of floats 152).  Floats throughout: 23 sequences, 15 heads of 80 under a window of 777: 108, of which few lines 13, the join 10.
 // Not kept: 64 lines to a wave (half the reads of LDS; heads of 64 211 us for 203, heads of 128 spill), eight waves to a workgroup (618 for 563), the next
 // tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219).
 #pragma once
@@ -48,10 +49,12 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int GROUP = 64 / CHUNKS;
   static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
-  // Registers are short: values are under way while the scores are multiplied, keys while the weights are (KEYS_LATE:
-  // never), not both; and queries are read and split
-  // again for every tile.  (No kernel may spill: this compiler has stored and reloaded three registers of a spilled four.)
-  static constexpr bool LATE = KP == 3 && D32 > 2 && !FEW, KEYS_LATE = LATE && D32 == 4, QUERIES_AGAIN = QP == 3 && DP == 256;
+  // Registers are short: values are under way while the scores are multiplied, keys while the weights are (KEYS_LATE: while nothing is), not both;
+  // queries are read and split again for every tile, or are in LDS, once for the waves of few lines.  (No kernel may spill: this compiler has stored
+  // and reloaded three registers of a spilled four.)
+  static constexpr bool LATE = FEW ? DP == 256 : KP == 3 && D32 > 2, KEYS_LATE = LATE && KP == 3 && D32 == 4;
+  static constexpr bool QUERIES_AGAIN = QP == 3 && DP == 256, QUERIES_LDS = FEW && DP == 256;
+  static_assert(!QUERIES_LDS || QP == 1, "queries as they are");
   // Where 16 bytes of a row lie in LDS: 16 rows that read the same chunk of keys, and four neighbouring rows that read four chunks of values,
   // touch every bank once, at distances that instructions mostly have as constants.  Through registers: rows 16 (keys) and 64 (values) bytes
   // more than their length apart.  DIRECT: chunk ^ turn of the row in its group, and groups at distances of more than 1 KB.
@@ -74,7 +77,7 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int LOADS = TILE * CHUNKS / LOADERS;
   static constexpr int STAGES = FEW || KP == 3 ? 1 : 2; // tiles that there is room for
   static constexpr int PER_SIMD = D32 <= 4 && (KP == 1 ? QP == 1 || D32 <= 2 : !FEW) ? 2 : 1; // waves, as the registers allow
-  static constexpr int TILES = FEW ? KEY_WAVES : STAGES, LDS = TILES * TILE_VALUES * 2;
+  static constexpr int TILES = FEW ? KEY_WAVES : STAGES, LDS = TILES * TILE_VALUES * 2 + (QUERIES_LDS ? STEPS * 1024 : 0);
   static_assert(!FEW || TILE_VALUES * 2 >= 32 * DP * 4, "the sums of a wave fit where its tile was");
 };
 
@@ -242,8 +245,16 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
       for (int j = 0; j < QP; ++j) put(j, out[j]);
     }
   };
-  u32x4 q[QP][S::QUERIES_AGAIN ? 1 : STEPS];
-  if constexpr (!S::QUERIES_AGAIN) {
+  u32x4 q[QP][S::QUERIES_AGAIN || S::QUERIES_LDS ? 1 : STEPS];
+  uint16_t *const q_lds = attend_lds + S::TILES * S::TILE_VALUES + lane * 8;
+  if constexpr (S::QUERIES_LDS) { // the waves' lines are the same
+#pragma unroll
+    for (int k = 0; k < STEPS / S::WAVES; ++k) {
+      const int i = wave * (STEPS / S::WAVES) + k;
+      parts_of_query(query_at(i), i, [&](int, u32x4 v) { *reinterpret_cast<u32x4 *>(q_lds + i * 512) = v; });
+    }
+    __syncthreads();
+  } else if constexpr (!S::QUERIES_AGAIN) {
     Packed8<T> p[STEPS];
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) p[i] = query_at(i);
@@ -397,7 +408,8 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
     for (int n = 0; n < BLOCKS; ++n) score[n] = floatx16{};
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) {
-      const int slot = S::QUERIES_AGAIN ? 0 : i;
+      const int slot = S::QUERIES_AGAIN || S::QUERIES_LDS ? 0 : i;
+      if constexpr (S::QUERIES_LDS) q[0][0] = *reinterpret_cast<const u32x4 *>(q_lds + i * 512);
       if constexpr (S::QUERIES_AGAIN) parts_of_query(query_at(i), i, [&](int j, u32x4 v) { q[j][0] = v; });
 #pragma unroll
       for (int n = 0; n < BLOCKS; ++n)
@@ -651,7 +663,7 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
         put_keys(keys, here, whole);
         all_there();
         load(v_ahead, a.c.v, at_now);
-        if (base <= wave_last) scores_of(keys, score);
+        if (FEW || base <= wave_last) scores_of(keys, score);
         bad = everybody(masked, put_values(values, here, whole, masked));
         if (!S::KEYS_LATE && more) load(k_ahead, a.c.k, at);
         at_now = at;
@@ -782,7 +794,7 @@ template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t 
       if (!jobs) return;
       hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
     };
-    if constexpr (D32 <= 4) go(Int<1>{}, a.few_jobs); // (longer heads have no few lines)
+    if constexpr (D32 <= 4 || sizeof(T) == 2) go(Int<1>{}, a.few_jobs); // (longer heads of floats have no few lines)
     go(Int<0>{}, a.jobs);
   };
   if (a.c.head <= 64) with(Int<2>{});

@@ -27,7 +27,7 @@ void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cu
 // have their positions shared by the waves of a workgroup, others have tiles of lines.  Of both, the positions may go in parts to several
 // workgroups, whose sums are joined.
 constexpr int ATTEND_FEW = 32, ATTEND_LINES = 128; // lines of a sequence that are few; of a tile
-constexpr int ATTEND_FEW_HEAD = 128;               // of heads up to so many values; of longer ones all go in tiles of lines
+constexpr int ATTEND_FEW_HEAD = 128;               // of heads up to so many values; of longer ones of floats all go in tiles of lines
 constexpr int ATTEND_FEW_LEAST = 4;                // tiles of 32 positions that a part has at least
 struct AttendPlan {
   int few, few_splits, splits, tiles;              // few: the most lines of a sequence that goes that way, 0: none

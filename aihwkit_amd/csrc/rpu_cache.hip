@@ -60,7 +60,7 @@ int splits_for(long units, long longest, long least, long together, long many) {
   const long fill = std::min(together / units, (longest + least - 1) / least), more = std::min(many / units, longest / 1024);
   return (int)std::max(1l, std::min(64l, std::max(fill, more)));
 }
-AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int window, int sinks, int longest) {
+AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads, int dtype, int window, int sinks, int longest) {
   AttendPlan p{};
   if ((long)r.rows * (q_heads / c.heads) > (1 << 30)) throw RpuError("So many rows and heads are too many for a call.");
   const long group = q_heads / c.heads, places = (long)r.table_width * c.page_size;
@@ -70,13 +70,13 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     const long all = longest && longest < places ? longest : places;
     return window ? std::min(all, (long)window + sinks + tokens + 64) : all;
   };
-  const bool long_head = c.head_size > ATTEND_FEW_HEAD;
-  if (!long_head && (r.starts_dev || lines <= ATTEND_FEW)) {
+  const bool all_tiles = c.head_size > ATTEND_FEW_HEAD && dtype == RPU_F32;
+  if (!all_tiles && (r.starts_dev || lines <= ATTEND_FEW)) {
     p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
     p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 512, 4096);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
-  if (long_head || r.starts_dev || lines > ATTEND_FEW) {
+  if (all_tiles || r.starts_dev || lines > ATTEND_FEW) {
     const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
@@ -85,8 +85,8 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     // (Positions of floats cost most, so shorter parts pay: of at least 256 in 768 workgroups 109 and 36 us, of 512 in 256 137 and 49, for 23 sequences
     // of up to 275 tokens, 15 heads of 80 under a window of 777, and for 760 tokens of one, 14 heads of 72.  Of 16 bits the same parts lose: 84 to 108
     // and 13.6 to 16.6 us for 2865 tokens of 18 heads of 232 and 2 sequences of 261, 10 heads of 104.)
-    const bool costly = c.dtype == RPU_F32 && !long_head;
-    p.splits = splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), costly ? 256 : 512, costly ? 768 : c.dtype == RPU_F32 ? 256 : 512, long_head ? 2048 : 0);
+    const bool costly = c.dtype == RPU_F32 && !all_tiles;
+    p.splits = splits_for(least * c.heads, seen(ATTEND_LINES / group + 1), costly ? 256 : 512, costly ? 768 : c.dtype == RPU_F32 ? 256 : 512, all_tiles ? 2048 : 0);
     p.splits = (int)std::max(1l, std::min<long>(p.splits, 2048 / (tiles * c.heads)));
     p.jobs = tiles * c.heads * p.splits;
   }
@@ -153,7 +153,7 @@ size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *ro
   (void)guarded([&] {
     (void)cache_dev(cache, dtype);
     if (rows_dev(*cache, rows).rows && width_of(q_heads, *cache) && q_heads % cache->heads == 0 && window >= 0 && sinks >= 0 && longest >= 0)
-      bytes = attend_plan(*cache, *rows, q_heads, window, sinks, longest).bytes;
+      bytes = attend_plan(*cache, *rows, q_heads, dtype, window, sinks, longest).bytes;
   });
   return bytes;
 }
@@ -172,7 +172,7 @@ int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const v
     if (window < 0 || sinks < 0) throw RpuError("window and sinks must not be negative.");
     if (sinks && !window) throw RpuError("Only a window has first tokens that stay visible.");
     if (longest < 0) throw RpuError("longest must not be negative.");
-    const AttendPlan p = a.r.rows ? attend_plan(*cache, *rows, q_heads, window, sinks, longest) : AttendPlan{};
+    const AttendPlan p = a.r.rows ? attend_plan(*cache, *rows, q_heads, dtype, window, sinks, longest) : AttendPlan{};
     const size_t need = p.bytes;
     if (scratch_bytes < need) throw RpuError("The scratch memory is too small.");
     const Span q = matrix("q", q_dev, q_ld, a.r.rows, width, e), out = matrix("the output", out_dev, out_ld, a.r.rows, width, e),
