@@ -25,6 +25,7 @@
 #pragma once
 #include "cache.h"
 
+#include <algorithm>
 #include <type_traits>
 
 namespace rpu_amd {
@@ -184,14 +185,14 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
 }
 
 template <typename T, typename TC, int D32, bool FEW>
-__global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a) {
+__global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a, long from_job) {
   using S = Shape<T, TC, D32, FEW>;
   using M = typename S::M;
   constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
   extern __shared__ __attribute__((aligned(16))) uint16_t attend_lds[];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), half = lane >> 5;
   Job job;
-  if (FEW ? !job_few(a, blockIdx.x, job) : !job_many<S::LINES>(a, blockIdx.x, job)) return;
+  if (FEW ? !job_few(a, from_job + blockIdx.x, job) : !job_many<S::LINES>(a, from_job + blockIdx.x, job)) return;
   const int group = a.group, head = a.c.head;
   // (the same in all lanes, which the compiler does not see of what comes from memory)
   job.s.begin = __builtin_amdgcn_readfirstlane(job.s.begin);
@@ -791,8 +792,8 @@ template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t 
     const auto go = [&](auto few, long jobs) {
       constexpr bool FEW = decltype(few)::value;
       using Sh = Shape<T, TC, D32, FEW>;
-      if (!jobs) return;
-      hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)jobs), dim3(Sh::WAVES * 64), Sh::LDS, s, a);
+      for (long from = 0; from < jobs; from += MOST_GROUPS)
+        hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)std::min(MOST_GROUPS, jobs - from)), dim3(Sh::WAVES * 64), Sh::LDS, s, a, from);
     };
     if constexpr (D32 <= 4 || sizeof(T) == 2) go(Int<1>{}, a.few_jobs); // (longer heads of floats have no few lines)
     go(Int<0>{}, a.jobs);

@@ -15,6 +15,7 @@ struct CacheRowsDev {
   int n, places, rows; // places: positions that a table holds
 };
 
+constexpr long MOST_GROUPS = 1 << 23; // workgroups of 256 threads in a launch: all threads are counted in 32 bits
 struct AppendArgs {
   CacheDev c;
   CacheRowsDev r;

@@ -25,12 +25,12 @@ constexpr int THREADS = 256, MOST_ROWS_EACH = 2;
 // length, the page), are found.  SHORT: some part of a head is no row of eight columns and more.
 // Bound by memory: 16384 rows of 32 query and 8 + 8 other heads of 128 bf16 in 80 us (403 MB, 5.0 TB/s; a copy of 2 GB takes 4.9), with 8 rows to a
 // workgroup 89; few rows by the chain: 8 rows in 4.3 us, a launch, 3216 rows of 18 heads of 80 halves that are searched among 37 sequences in 9.1.
-template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THREADS) void k_cache_append(AppendArgs a, int each) {
+template <typename T, typename TC, bool SHORT> __global__ __launch_bounds__(THREADS) void k_cache_append(AppendArgs a, int each, int from) {
   __shared__ int page[MOST_ROWS_EACH];
   __shared__ long at[MOST_ROWS_EACH];
   __shared__ float2 angles[MOST_ROWS_EACH * (RPU_CACHE_MAX_HEAD / 2)];
   static_assert(MOST_ROWS_EACH <= THREADS / 64, "a wave has one row's entry");
-  const int first = blockIdx.x * each, count = min(each, a.r.rows - first), tid = threadIdx.x;
+  const int first = from + blockIdx.x * each, count = min(each, a.r.rows - first), tid = threadIdx.x;
   const int pairs = a.c.pairs, head = a.c.head, rest = head - 2 * pairs;
   // groups of a head: of its pairs, then of what is not rotated; values go over whole
   const int of_pairs = ((a.c.neighbours ? 2 * pairs : pairs) + 7) / 8, of_head = of_pairs + (rest + 7) / 8, of_value = head / 8;
@@ -148,12 +148,14 @@ void launch_cache_append(const AppendArgs &a, int dtype, int cache_dtype, int cu
   const int rotated = a.c.neighbours ? 2 * a.c.pairs : a.c.pairs, rest = a.c.head - 2 * a.c.pairs;
   const bool is_short = (rotated && rotated < 8) || (rest && rest < 8);
   const int each = (int)std::min<long>(MOST_ROWS_EACH, (a.r.rows + 8l * cus - 1) / (8l * cus));
-  const dim3 grid((unsigned)((a.r.rows + each - 1) / each));
   with_adapter_types(dtype, cache_dtype, [&](auto x, auto c) {
     using T = decltype(x);
     using TC = decltype(c);
-    if (is_short) hipLaunchKernelGGL((k_cache_append<T, TC, true>), grid, dim3(THREADS), 0, s, a, each);
-    else hipLaunchKernelGGL((k_cache_append<T, TC, false>), grid, dim3(THREADS), 0, s, a, each);
+    for (long from = 0; from < a.r.rows; from += MOST_GROUPS * each) {
+      const dim3 grid((unsigned)std::min(MOST_GROUPS, (a.r.rows - from + each - 1) / each));
+      if (is_short) hipLaunchKernelGGL((k_cache_append<T, TC, true>), grid, dim3(THREADS), 0, s, a, each, (int)from);
+      else hipLaunchKernelGGL((k_cache_append<T, TC, false>), grid, dim3(THREADS), 0, s, a, each, (int)from);
+    }
   });
 }
 

@@ -311,6 +311,27 @@ def test_offsets_beyond_32_bits():
 
 # -- append --------------------------------------------------------------------------------------------------------------
 
+def test_more_workgroups_than_a_launch_has():
+    """Of 256 threads each, 2^24 workgroups: what they do is the same as in a small call, all the way to the last."""
+    n, period = (1 << 24) + 37, 512
+    keys, values = (rand(seed, 3, 1, 8, 8, dtype=F16).cuda() for seed in (51, 52))
+    cache = digital.PagedCache(keys, values)
+    tables = numbers([[k % 4 - 1] for k in range(period)])
+    lengths, q = numbers([k % 9 for k in range(period)]), rand(53, period, 1, 8, dtype=F16).cuda()
+    times = -(-n // period)
+    few = cache.attend(q, tables, lengths)
+    many = cache.attend(q.repeat(times, 1, 1)[:n], tables.repeat(times, 1)[:n], lengths.repeat(times)[:n])
+    assert torch.equal(many, few.repeat(times, 1, 1)[:n])
+    # rows of a key and a value each: two to a workgroup
+    rows = (1 << 25) + 37
+    pages = -(-rows // 65536)
+    k = torch.arange(8 * rows, dtype=torch.int32, device="cuda").remainder_(2039).to(F16).view(rows, 1, 8)
+    cache = digital.PagedCache(torch.full((pages, 1, 65536, 8), -1.0, dtype=F16, device="cuda"), torch.full((pages, 1, 65536, 8), -1.0, dtype=F16, device="cuda"))
+    cache.append(k, k, numbers([list(range(pages))]), numbers([rows]))
+    for held in (cache.keys, cache.values):
+        assert torch.equal(held.view(-1, 1, 8)[:rows], k) and (held.view(-1, 8)[rows:] == -1).all()
+
+
 def check_append(batch, frequencies, neighbours, starts=True, layout=lambda t: t):
     """Against the formula; what is not a new row's place keeps its bits."""
     cache = digital.PagedCache(batch.keys.cuda(), batch.values.cuda(), frequencies, neighbours)
