@@ -228,7 +228,27 @@ def test_starts_and_lengths_out_of_range_touch_nothing_else():
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 def test_what_is_not_seen_does_not_reach_a_row(bad, dtype, cache_dtype):
     """Values and keys of later positions, of positions behind the window, of another head and of unused places."""
-    batch = Batch([(140, 60), (3, 130), (1, 300)], 4, 2, 64, 16, dtype, cache_dtype, seed=14)
+    check_poisoned(bad, 64, dtype, cache_dtype)
+
+
+@pytest.mark.parametrize("bad", [NAN, INF])
+@pytest.mark.parametrize("head", [40, 80, 128, 176, 256])
+@pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
+def test_what_is_not_seen_does_not_reach_rows_of_other_heads(head, bad, dtype, cache_dtype):
+    check_poisoned(bad, head, dtype, cache_dtype)
+
+
+@pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("window, sinks", [(1, 1), (64, 4), (100, 64), (3, 130)])
+@pytest.mark.parametrize("heads, kv, head", [(5, 5, 80), (2, 1, 200), (3, 1, 256)])
+def test_windows_of_other_heads(heads, kv, head, window, sinks, dtype, cache_dtype):
+    for layout in ("tokens", "mixed"):
+        batch = Batch(LAYOUTS[layout], heads, kv, head, 32, dtype, cache_dtype, seed=23).gpu()
+        batch.check(batch.attend(window=window, sinks=sinks), window=window, sinks=sinks)
+
+
+def check_poisoned(bad, head, dtype, cache_dtype):
+    batch = Batch([(140, 60), (3, 130), (1, 300)], 4, 2, head, 16, dtype, cache_dtype, seed=14)
     poisoned = {0: [100, 127, 150, 199], 1: [132, 5], 2: [7, 100]}
     for s, places in poisoned.items():
         for j in places:
@@ -239,7 +259,7 @@ def test_what_is_not_seen_does_not_reach_a_row(bad, dtype, cache_dtype):
     for kw in (dict(), dict(window=33, sinks=4), dict(window=70, sinks=0)):
         out = batch.attend(**kw).double().cpu()
         expected, parts = batch.expected(**kw)
-        limit = bound_of(parts, 64, dtype)
+        limit = bound_of(parts, head, dtype)
         fine = torch.ones(batch.rows, dtype=torch.bool)
         for s, places in poisoned.items():
             for i in range(batch.new[s]):
