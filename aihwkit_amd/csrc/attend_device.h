@@ -45,8 +45,9 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr int TILE = FEW || KP == 3 || (DP == 256 && QP > 1) ? 32 : 64; // positions
   // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
   static constexpr bool DIRECT = !FEW && KP == 1;
-  // The scores of the next tile among the weights of this one, where a third wave to a SIMD has no registers anyway.
-  static constexpr bool AHEAD = DIRECT && (DP == 128 || (DP == 256 && QP == 1));
+  // The scores of the next tile among the weights of this one, where a third wave to a SIMD has no registers anyway (of longer heads, 4 % in time, the
+  // registers are all taken, and the compiler may spill).
+  static constexpr bool AHEAD = DIRECT && DP == 128;
   static constexpr int GROUP = 64 / CHUNKS;
   static_assert(GROUP <= RPU_CACHE_MIN_PAGE, "a group of rows is of one page");
   static constexpr int BLOCKS = TILE / 32, STEPS = 2 * D32;
@@ -184,8 +185,7 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
   return true;
 }
 
-template <typename T, typename TC, int D32, bool FEW>
-__global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a, long from_job) {
+template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__ void attend_job(AttendArgs a, long from_job) {
   using S = Shape<T, TC, D32, FEW>;
   using M = typename S::M;
   constexpr int TILE = S::TILE, BLOCKS = S::BLOCKS, STEPS = S::STEPS, KP = S::KP, QP = S::QP, CHUNKS = S::CHUNKS, DP = S::DP, LOADS = S::LOADS;
@@ -323,11 +323,13 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   // what this thread fetched: zeros where there is nothing; whether some value is not finite
   const auto clean = [&](uint16_t *values, uint64_t here) {
     bool bad = false;
+    int column = lane * 8, r = r_lane;
+    asm volatile("" : "+v"(column), "+v"(r)); // few tiles come here: no addresses and masks kept in registers for them
 #pragma unroll
     for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
       const int g = 4 * i + wave;
-      u32x4 *const v = reinterpret_cast<u32x4 *>(values + g * S::V_GROUP + lane * 8);
-      if (!((here >> (g * S::GROUP + r_lane)) & 1)) *v = u32x4{};
+      u32x4 *const v = reinterpret_cast<u32x4 *>(values + g * S::V_GROUP + column);
+      if (!((here >> (g * S::GROUP + r)) & 1)) *v = u32x4{};
       else {
         const u32x4 w = *v;
 #pragma unroll
@@ -786,17 +788,35 @@ __global__ __launch_bounds__((Shape<T, TC, D32, FEW>::WAVES * 64), (Shape<T, TC,
   }
 }
 
+template <typename T, typename TC, int D32, bool FEW>
+__global__ __launch_bounds__(256, (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_attend(AttendArgs a, long from) {
+  attend_job<T, TC, D32, FEW>(a, from);
+}
+// Sequences of many and of few lines in one launch, where both take as many waves to a SIMD: tiles, which take longest, first.  (bf16; 64 sequences of up
+// to 40 and 16040 tokens, 8 heads of 128: 434 us, in two launches 546; 16 of up to 100 and 600, 2 heads of 64: 17 and 23.)
+template <typename T, typename TC, int D32>
+__global__ __launch_bounds__(256, (Shape<T, TC, D32, false>::PER_SIMD)) void k_attend_mixed(AttendArgs a, long from) {
+  if (from + blockIdx.x < a.jobs) attend_job<T, TC, D32, false>(a, from);
+  else attend_job<T, TC, D32, true>(a, from - a.jobs);
+}
+
 template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t s) {
+  const auto go = [&](auto kernel, long jobs, int lds) {
+    for (long from = 0; from < jobs; from += MOST_GROUPS) hipLaunchKernelGGL(kernel, dim3((unsigned)std::min(MOST_GROUPS, jobs - from)), dim3(256), lds, s, a, from);
+  };
   const auto with = [&](auto d32) {
     constexpr int D32 = decltype(d32)::value;
-    const auto go = [&](auto few, long jobs) {
-      constexpr bool FEW = decltype(few)::value;
-      using Sh = Shape<T, TC, D32, FEW>;
-      for (long from = 0; from < jobs; from += MOST_GROUPS)
-        hipLaunchKernelGGL((k_attend<T, TC, D32, FEW>), dim3((unsigned)std::min(MOST_GROUPS, jobs - from)), dim3(Sh::WAVES * 64), Sh::LDS, s, a, from);
-    };
-    if constexpr (D32 <= 4 || sizeof(T) == 2) go(Int<1>{}, a.few_jobs); // (longer heads of floats have no few lines)
-    go(Int<0>{}, a.jobs);
+    using Many = Shape<T, TC, D32, false>;
+    static_assert(Many::WAVES == 4);
+    if constexpr (D32 <= 4 || sizeof(T) == 2) { // (longer heads of floats have no few lines)
+      using Few = Shape<T, TC, D32, true>;
+      static_assert(Few::WAVES == 4);
+      if constexpr (D32 <= 4 && Many::PER_SIMD == Few::PER_SIMD) { // (longer heads spill)
+        if (a.jobs && a.few_jobs) return go(k_attend_mixed<T, TC, D32>, a.jobs + a.few_jobs, std::max(Many::LDS, Few::LDS));
+      }
+      go(k_attend<T, TC, D32, true>, a.few_jobs, Few::LDS);
+    }
+    go(k_attend<T, TC, D32, false>, a.jobs, Many::LDS);
   };
   if (a.c.head <= 64) with(Int<2>{});
   else if (a.c.head <= 96) with(Int<3>{});

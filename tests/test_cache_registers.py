@@ -22,8 +22,9 @@ def test_no_attention_kernel_spills(tmp_path):
         notes = subprocess.run([READELF, "--notes", str(path)], capture_output=True, text=True, check=True).stdout
         for kernel in re.split(r"\n  - ", notes)[1:]:
             name = re.search(r"\.name: +(\S+)", kernel)
-            if name and "8k_attend" in name.group(1):
+            if name and re.search("8k_attend|14k_attend_mixed", name.group(1)):
                 found[name.group(1)] = (int(re.search(r"\.vgpr_spill_count: +(\d+)", kernel).group(1)),
                                         int(re.search(r"\.private_segment_fixed_size: +(\d+)", kernel).group(1)))
-    assert len(found) == 37, len(found)      # five pairs of types; four widths in tiles of lines, three (beside 16-bit rows four) with few lines
+    # five pairs of types; four widths in tiles of lines, three (beside 16-bit rows four) with few lines, three (floats: none) with both
+    assert len(found) == 49, len(found)
     assert set(found.values()) == {(0, 0)}, {name: v for name, v in found.items() if v != (0, 0)}
