@@ -46,42 +46,46 @@ __device__ __forceinline__ bool join_line(const float *sums, const float2 *stats
   return true;
 }
 
-// Few parts of many lines: a workgroup for a row, four columns to a lane, all of their loads under way together.
+// Few parts: a wave for 64 times four columns of a row, whose parts' loads are all under way together.  (By a workgroup to a line, 29000 lines in four
+// parts took 49 us, now 11.)
 constexpr int JOIN_PARTS = 8;
-template <typename T> __device__ __forceinline__ void join_row(const AttendArgs &a, int row) {
+template <typename T> __device__ __forceinline__ void join_row(const AttendArgs &a, int row, int i, bool with_few) {
   const Sequence s = sequence_of(a.r, row);
-  if (s.which < 0 || (long)(s.end - s.begin) * a.group <= a.few) return;
-  const int q_heads = a.c.heads * a.group, head = a.c.head, pieces = head / 4;
-  const long stride = (long)a.r.rows * q_heads;
-  for (int i = threadIdx.x; i < q_heads * pieces; i += 64 * JOIN_WAVES) {
-    const int h = i / pieces, d = i % pieces * 4;
-    const long unit = (long)row * q_heads + h;
-    float2 stats[JOIN_PARTS];
-    f32x4 part[JOIN_PARTS];
+  const int q_heads = a.c.heads * a.group, head = a.c.head, pieces = head / 4, h = i / pieces, d = i % pieces * 4;
+  const long lines = (long)(s.end - s.begin) * a.group;
+  const bool few = lines <= a.few;
+  const int parts = few ? with_few ? a.few_splits : 1 : a.splits;
+  if (s.which < 0 || parts < 2 || h >= q_heads) return;
+  const long stride = few ? (long)a.r.n * a.c.heads * a.few : (long)a.r.rows * q_heads;
+  const long unit = few ? ((long)s.which * a.c.heads + h / a.group) * a.few + (row - s.begin) * a.group + h % a.group : (long)row * q_heads + h;
+  const float *const sums = (few ? a.few_part : a.part) + unit * head + d;
+  const float2 *const of = (few ? a.few_stats : a.stats) + unit;
+  float2 stats[JOIN_PARTS];
+  f32x4 part[JOIN_PARTS];
 #pragma unroll
-    for (int p = 0; p < JOIN_PARTS; ++p) stats[p] = a.stats[min(p, a.splits - 1) * stride + unit];
+  for (int p = 0; p < JOIN_PARTS; ++p) stats[p] = of[min(p, parts - 1) * stride];
 #pragma unroll
-    for (int p = 0; p < JOIN_PARTS; ++p) part[p] = *reinterpret_cast<const f32x4 *>(a.part + (min(p, a.splits - 1) * stride + unit) * head + d);
-    float top = NONE, total = 0.0f;
+  for (int p = 0; p < JOIN_PARTS; ++p) part[p] = *reinterpret_cast<const f32x4 *>(sums + min(p, parts - 1) * stride * head);
+  float top = NONE, total = 0.0f;
 #pragma unroll
-    for (int p = 0; p < JOIN_PARTS; ++p) top = fmaxf(top, stats[p].x);
-    f32x4 v = {};
+  for (int p = 0; p < JOIN_PARTS; ++p) top = fmaxf(top, stats[p].x);
+  f32x4 v = {};
 #pragma unroll
-    for (int p = 0; p < JOIN_PARTS; ++p) {
-      const float f = p < a.splits && stats[p].x != NONE ? __builtin_amdgcn_exp2f(stats[p].x - top) : 0.0f;
-      if (p < a.splits && stats[p].x != NONE) total += stats[p].y * f;
-      if (f != 0.0f) v += part[p] * f;
-    }
-    const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
-    float r[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) r[k] = total == 0.0f ? 0.0f : v[k] * inverse;
-    store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * head + d, r, 4);
+  for (int p = 0; p < JOIN_PARTS; ++p) {
+    const bool seen = p < parts && stats[p].x != NONE;
+    const float f = seen ? __builtin_amdgcn_exp2f(stats[p].x - top) : 0.0f;
+    if (seen) total += stats[p].y * f;
+    if (f != 0.0f) v += part[p] * f; // 0: nothing seen, nothing left of it, or never written
   }
+  const float inverse = total == 0.0f ? 0.0f : 1.0f / total;
+  float r[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) r[k] = total == 0.0f ? 0.0f : v[k] * inverse;
+  store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * head + d, r, 4);
 }
 
-// Lines of sequences of few lines first, then rows, or the lines of rows.
-template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attend_join(AttendArgs a, long few_units) {
+// Lines of sequences of few lines first, then rows (`per_row` waves each) or, of many parts, their lines (0).
+template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attend_join(AttendArgs a, long few_units, int per_row) {
   const int q_heads = a.c.heads * a.group;
   long unit = blockIdx.x;
   const long units = gridDim.x - few_units;
@@ -98,7 +102,12 @@ template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_atten
     mine = join_line(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, v);
   } else {
     unit -= few_units;
-    if (a.splits <= JOIN_PARTS) return join_row<T>(a, (int)unit);
+    if (per_row) {
+      const long w = unit * JOIN_WAVES + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+      row = (int)(w / per_row);
+      if (row < a.r.rows) join_row<T>(a, row, (int)(w % per_row) * 64 + (threadIdx.x & 63), !few_units);
+      return;
+    }
     row = (int)(unit / q_heads);
     h = (int)(unit % q_heads);
     const Sequence s = sequence_of(a.r, row);
@@ -115,8 +124,14 @@ void launch_cache_attend(const AttendArgs &a, int dtype, int cache_dtype, hipStr
   with_adapter_types(dtype, cache_dtype, [&](auto x, auto c) {
     using T = decltype(x);
     attend::launch<T, decltype(c)>(a, s);
-    const long few = a.few_jobs && a.few_splits > 1 ? (long)a.r.n * a.c.heads * a.few : 0, rows = a.jobs && a.splits > 1 ? (long)a.r.rows * (a.splits > JOIN_PARTS ? a.c.heads * a.group : 1) : 0;
-    if (few + rows) hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(few + rows)), dim3(64 * JOIN_WAVES), 0, s, a, few);
+    const int few = a.few_jobs ? a.few_splits : 1, many = a.jobs ? a.splits : 1;
+    if (few < 2 && many < 2) return;
+    const int q_heads = a.c.heads * a.group, per_row = many > JOIN_PARTS ? 0 : (q_heads * (a.c.head / 4) + 63) / 64;
+    const long few_lines = (long)a.r.n * a.c.heads * a.few, units = per_row ? ((long)a.r.rows * per_row + JOIN_WAVES - 1) / JOIN_WAVES : (long)a.r.rows * q_heads;
+    // (rows that have nothing to join cost their workgroups all the same)
+    const bool by_line = few > JOIN_PARTS || !per_row || (many < 2 && few_lines < units);
+    const long few_units = few > 1 && by_line ? few_lines : 0;
+    hipLaunchKernelGGL(k_attend_join<T>, dim3((unsigned)(few_units + (many > 1 || !few_units ? units : 0))), dim3(64 * JOIN_WAVES), 0, s, a, few_units, per_row);
   });
 }
 
