@@ -73,7 +73,12 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
   const bool all_tiles = c.head_size > ATTEND_FEW_HEAD && dtype == RPU_F32;
   if (!all_tiles && (r.starts_dev || lines <= ATTEND_FEW)) {
     p.few = r.starts_dev ? ATTEND_FEW : (int)lines;
-    p.few_splits = splits_for((long)r.n * c.heads, seen(ATTEND_FEW / group + 1), 32 * ATTEND_FEW_LEAST, 512, 4096);
+    // Parts cost a join, 3 us, which so few positions do not take.  (us without and with parts.  36 units, heads of 64 bf16: 384 positions 7.7 and 8.8,
+    // 768 10.9 and 8.9; float rows: 256 7.2 and 9.0, 512 9.8 and 9.1; floats: 256 10.3 and 10.7, 512 16 and 11.  144 units: bf16 768 11.8 and 12.5, 1024 14.8
+    // and 13.7; floats 768 23 and 26, 1024 29 and 29.)
+    const long units = (long)r.n * c.heads, most = seen(ATTEND_FEW / group + 1);
+    const long alone = units >= 128 ? 768 : c.dtype == RPU_F32 ? 128 : dtype == RPU_F32 ? 256 : 384;
+    p.few_splits = most <= alone ? 1 : splits_for(units, most, 32 * ATTEND_FEW_LEAST, 512, 4096);
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
   if (all_tiles || r.starts_dev || lines > ATTEND_FEW) {
