@@ -15,13 +15,13 @@
 //                          one of 131072 positions (0.5 GB): 100; a window of 1024 (0.3 GB): 54; one of 1024 positions, 12 heads of 64: 9.1, two launches.
 //                          (One wave for a line, without matrix instructions: 7551, 119976, 1026, 263.)  Heads of 256, 16 sequences of 4096, 8 heads bf16
 //                          (0.3 GB): 78, in tiles of lines 113; one of 1024, 4 heads: 13, in tiles 35.
-//   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 560 us (980 TFLOP/s; a large matrix product 1320), the matrix pipes are
+//   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 560 to 585 us (940 to 980 TFLOP/s; a large matrix product 1320), the matrix pipes are
 //                          busy for 45 %, vector instructions take 50 %, LDS 45 %.  Without the loads of keys and values it takes 476, without
 //                          exponentials 541, without barriers 551.  16384 tokens under a window of 2048, 16 heads of 64 halves: 203 (635 TFLOP/s).
 //   float rows             the products of parts: 3 (bf16 cache), 2 (halves), 6 (floats).  8 x 1024 tokens, 12 heads of 64, bf16 cache: 54 (237 TFLOP/s, a matrix
 //                          product of floats 152).  Floats throughout: 23 sequences, 15 heads of 80 under a window of 777: 107, of which few lines 13, the join 10.
 // Not kept: 64 lines to a wave (half the reads of LDS; heads of 64 211 us for 203, heads of 128 spill), eight waves to a workgroup (618 for 563), the next
-// tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219).
+// tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219), waves' priorities and other orders of the instructions (1 %).
 #pragma once
 #include "cache.h"
 
