@@ -23,6 +23,7 @@
 // Not kept: 64 lines to a wave (half the reads of LDS; heads of 64 211 us for 203, heads of 128 spill), eight waves to a workgroup (618 for 563), the next
 // tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219), waves' priorities and other orders of the instructions (1 %).
 #pragma once
+#include "attend_tiles.h"
 #include "cache.h"
 
 #include <algorithm>
@@ -151,8 +152,7 @@ __device__ __forceinline__ bool job_few(const AttendArgs &a, long at, Job &job) 
   return job.lines > 0 && job.lines <= a.few;
 }
 // Tiles of LINES lines, the last of the sequences first: they see most.  Where heads (of all sequences, if these have as many rows each) divide
-// by the eight L2 caches, each cache has some of them; otherwise all go in turn.  Sequences of unlike rows have the tiles from
-// (starts[s] * group) / LINES + s on, one more than they can need at most.
+// by the eight L2 caches, each cache has some of them; otherwise all go in turn.  Sequences of unlike rows: attend_tiles.h.
 template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &a, long at, Job &job) {
   if (at >= a.jobs) return false;
   const int each = a.r.starts ? a.tiles : a.tiles / a.r.n, sets = a.r.starts ? a.c.heads : a.c.heads * a.r.n; // tiles of a set
@@ -174,9 +174,10 @@ template <int LINES> __device__ __forceinline__ bool job_many(const AttendArgs &
   job.head = set % a.c.heads;
   int which = set / a.c.heads;
   if (a.r.starts) {
-    const auto base = [&](int start, int s) { return (long)min(max(start, 0), a.r.rows) * a.group / LINES + s; };
-    which = max(last_of(a.r.starts, a.r.n, [&](int start, int s) { return base(start, s) <= tile; }), 0);
-    tile = (int)max(tile - base(a.r.starts[which], which), 0l);
+    const TileOf t = tile_of(tile, a.r.starts, a.r.rows, a.group, LINES, [&](auto &&held) { return last_of(a.r.starts, a.r.n, held); });
+    if (t.which < 0) return false;
+    which = t.which;
+    tile = (int)t.tile;
   }
   job.s = sequence_at(a.r, which);
   job.lines = lines_of(job.s, a.group);

@@ -1,4 +1,5 @@
 // C entry points of attention over a paged cache: what they check on the host before anything is launched.
+#include "attend_tiles.h"
 #include "cache.h"
 #include "operand_checks.h"
 
@@ -82,7 +83,7 @@ AttendPlan attend_plan(const rpu_cache &c, const rpu_cache_rows &r, int q_heads,
     p.few_jobs = (long)r.n * c.heads * p.few_splits;
   }
   if (all_tiles || r.starts_dev || lines > ATTEND_FEW) {
-    const long tiles = r.starts_dev ? r.rows * group / ATTEND_LINES + r.n : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
+    const long tiles = r.starts_dev ? attend::numbers_of(r.rows, (int)group, ATTEND_LINES, r.n) : (lines + ATTEND_LINES - 1) / ATTEND_LINES * r.n;
     if (tiles > INT_MAX) throw RpuError("So many rows and heads are too many for a call.");
     p.tiles = (int)tiles;
     // (tiles that there are if the rows are of one sequence, at most about as many workgroups without work as with it)
