@@ -274,7 +274,10 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) parts_of_query(p[i], i, [&](int j, u32x4 v) { q[j][i] = v; });
   }
-  const float c = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift); // of the exponents, in powers of two
+  float c = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift); // of the exponents, in powers of two
+  // A lift may take it out of the numbers that floats hold whole.  Lifted scores are less than 2^40 and multiples of 2^-48: with any factor below
+  // 2^-126 all weights are 1, with any beyond floats only the largest score has one.
+  if constexpr (QP == 2) c = __builtin_amdgcn_fmed3f(c, 0x1p-126f, 0x1.fffffep127f);
 
   // Tiles: page numbers are under way two tiles ahead, keys and values one.
   const int *table = a.r.tables + job.s.which * a.r.table_ld;
