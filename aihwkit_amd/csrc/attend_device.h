@@ -34,7 +34,7 @@ namespace attend {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-constexpr float NONE = -__builtin_inff(), LOG2E = 1.44269504088896340736f;
+constexpr float NONE = -__builtin_inff();
 
 // How rows of T beside a cache of TC, heads of up to 32 D32 values, are worked on.
 template <typename T, typename TC, int D32, bool FEW> struct Shape {
@@ -274,7 +274,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
 #pragma unroll
     for (int i = 0; i < STEPS; ++i) parts_of_query(p[i], i, [&](int j, u32x4 v) { q[j][i] = v; });
   }
-  float c = none ? LOG2E : fabsf(a.scale * LOG2E) * inverse_of(lift); // of the exponents, in powers of two
+  float c = none ? LOG2E : exponent_factor(a.scale) * inverse_of(lift); // of the exponents, in powers of two
   // A lift may take it out of the numbers that floats hold whole.  Lifted scores are less than 2^40 and multiples of 2^-48: with any factor below
   // 2^-126 all weights are 1, with any beyond floats only the largest score has one.
   if constexpr (QP == 2) c = __builtin_amdgcn_fmed3f(c, 0x1p-126f, 0x1.fffffep127f);
@@ -444,11 +444,12 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     }
   };
   // The score that weights are relative to, as a power of two too, and their sum (of this lane's positions).  It follows the maximum where that is
-  // more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.
+  // more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.  Beyond ATTEND_FAR the power is too
+  // coarse to be subtracted from others; it is NaN then (and before anything is seen) and every tile's scores have the score itself subtracted.
   constexpr float SLACK = 8.0f;
-  float m = NONE, power = NONE, total = 0.0f;
+  float m = NONE, power = __builtin_nanf(""), total = 0.0f;
   floatx16 sums[D32] = {};
-  const auto raise = [&](const Scores &score) {
+  const auto raise = [&](Scores &score) {
     float now = score[0][0], other;
 #pragma unroll
     for (int n = 0; n < BLOCKS; ++n)
@@ -456,17 +457,25 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
       for (int i = 0; i < 16; ++i) now = most(now, score[n][i]);
     now = half_and_half(now, other);
     now = most(now, other);
-    const bool far = !(now * c <= power + SLACK) && now != NONE; // (NaN is)
-    if (__any(far)) {
-      now = far ? most(now, m) : m;
-      const float next = now == NONE ? NONE : now * c, shrink = far ? __builtin_amdgcn_exp2f(power - next) : 1.0f;
+    const bool up = !(now * c <= power + SLACK);
+    if (__any(up)) {
+      now = up ? most(now, m) : m;
+      const float shrink = up ? __builtin_amdgcn_exp2f(m == NONE ? NONE : weight_between(m, now, c)) : 1.0f;
       total *= shrink;
 #pragma unroll
       for (int n = 0; n < D32; ++n) sums[n] *= shrink;
       m = now;
-      power = next;
+      const bool far = !(fabsf(m * c) <= ATTEND_FAR);
+      power = far ? __builtin_nanf("") : m * c;
+      if (__any(far)) {
+        const float most_seen = far && m != NONE ? m : 0.0f;
+#pragma unroll
+        for (int n = 0; n < BLOCKS; ++n)
+#pragma unroll
+          for (int i = 0; i < 16; ++i) score[n][i] -= most_seen;
+      }
     }
-    return power == NONE ? 0.0f : power;
+    return power != power ? 0.0f : power;
   };
   // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
   const auto repair = [&](uint16_t *values, const Seen &seen) {
@@ -722,7 +731,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     const long unit = (long)row * (a.c.heads * group) + q_head;
     if (a.splits > 1) {
       const long part = (long)job.split * a.r.rows * (a.c.heads * group) + unit;
-      if (!half) a.stats[part] = float2{power, total};
+      if (!half) a.stats[part] = float2{m * inverse_of(lift), total};
 #pragma unroll
       for (int n = 0; n < D32; ++n)
 #pragma unroll
@@ -748,16 +757,16 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     // the waves' parts meet in LDS, each where its tile was
     __shared__ float2 stats[S::KEY_WAVES][32];
     __shared__ float2 joined[32];
-    if (!half) stats[wave][lane & 31] = float2{power, total};
+    if (!half) stats[wave][lane & 31] = float2{m, total};
     __syncthreads();
     float top = NONE, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < S::KEY_WAVES; ++w) top = most(top, stats[w][lane & 31].x);
-    const auto shrink_of = [&](float p) { return p == NONE ? 0.0f : __builtin_amdgcn_exp2f(p - top); };
+    const auto shrink_of = [&](float of) { return of == NONE ? 0.0f : __builtin_amdgcn_exp2f(weight_between(of, top, c)); };
 #pragma unroll
     for (int w = 0; w < S::KEY_WAVES; ++w) sum = fmaf(stats[w][lane & 31].y, shrink_of(stats[w][lane & 31].x), sum);
-    if (wave == 0 && !half) joined[lane & 31] = float2{top, sum};
-    const float shrink = shrink_of(power);
+    if (wave == 0 && !half) joined[lane & 31] = float2{top * inverse_of(lift), sum};
+    const float shrink = shrink_of(m);
     float *const mine = reinterpret_cast<float *>(attend_lds + wave * S::TILE_VALUES) + (lane & 31) * DP;
     if (live)
 #pragma unroll

@@ -46,7 +46,7 @@ struct AttendArgs {
   int few, few_splits, splits, tiles;
   long few_jobs, jobs;
   float *few_part, *part;      // sums of a part of the positions: [few_splits][n][heads][few][head], [splits][rows][q heads][head]
-  float2 *few_stats, *stats;   // maximum (as a power of two) and sum of the weights
+  float2 *few_stats, *stats;   // the score that weights are relative to (before the scale), and their sum
 };
 namespace attend {
 template <typename T, typename TC> void launch(const AttendArgs &a, hipStream_t s);
@@ -102,6 +102,17 @@ __device__ __forceinline__ int page_of(const CacheDev &c, const CacheRowsDev &r,
   if (position < 0 || position >= r.places) return -1;
   const int page = table[position >> c.page_shift];
   return page >= 0 && page < c.pages ? page : -1;
+}
+// Weights are 2^(c score - c reference), c of the scale's magnitude.
+constexpr float LOG2E = 1.44269504088896340736f;
+__device__ __forceinline__ float exponent_factor(float scale) { return fabsf(scale * LOG2E); }
+// The exponent of a weight relative to one score, relative to another.  Up to ATTEND_FAR, weights were made with c reference rounded (to 2^-8 at most), so
+// that this is the difference of the rounded ones.  Beyond, where a float has c reference to 2^-7 at best (from 2^31 on to 128, and with scales up to 1e30
+// not at all), they were made of the difference of the scores.
+constexpr float ATTEND_FAR = 0x1p16f;
+__device__ __forceinline__ float weight_between(float of, float to, float c) {
+  const float p = of * c, q = to * c;
+  return fabsf(p) <= ATTEND_FAR && fabsf(q) <= ATTEND_FAR ? p - q : (of - to) * c;
 }
 // value 0 of a head at a position
 __device__ __forceinline__ long place_of(const CacheDev &c, int page, int head, long position) {
