@@ -89,13 +89,14 @@ template <typename M> __device__ __forceinline__ floatx16 multiply(u32x4 a, u32x
   else return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 
-// two floats as PARTS of type M each (rounded, what is left goes on); the largest floats stay finite, an infinity is in the second part
-template <typename M, int PARTS> __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[PARTS]) {
+// two floats as PARTS of type M each (rounded, what is left goes on); the largest floats stay finite, an infinity is in the second part (not SMALL: there are
+// none)
+template <typename M, bool SMALL = false, int PARTS> __device__ __forceinline__ void split2(float a, float b, uint32_t (&part)[PARTS]) {
 #pragma unroll
   for (int k = 0; k < PARTS; ++k) {
     if constexpr (__is_same(M, __bf16)) {
       constexpr float MOST = 0x1.fep127f;
-      part[k] = PARTS == 1 || k ? pack2(a, b, __bf16{}) : pack2(__builtin_amdgcn_fmed3f(a, -MOST, MOST), __builtin_amdgcn_fmed3f(b, -MOST, MOST), __bf16{});
+      part[k] = PARTS == 1 || k || SMALL ? pack2(a, b, __bf16{}) : pack2(__builtin_amdgcn_fmed3f(a, -MOST, MOST), __builtin_amdgcn_fmed3f(b, -MOST, MOST), __bf16{});
       if (k + 1 < PARTS) {
         a -= __uint_as_float(part[k] << 16);
         b -= __uint_as_float(part[k] & 0xffff0000u);
@@ -443,11 +444,12 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
       for (int i = 0; i < 16; ++i) score[n][i] = mine & (1u << (8 * (i / 4) + i % 4)) ? score[n][i] : NONE;
     }
   };
-  // The score that weights are relative to, as a power of two too, and their sum (of this lane's positions).  It follows the maximum where that is
-  // more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.  Beyond ATTEND_FAR the power is too
-  // coarse to be subtracted from others; it is NaN then (and before anything is seen) and every tile's scores have the score itself subtracted.
-  constexpr float SLACK = 8.0f;
-  float m = NONE, power = __builtin_nanf(""), total = 0.0f;
+  // The score that weights are relative to, what their exponents have subtracted (it as a power of two, raised), and their sum (of this lane's positions).
+  // It follows the maximum where that is more than 2^SLACK away: a maximum that grows by little with every tile, as of many like scores, rescales nothing.
+  // Beyond ATTEND_FAR a power of two is too coarse to be subtracted from others; the reference is NaN then (and before anything is seen) and every tile's
+  // scores have the score itself subtracted.
+  using R = References<T>;
+  float m = NONE, reference = __builtin_nanf(""), total = 0.0f;
   floatx16 sums[D32] = {};
   const auto raise = [&](Scores &score) {
     float now = score[0][0], other;
@@ -457,16 +459,16 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
       for (int i = 0; i < 16; ++i) now = most(now, score[n][i]);
     now = half_and_half(now, other);
     now = most(now, other);
-    const bool up = !(now * c <= power + SLACK);
+    const bool up = !(now * c <= (R::SLACK == R::RAISED ? reference : reference + (R::SLACK - R::RAISED)));
     if (__any(up)) {
       now = up ? most(now, m) : m;
-      const float shrink = up ? __builtin_amdgcn_exp2f(m == NONE ? NONE : weight_between(m, now, c)) : 1.0f;
+      const float shrink = up ? __builtin_amdgcn_exp2f(m == NONE ? NONE : weight_between<R>(m, now, c)) : 1.0f;
       total *= shrink;
 #pragma unroll
       for (int n = 0; n < D32; ++n) sums[n] *= shrink;
       m = now;
       const bool far = !(fabsf(m * c) <= ATTEND_FAR);
-      power = far ? __builtin_nanf("") : m * c;
+      reference = far ? __builtin_nanf("") : m * c + R::RAISED;
       if (__any(far)) {
         const float most_seen = far && m != NONE ? m : 0.0f;
 #pragma unroll
@@ -475,7 +477,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
           for (int i = 0; i < 16; ++i) score[n][i] -= most_seen;
       }
     }
-    return power != power ? 0.0f : power;
+    return reference != reference ? R::RAISED : reference;
   };
   // rare: what is not finite goes to the lines that see it by itself, and is zero for the product
   const auto repair = [&](uint16_t *values, const Seen &seen) {
@@ -501,10 +503,9 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     all_there();
   };
   // Weights of 16 positions each (4 half + 8 (e / 4) + e % 4), and their products with four positions of 16 columns to 16 lanes.
-  // Halves are up to 2^15, so that small ones keep their bits: of half rows by the exponent, of floats, whose `total` is of the weights, by a product.
-  constexpr float LIFT = 0x1p7f;
+  // Of floats they come from exponents near 0, which have more bits, and are lifted by a product; their `total` is of the weights before it.
+  constexpr float LIFT = S::HALF ? 0x1p7f : 0x1p-8f;
   const auto add = [&](uint16_t *values, const Scores &score, float less) {
-    const float exponent = S::HALF && QP == 1 ? less - (15.0f - SLACK) : less;
     constexpr int COLUMNS = S::DIRECT ? (DP == 64 ? 2 : 4) : 1;
     uint16_t *columns[COLUMNS];
 #pragma unroll
@@ -515,14 +516,14 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const int at = 8 * (b & 1) + i;
-        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -exponent)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -exponent));
+        float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -less));
         if constexpr (QP > 1) total += w0 + w1;
-        if constexpr (S::HALF && QP > 1) {
+        if constexpr (QP > 1) {
           w0 *= LIFT;
           w1 *= LIFT;
         }
         uint32_t part[QP];
-        split2<M>(w0, w1, part);
+        split2<M, true>(w0, w1, part);
         if constexpr (QP == 1) total = add2<M>(part[0], total); // of the rounded ones: those that the values are multiplied with
 #pragma unroll
         for (int l = 0; l < QP; ++l) weights[l][i / 2] = part[l];
@@ -725,7 +726,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     const float mine = half_and_half(total, other);
     total = mine + other;
   }
-  if constexpr (S::HALF && QP > 1) total *= LIFT;
+  if constexpr (QP > 1) total *= LIFT;
   if constexpr (!FEW) {
     if (!live) return;
     const long unit = (long)row * (a.c.heads * group) + q_head;
@@ -762,7 +763,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     float top = NONE, sum = 0.0f;
 #pragma unroll
     for (int w = 0; w < S::KEY_WAVES; ++w) top = most(top, stats[w][lane & 31].x);
-    const auto shrink_of = [&](float of) { return of == NONE ? 0.0f : __builtin_amdgcn_exp2f(weight_between(of, top, c)); };
+    const auto shrink_of = [&](float of) { return of == NONE ? 0.0f : __builtin_amdgcn_exp2f(weight_between<R>(of, top, c)); };
 #pragma unroll
     for (int w = 0; w < S::KEY_WAVES; ++w) sum = fmaf(stats[w][lane & 31].y, shrink_of(stats[w][lane & 31].x), sum);
     if (wave == 0 && !half) joined[lane & 31] = float2{top * inverse_of(lift), sum};

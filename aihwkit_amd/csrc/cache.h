@@ -106,13 +106,18 @@ __device__ __forceinline__ int page_of(const CacheDev &c, const CacheRowsDev &r,
 // Weights are 2^(c score - c reference), c of the scale's magnitude.
 constexpr float LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float exponent_factor(float scale) { return fabsf(scale * LOG2E); }
-// The exponent of a weight relative to one score, relative to another.  Up to ATTEND_FAR, weights were made with c reference rounded (to 2^-8 at most), so
-// that this is the difference of the rounded ones.  Beyond, where a float has c reference to 2^-7 at best (from 2^31 on to 128, and with scales up to 1e30
-// not at all), they were made of the difference of the scores.
+// Exponents have c reference + RAISED subtracted, rounded.  Scores may be up to SLACK powers of two above the reference: weights are at most 1 when they meet
+// the values, so that the largest of these stay finite, of halves 2^15, so that small weights keep their bits.  (Floats are lifted afterwards.)
+template <typename T> struct References { // of rows of T
+  static constexpr float SLACK = 8.0f, RAISED = sizeof(T) == 4 ? 0.0f : __is_same(T, _Float16) ? SLACK - 15.0f : SLACK;
+};
+// The exponent of a weight relative to one score, relative to another.  Up to ATTEND_FAR, weights were made with the rounded reference (by up to 2^-8), so that
+// this is the difference of those.  Beyond, where a float has c reference to 2^-7 at best (from 2^31 on to 128, and with scales up to 1e30 not at all),
+// they were made of the difference of the scores.
 constexpr float ATTEND_FAR = 0x1p16f;
-__device__ __forceinline__ float weight_between(float of, float to, float c) {
+template <typename R> __device__ __forceinline__ float weight_between(float of, float to, float c) {
   const float p = of * c, q = to * c;
-  return fabsf(p) <= ATTEND_FAR && fabsf(q) <= ATTEND_FAR ? p - q : (of - to) * c;
+  return fabsf(p) <= ATTEND_FAR && fabsf(q) <= ATTEND_FAR ? (p + R::RAISED) - (q + R::RAISED) : (of - to) * c;
 }
 // value 0 of a head at a position
 __device__ __forceinline__ long place_of(const CacheDev &c, int page, int head, long position) {

@@ -9,14 +9,14 @@ constexpr float NONE = -__builtin_inff();
 // out = sum over the parts 2^(c m_p - c m) sums_p / sum over the parts 2^(c m_p - c m) total_p.  A workgroup for a line: the parts' factors to the lanes
 // of every wave, their sums to the waves, four columns to a lane (and two parts to a wave, of heads of up to 128 columns).
 constexpr int JOIN_WAVES = 4;
-__device__ __forceinline__ bool join_line(const float *sums, const float2 *stats, long unit, long stride, int parts, int head, float c, f32x4 &v) {
+template <typename T> __device__ __forceinline__ bool join_line(const float *sums, const float2 *stats, long unit, long stride, int parts, int head, float c, f32x4 &v) {
   __shared__ f32x4 room[JOIN_WAVES][64];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const float2 mine = lane < parts ? stats[lane * stride + unit] : float2{NONE, 0.0f};
   float top = mine.x;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) top = fmaxf(top, __shfl_xor(top, m));
-  const float factor = mine.x == NONE ? 0.0f : __builtin_amdgcn_exp2f(weight_between(mine.x, top, c));
+  const float factor = mine.x == NONE ? 0.0f : __builtin_amdgcn_exp2f(weight_between<References<T>>(mine.x, top, c));
   float total = mine.x == NONE ? 0.0f : mine.y * factor;
 #pragma unroll
   for (int m = 32; m > 0; m >>= 1) total += __shfl_xor(total, m);
@@ -74,7 +74,7 @@ template <typename T> __device__ __forceinline__ void join_row(const AttendArgs 
 #pragma unroll
   for (int p = 0; p < JOIN_PARTS; ++p) {
     const bool seen = p < parts && stats[p].x != NONE;
-    const float f = seen ? __builtin_amdgcn_exp2f(weight_between(stats[p].x, top, c)) : 0.0f;
+    const float f = seen ? __builtin_amdgcn_exp2f(weight_between<References<T>>(stats[p].x, top, c)) : 0.0f;
     if (seen) total += stats[p].y * f;
     if (f != 0.0f) v += part[p] * f; // 0: nothing seen, nothing left of it, or never written
   }
@@ -100,7 +100,7 @@ template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_atten
     if (lines > a.few || l >= lines) return;
     row = s.begin + l / a.group;
     h = head * a.group + l % a.group;
-    mine = join_line(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, exponent_factor(a.scale), v);
+    mine = join_line<T>(a.few_part, a.few_stats, unit, few_units, a.few_splits, a.c.head, exponent_factor(a.scale), v);
   } else {
     unit -= few_units;
     if (per_row) {
@@ -113,7 +113,7 @@ template <typename T> __global__ __launch_bounds__(64 * JOIN_WAVES) void k_atten
     h = (int)(unit % q_heads);
     const Sequence s = sequence_of(a.r, row);
     if (s.which < 0 || (long)(s.end - s.begin) * a.group <= a.few) return;
-    mine = join_line(a.part, a.stats, unit, units, a.splits, a.c.head, exponent_factor(a.scale), v);
+    mine = join_line<T>(a.part, a.stats, unit, units, a.splits, a.c.head, exponent_factor(a.scale), v);
   }
   const float r[4] = {v[0], v[1], v[2], v[3]};
   if (mine) store_first(static_cast<T *>(a.out.p) + row * a.out.ld + h * a.c.head + threadIdx.x * 4, r, 4);

@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from cache_oracle import bound_of
-from test_gpu_cache import LAYOUTS, PAIR_IDS, PAIRS, Batch
+from test_gpu_cache import BF16, F32, LAYOUTS, PAIR_IDS, PAIRS, Batch
 from test_gpu_digital import close
 
 pytestmark = pytest.mark.gpu
@@ -82,3 +82,22 @@ def test_large_scales(scale, name, dtype, cache_dtype):
 def test_scores_far_from_zero(scale, offset, name, dtype, cache_dtype):
     """2^18 and more beside differences of a few: 2^-64 and less of a weight does not count."""
     check_exact(whole_scores(name, dtype, cache_dtype, offset), 64.0, scale=scale)
+
+
+@pytest.mark.parametrize("dtype, cache_dtype", [(F32, F32), (F32, BF16), (BF16, BF16)], ids=["f32-f32", "f32-bf16", "bf16-bf16"])
+@pytest.mark.parametrize("heads, kv, head", [(4, 2, 64), (2, 1, 128), (2, 1, 200)])
+@pytest.mark.parametrize("rise", [0.5, 1.375, 5.375])
+def test_largest_values_under_rising_scores(rise, heads, kv, head, dtype, cache_dtype):
+    """Two values of 1.5e38 in a head's column, whose scores are above the first that a row meets."""
+    batch = Batch([(70, 200), (1, 300), (2, 5000), (40, 2000)], heads, kv, head, 16, dtype, cache_dtype, seed=65)
+    batch.keys = torch.where(batch.keys.isnan(), batch.keys, torch.zeros((), dtype=cache_dtype))
+    batch.q.zero_()
+    batch.q[..., 0] = 1.0
+    for s, length in enumerate(batch.lengths):
+        for j in (100, batch.lengths[s] - batch.new[s] - 20):
+            at = int(batch.tables_host[s, j // 16])
+            batch.keys[at, :, j % 16, 0] = rise
+            batch.values[at, :, j % 16, 5] = 1.5e38
+    batch.gpu()
+    assert torch.isfinite(batch.attend(scale=1.0)[batch.starts_host[0]:batch.starts_host[-1]]).all()
+    check_exact(batch, 64.0, scale=1.0)
