@@ -320,7 +320,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
 #pragma unroll
       for (int i = 0; i < TILE / S::GROUP / 4; ++i) {
         const int to_group = __builtin_amdgcn_readfirstlane(to + (4 * i + wave) * group_bytes);
-        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p[i]), "s"(to_group) : "memory");
+        asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(p[i]), "s"(to_group) : "memory", "m0");
       }
   };
   const auto fetch_keys = [&](uint64_t at, int stage) { fetch(a.c.k, at, k_lane, S::K_GROUP * 2, lds_at + stage * S::K_PLANE * 2); };
