@@ -2,8 +2,9 @@
 import pytest
 import torch
 
+from aihwkit_amd import digital
 from cache_oracle import bound_of
-from test_gpu_cache import BF16, F32, LAYOUTS, PAIR_IDS, PAIRS, Batch
+from test_gpu_cache import BF16, F32, LAYOUTS, PAIR_IDS, PAIRS, Batch, numbers
 from test_gpu_digital import close
 
 pytestmark = pytest.mark.gpu
@@ -101,3 +102,50 @@ def test_largest_values_under_rising_scores(rise, heads, kv, head, dtype, cache_
     batch.gpu()
     assert torch.isfinite(batch.attend(scale=1.0)[batch.starts_host[0]:batch.starts_host[-1]]).all()
     check_exact(batch, 64.0, scale=1.0)
+
+
+def named_places(batch, starts, lengths):
+    """What rows of those starts and lengths, clamped to the rows and tables that there are, may be written to."""
+    named = torch.zeros(batch.keys.shape[0], batch.keys.shape[2], dtype=torch.bool)
+    page_size = batch.keys.size(2)
+    for s in range(len(lengths)):
+        begin = min(max(starts[s], 0), batch.rows)
+        m = min(max(starts[s + 1], begin), batch.rows) - begin
+        for p in range(max(lengths[s] - m, 0), min(lengths[s], batch.tables_host.size(1) * page_size)):
+            page = int(batch.tables_host[s, p // page_size])
+            if 0 <= page < batch.keys.size(0):
+                named[page, p % page_size] = True
+    return named
+
+
+@pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
+@pytest.mark.parametrize("neighbours", [False, True], ids=["halves", "neighbours"])
+def test_starts_lengths_and_tables_out_of_range_write_nowhere_else(neighbours, dtype, cache_dtype):
+    """Cache, queries and output lie in larger memory: what is beside them, and every place of the cache that no row's sequence names, keeps its bits."""
+    batch = Batch([(4, 30), (4, 0), (40, 9)], 4, 2, 64, 16, dtype, cache_dtype, seed=66)
+    batch.tables_host[0, 1], batch.tables_host[2, 2] = 2 ** 31 - 1, batch.keys.size(0)
+    count, bits = batch.keys.numel(), torch.int32 if cache_dtype == F32 else torch.int16
+    room = torch.randint(-2 ** 15, 2 ** 15, (3 * 4096 + 2 * count,), generator=torch.Generator().manual_seed(67)).to(bits).cuda()
+    keys, values = (room[4096 + k * (4096 + count):][:count].view(cache_dtype).view(batch.keys.shape) for k in range(2))
+    cache = digital.PagedCache(keys, values, digital.rotation_frequencies(64)[:19], neighbours)
+    whole = torch.full((batch.rows + 20, 4, 64), 7.0, dtype=dtype, device="cuda")
+    out = whole[10:10 + batch.rows]
+    rows = torch.ones(batch.rows, 2, 64, dtype=dtype, device="cuda")
+    tables = batch.tables_host.cuda()
+    for starts in ([-5, 4, 8, 1000], [40, 30, 20, 10], [2 ** 31 - 1, -(2 ** 31), 0, 5], [48, 48, 48, 48], [0, 4, 8, 48]):
+        for lengths in ([2 ** 31 - 1] * 3, [-(2 ** 31)] * 3, [34, 4, 49]):
+            given = dict(starts=numbers(starts), out=out)
+            before = room.clone()
+            cache.attend(batch.q, tables, numbers(lengths), **given)
+            assert torch.equal(room, before)
+            cache.append(rows, rows, tables, numbers(lengths), queries=batch.q, **given)
+            named = named_places(batch, starts, lengths)
+            if starts == [0, 4, 8, 48] and lengths == [34, 4, 49]:
+                assert int(named.sum()) > 20 and (values.cpu().permute(0, 2, 1, 3)[named] == 1).all()
+            for k, now in enumerate((keys, values)):
+                then = before[4096 + k * (4096 + count):][:count].view(batch.keys.shape)
+                now = now.view(bits)
+                assert torch.equal(now.cpu().permute(0, 2, 1, 3)[~named], then.cpu().permute(0, 2, 1, 3)[~named])
+                now.copy_(then)
+            assert torch.equal(room, before)          # beside the cache
+            assert (whole[:10] == 7).all() and (whole[10 + batch.rows:] == 7).all()
