@@ -6,9 +6,12 @@
 // columns are the lines -- maximum, sum and rescaling stay in the lane, and the weights are the second product's operand as the first leaves
 // them: its terms may come in any order, so that values are read (transposed, from LDS) in the order that the lanes have.
 //
-// Matrix operands are 16-bit.  Of 16-bit rows and caches they are the numbers themselves, weights are rounded to that type (half a step of it,
-// relative to each weight, in a mean of values).  Floats go in parts: beside bf16 and floats three bf16 each, beside halves two halves, lifted
-// by a power of two; products of parts that add up to less than 2^-24 of the largest are left out.
+// Matrix operands are 16-bit.  Of 16-bit rows and caches they are the numbers themselves; weights of few lines, which memory bounds, are two of them (16 bits of
+// bf16, 22 of halves: the result is as near as its own rounding lets it be), of tiles of lines they are rounded to that type: half a step of it, relative to each
+// weight, in a mean of values, an error 1.27 times that of the result's rounding alone (8192 tokens, 32 heads of 128 bf16: 2.10e-3 for 1.65e-3 of the norm).
+// In two parts there, products take half as many again: 810 us for 576, 16384 tokens under a window of 2048, 16 heads of 64 halves 266 for 212.
+// Floats go in parts: beside bf16 and floats three bf16 each, beside halves two halves, lifted by a power of two; products of parts that add up to
+// less than 2^-24 of the largest are left out.
 //
 // What bounds it, and what it reaches (us; MI355X):
 //   one token a sequence   memory: keys and values are read once.  64 sequences of up to 8192 positions, 8 heads of 128 bf16 (1.3 GB): 241, 5.5 TB/s;
@@ -41,7 +44,8 @@ template <typename T, typename TC, int D32, bool FEW> struct Shape {
   static constexpr bool HALF = __is_same(TC, _Float16);
   using M = std::conditional_t<__is_same(TC, float), __bf16, TC>; // of matrix operands
   static constexpr int KP = sizeof(TC) == 4 ? 3 : 1;                         // parts of keys and values
-  static constexpr int QP = sizeof(T) == 2 ? 1 : HALF ? 2 : 3;               // of queries and weights
+  static constexpr int QP = sizeof(T) == 2 ? 1 : HALF ? 2 : 3;               // of queries
+  static constexpr int WP = sizeof(T) == 2 && FEW ? 2 : QP;                  // of weights
   static constexpr int DP = D32 <= 2 ? 64 : D32 <= 4 ? 128 : 256, CHUNKS = DP / 8; // a head in LDS, and its pieces of 16 bytes
   static constexpr int TILE = FEW || KP == 3 || (DP == 256 && QP > 1) ? 32 : 64; // positions
   // Keys and values as they are go to LDS without a register in between (DIRECT), 1 KB to a wave's load: GROUP rows.
@@ -512,21 +516,21 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
     for (int n = 0; n < COLUMNS; ++n) columns[n] = values + S::v_at(4 * half + ((lane & 15) >> 2), 4 * n + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) + (lane & 1) * 4;
 #pragma unroll
     for (int b = 0; b < 2 * BLOCKS; ++b) {
-      u32x4 weights[QP];
+      u32x4 weights[S::WP];
 #pragma unroll
       for (int i = 0; i < 8; i += 2) {
         const int at = 8 * (b & 1) + i;
         float w0 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at], c, -less)), w1 = __builtin_amdgcn_exp2f(fmaf(score[b / 2][at + 1], c, -less));
-        if constexpr (QP > 1) total += w0 + w1;
+        if constexpr (S::WP > 1) total += w0 + w1;
         if constexpr (QP > 1) {
           w0 *= LIFT;
           w1 *= LIFT;
         }
-        uint32_t part[QP];
+        uint32_t part[S::WP];
         split2<M, true>(w0, w1, part);
-        if constexpr (QP == 1) total = add2<M>(part[0], total); // of the rounded ones: those that the values are multiplied with
+        if constexpr (S::WP == 1) total = add2<M>(part[0], total); // of the rounded ones: those that the values are multiplied with
 #pragma unroll
-        for (int l = 0; l < QP; ++l) weights[l][i / 2] = part[l];
+        for (int l = 0; l < S::WP; ++l) weights[l][i / 2] = part[l];
       }
 #pragma unroll
       for (int n = 0; n < D32; ++n)
@@ -542,7 +546,7 @@ template <typename T, typename TC, int D32, bool FEW> __device__ __forceinline__
           const u32x2 v0 = __builtin_bit_cast(u32x2, v[0]), v1 = __builtin_bit_cast(u32x2, v[1]);
           const u32x4 both = {v0[0], v0[1], v1[0], v1[1]};
 #pragma unroll
-          for (int l = 0; l < QP; ++l)
+          for (int l = 0; l < S::WP; ++l)
             if (j + l < 3) sums[n] = multiply<M>(both, weights[l], sums[n]);
         }
     }

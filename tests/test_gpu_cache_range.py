@@ -3,8 +3,8 @@ import pytest
 import torch
 
 from aihwkit_amd import digital
-from cache_oracle import bound_of
-from test_gpu_cache import BF16, F32, LAYOUTS, PAIR_IDS, PAIRS, Batch, numbers
+from cache_oracle import U, bound_of
+from test_gpu_cache import BF16, F16, F32, LAYOUTS, PAIR_IDS, PAIRS, Batch, numbers
 from test_gpu_digital import close
 
 pytestmark = pytest.mark.gpu
@@ -26,14 +26,14 @@ def test_many_rows_of_no_sequence_before_the_first(heads, kv, head, dtype, cache
 
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 @pytest.mark.parametrize("heads, kv, head", [(4, 2, 64), (2, 1, 128), (2, 1, 200)])
-@pytest.mark.parametrize("scale", [1e-12, -1e-20, 1e-37, 1e-42, 2.0 ** -149])
-def test_scales_near_zero(scale, heads, kv, head, dtype, cache_dtype):
+def test_scales_near_zero(heads, kv, head, dtype, cache_dtype):
     """The mean of what a row sees, of rows of zeros too (whose lift beside halves is the largest that there is)."""
     for layout in ("tokens", "mixed", "prompt"):
         batch = Batch(LAYOUTS[layout], heads, kv, head, 16, dtype, cache_dtype, seed=62).gpu()
         batch.q[::2] = 0.0
         batch.q[1::3, 1] = 1e-30
-        batch.check(batch.attend(scale=scale), scale=scale)
+        for scale in (1e-12, -1e-20, 1e-37, 1e-42, 2.0 ** -149):
+            batch.check(batch.attend(scale=scale), scale=scale)
         batch.check(batch.attend(scale=scale, window=50, sinks=3), scale=scale, window=50, sinks=3)
 
 
@@ -67,22 +67,22 @@ def check_exact(batch, difference, **kw):
 
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 @pytest.mark.parametrize("name", LONG)
-@pytest.mark.parametrize("scale", [300.0, 1e5, -1e9, 1e10, 3e17, -1e30])
-def test_large_scales(scale, name, dtype, cache_dtype):
+def test_large_scales(name, dtype, cache_dtype):
     """Only the largest scores count, all of them alike: they are whole numbers."""
     batch = whole_scores(name, dtype, cache_dtype)
-    check_exact(batch, 0.0, scale=scale)
+    for scale in (300.0, 1e5, -1e9, 1e10, 3e17, -1e30):
+        check_exact(batch, 0.0, scale=scale)
     check_exact(batch, 0.0, scale=scale, window=90, sinks=2)
 
 
 @pytest.mark.parametrize("dtype, cache_dtype", PAIRS, ids=PAIR_IDS)
 @pytest.mark.parametrize("name", LONG)
-@pytest.mark.parametrize("offset", [lambda j: 1024.0, lambda j: -1024.0, lambda j: -1024.0 if j < 700 else 1024.0, lambda j: 1024.0 if j % 64 == 7 else -8.0],
-                         ids=["high", "low", "rising", "few"])
-@pytest.mark.parametrize("scale", [0.05, 0.25, 1.0])
-def test_scores_far_from_zero(scale, offset, name, dtype, cache_dtype):
+def test_scores_far_from_zero(name, dtype, cache_dtype):
     """2^18 and more beside differences of a few: 2^-64 and less of a weight does not count."""
-    check_exact(whole_scores(name, dtype, cache_dtype, offset), 64.0, scale=scale)
+    for offset in (lambda j: 1024.0, lambda j: -1024.0, lambda j: -1024.0 if j < 700 else 1024.0, lambda j: 1024.0 if j % 64 == 7 else -8.0):
+        batch = whole_scores(name, dtype, cache_dtype, offset)
+        for scale in (0.05, 0.25, 1.0):
+            check_exact(batch, 64.0, scale=scale)
 
 
 @pytest.mark.parametrize("dtype, cache_dtype", [(F32, F32), (F32, BF16), (BF16, BF16)], ids=["f32-f32", "f32-bf16", "bf16-bf16"])
@@ -149,3 +149,19 @@ def test_starts_lengths_and_tables_out_of_range_write_nowhere_else(neighbours, d
                 now.copy_(then)
             assert torch.equal(room, before)          # beside the cache
             assert (whole[:10] == 7).all() and (whole[10 + batch.rows:] == 7).all()
+
+
+@pytest.mark.parametrize("dtype", [BF16, F16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("heads, kv, head", [(12, 12, 64), (14, 2, 80), (8, 2, 128), (3, 1, 256)])
+def test_few_rows_of_16_bits_have_what_their_rounding_leaves(heads, kv, head, dtype):
+    """Weights in two parts: each is off by half a step of what its rounding leaves, a quarter of eps squared, of halves at least 2^-25 / 2^7 of the largest
+    (which is 2^7 and more when it is rounded).  What is stored is the number nearest to some value that near."""
+    step = torch.finfo(dtype).eps ** 2 / 4
+    for layout in ([(1, 0), (1, 30), (1, 129), (1, 500), (1, 1000)], [(3, 61), (2, 0), (2, 200)], [(1, 2500), (4, 40)]):
+        batch = Batch(layout, heads, kv, head, 16, dtype, dtype, seed=68).gpu()
+        for kw in (dict(), dict(window=70, sinks=3)):
+            expected, parts = batch.expected(**kw)
+            each = (head + 6) * U * parts["magnitude"] + 12 * U + parts["count"] * U
+            limit = (2 * each + step) * parts["plain"] * (1 + 2 * each + step) + (2.0 ** -32 * parts["flat"] if dtype == F16 else 0.0) + 2 * U * expected.abs()
+            got = batch.attend(**kw).cpu()
+            assert (got >= (expected - limit).to(dtype)).all() and (got <= (expected + limit).to(dtype)).all()
