@@ -97,12 +97,6 @@ __device__ __forceinline__ Sequence sequence_of(const CacheRowsDev &r, int row) 
   if (row < s.begin || row >= s.end) s.which = -1;
   return s;
 }
-// the page of a position of a sequence; -1: none
-__device__ __forceinline__ int page_of(const CacheDev &c, const CacheRowsDev &r, const int *table, long position) {
-  if (position < 0 || position >= r.places) return -1;
-  const int page = table[position >> c.page_shift];
-  return page >= 0 && page < c.pages ? page : -1;
-}
 // Weights are 2^(c score - c reference), c of the scale's magnitude.
 constexpr float LOG2E = 1.44269504088896340736f;
 __device__ __forceinline__ float exponent_factor(float scale) { return fabsf(scale * LOG2E); }
