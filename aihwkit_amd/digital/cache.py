@@ -196,7 +196,9 @@ class PagedCache:
         multiple of the cache's, each of which serves as many neighbouring ones.  ``scale`` (None: ``head_size ** -0.5``; up to 1e30)
         multiplies the products of queries and keys.  ``longest``: a number that no length exceeds (None: what the tables hold); how the work is
         shared goes by it, the results are right without it.  A row that sees nothing becomes zeros, and so does one whose weights are all
-        zero.  What a row does not see does not reach it, infinities and NaN included.  ``out`` may be ``queries``."""
+        zero.  What a row does not see does not reach it, infinities and NaN included; one among the values that a head of a row sees makes its
+        column of that head infinite or NaN, one among the keys that it sees, or in its query, may make all of its columns so.  The products of
+        queries and keys, and the sums of the values by weights of up to 1, are to stay below the largest float.  ``out`` may be ``queries``."""
         done = torch_calls().cache_attend(self.keys, self.values, self._shape, queries, tables, lengths, starts, scale, window, sinks, longest, out,
                                           non_blocking)
         if done is not None:
