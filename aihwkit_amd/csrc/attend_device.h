@@ -11,18 +11,18 @@
 // weight, in a mean of values, an error 1.27 times that of the result's rounding alone (8192 tokens, 32 heads of 128 bf16: 2.10e-3 for 1.65e-3 of the norm).
 // In two parts there, products take half as many again: 810 us for 576, 16384 tokens under a window of 2048, 16 heads of 64 halves 266 for 212.
 // Floats go in parts: beside bf16 and floats three bf16 each, beside halves two halves, lifted by a power of two; products of parts that add up to
-// less than 2^-24 of the largest are left out.
+// less than 2^-24 of the largest are left out (two halves have 22 to 23 bits).
 //
 // What bounds it, and what it reaches (us; MI355X):
-//   one token a sequence   memory: keys and values are read once.  64 sequences of up to 8192 positions, 8 heads of 128 bf16 (1.3 GB): 241, 5.5 TB/s;
-//                          one of 131072 positions (0.5 GB): 100; a window of 1024 (0.3 GB): 54; one of 1024 positions, 12 heads of 64: 9.1, two launches.
+//   one token a sequence   memory: keys and values are read once.  64 sequences of up to 8192 positions, 8 heads of 128 bf16 (1.3 GB): 240, 5.5 TB/s;
+//                          one of 131072 positions (0.5 GB): 101; a window of 1024 (0.3 GB): 55; one of 1024 positions, 12 heads of 64: 9.2, two launches.
 //                          (One wave for a line, without matrix instructions: 7551, 119976, 1026, 263.)  Heads of 256, 16 sequences of 4096, 8 heads bf16
-//                          (0.3 GB): 78, in tiles of lines 113; one of 1024, 4 heads: 13, in tiles 35.
-//   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 560 to 585 us (940 to 980 TFLOP/s; a large matrix product 1320), the matrix pipes are
-//                          busy for 45 %, vector instructions take 50 %, LDS 45 %.  Without the loads of keys and values it takes 476, without
-//                          exponentials 541, without barriers 551.  16384 tokens under a window of 2048, 16 heads of 64 halves: 203 (635 TFLOP/s).
-//   float rows             the products of parts: 3 (bf16 cache), 2 (halves), 6 (floats).  8 x 1024 tokens, 12 heads of 64, bf16 cache: 54 (237 TFLOP/s, a matrix
-//                          product of floats 152).  Floats throughout: 23 sequences, 15 heads of 80 under a window of 777: 107, of which few lines 13, the join 10.
+//                          (0.3 GB): 79, in tiles of lines 113; one of 1024, 4 heads: 13, in tiles 35.
+//   prompts                nothing alone: of the time of 8192 tokens, 32 heads of 128 bf16, 554 to 588 us (935 to 990 TFLOP/s; a large matrix product 1320), the matrix pipes are
+//                          busy for 46 %, vector instructions take 50 %, LDS 45 %.  Of 565, without the loads of keys and values it takes 476,
+//                          without exponentials 541, without barriers 551.  16384 tokens under a window of 2048, 16 heads of 64 halves: 205 to 215 (600 to 630 TFLOP/s).
+//   float rows             the products of parts: 3 (bf16 cache), 2 (halves), 6 (floats).  8 x 1024 tokens, 12 heads of 64, bf16 cache: 54 (239 TFLOP/s, a matrix
+//                          product of floats 152), halves 44 (293).  Floats throughout: 23 sequences, 15 heads of 80 under a window of 777: 107, of which few lines 14, the join 10.
 // Not kept: 64 lines to a wave (half the reads of LDS; heads of 64 211 us for 203, heads of 128 spill), eight waves to a workgroup (618 for 563), the next
 // tile's scores ahead for heads of 64 (a third wave to a SIMD is worth more: 254 for 219), waves' priorities and other orders of the instructions (1 %).
 #pragma once
@@ -811,7 +811,7 @@ __global__ __launch_bounds__(256, (Shape<T, TC, D32, FEW>::PER_SIMD)) void k_att
   attend_job<T, TC, D32, FEW>(a, from);
 }
 // Sequences of many and of few lines in one launch, where both take as many waves to a SIMD: tiles, which take longest, first.  (bf16; 64 sequences of up
-// to 40 and 16040 tokens, 8 heads of 128: 434 us, in two launches 546; 16 of up to 100 and 600, 2 heads of 64: 17 and 23.)
+// to 40 and 16040 tokens, 8 heads of 128: 434 us, in two launches 546 (414 since); 16 of up to 100 and 600, 2 heads of 64: 17 and 23.)
 template <typename T, typename TC, int D32>
 __global__ __launch_bounds__(256, (Shape<T, TC, D32, false>::PER_SIMD)) void k_attend_mixed(AttendArgs a, long from) {
   if (from + blockIdx.x < a.jobs) attend_job<T, TC, D32, false>(a, from);
