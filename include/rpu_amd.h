@@ -845,8 +845,8 @@ int rpu_cache_append(const rpu_cache *cache, const rpu_cache_rows *rows, const v
  * scale: up to 1e30 in magnitude.  out_dev may be q_dev; rows of no sequence are left as they are.  longest: what no length exceeds (0: what the
  * tables hold); how the work is shared goes by it, results are right without it.  Values of places that a row does not see do not reach it, infinities
  * and NaN included; one among the values that a head of a row sees makes its column of that head infinite or NaN, one among the keys that it sees, or in its
- * query, may make all of its columns so.  The products q k_j, and the sums of the values by weights of up to 1, are to stay below the largest float.  16-bit rows of sequences
- * of more than 32 (rows * q_heads / heads) have their weights rounded to their type.
+ * query, may make all of its columns so.  The products q k_j, and the sums of the values by weights of up to 1, are to stay below the largest float; float rows have fewer
+ * than 22 bits of values below 2^-110.  16-bit rows of sequences of more than 32 (rows * q_heads / heads) have their weights rounded to their type.
  * scratch: rpu_cache_attend_scratch bytes (0: may be null), aligned to 16, used until the call's work is done. */
 size_t rpu_cache_attend_scratch(const rpu_cache *cache, const rpu_cache_rows *rows, int q_heads, int dtype, int window, int sinks, int longest);
 int rpu_cache_attend(const rpu_cache *cache, const rpu_cache_rows *rows, const void *q_dev, long q_ld, void *out_dev, long out_ld, int q_heads,
